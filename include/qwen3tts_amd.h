@@ -375,6 +375,122 @@ int q3t_prefill_rope_write(const q3t_prefill_rope_write_args *args, void *stream
  */
 int q3t_prefill_step(const q3t_prefill_rope_write_args *write, const q3t_prefill_args *attend, void *stream);
 
+/* ---- paged key-value cache ------------------------------------------------------------- */
+
+/*
+ * A cache kept in pages: pools of `pages` pages, each holding `page_size` key (value) rows of
+ * every KV head; row j of request b is row j % page_size of page
+ * page_table[b * table_stride_b + j / page_size].  The pools are (pages, kv_heads, page_size,
+ * head_dim) by strides (p, h, t) in elements, rows unit-stride; any order of the first three
+ * dimensions is a choice of strides.  A page number outside [0, pages) names no page: rows on
+ * it are not written, and keys on it do not exist.
+ */
+
+/*
+ * Paired write of new rows: with j = positions[b] + t,
+ *   key_pages  [page_table[b, j / page_size], h, j % page_size, :] = keys  [b, h, t, :]
+ *   value_pages[page_table[b, j / page_size], h, j % page_size, :] = values[b, h, t, :]
+ * for b < batch, h < heads, t < min(tokens, lengths[b]) (lengths == NULL: all tokens), bit-exact
+ * copies of elem_size-byte elements.  Rows whose j lies outside [0, table_width * page_size) or
+ * that are on no page are skipped on the device, as q3t_kv_write skips rows outside the arena.
+ * Two rows of one launch for the same place of the pool leave one of the two, either one.
+ * The counterpart of q3t_kv_write (SlotCache.update's scatter, continuous.py:152-166) and, with
+ * lengths, of the prefix copies of an admitted batch (continuous.py:118-132, 468-469).
+ */
+typedef struct q3t_paged_write_args {
+    int64_t batch, heads, tokens, width, elem_size; /* elem_size 2 or 4 */
+    const void *keys, *values;                      /* rows (b, h, t), unit-stride elements */
+    int64_t k_stride_b, k_stride_h, k_stride_t;
+    int64_t v_stride_b, v_stride_h, v_stride_t;
+    void *key_pages, *value_pages;
+    int64_t kp_stride_p, kp_stride_h, kp_stride_t;
+    int64_t vp_stride_p, vp_stride_h, vp_stride_t;
+    int64_t pages, page_size;
+    const int32_t *page_table; /* device (batch, table_width) */
+    int64_t table_width, table_stride_b;
+    const int64_t *positions;  /* device (batch): j of each request's row t = 0 */
+    const int32_t *lengths;    /* optional device (batch) */
+} q3t_paged_write_args;
+
+int q3t_paged_write(const q3t_paged_write_args *args, void *stream);
+
+/*
+ * Grouped-query attention of one new token per request over a paged cache.  Request b attends
+ * its keys 0 ... positions[b] (a position outside [0, ctx) attends nothing), ctx being at most
+ * table_width * page_size; with a mask (batch, ctx), added to the scaled scores in float32 as
+ * SDPA adds one (bool: nonzero attends).  A key whose mask term is minus infinity (or false),
+ * or that is on no page, does not exist: whatever its rows hold, none of it reaches the output.
+ * A request that attends nothing gets zero rows.  Query head hq reads KV head
+ * hq / (q_heads / kv_heads).  The counterpart of q3t_decode_attention with query_len 1
+ * (packed_attention.py:75-84) over pages instead of slots.
+ *
+ * dtype Q3T_BF16, Q3T_F16 or Q3T_F32; head_dim 64 or 128; pool bases and strides, query rows:
+ * 16-byte multiples.
+ */
+typedef struct q3t_paged_args {
+    int64_t batch, q_heads, kv_heads, head_dim, dtype;
+    int64_t ctx;   /* keys that a request may have, 1 ... table_width * page_size, below 2^30 */
+    float scale;   /* softmax scale, normally head_dim ** -0.5 */
+    int32_t reserved; /* 0 */
+    const void *query; /* (batch, q_heads, head_dim) */
+    int64_t q_stride_b, q_stride_h;
+    const void *key_pages, *value_pages;
+    int64_t kp_stride_p, kp_stride_h, kp_stride_t;
+    int64_t vp_stride_p, vp_stride_h, vp_stride_t;
+    int64_t pages, page_size;
+    const int32_t *page_table;
+    int64_t table_width, table_stride_b;
+    const int64_t *positions;  /* device (batch): the new token's position */
+    const void *mask;          /* optional (batch, ctx) */
+    int64_t mask_dtype, mask_stride_b, mask_stride_t;
+    void *out;                 /* (batch, q_heads, head_dim), query's dtype */
+    int64_t o_stride_b, o_stride_h;
+    void *workspace;           /* q3t_paged_workspace_bytes bytes, a decode workspace */
+    int64_t workspace_bytes;
+} q3t_paged_args;
+
+/* Bytes of workspace q3t_paged_attention needs for these sizes (pointers are not read); -1 for
+   malformed ones.  The workspace is one as q3t_decode_attention takes (its counter region in
+   front, zeroed before first use and by every launch's end; q3t_decode_reset_workspace clears it),
+   so launches of both that follow each other on a stream may share one. */
+int64_t q3t_paged_workspace_bytes(const q3t_paged_args *args);
+
+int q3t_paged_attention(const q3t_paged_args *args, void *stream);
+
+/* ---- rotary positions with several axes --------------------------------------------------- */
+
+/*
+ * Rotate-half RoPE of query and key rows whose tokens have a position on each of `axes` axes
+ * (time, height, width of images and video; the talker's mrope_section).  Frequency i of
+ * half = sum(sections) turns by positions[axis(i), b, s] * turns[i] full turns, where axis(i) is
+ * the section that i falls in or, interleaved, a = i % axes where i < axes * sections[a], and 0
+ * otherwise:
+ *   y[i] = x[i] cos - x[i + half] sin,  y[i + half] = x[i + half] cos + x[i] sin
+ * with cos and sin multiplied by `scaling`; elements past 2 * half are copied.  Angles are formed
+ * in 64 bits and reduced before cos and sin, products and sums in float32, and each element is
+ * rounded once (q3t_rotary, given cos/sin rows, rounds as torch-eager does).  Outputs may be the
+ * inputs themselves.  turns: device, `half` doubles, frequency / (2 pi).
+ * Replaces: the talker's rotary_emb and apply_multimodal_rotary_pos_emb on unequal axes
+ * (continuous.py:193, packed_attention.py:66-69).
+ */
+typedef struct q3t_rotary_axes_args {
+    int64_t batch, tokens, q_heads, k_heads, width, dtype; /* k_heads 0: no keys */
+    int64_t axes, sections[4];                             /* 1 ... 4 axes */
+    int32_t interleaved;
+    float scaling;
+    const double *turns;
+    const int64_t *positions; /* device (axes, batch, tokens) */
+    int64_t p_stride_a, p_stride_b, p_stride_s;
+    const void *query, *key;  /* (batch, tokens, heads, width), rows unit-stride */
+    int64_t q_stride_b, q_stride_s, q_stride_h;
+    int64_t k_stride_b, k_stride_s, k_stride_h;
+    void *q_out, *k_out;
+    int64_t qo_stride_b, qo_stride_s, qo_stride_h;
+    int64_t ko_stride_b, ko_stride_s, ko_stride_h;
+} q3t_rotary_axes_args;
+
+int q3t_rotary_axes(const q3t_rotary_axes_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@ library is missing or a call is rejected, the wrappers raise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -87,6 +88,57 @@ class PrefillRopeWriteArgs(ctypes.Structure):
     ]
 
 
+class PagedWriteArgs(ctypes.Structure):
+    """Mirror of ``q3t_paged_write_args``."""
+    _fields_ = [
+        ("batch", c_i64), ("heads", c_i64), ("tokens", c_i64), ("width", c_i64), ("elem_size", c_i64),
+        ("keys", c_vp), ("values", c_vp),
+        ("k_stride_b", c_i64), ("k_stride_h", c_i64), ("k_stride_t", c_i64),
+        ("v_stride_b", c_i64), ("v_stride_h", c_i64), ("v_stride_t", c_i64),
+        ("key_pages", c_vp), ("value_pages", c_vp),
+        ("kp_stride_p", c_i64), ("kp_stride_h", c_i64), ("kp_stride_t", c_i64),
+        ("vp_stride_p", c_i64), ("vp_stride_h", c_i64), ("vp_stride_t", c_i64),
+        ("pages", c_i64), ("page_size", c_i64),
+        ("page_table", c_vp), ("table_width", c_i64), ("table_stride_b", c_i64),
+        ("positions", c_vp), ("lengths", c_vp),
+    ]
+
+
+class PagedArgs(ctypes.Structure):
+    """Mirror of ``q3t_paged_args``."""
+    _fields_ = [
+        ("batch", c_i64), ("q_heads", c_i64), ("kv_heads", c_i64), ("head_dim", c_i64), ("dtype", c_i64),
+        ("ctx", c_i64), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("query", c_vp), ("q_stride_b", c_i64), ("q_stride_h", c_i64),
+        ("key_pages", c_vp), ("value_pages", c_vp),
+        ("kp_stride_p", c_i64), ("kp_stride_h", c_i64), ("kp_stride_t", c_i64),
+        ("vp_stride_p", c_i64), ("vp_stride_h", c_i64), ("vp_stride_t", c_i64),
+        ("pages", c_i64), ("page_size", c_i64),
+        ("page_table", c_vp), ("table_width", c_i64), ("table_stride_b", c_i64),
+        ("positions", c_vp),
+        ("mask", c_vp), ("mask_dtype", c_i64), ("mask_stride_b", c_i64), ("mask_stride_t", c_i64),
+        ("out", c_vp), ("o_stride_b", c_i64), ("o_stride_h", c_i64),
+        ("workspace", c_vp), ("workspace_bytes", c_i64),
+    ]
+
+
+class RotaryAxesArgs(ctypes.Structure):
+    """Mirror of ``q3t_rotary_axes_args``."""
+    _fields_ = [
+        ("batch", c_i64), ("tokens", c_i64), ("q_heads", c_i64), ("k_heads", c_i64), ("width", c_i64),
+        ("dtype", c_i64), ("axes", c_i64), ("sections", c_i64 * 4),
+        ("interleaved", ctypes.c_int32), ("scaling", ctypes.c_float),
+        ("turns", c_vp), ("positions", c_vp),
+        ("p_stride_a", c_i64), ("p_stride_b", c_i64), ("p_stride_s", c_i64),
+        ("query", c_vp), ("key", c_vp),
+        ("q_stride_b", c_i64), ("q_stride_s", c_i64), ("q_stride_h", c_i64),
+        ("k_stride_b", c_i64), ("k_stride_s", c_i64), ("k_stride_h", c_i64),
+        ("q_out", c_vp), ("k_out", c_vp),
+        ("qo_stride_b", c_i64), ("qo_stride_s", c_i64), ("qo_stride_h", c_i64),
+        ("ko_stride_b", c_i64), ("ko_stride_s", c_i64), ("ko_stride_h", c_i64),
+    ]
+
+
 # Every exported entry point with its ctypes signature.
 SIGNATURES = {
     "q3t_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -111,6 +163,10 @@ SIGNATURES = {
     "q3t_prefill_attention": (ctypes.c_int, [ctypes.POINTER(PrefillArgs), c_vp]),
     "q3t_prefill_rope_write": (ctypes.c_int, [ctypes.POINTER(PrefillRopeWriteArgs), c_vp]),
     "q3t_prefill_step": (ctypes.c_int, [ctypes.POINTER(PrefillRopeWriteArgs), ctypes.POINTER(PrefillArgs), c_vp]),
+    "q3t_paged_write": (ctypes.c_int, [ctypes.POINTER(PagedWriteArgs), c_vp]),
+    "q3t_paged_workspace_bytes": (c_i64, [ctypes.POINTER(PagedArgs)]),
+    "q3t_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedArgs), c_vp]),
+    "q3t_rotary_axes": (ctypes.c_int, [ctypes.POINTER(RotaryAxesArgs), c_vp]),
 }
 
 _lock = threading.Lock()
@@ -159,6 +215,14 @@ def check(status: int, what: str) -> None:
 def stream_handle(device: torch.device) -> int:
     """Raw hipStream_t of torch's current stream on ``device``."""
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """``device`` as the current device for a launch; nothing to do where it is already."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 _HIP = None

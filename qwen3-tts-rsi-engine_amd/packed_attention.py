@@ -25,6 +25,8 @@ signature compatibility):
   for two queries): ``decode_step`` writes positions 0 and 1 and attends them causally.  The
   mask's values are read once, outside graph capture, and the result is kept per mask
   tensor;
+* a one-token step over a ``PagedCache`` rotates q and k, writes the new rows into their pages
+  and attends them with ``paged_attention`` under the layer's mask, if any;
 * every other call rotates q/k with ``rotary`` (bf16-exact to torch eager), lets the cache
   update and calls ``attention`` (the npu_attention.attention drop-in).
 
@@ -39,6 +41,7 @@ from __future__ import annotations
 import torch
 
 from .attention import attention, decode_step, plan_shape, prefill_attention
+from .paged import PagedCache, paged_attention
 from .prefill import prefill_rope_write
 from .rotary import rotary
 from .slots import PredictorCache, PrefillCache, SlotCache
@@ -249,6 +252,13 @@ class PackedAttention(torch.nn.Module):
         query = rotary(query.contiguous(), cos, sin).transpose(1, 2)
         key = rotary(key.contiguous(), cos, sin).transpose(1, 2)
         value = value.transpose(1, 2)
+        if isinstance(past_key_values, PagedCache):
+            if reference.training or getattr(reference, 'sliding_window', None) is not None:
+                raise ValueError('Paged attention is inference-only and without a sliding window')
+            pages = past_key_values.update(key, value, reference.layer_idx)
+            output = paged_attention(query.transpose(1, 2), *pages, past_key_values.page_table,
+                                     past_key_values.positions, scale=reference.scaling, mask=attention_mask)
+            return reference.o_proj(output.reshape(*shape, -1)), None
         if past_key_values is not None:
             key, value = past_key_values.update(key, value, reference.layer_idx,
                                                 {'sin': sin, 'cos': cos, 'cache_position': cache_position})

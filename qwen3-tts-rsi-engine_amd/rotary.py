@@ -6,7 +6,12 @@ output tensor, and torch-eager rounding after every op (kernel ``q3t_rotary``); 
 are accepted too, with torch-eager fp32 rounding.
 ``rope_tables`` produces the default-RoPE cos/sin rows for integer positions
 (kernel ``q3t_rope_tables``); ``inverse_frequencies`` is the host-side fp32 table it uses.
+``rotary_axes`` rotates queries and keys of tokens with a position on each of several axes (the
+talker's ``mrope_section``; time, height and width of images and video; kernel
+``q3t_rotary_axes``).
 """
+import math
+
 import torch
 
 from . import _lib
@@ -67,3 +72,75 @@ def rope_tables(positions, head_dim, theta=DEFAULT_THETA, scaling=1.0, dtype=tor
                                             sin.data_ptr(), _lib.stream_handle(positions.device))
     _lib.check(status, 'rope tables')
     return cos, sin
+
+
+_TURNS = {}
+
+
+def _turns(half, theta, device):
+    """Full turns per position of every frequency, theta**(-i/half) / 2 pi, in float64."""
+    key = (device, half, float(theta))
+    turns = _TURNS.get(key)
+    if turns is None:  # cached so that captured graphs never see a host copy
+        exponent = torch.arange(half, dtype=torch.float64) / half
+        turns = _TURNS[key] = (float(theta) ** -exponent / (2 * math.pi)).to(device)
+    return turns
+
+
+def rotary_axes(query, key, positions, sections, *, interleaved=False, theta=DEFAULT_THETA, inv_freq=None,
+                scaling=1.0, inplace=False):
+    """Rotate-half RoPE of tokens that have a position on each of several axes.
+
+    query (B, S, Hq, D) and key (B, S, Hkv, D), or None: bf16, fp16 or fp32 rows of any strides
+    with unit-stride elements (views of the fused QKV projection are fine); positions (A, B, S)
+    int64, A in 1 ... 4.  ``sections`` are the axes' shares of the ``half = sum(sections)``
+    frequencies theta**(-i/half), or of ``inv_freq`` (half,), consecutively, or ``interleaved``:
+    frequency i then belongs to axis ``a = i % A`` where ``i < A * sections[a]``, else to axis 0
+    (the talker's ``mrope_section`` with ``interleaved``).  Elements i and i + half turn by
+    ``positions[axis(i)] * frequency_i``; elements past ``2 * half`` are copied; cos and sin are
+    multiplied by ``scaling``.  Angles are formed in float64, the rest in float32, and each element
+    is rounded once (``rotary``, given cos/sin rows, rounds as torch-eager does).
+
+    Returns (query, key) rotated: new contiguous tensors, or with ``inplace`` the given ones,
+    rotated where they are."""
+    tensors = [query] if key is None else [query, key]
+    if any(t.ndim != 4 for t in tensors) or (key is not None and (key.shape[:2] != query.shape[:2]
+                                                                  or key.shape[3] != query.shape[3])):
+        raise ValueError('expected BSND query and key rows of one batch, length and width')
+    batch, tokens, q_heads, width = query.shape
+    if query.dtype not in _lib.DTYPE_CODES or query.dtype == torch.bool or tensors[-1].dtype != query.dtype:
+        raise ValueError('rotary supports bf16, fp16 or fp32 tensors of one dtype')
+    sections = tuple(sections)
+    if not 1 <= len(sections) <= 4 or any(not isinstance(n, int) or n < 0 for n in sections):
+        raise ValueError('sections must be one to four counts of frequencies')
+    half = sum(sections)
+    if not 1 <= half or 2 * half > width or half > 512:
+        raise ValueError('sections must sum to at least one and at most half of the width (512 at most)')
+    if positions.dtype != torch.int64 or tuple(positions.shape) != (len(sections), batch, tokens):
+        raise ValueError('positions must be an int64 (axes, batch, length) tensor')
+    if any(t.shape[2] < 1 or t.stride(3) != 1 for t in tensors):
+        raise ValueError('rows must be unit-stride, at least one per token')
+    device = _lib.require_gpu(*tensors, positions)
+    if inplace and any(n > 1 and s == 0 for t in tensors for n, s in zip(t.shape, t.stride())):
+        raise ValueError('rows that share memory cannot be rotated in place')
+    if inv_freq is None:
+        turns = _turns(half, theta, device)
+    else:
+        if inv_freq.shape != (half,):
+            raise ValueError('inv_freq must have one entry per frequency')
+        turns = inv_freq.to(device=device, dtype=torch.float64) / (2 * math.pi)
+    outs = tensors if inplace else [torch.empty(t.shape, device=device, dtype=t.dtype) for t in tensors]
+    if query.numel() == 0:
+        return outs[0], None if key is None else outs[1]
+    k, ko = (None, None) if key is None else (key, outs[1])
+    none = (0, 0, 0)
+    a = _lib.RotaryAxesArgs(
+        batch, tokens, q_heads, 0 if key is None else key.shape[2], width, _lib.DTYPE_CODES[query.dtype],
+        len(sections), (_lib.c_i64 * 4)(*sections), bool(interleaved), scaling, turns.data_ptr(),
+        positions.data_ptr(), *positions.stride(), query.data_ptr(), _lib.ptr(k),
+        *query.stride()[:3], *(none if k is None else k.stride()[:3]), outs[0].data_ptr(), _lib.ptr(ko),
+        *outs[0].stride()[:3], *(none if ko is None else ko.stride()[:3]))
+    with _lib.on_device(device):
+        status = _lib.library().q3t_rotary_axes(a, _lib.stream_handle(device))
+    _lib.check(status, 'rotary axes')
+    return outs[0], None if key is None else outs[1]
