@@ -27,4 +27,67 @@ Q3T_BOTH uint32_t divide(uint32_t n, const Divisor &v) {
     return ((uint32_t)(((uint64_t)v.m * n) >> 32) + n) >> v.l;
 }
 
+// ---- how the paged attention's work is shared out ------------------------------------------
+//
+// A pair is a request with one KV head (and up to 16 of its query heads).  A pair's keys are read
+// in rounds of a fixed number of keys, at least one.  All pairs' rounds lie on one line, request
+// by request, head by head, and workgroup w takes the share [w * share, (w + 1) * share) of it.  A
+// pair that lies in several shares is merged from its parts.
+//   * When every pair cut into pieces of `kShareRounds` rounds gives no more pieces than there are
+//     workgroups, each piece is a share of its own: pairs take a multiple of that many places on
+//     the line (`unit`), the last piece the rest of the pair.
+//   * Otherwise the line holds the rounds alone and the shares are equal.
+
+struct Sharing {
+    uint32_t unit;   // places of a pair are a multiple of it
+    uint32_t share;  // places of a workgroup
+    uint32_t total;  // places in all
+};
+
+// From the pairs' rounds, and their pieces of `least` rounds, over all pairs.
+Q3T_BOTH Sharing sharing(uint32_t rounds, uint32_t pieces, uint32_t least, uint32_t workgroups) {
+    if (pieces <= workgroups) return {least, least, pieces * least};
+    return {1u, (uint32_t)(((uint64_t)rounds + workgroups - 1) / workgroups), rounds};
+}
+
+Q3T_BOTH uint32_t places(uint32_t rounds, uint32_t unit) { return (rounds + unit - 1) / unit * unit; }
+
+// Where a workgroup is on the line: place x, `left` places to go, at place `off` of pair (b, head).
+struct Cursor {
+    uint32_t x, left, b, head, off;
+};
+
+// A run of one pair's rounds [lo, hi) in one share: part `x / share` - first of the pair's `parts`.
+// Its state's slot is 2 w for a pair that began in an earlier share (a workgroup's first run at
+// most), 2 w + 1 for one that begins in this one (the last at most, if there are more parts).
+struct Run {
+    uint32_t b, head, lo, hi, first, parts, begins;
+};
+
+// The run at the cursor, for a pair of `rounds` rounds, and the cursor moved past it.
+Q3T_BOTH Run next_run(Cursor &c, uint32_t rounds, uint32_t heads, const Sharing &s) {
+    const uint32_t length = places(rounds, s.unit), rest = length - c.off;
+    const uint32_t take = rest < c.left ? rest : c.left, end = c.off + take;
+    Run r;
+    r.b = c.b;
+    r.head = c.head;
+    r.lo = c.off;
+    r.hi = end < rounds ? end : rounds;
+    r.begins = c.off == 0;
+    const uint32_t start = c.x - c.off;
+    r.first = start / s.share;
+    r.parts = (start + length - 1) / s.share - r.first + 1;
+    c.x += take;
+    c.left -= take;
+    c.off = end;
+    if (end == length) {
+        c.off = 0;
+        if (++c.head == heads) {
+            c.head = 0;
+            ++c.b;
+        }
+    }
+    return r;
+}
+
 }  // namespace q3t

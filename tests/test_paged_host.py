@@ -32,6 +32,18 @@ def index(tmp_path_factory):
     (where / 'index.cpp').write_text(f'''
 #include "{CSRC / 'paged_index.hpp'}"
 extern "C" uint32_t quotient(uint32_t n, uint32_t d) {{ return q3t::divide(n, q3t::divisor(d)); }}
+extern "C" void share_out(uint32_t rounds, uint32_t pieces, uint32_t least, uint32_t workgroups, uint32_t *out) {{
+    const q3t::Sharing s = q3t::sharing(rounds, pieces, least, workgroups);
+    out[0] = s.unit; out[1] = s.share; out[2] = s.total;
+}}
+extern "C" uint32_t places(uint32_t rounds, uint32_t unit) {{ return q3t::places(rounds, unit); }}
+extern "C" void next_run(uint32_t *cursor, uint32_t rounds, uint32_t heads, const uint32_t *sharing, uint32_t *out) {{
+    q3t::Cursor c = {{cursor[0], cursor[1], cursor[2], cursor[3], cursor[4]}};
+    const q3t::Run r = q3t::next_run(c, rounds, heads, q3t::Sharing{{sharing[0], sharing[1], sharing[2]}});
+    const uint32_t after[5] = {{c.x, c.left, c.b, c.head, c.off}}, run[7] = {{r.b, r.head, r.lo, r.hi, r.first, r.parts, r.begins}};
+    for (int i = 0; i < 5; ++i) cursor[i] = after[i];
+    for (int i = 0; i < 7; ++i) out[i] = run[i];
+}}
 ''')
     subprocess.run(['g++', '-std=c++17', '-O2', '-shared', '-fPIC', '-fsanitize=undefined', '-fno-sanitize-recover',
                     str(where / 'index.cpp'), '-o', str(where / 'index.so')], check=True)
@@ -48,6 +60,53 @@ def test_division(index):
         for n in [0, 1, d - 1, d, min(d + 1, top), 2 * d - 1 if 2 * d - 1 <= top else top, top // d * d, max(top // d * d - 1, 0), top] + \
                  [rng.randrange(0, top) for _ in range(20)]:
             assert index.quotient(n, d) == n // d, (n, d)
+
+
+@pytest.mark.parametrize('seed', range(60))
+def test_shares_cover_every_pair_once(index, seed):
+    """Every workgroup's runs, together: each round of each pair exactly once, in one run per share,
+    parts numbered from the pair's first share, at most two unfinished states a workgroup and no slot
+    of them twice, no share longer than it says."""
+    rng = random.Random(seed)
+    heads, workgroups, least = rng.choice([1, 2, 3, 8]), rng.choice([1, 3, 16, 64, 512]), rng.choice([1, 4])
+    rounds = [rng.choice([1, 1, 2, 3, rng.randrange(1, 17), rng.randrange(1, 900)]) for _ in range(rng.choice([1, 2, 7, 40]))]
+    u32 = ctypes.c_uint32
+    sharing = (u32 * 3)()
+    index.share_out(sum(rounds) * heads, sum(-(-r // least) for r in rounds) * heads, least, workgroups, sharing)
+    unit, share, total = sharing
+    length = [index.places(r, unit) for r in rounds]
+    assert total == heads * sum(length) and share * workgroups >= total and share >= 1
+    covered, parts, slots = {}, {}, set()
+    for w in range(workgroups):
+        x = w * share
+        if x >= total:
+            continue
+        off, b = x, 0
+        while off >= length[b] * heads:
+            off -= length[b] * heads
+            b += 1
+        cursor = (u32 * 5)(x, min(share, total - x), b, off // length[b], off % length[b])
+        unfinished = 0
+        while cursor[1]:
+            out = (u32 * 7)()
+            index.next_run(cursor, rounds[cursor[2]], heads, sharing, out)
+            rb, head, lo, hi, first, count, begins = out
+            assert lo < hi <= rounds[rb]
+            for r in range(lo, hi):
+                assert (rb, head, r) not in covered
+                covered[rb, head, r] = w
+            assert begins == (lo == 0) and first <= w < first + count
+            assert parts.setdefault((rb, head), (first, count)) == (first, count)
+            assert (w == first) == bool(begins)
+            if count > 1:
+                unfinished += 1
+                slot = 2 * w + begins
+                assert slot not in slots
+                slots.add(slot)
+        assert unfinished <= 2
+    assert len(covered) == heads * sum(rounds)
+    for (rb, head), (first, count) in parts.items():
+        assert {covered[rb, head, r] for r in range(rounds[rb])} == set(range(first, first + count))
 
 
 def _attend_args(pkg, **changes):
