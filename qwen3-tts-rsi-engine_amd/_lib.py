@@ -214,7 +214,13 @@ def check(status: int, what: str) -> None:
 
 def stream_handle(device: torch.device) -> int:
     """Raw hipStream_t of torch's current stream on ``device``."""
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# the same handle without a Stream object in between, where torch has it (2 us a call less)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
 
 
 _HERE = contextlib.nullcontext()

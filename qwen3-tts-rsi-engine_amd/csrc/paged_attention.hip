@@ -12,9 +12,10 @@
 //     workspace, and the workgroup that arrives last merges them, in the parts' order.
 //   * A wave takes every fourth stage of 16 (rows of 128 bytes: 32) keys of a pair.  A stage's rows
 //     go straight from memory to the wave's own two LDS slots, one stage ahead of the one that is
-//     scored, over the ends of pairs: no barrier but where a pair ends.  The stages' page numbers
-//     come the same way, two stages before the rows that they place; each lane works out the
-//     address of its own row, so that any page size will do.
+//     scored, over the ends of pairs: no barrier but where a pair ends.  The page numbers of up to 64
+//     stages come the same way, while the stages before them are read.  Where pages hold whole
+//     stages a stage's rows are one range of memory; for other page sizes each lane works out the
+//     address of its own row.
 //   * The rows of a KV head's query heads are the columns of 16x16 products, S^T = K . Q^T and
 //     O^T += V^T . P^T.  The matrix cores idle (under a twentieth of their rate), so the weights are
 //     not rounded to the cache's type: bf16 weights go in three parts (all 24 bits of their
@@ -25,30 +26,32 @@
 #include "paged_index.hpp"
 #include "q3t_common.hpp"
 
+#include <type_traits>
+
 namespace q3t {
 namespace paged {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kColumns = 16;           // query heads of a workgroup: columns of a product
-constexpr int kWindow = 256;           // requests whose lengths are at hand
-constexpr uint32_t kLeastRounds = 4;   // rounds that are not shared out
-constexpr int kCounters = 65536;       // counter words in front of a decode workspace
+constexpr uint32_t kLeastRounds = 2;   // rounds that are not shared out
+constexpr int kCounters = 65536;       // counter words in front of a decode workspace: of the pairs,
+constexpr int kPairs = kCounters - 1024;  // then of the state slots
+constexpr int kWorkgroups = 512;       // at most
+constexpr uint32_t kTogether = 16;     // parts that are merged in one step
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
     const char *q, *kp, *vp, *mask;
     char *out;
     const int32_t *table;
-    const int64_t *positions;
     int32_t *counters;
     float *states;
-    int64_t q_sb, q_sh, o_sb, o_sh;                    // bytes
-    int64_t m_sb, m_st, table_sb;                      // elements
-    uint32_t kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st; // 16 bytes
-    int32_t ctx, mask_dtype, stream, vec_out;
-    uint32_t batch, pages, group, heads, blocks;       // heads: pairs of a request; blocks: of a KV head
+    uint32_t q_sb, q_sh, kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;  // 16 bytes
+    uint32_t o_sb, o_sh, m_sb, m_st, table_sb;                      // elements
+    int32_t mask_dtype, vec_out;
+    uint32_t pages, group, heads, blocks;       // heads: pairs of a request; blocks: of a KV head
     uint32_t columns;                                  // of a state
-    Divisor by_page;
+    Divisor by_page, by_grid;
     float scale;                                       // unmasked: times log2(e)
 };
 
@@ -74,12 +77,10 @@ template <typename T, int D, bool MASK>
 struct Lds {
     alignas(1024) char ring[kWaves][2][Shape<T, D>::stage];
     alignas(16) char shared[Shape<T, D>::shared];
-    alignas(16) int32_t ids[kWaves][4][Shape<T, D>::keys];
+    uint32_t ids[kWaves][2][64];
     alignas(16) uint32_t maskw[MASK ? kWaves : 1][2][MASK ? Shape<T, D>::keys : 4];
     float ml[kWaves][kColumns][2];
-    int32_t lengths[kWindow];
-    uint32_t sums[kWaves][2];
-    uint32_t start[4];
+    uint32_t count;
 };
 
 #define Q3T_LDS __attribute__((address_space(3)))
@@ -88,18 +89,22 @@ Q3T_DEVICE uint32_t lds_at(const void *x) { return (uint32_t)(uintptr_t)(Q3T_LDS
 Q3T_DEVICE uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
 // Four 16-byte loads per lane into LDS, 1 KiB apart there: the instructions' offsets move both
-// addresses, so load i's pointer is 1024 i short of its row.
-#define Q3T_LOAD4(POLICY)                                                                             \
-    asm volatile("s_mov_b32 m0, %0\n\t" Q3T_VMEM_SGPR_WAIT                                            \
-                 "global_load_lds_dwordx4 %1, off" POLICY "\n\t"                                      \
-                 "global_load_lds_dwordx4 %2, off offset:1024" POLICY "\n\t"                          \
-                 "global_load_lds_dwordx4 %3, off offset:2048" POLICY "\n\t"                          \
-                 "global_load_lds_dwordx4 %4, off offset:3072" POLICY                                 \
-                 :: "s"(base), "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]) : "memory", "m0")
-Q3T_DEVICE void load_rows(const uint64_t *p, uint32_t base, bool stream) {
-    if (stream) Q3T_LOAD4(" nt");
-    else Q3T_LOAD4("");
+// addresses, so load i's address is 1024 i short of its row.
+#define Q3T_LOAD4(OPCODE, ADDRESS, POLICY, ...)                                                    \
+    asm volatile("s_mov_b32 m0, %0\n\t" Q3T_VMEM_SGPR_WAIT                                         \
+                 OPCODE " %1, " ADDRESS POLICY "\n\t"                                              \
+                 OPCODE " %2, " ADDRESS " offset:1024" POLICY "\n\t"                               \
+                 OPCODE " %3, " ADDRESS " offset:2048" POLICY "\n\t"                               \
+                 OPCODE " %4, " ADDRESS " offset:3072" POLICY                                      \
+                 :: "s"(base), "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]) __VA_ARGS__ : "memory", "m0")
+// from a pointer per lane
+Q3T_DEVICE void load_rows(const uint64_t *p, uint32_t base) { Q3T_LOAD4("global_load_lds_dwordx4", "off", " nt"); }
+// from an offset per lane into a resource; past its range zeros are written without a memory access
+#define Q3T_RSRC , "s"(rsrc)
+Q3T_DEVICE void load_rows(i32x4_t rsrc, const uint32_t *p, uint32_t base) {
+    Q3T_LOAD4("buffer_load_dwordx4", "%5, 0 offen", " nt lds", Q3T_RSRC);
 }
+#undef Q3T_RSRC
 #undef Q3T_LOAD4
 Q3T_DEVICE void load_lds16(uint64_t from, uint32_t base) {
     asm volatile("s_mov_b32 m0, %0\n\t" Q3T_VMEM_SGPR_WAIT "global_load_lds_dwordx4 %1, off"
@@ -116,10 +121,9 @@ Q3T_DEVICE void publish(float *p, float a, float b) {
     const uint64_t v = (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32;
     __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-Q3T_DEVICE void collect(const float *p, float &a, float &b) {
+Q3T_DEVICE f32x2_t collect(const float *p) {
     const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    a = __uint_as_float((uint32_t)v);
-    b = __uint_as_float((uint32_t)(v >> 32));
+    return f32x2_t{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
 }
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -188,15 +192,24 @@ template <typename T, int D> struct Tile {
             rest[d] *= a;
         }
     }
-    Q3T_DEVICE f32x4_t scores(uint32_t keys, int t, int g, int c) const {
-        const int r = 16 * t + c;
+    uint32_t key_at[D / 32], value_at[D / 16];  // the lane's places in a stage's first 16 rows (the swizzles repeat every 16)
+
+    Q3T_DEVICE void place(uint32_t ring, int g, int c) {
+        const int r = 4 * g + (c >> 2);
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk) key_at[kk] = ring + c * S::row + (((4 * kk + g) ^ S::key_swizzle(c)) & (S::chunks - 1)) * 16;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+            value_at[d] = ring + (S::keys + r) * S::row + (((2 * d + ((c >> 1) & 1)) ^ S::value_swizzle(r)) & (S::chunks - 1)) * 16 + 8 * (c & 1);
+    }
+    // tile t of the stage at byte `stage` of the ring
+    Q3T_DEVICE f32x4_t scores(uint32_t stage, int t) const {
         f32x4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < D / 32; ++kk)
-            s = Half<T>::scores(lds_read16(keys + r * S::row + (((4 * kk + g) ^ S::key_swizzle(r)) & (S::chunks - 1)) * 16), q[kk], s);
+        for (int kk = 0; kk < D / 32; ++kk) s = Half<T>::scores(lds_read16(key_at[kk] + stage + t * 16 * S::row), q[kk], s);
         return s;
     }
-    Q3T_DEVICE void values(uint32_t rows, int t, int g, int c, const float (&w)[4]) {
+    Q3T_DEVICE void values(uint32_t stage, int t, const float (&w)[4]) {
         uint2 part[3];
         float x[4] = {w[0], w[1], w[2], w[3]};
 #pragma unroll
@@ -207,11 +220,9 @@ template <typename T, int D> struct Tile {
             x[2] -= Half<T>::lo(part[i].y);
             x[3] -= Half<T>::hi(part[i].y);
         }
-        const int r = 16 * t + 4 * g + (c >> 2);
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
-            const int chunk = ((2 * d + ((c >> 1) & 1)) ^ S::value_swizzle(r)) & (S::chunks - 1);
-            const uint2 v = lds_read_tr16(rows + r * S::row + chunk * 16 + 8 * (c & 1));
+            const uint2 v = lds_read_tr16(value_at[d] + stage + t * 16 * S::row);
             first[d] = Half<T>::values(v, part[0], first[d]);
 #pragma unroll
             for (int i = 1; i < Half<T>::parts; ++i) rest[d] = Half<T>::values(v, part[i], rest[d]);
@@ -249,23 +260,29 @@ template <int D> struct Tile<float, D> {
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) acc[d] *= a;
     }
-    Q3T_DEVICE f32x4_t scores(uint32_t keys, int t, int g, int c) const {
-        const int r = 16 * t + c;
+    uint32_t key_at[D / 16], value_at;
+
+    Q3T_DEVICE void place(uint32_t ring, int g, int c) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) key_at[kk] = ring + c * S::row + ((4 * kk + g) ^ S::key_swizzle(c)) * 16;
+        value_at = ring + (S::keys + 4 * g) * S::row + c * 16;
+    }
+    Q3T_DEVICE f32x4_t scores(uint32_t stage, int t) const {
         f32x4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-            const f32x4_t k = read(keys + r * S::row + ((4 * kk + g) ^ S::key_swizzle(r)) * 16);
+            const f32x4_t k = read(key_at[kk] + stage + t * 16 * S::row);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[kk][e], s, 0, 0, 0);
         }
         return s;
     }
-    Q3T_DEVICE void values(uint32_t rows, int t, int g, int c, const float (&w)[4]) {
+    Q3T_DEVICE void values(uint32_t stage, int t, const float (&w)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
-                const f32x4_t v = read(rows + (16 * t + 4 * g + i) * S::row + (16 * j + c) * 16);
+                const f32x4_t v = read(value_at + stage + (16 * t + i) * S::row + j * 256);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[4 * j + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], w[i], acc[4 * j + e], 0, 0, 0);
             }
@@ -281,13 +298,18 @@ template <int D> struct Tile<float, D> {
     }
 };
 
-// The mask term of a word that holds the element at byte `low` of it.
-Q3T_DEVICE float mask_term(uint32_t word, uint32_t low, int dtype) {
+// Four mask terms from four words, each holding its element at byte (low + i step) % 4.
+Q3T_DEVICE void mask_terms(const U4 &words, uint32_t low, uint32_t step, int dtype, float (&x)[4]) {
+    const uint32_t w[4] = {words.x, words.y, words.z, words.w};
+    auto each = [&](auto term) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = term(w[i] >> (8 * ((low + i * step) & 3u)));
+    };
     switch (dtype) {
-        case Q3T_BF16: return bf16_to_float((word >> (8 * low)) & 0xffffu);
-        case Q3T_F16: return (float)__builtin_bit_cast(_Float16, (uint16_t)(word >> (8 * low)));
-        case Q3T_F32: return __uint_as_float(word);
-        default: return (word >> (8 * low)) & 0xffu ? 0.0f : -INFINITY;  // bool: true attends
+        case Q3T_BF16: each([](uint32_t e) { return bf16_to_float(e & 0xffffu); }); break;
+        case Q3T_F16: each([](uint32_t e) { return (float)__builtin_bit_cast(_Float16, (uint16_t)e); }); break;
+        case Q3T_F32: each([](uint32_t e) { return __uint_as_float(e); }); break;
+        default: each([](uint32_t e) { return e & 0xffu ? 0.0f : -INFINITY; });  // bool: true attends
     }
 }
 
@@ -306,14 +328,64 @@ Q3T_DEVICE void store_out(char *at, const float (&y)[4], bool vec) {
     }
 }
 
-// A wave's stage: keys from key0 on of request b (length keys) under pair `head`, in the share's run.
-struct Stage {
-    uint32_t b, head, length, key0;
-    int32_t run;  // -1: none
+// Four elements of a column's softmax state: maximum, sum, weighted values.
+struct State {
+    float m, l;
+    f32x4_t a;
+    // Another state's keys added; fused products by name, so that every copy of this code rounds alike.
+    Q3T_DEVICE void add(const State &o, float unit) {
+        const float top = fmaxf(m, o.m), from = top == -INFINITY ? 0.f : top;
+        const float e0 = fexp2((m - from) * unit), e1 = fexp2((o.m - from) * unit);
+        l = __builtin_fmaf(l, e0, o.l * e1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = __builtin_fmaf(a[i], e0, o.a[i] * e1);
+        m = top;
+    }
+    Q3T_DEVICE void publish(float *to, uint32_t sums, uint32_t column, uint32_t d, int D) const {
+        paged::publish(to + column * D + d, a[0], a[1]);
+        paged::publish(to + column * D + d + 2, a[2], a[3]);
+        if (d == 0) paged::publish(to + sums + 2 * column, m, l);
+    }
+    Q3T_DEVICE void collect(const float *from, uint32_t sums, uint32_t column, uint32_t d, int D) {
+        const f32x2_t ml = paged::collect(from + sums + 2 * column);
+        const f32x2_t lo = paged::collect(from + column * D + d), hi = paged::collect(from + column * D + d + 2);
+        m = ml[0];
+        l = ml[1];
+        a = f32x4_t{lo[0], lo[1], hi[0], hi[1]};
+    }
 };
 
-template <typename T, int D, bool MASK>
-__global__ void __launch_bounds__(kThreads, (Shape<T, D>::per_cu)) paged_kernel(Params p) {
+// Stages of a wave in one run, keys `key`, key + a round, ... below `end`, up to the number of
+// stages whose page numbers fit its 64 words.
+struct Batch {
+    uint32_t b, kv_head, length, key, end;
+    int32_t run;  // of the share; -1: none
+};
+// A wave's stage; bit k of `exists`: key0 + k is a key of the request and on a page.
+struct Stage {
+    uint32_t b, key0, exists;
+    int32_t run;
+};
+
+// Sums over the wave's lanes up to and with each lane.
+Q3T_DEVICE uint32_t scan(uint32_t x) {
+    auto add = [&](auto control, auto rows) {
+        x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(control)::value, decltype(rows)::value, 0xf, false);
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // from 1, 2, 4 and 8 lanes
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});  // below in rows of 16
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // lanes 15 and 47 to the next rows
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // lane 31 to the upper half
+    return x;
+}
+
+// WHOLE: a stage's keys share a page (page sizes that are multiples of a stage), so their rows are one
+// range of memory.
+template <typename T, int D, bool MASK, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, (Shape<T, D>::per_cu))
+paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     typedef Shape<T, D> S;
     typedef Tile<T, D> Products;
     constexpr int LOADS = 2 * S::loads;
@@ -321,151 +393,188 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, D>::per_cu)) paged_kernel(
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = (int)uniform(tid >> 6);
 
-    // ---- the share: all requests' rounds and pieces, then the request that it starts in --------
-    auto length_of = [&](int64_t pos) { return pos >= 0 && pos < p.ctx ? (int)pos + 1 : 0; };
-    auto rounds_of = [&](int length) { return (uint32_t)max(1, (length + S::round - 1) >> S::log_round); };
-    const uint32_t each = (p.batch + kThreads - 1) / kThreads;  // requests of a thread, one after the other
-    uint32_t rounds = 0, pieces = 0;
+    // ---- the share: every wave adds up all requests' rounds and pieces for itself ---------------
+    auto length_at = [&](uint32_t b) {
+        const int64_t pos = b < batch ? positions[b] : -1;
+        return pos >= 0 && pos < (int64_t)ctx ? (uint32_t)pos + 1 : 0u;
+    };
+    auto rounds_of = [&](uint32_t length) { return max(1u, (length + S::round - 1) >> S::log_round); };
+    const uint32_t each = (batch + 63) / 64;  // requests of a lane, one after the other
+    uint32_t lengths = length_at(lane);       // of requests window + lane
+    uint32_t rounds = 0, pieces = 0, window = 0;
     for (uint32_t i = 0; i < each; ++i) {
-        const uint32_t b = tid * each + i;
-        if (b >= p.batch) break;
-        const int length = length_of(p.positions[b]);
-        if (each == 1) s.lengths[tid] = length;
-        rounds += rounds_of(length);
-        pieces += (rounds_of(length) + kLeastRounds - 1) / kLeastRounds;
+        const uint32_t b = lane * each + i, r = rounds_of(each == 1 ? lengths : length_at(b));
+        if (b >= batch) break;
+        rounds += r;
+        pieces += (r + kLeastRounds - 1) / kLeastRounds;
     }
-    uint32_t rounds_to = rounds, pieces_to = pieces;  // sums up to and with this thread
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t a = __shfl_up(rounds_to, o), b = __shfl_up(pieces_to, o);
-        if (lane >= o) {
-            rounds_to += a;
-            pieces_to += b;
-        }
-    }
-    if (lane == 63) {
-        s.sums[wave][0] = rounds_to;
-        s.sums[wave][1] = pieces_to;
-    }
-    __syncthreads();
-    uint32_t all_rounds = 0, all_pieces = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        if (w == wave) {
-            rounds_to += all_rounds;
-            pieces_to += all_pieces;
-        }
-        all_rounds += s.sums[w][0];
-        all_pieces += s.sums[w][1];
-    }
-    const Sharing sh = sharing(uniform(all_rounds) * p.heads, uniform(all_pieces) * p.heads, kLeastRounds, gridDim.x);
+    const uint32_t rounds_to = scan(rounds), pieces_to = scan(pieces);
+    auto last_lane = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); };
+    const Sharing sh = sharing(last_lane(rounds_to) * p.heads, last_lane(pieces_to) * p.heads, kLeastRounds, p.by_grid);
     Cursor at = {};
     at.x = blockIdx.x * sh.share;
     if (at.x >= sh.total) return;
     at.left = min(sh.share, sh.total - at.x);
     {
-        const bool cut = sh.unit > 1;
-        const uint32_t mine = cut ? pieces * kLeastRounds : rounds;
-        uint32_t from = ((cut ? pieces_to * kLeastRounds : rounds_to) - mine) * p.heads;
-        if (at.x >= from && at.x - from < mine * p.heads) {
-            for (uint32_t i = 0; i < each; ++i) {
-                const uint32_t b = tid * each + i, one = places(rounds_of(length_of(p.positions[b])), sh.unit);
-                if (at.x - from < one * p.heads) {
-                    s.start[0] = b;
-                    s.start[1] = (at.x - from) / one;
-                    s.start[2] = (at.x - from) % one;
-                    break;
-                }
-                from += one * p.heads;
+        // the lane whose requests hold the share's first place, then the request
+        auto holder = [&](uint32_t to, uint32_t &from) {  // `from`: the first place of the lane found
+            const uint64_t below = __builtin_amdgcn_ballot_w64(to * p.heads <= at.x - from);
+            const int j = __builtin_popcountll(below);
+            if (j) from += (uint32_t)__builtin_amdgcn_readlane((int)to, j - 1) * p.heads;
+            return (uint32_t)j;
+        };
+        uint32_t from = 0, length;
+        at.b = holder(sh.unit > 1 ? pieces_to * kLeastRounds : rounds_to, from);
+        if (each > 1) {
+            window = at.b * each;
+            while (true) {  // (once, for up to 4096 requests)
+                lengths = length_at(window + lane);
+                const uint32_t j = holder(scan(window + lane < batch ? places(rounds_of(lengths), sh.unit) : 0), from);
+                at.b = window + j;
+                if (j < 64) break;
+                window += 64;
             }
         }
-    }
-    __syncthreads();
-    at.b = uniform(s.start[0]);
-    at.head = uniform(s.start[1]);
-    at.off = uniform(s.start[2]);
-    const uint32_t window = each == 1 ? 0 : at.b;  // s.lengths holds the requests from here on
-    if (each > 1) {
-        s.lengths[tid] = window + tid < p.batch ? length_of(p.positions[window + tid]) : 0;
-        __syncthreads();
+        length = places(rounds_of((uint32_t)__builtin_amdgcn_readlane((int)lengths, (int)(at.b - window))), sh.unit);
+        at.head = (at.x - from) / length;
+        at.off = (at.x - from) % length;
     }
     auto request_length = [&](uint32_t b) {
-        return b - window < kWindow ? uniform(s.lengths[b - window]) : uniform(length_of(p.positions[b]));
+        return b - window < 64 ? (uint32_t)__builtin_amdgcn_readlane((int)lengths, (int)(b - window)) : uniform(length_at(b));
     };
 
     // ---- the wave's stages, in the order of the share ------------------------------------------
+    // pairs of a request: the blocks of up to 16 query heads of each KV head
+    auto kv_head = [&](uint32_t head) { return p.blocks == 1 ? head : head / p.blocks; };
     Cursor ahead = at;
-    Run run = {};
-    uint32_t run_length = 0, round = 0;
-    int32_t run_index = -1;
-    auto next_stage = [&]() {
-        ++round;
-        while (true) {
-            const uint32_t key0 = (round * kWaves + wave) * S::keys;
-            if (run_index >= 0 && round < run.hi && key0 < run_length) return Stage{run.b, run.head, run_length, key0, run_index};
-            if (ahead.left == 0) return Stage{0u, 0u, 1u, 0u, -1};
-            run_length = request_length(ahead.b);
-            run = next_run(ahead, rounds_of(run_length), p.heads, sh);
-            round = run.lo;
-            ++run_index;
+    int32_t runs = -1;
+    constexpr uint32_t kStep = S::round, kBatch = (WHOLE ? 64 : 64 / S::keys) * kStep;  // keys
+    Batch batches = {0u, 0u, 0u, 0u, 0u, -1};  // the next one, whose page numbers are on their way
+    auto next_batch = [&]() {
+        if (batches.key + kBatch < batches.end) {
+            batches.key += kBatch;
+            return;
         }
+        while (ahead.left) {
+            const uint32_t length = request_length(ahead.b);
+            const Run run = next_run(ahead, rounds_of(length), p.heads, sh);
+            ++runs;
+            batches.b = run.b;
+            batches.kv_head = kv_head(run.head);
+            batches.length = length;
+            batches.key = run.lo * kStep + wave * S::keys;
+            batches.end = min(run.hi * kStep, length);
+            batches.run = runs;
+            if (batches.key < batches.end) return;
+        }
+        batches = Batch{0u, 0u, 0u, 0u, 0u, -1};
     };
     const uint32_t ring = uniform(lds_at(&s.ring[wave][0][0]));
     const uint32_t ids = uniform(lds_at(&s.ids[wave][0][0]));
     const uint32_t maskw = MASK ? uniform(lds_at(&s.maskw[wave][0][0])) : 0u;
-    const int mask_size = !MASK ? 0 : p.mask_dtype == Q3T_F32 ? 4 : p.mask_dtype == Q3T_BOOL ? 1 : 2;
-    // page numbers of a stage's keys; past the request's end its last key's
-    auto load_ids = [&](const Stage &st, uint32_t n) {
-        const uint32_t key = min(st.key0 + lane, st.length - 1);
-        const uint64_t from = reinterpret_cast<uint64_t>(p.table + (int64_t)st.b * p.table_sb + divide(key, p.by_page));
-        if (lane < S::keys) load_lds4(from, uniform(ids + (n & 3) * S::keys * 4));
+    const uint32_t mask_size = !MASK ? 0 : p.mask_dtype == Q3T_F32 ? 4 : p.mask_dtype == Q3T_BOOL ? 1 : 2;
+    // The batch's page numbers: lane i's is stage i's (WHOLE), or that of key i % keys of stage i / keys;
+    // past the request's end that of its last key.
+    auto load_ids = [&](uint32_t half) {
+        const uint32_t key = batches.key + (WHOLE ? lane * kStep : lane / S::keys * kStep + lane % S::keys);
+        const uint32_t at_page = divide(min(key, batches.length - 1), p.by_page);
+        load_lds4(reinterpret_cast<uint64_t>(p.table + (uint64_t)batches.b * p.table_sb + at_page), uniform(ids + half * 256));
     };
-    auto mask_byte = [&](uint32_t b, uint32_t key) { return ((int64_t)b * p.m_sb + (int64_t)key * p.m_st) * mask_size; };
-    auto load_stage = [&](const Stage &st, uint32_t n) {
-        if constexpr (MASK) {
-            const uint32_t key = min(st.key0 + lane, st.length - 1);
-            const uint64_t from = (reinterpret_cast<uint64_t>(p.mask) + (uint64_t)mask_byte(st.b, key)) & ~(uint64_t)3;
-            if (lane < S::keys) load_lds4(from, uniform(maskw + (n & 1) * S::keys * 4));
-        }
-        const uint32_t h = st.head / p.blocks, base = uniform(ring + (n & 1) * S::stage);
-        const uint64_t kh = (uint64_t)h * p.kp_sh, vh = (uint64_t)h * p.vp_sh;
-        uint64_t kf[S::loads], vf[S::loads];
+    // row and chunk of the lane's 16 bytes of load i, before the swizzle
+    auto row_of = [&](int i) { return (i * 64 + lane) / S::chunks; };
+    auto chunk_of = [&](int i) { return (i * 64 + lane) % S::chunks; };
+    uint32_t key_offset[WHOLE ? S::loads : 1], value_offset[WHOLE ? S::loads : 1];
+    if constexpr (WHOLE) {
 #pragma unroll
         for (int i = 0; i < S::loads; ++i) {
-            const int r = (i * 64 + lane) / S::chunks, slot = (i * 64 + lane) % S::chunks;
-            const uint32_t key = min(st.key0 + r, st.length - 1), at_row = key - divide(key, p.by_page) * p.by_page.d;
-            int32_t id = *(Q3T_LDS const int32_t *)(uintptr_t)(ids + ((n & 3) * S::keys + r) * 4);
-            if ((uint32_t)id >= p.pages) id = 0;  // a key on no page: not looked at
-            const uint64_t ko = (uint64_t)(uint32_t)id * p.kp_sp + (uint64_t)at_row * p.kp_st + kh;
-            const uint64_t vo = (uint64_t)(uint32_t)id * p.vp_sp + (uint64_t)at_row * p.vp_st + vh;
-            kf[i] = reinterpret_cast<uint64_t>(p.kp) + (ko + (uint32_t)(slot ^ S::key_swizzle(r))) * 16 - 1024 * (i & 3);
-            vf[i] = reinterpret_cast<uint64_t>(p.vp) + (vo + (uint32_t)(slot ^ S::value_swizzle(r))) * 16 - 1024 * (i & 3);
+            const int r = row_of(i);
+            key_offset[i] = (uint32_t)(r * p.kp_st + (chunk_of(i) ^ S::key_swizzle(r))) * 16 - 1024 * (i & 3);
+            value_offset[i] = (uint32_t)(r * p.vp_st + (chunk_of(i) ^ S::value_swizzle(r))) * 16 - 1024 * (i & 3);
         }
+    }
+    // stage `index` of a batch into ring slot n % 2
+    auto load_stage = [&](const Batch &bt, uint32_t index, uint32_t half, uint32_t n) {
+        const uint32_t key0 = bt.key + index * kStep, at_ids = ids + half * 256 + index * (WHOLE ? 4 : 4 * S::keys);
+        if constexpr (MASK) {
+            const uint32_t key = min(key0 + lane, bt.length - 1);
+            const uint64_t byte = ((uint64_t)bt.b * p.m_sb + (uint64_t)key * p.m_st) * mask_size;
+            const uint64_t from = (reinterpret_cast<uint64_t>(p.mask) + byte) & ~(uint64_t)3;
+            if (lane < S::keys) load_lds4(from, uniform(maskw + (n & 1) * S::keys * 4));
+        }
+        const uint32_t base = uniform(ring + (n & 1) * S::stage);
+        Stage st = {bt.b, key0, 0u, bt.run};
+        const uint32_t rest = bt.length - key0;  // keys from key0 on
+        if constexpr (WHOLE) {
+            // the stage's rows that exist, none on no page
+            const uint32_t id = uniform(*(Q3T_LDS const uint32_t *)(uintptr_t)at_ids);
+            const uint32_t row = key0 - divide(key0, p.by_page) * p.by_page.d;
+            const uint32_t count = id < p.pages ? min((uint32_t)S::keys, rest) : 0u;
+            st.exists = count == 32 ? ~0u : (1u << count) - 1;
+            auto range = [&](const char *pool, uint32_t page_stride, uint32_t head_stride, uint32_t row_stride) {
+                const uint64_t from = reinterpret_cast<uint64_t>(pool) +
+                                      (count ? ((uint64_t)id * page_stride + (uint64_t)row * row_stride + (uint64_t)bt.kv_head * head_stride) * 16 : 0);
+                return i32x4_t{(int)(uint32_t)from, (int)((uint32_t)(from >> 32) & 0xffffu),
+                               (int)(count ? (count - 1) * row_stride * 16 + S::row : 0u), 0x00020000};
+            };
+            const i32x4_t keys = range(p.kp, p.kp_sp, p.kp_sh, p.kp_st), values = range(p.vp, p.vp_sp, p.vp_sh, p.vp_st);
 #pragma unroll
-        for (int i = 0; i < S::loads; i += 4) load_rows(kf + i, base + i * 1024, p.stream);
+            for (int i = 0; i < S::loads; i += 4) load_rows(keys, key_offset + i, base + i * 1024);
 #pragma unroll
-        for (int i = 0; i < S::loads; i += 4) load_rows(vf + i, base + (S::loads + i) * 1024, p.stream);
+            for (int i = 0; i < S::loads; i += 4) load_rows(values, value_offset + i, base + (S::loads + i) * 1024);
+        } else {
+            const uint32_t mine = *(Q3T_LDS const uint32_t *)(uintptr_t)(at_ids + lane % S::keys * 4);
+            st.exists = (uint32_t)__builtin_amdgcn_ballot_w64(lane < S::keys && (uint32_t)lane < rest && mine < p.pages);
+            const uint64_t kh = (uint64_t)bt.kv_head * p.kp_sh, vh = (uint64_t)bt.kv_head * p.vp_sh;
+            uint64_t kf[S::loads], vf[S::loads];
+#pragma unroll
+            for (int i = 0; i < S::loads; ++i) {
+                const int r = row_of(i);
+                const uint32_t key = min(key0 + r, bt.length - 1), row = key - divide(key, p.by_page) * p.by_page.d;
+                uint32_t id = *(Q3T_LDS const uint32_t *)(uintptr_t)(at_ids + r * 4);
+                if (id >= p.pages) id = 0;  // a key on no page: not looked at
+                const uint64_t ko = (uint64_t)id * p.kp_sp + (uint64_t)row * p.kp_st + kh;
+                const uint64_t vo = (uint64_t)id * p.vp_sp + (uint64_t)row * p.vp_st + vh;
+                kf[i] = reinterpret_cast<uint64_t>(p.kp) + (ko + (uint32_t)(chunk_of(i) ^ S::key_swizzle(r))) * 16 - 1024 * (i & 3);
+                vf[i] = reinterpret_cast<uint64_t>(p.vp) + (vo + (uint32_t)(chunk_of(i) ^ S::value_swizzle(r))) * 16 - 1024 * (i & 3);
+            }
+#pragma unroll
+            for (int i = 0; i < S::loads; i += 4) load_rows(kf + i, base + i * 1024);
+#pragma unroll
+            for (int i = 0; i < S::loads; i += 4) load_rows(vf + i, base + (S::loads + i) * 1024);
+        }
+        return st;
     };
     // the query rows of a pair, by the last wave, into one of two places
-    auto columns_of = [&](uint32_t head) { return min((uint32_t)kColumns, p.group - head % p.blocks * kColumns); };
-    auto first_head = [&](uint32_t head) { return head / p.blocks * p.group + head % p.blocks * kColumns; };
+    auto first_head = [&](uint32_t head) {
+        const uint32_t h = kv_head(head);
+        return h * p.group + (head - h * p.blocks) * kColumns;
+    };
+    auto columns_of = [&](uint32_t head) { return min((uint32_t)kColumns, (kv_head(head) + 1) * p.group - first_head(head)); };
     const uint32_t shared = uniform(lds_at(s.shared));
     auto load_query = [&](uint32_t b, uint32_t head, uint32_t place) {
         const uint32_t items = columns_of(head) * S::chunks;
         for (uint32_t i = 0; i < items; i += 64) {
             const uint32_t item = i + lane;
-            const uint64_t from = reinterpret_cast<uint64_t>(p.q) + (uint64_t)((int64_t)b * p.q_sb) +
-                                  (uint64_t)((int64_t)(first_head(head) + item / S::chunks) * p.q_sh) + item % S::chunks * 16;
+            const uint64_t from = reinterpret_cast<uint64_t>(p.q) + ((uint64_t)b * p.q_sb +
+                                  (uint64_t)(first_head(head) + item / S::chunks) * p.q_sh + item % S::chunks) * 16;
             if (item < items) load_lds16(from, uniform(shared + (place * p.columns * S::chunks + i) * 16));
         }
     };
 
-    Stage s0 = next_stage(), s1 = s0.run < 0 ? s0 : next_stage(), s2 = s1.run < 0 ? s1 : next_stage();
     if (wave == kWaves - 1) load_query(at.b, at.head, 0);
-    if (s0.run >= 0) load_ids(s0, 0);
-    if (s1.run >= 0) load_ids(s1, 1);
-    if (s2.run >= 0) load_ids(s2, 2);
-    wait_loads<0>();
-    if (s0.run >= 0) load_stage(s0, 0);
+    next_batch();
+    Batch now = batches;  // the batch whose rows are being loaded, its page numbers in half `half`
+    uint32_t index = 0, half = 0;
+    Stage s0 = {0u, 0u, 0u, -1};
+    if (now.run >= 0) {
+        load_ids(0);
+        next_batch();
+        if (batches.run >= 0) load_ids(1);
+        wait_loads<0>();
+        s0 = load_stage(now, 0, 0, 0);
+    } else {
+        wait_loads<0>();
+    }
     lds_barrier();  // the first query rows are there
 
     // ---- run by run -----------------------------------------------------------------------------
@@ -476,41 +585,46 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, D>::per_cu)) paged_kernel(
     const float threshold = MASK ? Products::threshold / kLog2e : Products::threshold;
     float m, l;
     uint32_t n = 0;
+    x.place(ring, g, c);
     auto score = [&](const Stage &st) {
-        const uint32_t keys = ring + (n & 1) * S::stage, rows = keys + S::keys * S::row;
+        const uint32_t stage = (n & 1) * S::stage;
         float v[S::keys / 16][4];
-        bool hidden[S::keys / 16][4], any = false;
+        bool hidden[S::keys / 16][4] = {}, any = false;
+        // Keys that do not exist.  Their value rows are zeroed, unless they are rows past a range, for
+        // which the loads left zeros.
+        if (MASK || st.exists != (uint32_t)((1ull << S::keys) - 1)) {
 #pragma unroll
-        for (int t = 0; t < S::keys / 16; ++t) {
-            const U4 id = lds_read16(ids + ((n & 3) * S::keys + 16 * t + 4 * g) * 4);
-            const uint32_t page[4] = {id.x, id.y, id.z, id.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t key = st.key0 + 16 * t + 4 * g + i;
-                hidden[t][i] = key >= st.length || page[i] >= p.pages;
+            for (int t = 0; t < S::keys / 16; ++t) {
                 if constexpr (MASK) {
-                    const uint32_t low = (uint32_t)(reinterpret_cast<uint64_t>(p.mask) + (uint64_t)mask_byte(st.b, min(key, st.length - 1))) & 3u;
-                    const uint32_t word = *(Q3T_LDS const uint32_t *)(uintptr_t)(maskw + ((n & 1) * S::keys + 16 * t + 4 * g + i) * 4);
-                    v[t][i] = mask_term(word, low, p.mask_dtype);
-                    hidden[t][i] = hidden[t][i] || v[t][i] == -INFINITY;
+                    const uint32_t step = p.m_st * mask_size;
+                    const uint32_t low = (uint32_t)reinterpret_cast<uint64_t>(p.mask) + st.b * p.m_sb * mask_size +
+                                         (st.key0 + 16 * t + 4 * g) * step;
+                    mask_terms(lds_read16(maskw + ((n & 1) * S::keys + 16 * t + 4 * g) * 4), low, step, p.mask_dtype, v[t]);
                 }
-                any = any || hidden[t][i];
+                const uint32_t exists = st.exists >> (16 * t + 4 * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    hidden[t][i] = !(exists & (1u << i));
+                    if constexpr (MASK) hidden[t][i] = hidden[t][i] || v[t][i] == -INFINITY;
+                    any = any || hidden[t][i];
+                }
             }
-        }
-        if (__builtin_amdgcn_ballot_w64(any)) {
-            const U4 zero = {0u, 0u, 0u, 0u};
+            if ((!WHOLE || MASK) && __builtin_amdgcn_ballot_w64(any)) {
+                const U4 zero = {0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int t = 0; t < S::keys / 16; ++t)
+                for (int t = 0; t < S::keys / 16; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (hidden[t][i])
-                        for (int chunk = c; chunk < S::chunks; chunk += 16) lds_write16(rows + (16 * t + 4 * g + i) * S::row + chunk * 16, zero);
-            asm volatile("" ::: "memory");
+                    for (int i = 0; i < 4; ++i)
+                        if (hidden[t][i])
+                            for (int chunk = c; chunk < S::chunks; chunk += 16)
+                                lds_write16(ring + stage + (S::keys + 16 * t + 4 * g + i) * S::row + chunk * 16, zero);
+                asm volatile("" ::: "memory");
+            }
         }
         float highest = -INFINITY;
 #pragma unroll
         for (int t = 0; t < S::keys / 16; ++t) {
-            const f32x4_t st4 = x.scores(keys, t, g, c);
+            const f32x4_t st4 = x.scores(stage, t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float scaled = MASK ? st4[i] * p.scale + v[t][i] : st4[i] * p.scale;
@@ -534,46 +648,58 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, D>::per_cu)) paged_kernel(
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = fexp2((v[t][i] - from) * unit + Products::shift);
             l += (w[0] + w[1]) + (w[2] + w[3]);
-            x.values(rows, t, g, c, w);
+            x.values(stage, t, w);
         }
     };
-    auto finish = [&](const Run &r, uint32_t column, uint32_t d, float sum, const float (&a)[4]) {
+    auto finish = [&](const Run &r, uint32_t column, uint32_t d, const State &sum) {
         float y[4];
+        const float inverse = sum.l == 0.f ? 0.f : 1.f / sum.l;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = sum == 0.f ? 0.f : a[i] / sum;
-        store_out<T>(p.out + (int64_t)r.b * p.o_sb + (int64_t)(first_head(r.head) + column) * p.o_sh + d * sizeof(T), y, p.vec_out);
+        for (int i = 0; i < 4; ++i) y[i] = sum.a[i] * inverse;
+        store_out<T>(p.out + ((uint64_t)r.b * p.o_sb + (uint64_t)(first_head(r.head) + column) * p.o_sh + d) * sizeof(T), y, p.vec_out);
     };
-    // what a state weighs against a maximum
-    auto weight = [&](float mine, float highest) { return fexp2((mine - (highest == -INFINITY ? 0.f : highest)) * unit); };
     const uint32_t state_size = p.columns * (D + 2);
 
-    for (int32_t index = 0; at.left > 0; ++index) {
+    for (int32_t order = 0; at.left > 0; ++order) {
         const Run r = next_run(at, rounds_of(request_length(at.b)), p.heads, sh);
         const uint32_t columns = columns_of(r.head);
-        if (wave == kWaves - 1 && at.left > 0) load_query(at.b, at.head, (index + 1) & 1);
-        x.load_query(shared + (index & 1) * p.columns * S::row, g, c, (uint32_t)c < columns);
+        if (wave == kWaves - 1 && at.left > 0) load_query(at.b, at.head, (order + 1) & 1);
+        x.load_query(shared + (order & 1) * p.columns * S::row, g, c, (uint32_t)c < columns);
         x.clear();
         m = -INFINITY;
         l = 0.f;
-        if (s0.run != index) wait_loads<0>();  // no stage here: the next query rows may be in flight
-        while (s0.run == index) {
-            const Stage now = s0;
-            if (s1.run >= 0) {
-                // the next stage, into the slot that was scored last, once its reads have returned
-                const Stage s3 = s2.run < 0 ? s2 : next_stage();
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                load_ids(s3.run < 0 ? s1 : s3, n + 3);  // (always, so that the loads behind the stage can be counted)
-                load_stage(s1, n + 1);
-                wait_loads<LOADS + 1 + (MASK ? 1 : 0)>();
-                s0 = s1;
-                s1 = s2;
-                s2 = s3;
+        if (s0.run != order) wait_loads<0>();  // no stage here: the next query rows may be in flight
+        while (s0.run == order) {
+            // the next stage, into the slot that was scored last, once its reads have returned
+            Stage s1 = {0u, 0u, 0u, -1};
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            ++index;
+            if (index * kStep < kBatch && now.key + index * kStep < now.end) {
+                s1 = load_stage(now, index, half, n + 1);
+                wait_loads<LOADS + (MASK ? 1 : 0)>();
+            } else if (batches.run >= 0) {
+                wait_loads<LOADS + (MASK ? 1 : 0)>();  // the batch's page numbers, loaded ahead of the last batch's rows
+                now = batches;
+                index = 0;
+                half ^= 1;
+                next_batch();
+                const bool more = batches.run >= 0;
+                if (more) load_ids(half ^ 1);
+                s1 = load_stage(now, 0, half, n + 1);
+                if (more) wait_loads<LOADS + (MASK ? 1 : 0) + 1>();
+                else wait_loads<LOADS + (MASK ? 1 : 0)>();
             } else {
                 wait_loads<0>();
-                s0 = s1;
             }
-            score(now);
+            score(s0);
+            s0 = s1;
             ++n;
+            // Of two workgroups on a CU the older one's loads go first, and the younger one (the later
+            // half, as they are dealt out) would end after it: it goes first on every second stage.
+            if (blockIdx.x >= kWorkgroups / 2) {
+                if (n & 1) __builtin_amdgcn_s_setprio(2);
+                else __builtin_amdgcn_s_setprio(0);
+            }
         }
 
         // the waves' states into one, `pass` columns at a time
@@ -591,82 +717,100 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, D>::per_cu)) paged_kernel(
             lds_barrier();
             for (uint32_t item = tid; item < count * (D / 4); item += kThreads) {
                 const uint32_t column = c0 + item / (D / 4), d = item % (D / 4) * 4;
-                float highest = -INFINITY, sum = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) highest = fmaxf(highest, s.ml[w][column][0]);
+                State own = {};
+                own.m = fmaxf(fmaxf(s.ml[0][column][0], s.ml[1][column][0]), fmaxf(s.ml[2][column][0], s.ml[3][column][0]));
+                const float from = own.m == -INFINITY ? 0.f : own.m;
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) {
-                    const float e = weight(s.ml[w][column][0], highest);
-                    const f32x4_t part = __builtin_bit_cast(f32x4_t, lds_read16(buffer + ((w * pass + column - c0) * D + d) * 4));
-                    sum += s.ml[w][column][1] * e;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) a[i] += part[i] * e;
+                    const float e = fexp2((s.ml[w][column][0] - from) * unit);
+                    own.l += s.ml[w][column][1] * e;
+                    own.a += __builtin_bit_cast(f32x4_t, lds_read16(buffer + ((w * pass + column - c0) * D + d) * 4)) * e;
                 }
-                if (whole) {
-                    finish(r, column, d, sum, a);
-                } else {
-                    publish(state + column * D + d, a[0], a[1]);
-                    publish(state + column * D + d + 2, a[2], a[3]);
-                    if (d == 0) publish(state + p.columns * D + 2 * column, highest, sum);
-                }
+                if (whole) finish(r, column, d, own);
+                else own.publish(state, p.columns * D, column, d, D);
             }
             if (!whole && c0 + pass >= columns) wait_loads<0>();  // the state has been stored
             lds_barrier();
         }
         if (whole) continue;
 
-        int32_t *counter = p.counters + r.b * p.heads + r.head;
-        if (tid == 0) s.start[3] = (uint32_t)__hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        if (uniform(s.start[3]) != r.parts - 1) continue;
-        // the last to arrive: thread (part % groups, item) takes every groups-th part's four elements
-        const uint32_t items = columns * (D / 4), groups = max(1u, kThreads / items);
-        for (uint32_t first = 0; first < items; first += kThreads) {
-            const uint32_t item = first + tid % items, group = groups == 1 ? 0 : tid / items;
-            const bool live = groups == 1 ? first + tid < items : group < groups;
-            const uint32_t own = groups == 1 ? first + tid : item, column = own / (D / 4), d = own % (D / 4) * 4;
-            float highest = -INFINITY, sum = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
-            if (live) {
-                for (uint32_t i = group; i < r.parts; i += groups) {
-                    const float *from = p.states + (2 * (r.first + i) + (i == 0)) * (uint64_t)state_size;
-                    float pm, pl, v[4];
-                    collect(from + p.columns * D + 2 * column, pm, pl);
-                    collect(from + column * D + d, v[0], v[1]);
-                    collect(from + column * D + d + 2, v[2], v[3]);
-                    const float top = fmaxf(highest, pm), e0 = weight(highest, top), e1 = weight(pm, top);
-                    sum = sum * e0 + pl * e1;
+        // Parts beyond kTogether are merged in two steps: kTogether neighbours' last to arrive merges
+        // theirs into the first one's state, and the last of those merges them.
+        const uint32_t part = blockIdx.x - r.first;
+        auto slot_of = [&](uint32_t i) { return 2 * (r.first + i) + (i == 0); };  // part i's state
+        auto arrive = [&](int32_t *counter, uint32_t expected) {
+            if (tid == 0) s.count = (uint32_t)__hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();  // (and there are more barriers before the next count)
+            const bool last = uniform(s.count) == expected - 1;
+            if (last && tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            return last;
+        };
+        // every `step`-th part from `begin` on, `count` of them, in one order whoever merges them: thread
+        // (part % groups, item) adds up every groups-th part's four elements, and thread (0, item) the groups'
+        auto merge = [&](uint32_t begin, uint32_t step, uint32_t count, bool last) {
+            const uint32_t items = columns * (D / 4), groups = max(1u, kThreads / items);
+            for (uint32_t first = 0; first < items; first += kThreads) {
+                const uint32_t group = groups == 1 ? 0 : tid / items, item = groups == 1 ? first + tid : tid - group * items;
+                const bool live = group < groups && item < items;
+                const uint32_t column = item / (D / 4), d = item % (D / 4) * 4;
+                State sum = {};
+                sum.m = -INFINITY;
+                if (live) {
+                    constexpr uint32_t kFlight = 4;  // states on their way at once
+                    for (uint32_t i = group; i < count; i += kFlight * groups) {
+                        State parts[kFlight];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) a[j] = a[j] * e0 + v[j] * e1;
-                    highest = top;
+                        for (uint32_t j = 0; j < kFlight; ++j) {
+                            const uint32_t at_part = min(i + j * groups, count - 1);
+                            parts[j].collect(p.states + slot_of(begin + at_part * step) * (uint64_t)state_size, p.columns * D, column, d, D);
+                        }
+#pragma unroll
+                        for (uint32_t j = 0; j < kFlight; ++j)
+                            if (i + j * groups < count) sum.add(parts[j], unit);
+                    }
+                }
+                if (groups > 1) {
+                    const uint32_t mine = buffer + tid * 16, mine_ml = buffer + kThreads * 16 + tid * 8;
+                    if (live) {
+                        lds_write16(mine, __builtin_bit_cast(U4, sum.a));
+                        *(Q3T_LDS float *)(uintptr_t)mine_ml = sum.m;
+                        *(Q3T_LDS float *)(uintptr_t)(mine_ml + 4) = sum.l;
+                    }
+                    lds_barrier();
+                    if (live && group == 0) {
+                        for (uint32_t o = 1; o < min(groups, count); ++o) {
+                            const uint32_t ml = mine_ml + o * items * 8;
+                            State other;
+                            other.a = __builtin_bit_cast(f32x4_t, lds_read16(mine + o * items * 16));
+                            other.m = *(Q3T_LDS const float *)(uintptr_t)ml;
+                            other.l = *(Q3T_LDS const float *)(uintptr_t)(ml + 4);
+                            sum.add(other, unit);
+                        }
+                    }
+                    lds_barrier();  // the buffer is free again
+                }
+                if (!last) {  // the first part's state is written where other threads have read it
+                    wait_loads<0>();
+                    lds_barrier();
+                }
+                if (live && group == 0) {
+                    if (last) finish(r, column, d, sum);
+                    else sum.publish(p.states + slot_of(begin) * (uint64_t)state_size, p.columns * D, column, d, D);
                 }
             }
-            if (groups == 1) {
-                if (live) finish(r, column, d, sum, a);
-                continue;
-            }
-            const uint32_t mine = buffer + tid * 16, mine_ml = buffer + kThreads * 16 + tid * 8;
-            if (live) {
-                lds_write16(mine, U4{__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3])});
-                *(Q3T_LDS float *)(uintptr_t)mine_ml = highest;
-                *(Q3T_LDS float *)(uintptr_t)(mine_ml + 4) = sum;
-            }
-            lds_barrier();
-            if (live && group == 0) {
-                for (uint32_t o = 1; o < groups; ++o) {
-                    const uint32_t from = buffer + o * items * 16 + tid * 16, ml = buffer + kThreads * 16 + o * items * 8 + tid * 8;
-                    const f32x4_t v = __builtin_bit_cast(f32x4_t, lds_read16(from));
-                    const float pm = *(Q3T_LDS const float *)(uintptr_t)ml, pl = *(Q3T_LDS const float *)(uintptr_t)(ml + 4);
-                    const float top = fmaxf(highest, pm), e0 = weight(highest, top), e1 = weight(pm, top);
-                    sum = sum * e0 + pl * e1;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) a[j] = a[j] * e0 + v[j] * e1;
-                    highest = top;
-                }
-                finish(r, column, d, sum, a);
-            }
+        };
+        bool last = r.parts <= kTogether;
+        uint32_t begin = last ? 0 : part / kTogether * kTogether, step = 1, count = min(kTogether, r.parts - begin);
+        while (arrive(last ? p.counters + r.b * p.heads + r.head : p.counters + kPairs + slot_of(begin), count)) {
+            merge(begin, step, count, last);
+            if (last) break;
+            wait_loads<0>();
+            lds_barrier();  // the merged state has been stored
+            begin = 0;
+            step = kTogether;
+            count = (r.parts + kTogether - 1) / kTogether;
+            last = true;
         }
-        if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        lds_barrier();  // the buffer is free again
     }
 }
 
@@ -674,13 +818,20 @@ template <typename T, int D>
 struct Launch {
     static int64_t workgroups(const q3t_paged_args *a, int64_t pairs) {
         const int64_t rounds = (a->ctx + Shape<T, D>::round - 1) / Shape<T, D>::round;
-        const int64_t pieces = pairs * ((rounds + kLeastRounds - 1) / kLeastRounds), most = 256 * Shape<T, D>::per_cu;
+        const int64_t pieces = pairs * ((rounds + kLeastRounds - 1) / kLeastRounds), most = kWorkgroups / 2 * Shape<T, D>::per_cu;
         return pieces < most ? pieces : most;
     }
     static int64_t rounds(const q3t_paged_args *a, int64_t pairs) { return pairs * ((a->ctx + Shape<T, D>::round - 1) / Shape<T, D>::round); }
-    static void run(const Params &p, uint32_t blocks, hipStream_t s) {
-        if (p.mask) hipLaunchKernelGGL((paged_kernel<T, D, true>), dim3(blocks), dim3(kThreads), 0, s, p);
-        else hipLaunchKernelGGL((paged_kernel<T, D, false>), dim3(blocks), dim3(kThreads), 0, s, p);
+    static void run(const int64_t *positions, uint32_t batch, uint32_t ctx, const Params &p, uint32_t blocks, hipStream_t s) {
+        auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, s, positions, batch, ctx, p);
+        };
+        // rows of a stage as one range: whole pages, rows that do not overlap, 32-bit offsets
+        typedef Shape<T, D> S;
+        const bool whole = p.by_page.d % S::keys == 0 && p.kp_st * 16ull >= S::row && p.vp_st * 16ull >= S::row &&
+                           p.kp_st < (1u << 26) / S::keys && p.vp_st < (1u << 26) / S::keys;
+        if (p.mask) whole ? launch(paged_kernel<T, D, true, true>) : launch(paged_kernel<T, D, true, false>);
+        else whole ? launch(paged_kernel<T, D, false, true>) : launch(paged_kernel<T, D, false, false>);
     }
 };
 // f on the Launch of a call's type and width
@@ -705,13 +856,13 @@ static int sizes_of(const q3t_paged_args *a, Sizes &z) {
     if (a->head_dim != 64 && a->head_dim != 128) return Q3T_EUNSUPPORTED;
     if (a->pages > INT32_MAX || a->page_size > INT32_MAX || a->table_width > INT32_MAX) return Q3T_EUNSUPPORTED;
     if (a->ctx > a->table_width * a->page_size) return Q3T_EINVAL;
-    if (a->ctx >= 1 << 30 || a->batch > kCounters || a->q_heads > 1 << 16) return Q3T_EUNSUPPORTED;
+    if (a->ctx >= 1 << 30 || a->batch > kPairs || a->q_heads > 1 << 16) return Q3T_EUNSUPPORTED;
     z.group = a->q_heads / a->kv_heads;
     z.blocks = (z.group + kColumns - 1) / kColumns;
     z.pairs = a->batch * a->kv_heads * z.blocks;
     z.columns = z.group < kColumns ? z.group : kColumns;
-    if (z.pairs > kCounters) return Q3T_EUNSUPPORTED;  // a counter each
-    if (with(a, [&](auto l) { return l.rounds(a, z.pairs); }) >= INT32_MAX - kCounters) return Q3T_EUNSUPPORTED;
+    if (z.pairs > kPairs) return Q3T_EUNSUPPORTED;  // a counter each
+    if (with(a, [&](auto l) { return l.rounds(a, z.pairs); }) >= INT32_MAX / 2) return Q3T_EUNSUPPORTED;
     z.workgroups = with(a, [&](auto l) { return l.workgroups(a, z.pairs); });
     z.workspace = kCounters * 4 + 2 * z.workgroups * z.columns * (a->head_dim + 2) * 4;
     return Q3T_OK;
@@ -743,35 +894,39 @@ extern "C" int q3t_paged_attention(const q3t_paged_args *a, void *stream) {
         return Q3T_OK;
     };
     Params p = {};
-    const int64_t strides[6] = {a->kp_stride_p, a->kp_stride_h, a->kp_stride_t, a->vp_stride_p, a->vp_stride_h, a->vp_stride_t};
-    uint32_t *const to[6] = {&p.kp_sp, &p.kp_sh, &p.kp_st, &p.vp_sp, &p.vp_sh, &p.vp_st};
-    for (int i = 0; i < 6; ++i) {
+    const int64_t strides[8] = {a->q_stride_b, a->q_stride_h, a->kp_stride_p, a->kp_stride_h, a->kp_stride_t, a->vp_stride_p, a->vp_stride_h, a->vp_stride_t};
+    uint32_t *const to[8] = {&p.q_sb, &p.q_sh, &p.kp_sp, &p.kp_sh, &p.kp_st, &p.vp_sp, &p.vp_sh, &p.vp_st};
+    for (int i = 0; i < 8; ++i) {
         const int s = chunks(strides[i], *to[i]);
         if (s != Q3T_OK) return s;
     }
     p.q = (const char *)a->query; p.kp = (const char *)a->key_pages; p.vp = (const char *)a->value_pages;
     p.mask = (const char *)a->mask; p.out = (char *)a->out;
-    p.table = a->page_table; p.positions = a->positions;
-    p.q_sb = a->q_stride_b * es; p.q_sh = a->q_stride_h * es;
-    p.o_sb = a->o_stride_b * es; p.o_sh = a->o_stride_h * es;
-    p.m_sb = a->mask_stride_b; p.m_st = a->mask_stride_t; p.table_sb = a->table_stride_b;
+    p.table = a->page_table;
+    const int64_t elements[5] = {a->o_stride_b, a->o_stride_h, a->mask ? a->mask_stride_b : 0, a->mask ? a->mask_stride_t : 0, a->table_stride_b};
+    uint32_t *const in[5] = {&p.o_sb, &p.o_sh, &p.m_sb, &p.m_st, &p.table_sb};
+    for (int i = 0; i < 5; ++i) {
+        if (elements[i] < 0) return Q3T_EINVAL;
+        if (elements[i] > UINT32_MAX) return Q3T_EUNSUPPORTED;
+        *in[i] = (uint32_t)elements[i];
+    }
     const int64_t mask_size = a->mask_dtype == Q3T_F32 ? 4 : a->mask_dtype == Q3T_BOOL ? 1 : 2;
-    if ((p.q_sb | p.q_sh) % 16 || !aligned(p.q, 16) || !aligned(p.kp, 16) || !aligned(p.vp, 16) || !aligned(p.out, es) ||
-        !aligned(p.table, 4) || !aligned(p.positions, 8) || (p.mask && !aligned(p.mask, mask_size)))
+    if (!aligned(p.q, 16) || !aligned(p.kp, 16) || !aligned(p.vp, 16) || !aligned(p.out, es) ||
+        !aligned(p.table, 4) || !aligned(a->positions, 8) || (p.mask && !aligned(p.mask, mask_size)))
         return Q3T_EINVAL;
     if (!a->workspace || a->workspace_bytes < z.workspace) return Q3T_EWORKSPACE;
     if (!aligned(a->workspace, 16)) return Q3T_EINVAL;
     p.counters = (int32_t *)a->workspace;
     p.states = (float *)((char *)a->workspace + kCounters * 4);
-    p.ctx = (int32_t)a->ctx; p.mask_dtype = (int32_t)a->mask_dtype;
-    p.stream = 1;
-    p.vec_out = aligned(p.out, 4 * es) && (p.o_sb | p.o_sh) % (4 * es) == 0;
-    p.batch = (uint32_t)a->batch; p.pages = (uint32_t)a->pages;
+    p.mask_dtype = (int32_t)a->mask_dtype;
+    p.vec_out = aligned(p.out, 4 * es) && (p.o_sb | p.o_sh) % 4 == 0;
+    p.pages = (uint32_t)a->pages;
     p.group = (uint32_t)z.group; p.blocks = (uint32_t)z.blocks;
     p.heads = (uint32_t)(a->kv_heads * z.blocks);
     p.columns = (uint32_t)z.columns;
     p.by_page = divisor((uint32_t)a->page_size);
+    p.by_grid = divisor((uint32_t)z.workgroups);
     p.scale = a->mask ? a->scale : a->scale * kLog2e;
-    with(a, [&](auto l) { l.run(p, (uint32_t)z.workgroups, (hipStream_t)stream); });
+    with(a, [&](auto l) { l.run(a->positions, (uint32_t)a->batch, (uint32_t)a->ctx, p, (uint32_t)z.workgroups, (hipStream_t)stream); });
     return launch_status();
 }

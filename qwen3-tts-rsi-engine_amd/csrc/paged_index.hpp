@@ -44,10 +44,10 @@ struct Sharing {
     uint32_t total;  // places in all
 };
 
-// From the pairs' rounds, and their pieces of `least` rounds, over all pairs.
-Q3T_BOTH Sharing sharing(uint32_t rounds, uint32_t pieces, uint32_t least, uint32_t workgroups) {
-    if (pieces <= workgroups) return {least, least, pieces * least};
-    return {1u, (uint32_t)(((uint64_t)rounds + workgroups - 1) / workgroups), rounds};
+// From the pairs' rounds (fewer than 2^30), and their pieces of `least` rounds, over all pairs.
+Q3T_BOTH Sharing sharing(uint32_t rounds, uint32_t pieces, uint32_t least, const Divisor &workgroups) {
+    if (pieces <= workgroups.d) return {least, least, pieces * least};
+    return {1u, divide(rounds + workgroups.d - 1, workgroups), rounds};
 }
 
 Q3T_BOTH uint32_t places(uint32_t rounds, uint32_t unit) { return (rounds + unit - 1) / unit * unit; }
@@ -57,7 +57,8 @@ struct Cursor {
     uint32_t x, left, b, head, off;
 };
 
-// A run of one pair's rounds [lo, hi) in one share: part `x / share` - first of the pair's `parts`.
+// A run of one pair's rounds [lo, hi) in one share: part `x / share` - first of the pair's `parts`
+// (first only if there are several).
 // Its state's slot is 2 w for a pair that began in an earlier share (a workgroup's first run at
 // most), 2 w + 1 for one that begins in this one (the last at most, if there are more parts).
 struct Run {
@@ -74,9 +75,13 @@ Q3T_BOTH Run next_run(Cursor &c, uint32_t rounds, uint32_t heads, const Sharing 
     r.lo = c.off;
     r.hi = end < rounds ? end : rounds;
     r.begins = c.off == 0;
-    const uint32_t start = c.x - c.off;
-    r.first = start / s.share;
-    r.parts = (start + length - 1) / s.share - r.first + 1;
+    r.first = 0;
+    r.parts = 1;
+    if (c.off || take < rest) {  // (no division for a pair that lies in one share)
+        const uint32_t start = c.x - c.off;
+        r.first = start / s.share;
+        r.parts = (start + length - 1) / s.share - r.first + 1;
+    }
     c.x += take;
     c.left -= take;
     c.off = end;

@@ -31,15 +31,20 @@ _TYPES = {torch.bfloat16: _lib.Q3T_BF16, torch.float16: _lib.Q3T_F16, torch.floa
 
 
 def _check_pools(key_pages, value_pages, page_table, positions, batch):
+    """(strides of the key pages, of the value pages, of the page table, its width)."""
     if key_pages.ndim != 4 or value_pages.shape != key_pages.shape:
         raise ValueError('key and value pages must be (pages, kv_heads, page_size, head_dim) of one shape')
-    if key_pages.stride(3) != 1 or value_pages.stride(3) != 1:
+    ks, vs = key_pages.stride(), value_pages.stride()
+    if ks[3] != 1 or vs[3] != 1:
         raise ValueError('rows must be unit-stride along head_dim')
-    if (page_table.ndim != 2 or page_table.dtype != torch.int32 or page_table.shape[0] != batch
-            or page_table.shape[1] < 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
-        raise ValueError('page_table must be an int32 (batch, pages) tensor with unit-stride rows')
+    if page_table.ndim != 2 or page_table.dtype != torch.int32:
+        raise ValueError('page_table must be an int32 (batch, pages) tensor')
+    (rows, width), ts = page_table.shape, page_table.stride()
+    if rows != batch or width < 1 or (width > 1 and ts[1] != 1):
+        raise ValueError('page_table must have a unit-stride row of page numbers per request')
     if positions.dtype != torch.int64 or positions.shape != (batch,) or not positions.is_contiguous():
         raise ValueError('positions must be a contiguous int64 (batch,) tensor')
+    return ks, vs, ts[0], width
 
 
 def paged_write(keys, values, key_pages, value_pages, page_table, positions, lengths=None):
@@ -54,27 +59,28 @@ def paged_write(keys, values, key_pages, value_pages, page_table, positions, len
     if keys.ndim != 4 or values.shape != keys.shape:
         raise ValueError('Expected matching BNSD K/V')
     batch, heads, tokens, width = keys.shape
-    _check_pools(key_pages, value_pages, page_table, positions, batch)
-    if key_pages.shape[1] != heads or key_pages.shape[3] != width:
+    kps, vps, ts, table_width = _check_pools(key_pages, value_pages, page_table, positions, batch)
+    pages, page_heads, page_size, page_rows = key_pages.shape
+    if page_heads != heads or page_rows != width:
         raise ValueError('pages must have the rows\' KV heads and head_dim')
-    if (keys.dtype not in _TYPES or values.dtype != keys.dtype or key_pages.dtype != keys.dtype
-            or value_pages.dtype != keys.dtype):
+    dtype = keys.dtype
+    if dtype not in _TYPES or values.dtype != dtype or key_pages.dtype != dtype or value_pages.dtype != dtype:
         raise ValueError('paged K/V write supports bf16/fp16/fp32 tensors of one dtype')
-    if keys.stride(3) != 1 or values.stride(3) != 1:
+    ks, vs = keys.stride(), values.stride()
+    if ks[3] != 1 or vs[3] != 1:
         raise ValueError('K/V rows must be unit-stride along head_dim')
     device = _lib.require_gpu(keys, values, key_pages, value_pages, page_table, positions)
     if lengths is not None:
         if lengths.dtype != torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous():
             raise ValueError('lengths must be a contiguous int32 (batch,) tensor')
         _lib.require_gpu(keys, lengths)
-    if keys.numel() == 0:
+    if batch == 0 or tokens == 0:
         return
     a = _lib.PagedWriteArgs(
         batch, heads, tokens, width, keys.element_size(), keys.data_ptr(), values.data_ptr(),
-        *keys.stride()[:3], *values.stride()[:3], key_pages.data_ptr(), value_pages.data_ptr(),
-        *key_pages.stride()[:3], *value_pages.stride()[:3], key_pages.shape[0], key_pages.shape[2],
-        page_table.data_ptr(), page_table.shape[1], page_table.stride(0), positions.data_ptr(),
-        None if lengths is None else lengths.data_ptr())
+        ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], key_pages.data_ptr(), value_pages.data_ptr(),
+        kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], pages, page_size,
+        page_table.data_ptr(), table_width, ts, positions.data_ptr(), None if lengths is None else lengths.data_ptr())
     with _lib.on_device(device):
         status = _lib.library().q3t_paged_write(a, _lib.stream_handle(device))
     _lib.check(status, 'paged write')
@@ -95,17 +101,18 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     if query.ndim != 4 or query.shape[1] != 1:
         raise ValueError('paged attention takes one token per request, (batch, 1, heads, head_dim)')
     batch, _, q_heads, head_dim = query.shape
-    _check_pools(key_pages, value_pages, page_table, positions, batch)
+    kps, vps, ts, table_width = _check_pools(key_pages, value_pages, page_table, positions, batch)
     pages, kv_heads, page_size, width = key_pages.shape
     if width != head_dim or kv_heads < 1 or q_heads < 1 or q_heads % kv_heads:
         raise ValueError('head_dim mismatch or q_heads not a multiple of kv_heads')
     dtype = query.dtype
     if dtype not in _TYPES or key_pages.dtype != dtype or value_pages.dtype != dtype:
         raise ValueError('paged attention supports bf16, fp16 or fp32 tensors of one dtype')
-    if query.stride(3) != 1:
+    qs = query.stride()
+    if qs[3] != 1:
         raise ValueError('rows must be unit-stride along head_dim')
     device = _lib.require_gpu(query, key_pages, value_pages, page_table, positions)
-    ctx = page_table.shape[1] * page_size
+    ctx = table_width * page_size
     mask_fields = (None, 0, 0, 0)
     if mask is not None:
         if mask.dtype not in _lib.DTYPE_CODES:
@@ -120,19 +127,20 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
             raise ValueError('the mask must be broadcastable to (batch, 1, 1, keys)') from None
         mask_fields = (mask.data_ptr(), _lib.DTYPE_CODES[mask.dtype], rows.stride(0), rows.stride(3))
     if out is None:
-        out = torch.empty((batch, 1, q_heads, head_dim), device=device, dtype=dtype)
+        out, os = torch.empty((batch, 1, q_heads, head_dim), device=device, dtype=dtype), (q_heads * head_dim, 0, head_dim)
     else:
         _check_out(out, (batch, 1, q_heads, head_dim), dtype, device, 'paged attention')
+        os = out.stride()
     if batch == 0:
         return out
-    if query.data_ptr() % 16 or any(s * query.element_size() % 16 for s in (query.stride(0), query.stride(2))):
+    if query.data_ptr() % 16 or (qs[0] | qs[2]) * query.element_size() % 16:
         query = query.clone(memory_format=torch.contiguous_format)  # rows that 16-byte loads do not fit
+        qs = query.stride()
     a = _lib.PagedArgs(
         batch, q_heads, kv_heads, head_dim, _TYPES[dtype], ctx, head_dim ** -0.5 if scale is None else scale, 0,
-        query.data_ptr(), query.stride(0), query.stride(2), key_pages.data_ptr(), value_pages.data_ptr(),
-        *key_pages.stride()[:3], *value_pages.stride()[:3], pages, page_size,
-        page_table.data_ptr(), page_table.shape[1], page_table.stride(0), positions.data_ptr(), *mask_fields,
-        out.data_ptr(), out.stride(0), out.stride(2))
+        query.data_ptr(), qs[0], qs[2], key_pages.data_ptr(), value_pages.data_ptr(),
+        kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], pages, page_size,
+        page_table.data_ptr(), table_width, ts, positions.data_ptr(), *mask_fields, out.data_ptr(), os[0], os[2])
     lib = _lib.library()
     with _lib.on_device(device):
         stream = _lib.stream_handle(device)

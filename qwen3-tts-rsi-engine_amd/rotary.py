@@ -74,12 +74,13 @@ def rope_tables(positions, head_dim, theta=DEFAULT_THETA, scaling=1.0, dtype=tor
     return cos, sin
 
 
+_ROTARY_TYPES = {torch.bfloat16: _lib.Q3T_BF16, torch.float16: _lib.Q3T_F16, torch.float32: _lib.Q3T_F32}
 _TURNS = {}
 
 
 def _turns(half, theta, device):
     """Full turns per position of every frequency, theta**(-i/half) / 2 pi, in float64."""
-    key = (device, half, float(theta))
+    key = (device.index, half, theta)
     turns = _TURNS.get(key)
     if turns is None:  # cached so that captured graphs never see a host copy
         exponent = torch.arange(half, dtype=torch.float64) / half
@@ -103,44 +104,56 @@ def rotary_axes(query, key, positions, sections, *, interleaved=False, theta=DEF
 
     Returns (query, key) rotated: new contiguous tensors, or with ``inplace`` the given ones,
     rotated where they are."""
-    tensors = [query] if key is None else [query, key]
-    if any(t.ndim != 4 for t in tensors) or (key is not None and (key.shape[:2] != query.shape[:2]
-                                                                  or key.shape[3] != query.shape[3])):
-        raise ValueError('expected BSND query and key rows of one batch, length and width')
+    if query.ndim != 4 or (key is not None and key.ndim != 4):
+        raise ValueError('expected BSND query and key rows')
     batch, tokens, q_heads, width = query.shape
-    if query.dtype not in _lib.DTYPE_CODES or query.dtype == torch.bool or tensors[-1].dtype != query.dtype:
+    dtype, device = query.dtype, query.device
+    if dtype not in _ROTARY_TYPES or (key is not None and key.dtype != dtype):
         raise ValueError('rotary supports bf16, fp16 or fp32 tensors of one dtype')
-    sections = tuple(sections)
-    if not 1 <= len(sections) <= 4 or any(not isinstance(n, int) or n < 0 for n in sections):
-        raise ValueError('sections must be one to four counts of frequencies')
-    half = sum(sections)
-    if not 1 <= half or 2 * half > width or half > 512:
-        raise ValueError('sections must sum to at least one and at most half of the width (512 at most)')
-    if positions.dtype != torch.int64 or tuple(positions.shape) != (len(sections), batch, tokens):
+    half, axes = 0, len(sections)
+    for n in sections:
+        if not isinstance(n, int) or n < 0:
+            raise ValueError('sections must be counts of frequencies')
+        half += n
+    if not 1 <= axes <= 4 or half < 1 or 2 * half > width or half > 512:
+        raise ValueError('one to four sections must sum to at least one and at most half of the width (512 at most)')
+    if positions.dtype != torch.int64 or positions.shape != (axes, batch, tokens):
         raise ValueError('positions must be an int64 (axes, batch, length) tensor')
-    if any(t.shape[2] < 1 or t.stride(3) != 1 for t in tensors):
+    qs, ps, ks, k_heads = query.stride(), positions.stride(), (0, 0, 0, 1), 0
+    if key is None:
+        _lib.require_gpu(query, positions)
+    else:
+        key_batch, key_tokens, k_heads, key_width = key.shape
+        if key_batch != batch or key_tokens != tokens or key_width != width:
+            raise ValueError('query and key rows must have one batch, length and width')
+        ks = key.stride()
+        _lib.require_gpu(query, key, positions)
+    if qs[3] != 1 or ks[3] != 1 or q_heads < 1 or (key is not None and k_heads < 1):
         raise ValueError('rows must be unit-stride, at least one per token')
-    device = _lib.require_gpu(*tensors, positions)
-    if inplace and any(n > 1 and s == 0 for t in tensors for n, s in zip(t.shape, t.stride())):
-        raise ValueError('rows that share memory cannot be rotated in place')
     if inv_freq is None:
         turns = _turns(half, theta, device)
     else:
         if inv_freq.shape != (half,):
             raise ValueError('inv_freq must have one entry per frequency')
         turns = inv_freq.to(device=device, dtype=torch.float64) / (2 * math.pi)
-    outs = tensors if inplace else [torch.empty(t.shape, device=device, dtype=t.dtype) for t in tensors]
-    if query.numel() == 0:
-        return outs[0], None if key is None else outs[1]
-    k, ko = (None, None) if key is None else (key, outs[1])
-    none = (0, 0, 0)
+    if inplace:
+        for t in (query,) if key is None else (query, key):
+            if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+                raise ValueError('rows that share memory cannot be rotated in place')
+        q_out, k_out, qos, kos = query, key, qs, ks
+    else:
+        q_out, qos = torch.empty((batch, tokens, q_heads, width), device=device, dtype=dtype), (tokens * q_heads * width, q_heads * width, width)
+        k_out, kos = None, (0, 0, 0)
+        if key is not None:
+            k_out, kos = torch.empty((batch, tokens, k_heads, width), device=device, dtype=dtype), (tokens * k_heads * width, k_heads * width, width)
+    if batch == 0 or tokens == 0:
+        return q_out, k_out
     a = _lib.RotaryAxesArgs(
-        batch, tokens, q_heads, 0 if key is None else key.shape[2], width, _lib.DTYPE_CODES[query.dtype],
-        len(sections), (_lib.c_i64 * 4)(*sections), bool(interleaved), scaling, turns.data_ptr(),
-        positions.data_ptr(), *positions.stride(), query.data_ptr(), _lib.ptr(k),
-        *query.stride()[:3], *(none if k is None else k.stride()[:3]), outs[0].data_ptr(), _lib.ptr(ko),
-        *outs[0].stride()[:3], *(none if ko is None else ko.stride()[:3]))
+        batch, tokens, q_heads, k_heads, width, _ROTARY_TYPES[dtype], axes, (_lib.c_i64 * 4)(*sections), bool(interleaved),
+        scaling, turns.data_ptr(), positions.data_ptr(), ps[0], ps[1], ps[2],
+        query.data_ptr(), None if key is None else key.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
+        q_out.data_ptr(), None if key is None else k_out.data_ptr(), qos[0], qos[1], qos[2], kos[0], kos[1], kos[2])
     with _lib.on_device(device):
         status = _lib.library().q3t_rotary_axes(a, _lib.stream_handle(device))
     _lib.check(status, 'rotary axes')
-    return outs[0], None if key is None else outs[1]
+    return q_out, k_out

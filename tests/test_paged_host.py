@@ -33,7 +33,7 @@ def index(tmp_path_factory):
 #include "{CSRC / 'paged_index.hpp'}"
 extern "C" uint32_t quotient(uint32_t n, uint32_t d) {{ return q3t::divide(n, q3t::divisor(d)); }}
 extern "C" void share_out(uint32_t rounds, uint32_t pieces, uint32_t least, uint32_t workgroups, uint32_t *out) {{
-    const q3t::Sharing s = q3t::sharing(rounds, pieces, least, workgroups);
+    const q3t::Sharing s = q3t::sharing(rounds, pieces, least, q3t::divisor(workgroups));
     out[0] = s.unit; out[1] = s.share; out[2] = s.total;
 }}
 extern "C" uint32_t places(uint32_t rounds, uint32_t unit) {{ return q3t::places(rounds, unit); }}
@@ -95,6 +95,8 @@ def test_shares_cover_every_pair_once(index, seed):
             for r in range(lo, hi):
                 assert (rb, head, r) not in covered
                 covered[rb, head, r] = w
+            if count == 1:
+                first = w
             assert begins == (lo == 0) and first <= w < first + count
             assert parts.setdefault((rb, head), (first, count)) == (first, count)
             assert (w == first) == bool(begins)
