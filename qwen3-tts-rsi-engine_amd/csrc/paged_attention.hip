@@ -33,7 +33,8 @@ namespace paged {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kColumns = 16;           // query heads of a workgroup: columns of a product
-constexpr uint32_t kLeastRounds = 2;   // rounds that are not shared out
+constexpr uint32_t kLeastStages = 8;   // stages that are not shared out
+constexpr uint32_t kRunCost = 8;       // stages that the end of a run costs as much as
 constexpr int kCounters = 65536;       // counter words in front of a decode workspace: of the pairs,
 constexpr int kPairs = kCounters - 1024;  // then of the state slots
 constexpr int kWorkgroups = 512;       // at most
@@ -62,11 +63,9 @@ struct Shape {
     static constexpr int keys = row == 128 ? 32 : 16;      // of a wave's stage
     static constexpr int stage = 2 * keys * row;           // key rows, then value rows
     static constexpr int loads = keys * row / 1024;        // 1 KiB loads of either
-    static constexpr int round = kWaves * keys;
-    static constexpr int log_round = keys == 32 ? 7 : 6;
+    static constexpr int log_keys = keys == 32 ? 5 : 4;
     static constexpr bool f32 = sizeof(T) == 4;
-    // the queries of two pairs, and accumulators of at least 4 KiB (8 of 512-byte rows)
-    static constexpr int shared = 2 * kColumns * row + (row == 512 ? 8192 : 4096);
+    static_assert(kColumns * D * 4 <= stage, "a free slot holds a wave's accumulators");
     static constexpr int per_cu = row == 512 ? 1 : 2;      // workgroups that fit a CU's LDS
     // chunk c of key (value) row r sits at c ^ swizzle: the products' reads meet distinct banks
     static Q3T_DEVICE int key_swizzle(int r) { return chunks == 8 ? (r >> 1) & 7 : r & 15; }
@@ -76,10 +75,11 @@ struct Shape {
 template <typename T, int D, bool MASK>
 struct Lds {
     alignas(1024) char ring[kWaves][2][Shape<T, D>::stage];
-    alignas(16) char shared[Shape<T, D>::shared];
+    alignas(16) char query[2][kColumns * Shape<T, D>::row];  // of this run's pair and the next's
     uint32_t ids[kWaves][2][64];
     alignas(16) uint32_t maskw[MASK ? kWaves : 1][2][MASK ? Shape<T, D>::keys : 4];
     float ml[kWaves][kColumns][2];
+    uint32_t slot[kWaves];  // each wave's free slot
     uint32_t count;
 };
 
@@ -228,14 +228,14 @@ template <typename T, int D> struct Tile {
             for (int i = 1; i < Half<T>::parts; ++i) rest[d] = Half<T>::values(v, part[i], rest[d]);
         }
     }
-    // Elements of column c into its row of D floats.
-    Q3T_DEVICE void store(uint32_t to, int g) const {
+    // Elements of column c into its row of D floats, four to a chunk, chunk k at k ^ c.
+    Q3T_DEVICE void store(uint32_t to, int g, int c) const {
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
             f32x4_t x;
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = __builtin_fabsf(first[d][i]) < INFINITY ? first[d][i] + rest[d][i] : first[d][i];
-            lds_write16(to + (16 * d + 4 * g) * 4, __builtin_bit_cast(U4, x));
+            lds_write16(to + c * D * 4 + ((4 * d + g) ^ c) * 16, __builtin_bit_cast(U4, x));
         }
     }
 };
@@ -287,13 +287,13 @@ template <int D> struct Tile<float, D> {
                 for (int e = 0; e < 4; ++e) acc[4 * j + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], w[i], acc[4 * j + e], 0, 0, 0);
             }
     }
-    Q3T_DEVICE void store(uint32_t to, int g) const {
+    Q3T_DEVICE void store(uint32_t to, int g, int c) const {
 #pragma unroll
         for (int j = 0; j < D / 64; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4_t x = {acc[4 * j][i], acc[4 * j + 1][i], acc[4 * j + 2][i], acc[4 * j + 3][i]};
-                lds_write16(to + (64 * j + 4 * (4 * g + i)) * 4, __builtin_bit_cast(U4, x));
+                lds_write16(to + c * D * 4 + ((16 * j + 4 * g + i) ^ c) * 16, __builtin_bit_cast(U4, x));
             }
     }
 };
@@ -355,7 +355,7 @@ struct State {
     }
 };
 
-// Stages of a wave in one run, keys `key`, key + a round, ... below `end`, up to the number of
+// Stages of a wave in one run, every fourth from key `key` on below `end`, up to the number of
 // stages whose page numbers fit its 64 words.
 struct Batch {
     uint32_t b, kv_head, length, key, end;
@@ -393,24 +393,25 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = (int)uniform(tid >> 6);
 
-    // ---- the share: every wave adds up all requests' rounds and pieces for itself ---------------
+    // ---- the share: every wave adds up all requests' stages and pieces for itself ---------------
     auto length_at = [&](uint32_t b) {
         const int64_t pos = b < batch ? positions[b] : -1;
         return pos >= 0 && pos < (int64_t)ctx ? (uint32_t)pos + 1 : 0u;
     };
-    auto rounds_of = [&](uint32_t length) { return max(1u, (length + S::round - 1) >> S::log_round); };
+    auto stages_of = [&](uint32_t length) { return max(1u, (length + S::keys - 1) >> S::log_keys); };
     const uint32_t each = (batch + 63) / 64;  // requests of a lane, one after the other
     uint32_t lengths = length_at(lane);       // of requests window + lane
-    uint32_t rounds = 0, pieces = 0, window = 0;
+    uint32_t stages = 0, pieces = 0, window = 0;
     for (uint32_t i = 0; i < each; ++i) {
-        const uint32_t b = lane * each + i, r = rounds_of(each == 1 ? lengths : length_at(b));
+        const uint32_t b = lane * each + i, r = stages_of(each == 1 ? lengths : length_at(b));
         if (b >= batch) break;
-        rounds += r;
-        pieces += (r + kLeastRounds - 1) / kLeastRounds;
+        stages += r;
+        pieces += (r + kLeastStages - 1) / kLeastStages;
     }
-    const uint32_t rounds_to = scan(rounds), pieces_to = scan(pieces);
+    const uint32_t stages_to = scan(stages), pieces_to = scan(pieces);
     auto last_lane = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); };
-    const Sharing sh = sharing(last_lane(rounds_to) * p.heads, last_lane(pieces_to) * p.heads, kLeastRounds, p.by_grid);
+    const Sharing sh = sharing(batch * p.heads, last_lane(stages_to) * p.heads, last_lane(pieces_to) * p.heads,
+                               kLeastStages, kRunCost, p.by_grid);
     Cursor at = {};
     at.x = blockIdx.x * sh.share;
     if (at.x >= sh.total) return;
@@ -423,21 +424,25 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
             if (j) from += (uint32_t)__builtin_amdgcn_readlane((int)to, j - 1) * p.heads;
             return (uint32_t)j;
         };
-        uint32_t from = 0, length;
-        at.b = holder(sh.unit > 1 ? pieces_to * kLeastRounds : rounds_to, from);
+        uint32_t from = 0;
+        at.b = holder(sh.unit > 1 ? pieces_to * kLeastStages : stages_to + sh.cost * min((lane + 1) * each, batch), from);
         if (each > 1) {
             window = at.b * each;
             while (true) {  // (once, for up to 4096 requests)
                 lengths = length_at(window + lane);
-                const uint32_t j = holder(scan(window + lane < batch ? places(rounds_of(lengths), sh.unit) : 0), from);
+                const uint32_t j = holder(scan(window + lane < batch ? places(stages_of(lengths), sh) : 0), from);
                 at.b = window + j;
                 if (j < 64) break;
                 window += 64;
             }
         }
-        length = places(rounds_of((uint32_t)__builtin_amdgcn_readlane((int)lengths, (int)(at.b - window))), sh.unit);
+        const uint32_t stages_here = stages_of((uint32_t)__builtin_amdgcn_readlane((int)lengths, (int)(at.b - window)));
+        const uint32_t length = places(stages_here, sh);
         at.head = (at.x - from) / length;
-        at.off = (at.x - from) % length;
+        at.off = (at.x - from) - at.head * length;
+        if (at.off >= stages_here) end_pair(at, length, p.heads);
+        at = Cursor{uniform(at.x), uniform(at.left), uniform(at.b), uniform(at.head), uniform(at.off)};
+        if (at.left == 0) return;
     }
     auto request_length = [&](uint32_t b) {
         return b - window < 64 ? (uint32_t)__builtin_amdgcn_readlane((int)lengths, (int)(b - window)) : uniform(length_at(b));
@@ -448,7 +453,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     auto kv_head = [&](uint32_t head) { return p.blocks == 1 ? head : head / p.blocks; };
     Cursor ahead = at;
     int32_t runs = -1;
-    constexpr uint32_t kStep = S::round, kBatch = (WHOLE ? 64 : 64 / S::keys) * kStep;  // keys
+    constexpr uint32_t kStep = kWaves * S::keys, kBatch = (WHOLE ? 64 : 64 / S::keys) * kStep;  // keys
     Batch batches = {0u, 0u, 0u, 0u, 0u, -1};  // the next one, whose page numbers are on their way
     auto next_batch = [&]() {
         if (batches.key + kBatch < batches.end) {
@@ -457,13 +462,13 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         }
         while (ahead.left) {
             const uint32_t length = request_length(ahead.b);
-            const Run run = next_run(ahead, rounds_of(length), p.heads, sh);
+            const Run run = next_run(ahead, stages_of(length), p.heads, sh);
             ++runs;
             batches.b = run.b;
             batches.kv_head = kv_head(run.head);
             batches.length = length;
-            batches.key = run.lo * kStep + wave * S::keys;
-            batches.end = min(run.hi * kStep, length);
+            batches.key = (run.lo + ((wave - run.lo) & (kWaves - 1))) * S::keys;  // every fourth stage is the wave's
+            batches.end = min(run.hi * S::keys, length);
             batches.run = runs;
             if (batches.key < batches.end) return;
         }
@@ -513,8 +518,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
             auto range = [&](const char *pool, uint32_t page_stride, uint32_t head_stride, uint32_t row_stride) {
                 const uint64_t from = reinterpret_cast<uint64_t>(pool) +
                                       (count ? ((uint64_t)id * page_stride + (uint64_t)row * row_stride + (uint64_t)bt.kv_head * head_stride) * 16 : 0);
-                return i32x4_t{(int)(uint32_t)from, (int)((uint32_t)(from >> 32) & 0xffffu),
-                               (int)(count ? (count - 1) * row_stride * 16 + S::row : 0u), 0x00020000};
+                return scalar_rsrc(reinterpret_cast<const void *>(from), count ? (count - 1) * row_stride * 16 + S::row : 0u);
             };
             const i32x4_t keys = range(p.kp, p.kp_sp, p.kp_sh, p.kp_st), values = range(p.vp, p.vp_sp, p.vp_sh, p.vp_st);
 #pragma unroll
@@ -550,14 +554,14 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         return h * p.group + (head - h * p.blocks) * kColumns;
     };
     auto columns_of = [&](uint32_t head) { return min((uint32_t)kColumns, (kv_head(head) + 1) * p.group - first_head(head)); };
-    const uint32_t shared = uniform(lds_at(s.shared));
+    const uint32_t queries = uniform(lds_at(s.query[0]));
     auto load_query = [&](uint32_t b, uint32_t head, uint32_t place) {
         const uint32_t items = columns_of(head) * S::chunks;
         for (uint32_t i = 0; i < items; i += 64) {
             const uint32_t item = i + lane;
             const uint64_t from = reinterpret_cast<uint64_t>(p.q) + ((uint64_t)b * p.q_sb +
                                   (uint64_t)(first_head(head) + item / S::chunks) * p.q_sh + item % S::chunks) * 16;
-            if (item < items) load_lds16(from, uniform(shared + (place * p.columns * S::chunks + i) * 16));
+            if (item < items) load_lds16(from, uniform(queries + (place * kColumns * S::chunks + i) * 16));
         }
     };
 
@@ -579,8 +583,6 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 
     // ---- run by run -----------------------------------------------------------------------------
     Products x;
-    const uint32_t buffer = shared + 2 * p.columns * S::row;  // accumulators of `pass` columns per wave
-    const uint32_t pass = min(p.columns, (S::shared - 2 * p.columns * S::row) / (kWaves * D * 4));
     const float unit = MASK ? kLog2e : 1.f;  // scores are natural under a mask, else in log2 units
     const float threshold = MASK ? Products::threshold / kLog2e : Products::threshold;
     float m, l;
@@ -661,10 +663,10 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     const uint32_t state_size = p.columns * (D + 2);
 
     for (int32_t order = 0; at.left > 0; ++order) {
-        const Run r = next_run(at, rounds_of(request_length(at.b)), p.heads, sh);
+        const Run r = next_run(at, stages_of(request_length(at.b)), p.heads, sh);
         const uint32_t columns = columns_of(r.head);
         if (wave == kWaves - 1 && at.left > 0) load_query(at.b, at.head, (order + 1) & 1);
-        x.load_query(shared + (order & 1) * p.columns * S::row, g, c, (uint32_t)c < columns);
+        x.load_query(queries + (order & 1) * kColumns * S::row, g, c, (uint32_t)c < columns);
         x.clear();
         m = -INFINITY;
         l = 0.f;
@@ -702,36 +704,35 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
             }
         }
 
-        // the waves' states into one, `pass` columns at a time
+        // the waves' states, each in the slot that its next stage is not in, into one
         l += xor16(l);
         l += xor32(l);
+        const uint32_t slot = ring + ((n + 1) & 1) * S::stage;
         if (g == 0) {
             s.ml[wave][c][0] = m;
             s.ml[wave][c][1] = l;
         }
+        if (lane == 0) s.slot[wave] = slot;
+        if ((uint32_t)c < columns) x.store(slot, g, c);
+        lds_barrier();
         const bool whole = r.parts == 1;
         float *state = p.states + (2 * blockIdx.x + r.begins) * (uint64_t)state_size;
-        for (uint32_t c0 = 0; c0 < columns; c0 += pass) {
-            const uint32_t count = min(pass, columns - c0);
-            if (c >= c0 && c < c0 + count) x.store(buffer + (wave * pass + c - c0) * D * 4, g);
-            lds_barrier();
-            for (uint32_t item = tid; item < count * (D / 4); item += kThreads) {
-                const uint32_t column = c0 + item / (D / 4), d = item % (D / 4) * 4;
-                State own = {};
-                own.m = fmaxf(fmaxf(s.ml[0][column][0], s.ml[1][column][0]), fmaxf(s.ml[2][column][0], s.ml[3][column][0]));
-                const float from = own.m == -INFINITY ? 0.f : own.m;
+        for (uint32_t item = tid; item < columns * (D / 4); item += kThreads) {
+            const uint32_t column = item / (D / 4), chunk = item % (D / 4);
+            State own = {};
+            own.m = fmaxf(fmaxf(s.ml[0][column][0], s.ml[1][column][0]), fmaxf(s.ml[2][column][0], s.ml[3][column][0]));
+            const float from = own.m == -INFINITY ? 0.f : own.m;
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w) {
-                    const float e = fexp2((s.ml[w][column][0] - from) * unit);
-                    own.l += s.ml[w][column][1] * e;
-                    own.a += __builtin_bit_cast(f32x4_t, lds_read16(buffer + ((w * pass + column - c0) * D + d) * 4)) * e;
-                }
-                if (whole) finish(r, column, d, own);
-                else own.publish(state, p.columns * D, column, d, D);
+            for (int w = 0; w < kWaves; ++w) {
+                const float e = fexp2((s.ml[w][column][0] - from) * unit);
+                own.l += s.ml[w][column][1] * e;
+                own.a += __builtin_bit_cast(f32x4_t, lds_read16(s.slot[w] + column * D * 4 + (chunk ^ column) * 16)) * e;
             }
-            if (!whole && c0 + pass >= columns) wait_loads<0>();  // the state has been stored
-            lds_barrier();
+            if (whole) finish(r, column, chunk * 4, own);
+            else own.publish(state, p.columns * D, column, chunk * 4, D);
         }
+        if (!whole) wait_loads<0>();  // the state has been stored
+        lds_barrier();
         if (whole) continue;
 
         // Parts beyond kTogether are merged in two steps: kTogether neighbours' last to arrive merges
@@ -770,24 +771,22 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
                     }
                 }
                 if (groups > 1) {
-                    const uint32_t mine = buffer + tid * 16, mine_ml = buffer + kThreads * 16 + tid * 8;
+                    // 32 bytes a thread, in its wave's free slot
+                    auto place = [&](uint32_t t) { return s.slot[t >> 6] + (t & 63) * 32; };
                     if (live) {
-                        lds_write16(mine, __builtin_bit_cast(U4, sum.a));
-                        *(Q3T_LDS float *)(uintptr_t)mine_ml = sum.m;
-                        *(Q3T_LDS float *)(uintptr_t)(mine_ml + 4) = sum.l;
+                        lds_write16(place(tid), __builtin_bit_cast(U4, sum.a));
+                        lds_write16(place(tid) + 16, U4{__float_as_uint(sum.m), __float_as_uint(sum.l), 0u, 0u});
                     }
                     lds_barrier();
                     if (live && group == 0) {
                         for (uint32_t o = 1; o < min(groups, count); ++o) {
-                            const uint32_t ml = mine_ml + o * items * 8;
-                            State other;
-                            other.a = __builtin_bit_cast(f32x4_t, lds_read16(mine + o * items * 16));
-                            other.m = *(Q3T_LDS const float *)(uintptr_t)ml;
-                            other.l = *(Q3T_LDS const float *)(uintptr_t)(ml + 4);
+                            const U4 ml = lds_read16(place(tid + o * items) + 16);
+                            const State other = {__uint_as_float(ml.x), __uint_as_float(ml.y),
+                                                 __builtin_bit_cast(f32x4_t, lds_read16(place(tid + o * items)))};
                             sum.add(other, unit);
                         }
                     }
-                    lds_barrier();  // the buffer is free again
+                    lds_barrier();  // the slots are free again
                 }
                 if (!last) {  // the first part's state is written where other threads have read it
                     wait_loads<0>();
@@ -817,11 +816,11 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 template <typename T, int D>
 struct Launch {
     static int64_t workgroups(const q3t_paged_args *a, int64_t pairs) {
-        const int64_t rounds = (a->ctx + Shape<T, D>::round - 1) / Shape<T, D>::round;
-        const int64_t pieces = pairs * ((rounds + kLeastRounds - 1) / kLeastRounds), most = kWorkgroups / 2 * Shape<T, D>::per_cu;
+        const int64_t stages = (a->ctx + Shape<T, D>::keys - 1) / Shape<T, D>::keys;
+        const int64_t pieces = pairs * ((stages + kLeastStages - 1) / kLeastStages), most = kWorkgroups / 2 * Shape<T, D>::per_cu;
         return pieces < most ? pieces : most;
     }
-    static int64_t rounds(const q3t_paged_args *a, int64_t pairs) { return pairs * ((a->ctx + Shape<T, D>::round - 1) / Shape<T, D>::round); }
+    static int64_t stages(const q3t_paged_args *a, int64_t pairs) { return pairs * ((a->ctx + Shape<T, D>::keys - 1) / Shape<T, D>::keys + kRunCost); }
     static void run(const int64_t *positions, uint32_t batch, uint32_t ctx, const Params &p, uint32_t blocks, hipStream_t s) {
         auto launch = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, s, positions, batch, ctx, p);
@@ -862,7 +861,7 @@ static int sizes_of(const q3t_paged_args *a, Sizes &z) {
     z.pairs = a->batch * a->kv_heads * z.blocks;
     z.columns = z.group < kColumns ? z.group : kColumns;
     if (z.pairs > kPairs) return Q3T_EUNSUPPORTED;  // a counter each
-    if (with(a, [&](auto l) { return l.rounds(a, z.pairs); }) >= INT32_MAX / 2) return Q3T_EUNSUPPORTED;
+    if (with(a, [&](auto l) { return l.stages(a, z.pairs); }) >= INT32_MAX / 2) return Q3T_EUNSUPPORTED;
     z.workgroups = with(a, [&](auto l) { return l.workgroups(a, z.pairs); });
     z.workspace = kCounters * 4 + 2 * z.workgroups * z.columns * (a->head_dim + 2) * 4;
     return Q3T_OK;

@@ -30,68 +30,78 @@ Q3T_BOTH uint32_t divide(uint32_t n, const Divisor &v) {
 // ---- how the paged attention's work is shared out ------------------------------------------
 //
 // A pair is a request with one KV head (and up to 16 of its query heads).  A pair's keys are read
-// in rounds of a fixed number of keys, at least one.  All pairs' rounds lie on one line, request
-// by request, head by head, and workgroup w takes the share [w * share, (w + 1) * share) of it.  A
-// pair that lies in several shares is merged from its parts.
-//   * When every pair cut into pieces of `kShareRounds` rounds gives no more pieces than there are
-//     workgroups, each piece is a share of its own: pairs take a multiple of that many places on
-//     the line (`unit`), the last piece the rest of the pair.
-//   * Otherwise the line holds the rounds alone and the shares are equal.
+// in stages of a fixed number of keys, at least one.  All pairs lie on one line, request by request,
+// head by head, each with a place for every stage and some empty ones behind them, and workgroup w
+// takes the share [w * share, (w + 1) * share) of it.  A pair whose stages lie in several shares
+// is merged from its parts.
+//   * When every pair cut into pieces of `least` stages gives no more pieces than there are
+//     workgroups, each piece is a share of its own: a pair takes a multiple of that many places.
+//   * Otherwise a pair takes `cost` places more than it has stages, for what ends a run (the waves'
+//     merge, the output), and the shares are equal.
 
 struct Sharing {
-    uint32_t unit;   // places of a pair are a multiple of it
-    uint32_t share;  // places of a workgroup
-    uint32_t total;  // places in all
+    uint32_t unit, cost;  // places of a pair: a multiple of unit, and cost more
+    uint32_t share;       // places of a workgroup
+    uint32_t total;       // places in all
 };
 
-// From the pairs' rounds (fewer than 2^30), and their pieces of `least` rounds, over all pairs.
-Q3T_BOTH Sharing sharing(uint32_t rounds, uint32_t pieces, uint32_t least, const Divisor &workgroups) {
-    if (pieces <= workgroups.d) return {least, least, pieces * least};
-    return {1u, divide(rounds + workgroups.d - 1, workgroups), rounds};
+// From the number of pairs, their stages (fewer than 2^30 together), and their pieces of `least`
+// stages.
+Q3T_BOTH Sharing sharing(uint32_t pairs, uint32_t stages, uint32_t pieces, uint32_t least, uint32_t cost, const Divisor &workgroups) {
+    if (pieces <= workgroups.d) return {least, 0u, least, pieces * least};
+    const uint32_t total = stages + cost * pairs;
+    return {1u, cost, divide(total + workgroups.d - 1, workgroups), total};
 }
 
-Q3T_BOTH uint32_t places(uint32_t rounds, uint32_t unit) { return (rounds + unit - 1) / unit * unit; }
+Q3T_BOTH uint32_t places(uint32_t stages, const Sharing &s) {
+    return (s.unit == 1 ? stages : (stages + s.unit - 1) / s.unit * s.unit) + s.cost;
+}
 
 // Where a workgroup is on the line: place x, `left` places to go, at place `off` of pair (b, head).
 struct Cursor {
     uint32_t x, left, b, head, off;
 };
 
-// A run of one pair's rounds [lo, hi) in one share: part `x / share` - first of the pair's `parts`
-// (first only if there are several).
-// Its state's slot is 2 w for a pair that began in an earlier share (a workgroup's first run at
-// most), 2 w + 1 for one that begins in this one (the last at most, if there are more parts).
+// Past the pair's last stage: on to the next pair.
+Q3T_BOTH void end_pair(Cursor &c, uint32_t length, uint32_t heads) {
+    const uint32_t rest = length - c.off;
+    c.x += rest;
+    c.left -= rest < c.left ? rest : c.left;
+    c.off = 0;
+    if (++c.head == heads) {
+        c.head = 0;
+        ++c.b;
+    }
+}
+
+// A run of one pair's stages [lo, hi) in one share: part (its workgroup - first) of the pair's `parts`
+// (first only if there are several).  Its state's slot is 2 w for a pair that began in an earlier share
+// (a workgroup's first run at most), 2 w + 1 for one that begins in this one (the last at most, if
+// there are more parts).
 struct Run {
     uint32_t b, head, lo, hi, first, parts, begins;
 };
 
-// The run at the cursor, for a pair of `rounds` rounds, and the cursor moved past it.
-Q3T_BOTH Run next_run(Cursor &c, uint32_t rounds, uint32_t heads, const Sharing &s) {
-    const uint32_t length = places(rounds, s.unit), rest = length - c.off;
-    const uint32_t take = rest < c.left ? rest : c.left, end = c.off + take;
+// The run at the cursor, for a pair of `stages` stages, and the cursor moved past it.
+Q3T_BOTH Run next_run(Cursor &c, uint32_t stages, uint32_t heads, const Sharing &s) {
+    const uint32_t rest = stages - c.off, take = rest < c.left ? rest : c.left;
     Run r;
     r.b = c.b;
     r.head = c.head;
     r.lo = c.off;
-    r.hi = end < rounds ? end : rounds;
+    r.hi = c.off + take;
     r.begins = c.off == 0;
     r.first = 0;
     r.parts = 1;
     if (c.off || take < rest) {  // (no division for a pair that lies in one share)
         const uint32_t start = c.x - c.off;
         r.first = start / s.share;
-        r.parts = (start + length - 1) / s.share - r.first + 1;
+        r.parts = (start + stages - 1) / s.share - r.first + 1;
     }
     c.x += take;
     c.left -= take;
-    c.off = end;
-    if (end == length) {
-        c.off = 0;
-        if (++c.head == heads) {
-            c.head = 0;
-            ++c.b;
-        }
-    }
+    c.off = r.hi;
+    if (r.hi == stages) end_pair(c, places(stages, s), heads);
     return r;
 }
 

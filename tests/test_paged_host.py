@@ -32,16 +32,26 @@ def index(tmp_path_factory):
     (where / 'index.cpp').write_text(f'''
 #include "{CSRC / 'paged_index.hpp'}"
 extern "C" uint32_t quotient(uint32_t n, uint32_t d) {{ return q3t::divide(n, q3t::divisor(d)); }}
-extern "C" void share_out(uint32_t rounds, uint32_t pieces, uint32_t least, uint32_t workgroups, uint32_t *out) {{
-    const q3t::Sharing s = q3t::sharing(rounds, pieces, least, q3t::divisor(workgroups));
-    out[0] = s.unit; out[1] = s.share; out[2] = s.total;
+extern "C" void share_out(uint32_t pairs, uint32_t stages, uint32_t pieces, uint32_t least, uint32_t cost, uint32_t workgroups, uint32_t *out) {{
+    const q3t::Sharing s = q3t::sharing(pairs, stages, pieces, least, cost, q3t::divisor(workgroups));
+    out[0] = s.unit; out[1] = s.cost; out[2] = s.share; out[3] = s.total;
 }}
-extern "C" uint32_t places(uint32_t rounds, uint32_t unit) {{ return q3t::places(rounds, unit); }}
-extern "C" void next_run(uint32_t *cursor, uint32_t rounds, uint32_t heads, const uint32_t *sharing, uint32_t *out) {{
-    q3t::Cursor c = {{cursor[0], cursor[1], cursor[2], cursor[3], cursor[4]}};
-    const q3t::Run r = q3t::next_run(c, rounds, heads, q3t::Sharing{{sharing[0], sharing[1], sharing[2]}});
-    const uint32_t after[5] = {{c.x, c.left, c.b, c.head, c.off}}, run[7] = {{r.b, r.head, r.lo, r.hi, r.first, r.parts, r.begins}};
+static q3t::Sharing of(const uint32_t *s) {{ return {{s[0], s[1], s[2], s[3]}}; }}
+extern "C" uint32_t places(uint32_t stages, const uint32_t *sharing) {{ return q3t::places(stages, of(sharing)); }}
+static void put(const q3t::Cursor &c, uint32_t *cursor) {{
+    const uint32_t after[5] = {{c.x, c.left, c.b, c.head, c.off}};
     for (int i = 0; i < 5; ++i) cursor[i] = after[i];
+}}
+extern "C" void end_pair(uint32_t *cursor, uint32_t length, uint32_t heads) {{
+    q3t::Cursor c = {{cursor[0], cursor[1], cursor[2], cursor[3], cursor[4]}};
+    q3t::end_pair(c, length, heads);
+    put(c, cursor);
+}}
+extern "C" void next_run(uint32_t *cursor, uint32_t stages, uint32_t heads, const uint32_t *sharing, uint32_t *out) {{
+    q3t::Cursor c = {{cursor[0], cursor[1], cursor[2], cursor[3], cursor[4]}};
+    const q3t::Run r = q3t::next_run(c, stages, heads, of(sharing));
+    put(c, cursor);
+    const uint32_t run[7] = {{r.b, r.head, r.lo, r.hi, r.first, r.parts, r.begins}};
     for (int i = 0; i < 7; ++i) out[i] = run[i];
 }}
 ''')
@@ -62,19 +72,20 @@ def test_division(index):
             assert index.quotient(n, d) == n // d, (n, d)
 
 
-@pytest.mark.parametrize('seed', range(60))
+@pytest.mark.parametrize('seed', range(80))
 def test_shares_cover_every_pair_once(index, seed):
-    """Every workgroup's runs, together: each round of each pair exactly once, in one run per share,
+    """Every workgroup's runs, together: each stage of each pair exactly once, in one run per share,
     parts numbered from the pair's first share, at most two unfinished states a workgroup and no slot
-    of them twice, no share longer than it says."""
+    of them twice."""
     rng = random.Random(seed)
-    heads, workgroups, least = rng.choice([1, 2, 3, 8]), rng.choice([1, 3, 16, 64, 512]), rng.choice([1, 4])
-    rounds = [rng.choice([1, 1, 2, 3, rng.randrange(1, 17), rng.randrange(1, 900)]) for _ in range(rng.choice([1, 2, 7, 40]))]
+    heads, workgroups, least = rng.choice([1, 2, 3, 8]), rng.choice([1, 3, 16, 64, 512]), rng.choice([1, 4, 8])
+    cost = rng.choice([0, 1, 3, 7])
+    stages = [rng.choice([1, 1, 2, 3, rng.randrange(1, 17), rng.randrange(1, 900)]) for _ in range(rng.choice([1, 2, 7, 40]))]
     u32 = ctypes.c_uint32
-    sharing = (u32 * 3)()
-    index.share_out(sum(rounds) * heads, sum(-(-r // least) for r in rounds) * heads, least, workgroups, sharing)
-    unit, share, total = sharing
-    length = [index.places(r, unit) for r in rounds]
+    sharing = (u32 * 4)()
+    index.share_out(len(stages) * heads, sum(stages) * heads, sum(-(-r // least) for r in stages) * heads, least, cost, workgroups, sharing)
+    unit, extra, share, total = sharing
+    length = [index.places(r, sharing) for r in stages]
     assert total == heads * sum(length) and share * workgroups >= total and share >= 1
     covered, parts, slots = {}, {}, set()
     for w in range(workgroups):
@@ -86,12 +97,14 @@ def test_shares_cover_every_pair_once(index, seed):
             off -= length[b] * heads
             b += 1
         cursor = (u32 * 5)(x, min(share, total - x), b, off // length[b], off % length[b])
+        if cursor[4] >= stages[b]:
+            index.end_pair(cursor, length[b], heads)
         unfinished = 0
         while cursor[1]:
             out = (u32 * 7)()
-            index.next_run(cursor, rounds[cursor[2]], heads, sharing, out)
+            index.next_run(cursor, stages[cursor[2]], heads, sharing, out)
             rb, head, lo, hi, first, count, begins = out
-            assert lo < hi <= rounds[rb]
+            assert lo < hi <= stages[rb]
             for r in range(lo, hi):
                 assert (rb, head, r) not in covered
                 covered[rb, head, r] = w
@@ -106,9 +119,9 @@ def test_shares_cover_every_pair_once(index, seed):
                 assert slot not in slots
                 slots.add(slot)
         assert unfinished <= 2
-    assert len(covered) == heads * sum(rounds)
+    assert len(covered) == heads * sum(stages)
     for (rb, head), (first, count) in parts.items():
-        assert {covered[rb, head, r] for r in range(rounds[rb])} == set(range(first, first + count))
+        assert {covered[rb, head, r] for r in range(stages[rb])} == set(range(first, first + count))
 
 
 def _attend_args(pkg, **changes):
