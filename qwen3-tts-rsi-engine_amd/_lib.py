@@ -6,7 +6,6 @@ library is missing or a call is rejected, the wrappers raise.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -223,12 +222,44 @@ def stream_handle(device: torch.device) -> int:
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
 
 
-_HERE = contextlib.nullcontext()
+def gpu_index(*tensors: torch.Tensor) -> int:
+    """The index of the ROCm device that holds all tensors (``require_gpu`` for calls whose host time
+    counts)."""
+    index = tensors[0].get_device()
+    if index < 0 or tensors[0].device.type != "cuda":
+        raise ValueError("expected tensors on a ROCm GPU device")
+    for t in tensors:
+        if t.get_device() != index:
+            raise ValueError("tensors must share one device")
+    return index
 
 
-def on_device(device: torch.device):
-    """``device`` as the current device for a launch; nothing to do where it is already."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+class on_device:
+    """Device ``index`` as the current one, for launches; yields torch's current stream there."""
+    __slots__ = ('index', 'guard')
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self) -> int:
+        if _raw_stream is not None and torch._C._cuda_getDevice() == self.index:
+            self.guard = None
+            return _raw_stream(self.index)
+        self.guard = torch.cuda.device(self.index)
+        self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *error) -> None:
+        if self.guard is not None:
+            self.guard.__exit__(*error)
+
+
+def launch(entry, args, index: int, what: str) -> None:
+    """An entry point of an argument structure and a stream, on device ``index``."""
+    with on_device(index) as stream:
+        status = entry(args, stream)
+    if status != Q3T_OK:
+        check(status, what)
 
 
 _HIP = None

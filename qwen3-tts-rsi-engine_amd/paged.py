@@ -69,11 +69,11 @@ def paged_write(keys, values, key_pages, value_pages, page_table, positions, len
     ks, vs = keys.stride(), values.stride()
     if ks[3] != 1 or vs[3] != 1:
         raise ValueError('K/V rows must be unit-stride along head_dim')
-    device = _lib.require_gpu(keys, values, key_pages, value_pages, page_table, positions)
+    device = _lib.gpu_index(keys, values, key_pages, value_pages, page_table, positions)
     if lengths is not None:
         if lengths.dtype != torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous():
             raise ValueError('lengths must be a contiguous int32 (batch,) tensor')
-        _lib.require_gpu(keys, lengths)
+        _lib.gpu_index(keys, lengths)
     if batch == 0 or tokens == 0:
         return
     a = _lib.PagedWriteArgs(
@@ -81,9 +81,7 @@ def paged_write(keys, values, key_pages, value_pages, page_table, positions, len
         ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], key_pages.data_ptr(), value_pages.data_ptr(),
         kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], pages, page_size,
         page_table.data_ptr(), table_width, ts, positions.data_ptr(), None if lengths is None else lengths.data_ptr())
-    with _lib.on_device(device):
-        status = _lib.library().q3t_paged_write(a, _lib.stream_handle(device))
-    _lib.check(status, 'paged write')
+    _lib.launch(_lib.library().q3t_paged_write, a, device, 'paged write')
 
 
 def paged_attention(query, key_pages, value_pages, page_table, positions, *, scale=None, mask=None, out=None):
@@ -111,7 +109,7 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     qs = query.stride()
     if qs[3] != 1:
         raise ValueError('rows must be unit-stride along head_dim')
-    device = _lib.require_gpu(query, key_pages, value_pages, page_table, positions)
+    device = _lib.gpu_index(query, key_pages, value_pages, page_table, positions)
     ctx = table_width * page_size
     mask_fields = (None, 0, 0, 0)
     if mask is not None:
@@ -119,7 +117,7 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
             raise ValueError('attention mask must be bool, bf16, fp16 or fp32')
         if not 1 <= mask.ndim <= 4 or not 1 <= mask.shape[-1] <= ctx or any(n != 1 for n in mask.shape[-3:-1]):
             raise ValueError('the mask must be broadcastable to (batch, 1, 1, keys), its keys within the page table')
-        _lib.require_gpu(query, mask)
+        _lib.gpu_index(query, mask)
         ctx = mask.shape[-1]
         try:
             rows = mask.expand(batch, 1, 1, ctx)
@@ -127,9 +125,9 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
             raise ValueError('the mask must be broadcastable to (batch, 1, 1, keys)') from None
         mask_fields = (mask.data_ptr(), _lib.DTYPE_CODES[mask.dtype], rows.stride(0), rows.stride(3))
     if out is None:
-        out, os = torch.empty((batch, 1, q_heads, head_dim), device=device, dtype=dtype), (q_heads * head_dim, 0, head_dim)
+        out, os = query.new_empty((batch, 1, q_heads, head_dim)), (q_heads * head_dim, 0, head_dim)
     else:
-        _check_out(out, (batch, 1, q_heads, head_dim), dtype, device, 'paged attention')
+        _check_out(out, (batch, 1, q_heads, head_dim), dtype, query.device, 'paged attention')
         os = out.stride()
     if batch == 0:
         return out
@@ -142,16 +140,15 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
         kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], pages, page_size,
         page_table.data_ptr(), table_width, ts, positions.data_ptr(), *mask_fields, out.data_ptr(), os[0], os[2])
     lib = _lib.library()
-    with _lib.on_device(device):
-        stream = _lib.stream_handle(device)
-        need = lib.q3t_paged_workspace_bytes(a)
-        if need < 0:
-            raise ValueError('paged attention: unsupported shape or dtype')
-        if need > 0:
-            ws = workspace(device, need, stream)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    need = lib.q3t_paged_workspace_bytes(a)
+    if need < 0:
+        raise ValueError('paged attention: unsupported shape or dtype')
+    with _lib.on_device(device) as stream:
+        ws = workspace(query.device, need, stream)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
         status = lib.q3t_paged_attention(a, stream)
-    _lib.check(status, 'paged attention')
+    if status != _lib.Q3T_OK:
+        _lib.check(status, 'paged attention')
     return out
 
 

@@ -78,13 +78,13 @@ _ROTARY_TYPES = {torch.bfloat16: _lib.Q3T_BF16, torch.float16: _lib.Q3T_F16, tor
 _TURNS = {}
 
 
-def _turns(half, theta, device):
+def _turns(half, theta, like):
     """Full turns per position of every frequency, theta**(-i/half) / 2 pi, in float64."""
-    key = (device.index, half, theta)
+    key = (like.get_device(), half, theta)
     turns = _TURNS.get(key)
     if turns is None:  # cached so that captured graphs never see a host copy
         exponent = torch.arange(half, dtype=torch.float64) / half
-        turns = _TURNS[key] = (float(theta) ** -exponent / (2 * math.pi)).to(device)
+        turns = _TURNS[key] = (float(theta) ** -exponent / (2 * math.pi)).to(like.device)
     return turns
 
 
@@ -107,7 +107,7 @@ def rotary_axes(query, key, positions, sections, *, interleaved=False, theta=DEF
     if query.ndim != 4 or (key is not None and key.ndim != 4):
         raise ValueError('expected BSND query and key rows')
     batch, tokens, q_heads, width = query.shape
-    dtype, device = query.dtype, query.device
+    dtype = query.dtype
     if dtype not in _ROTARY_TYPES or (key is not None and key.dtype != dtype):
         raise ValueError('rotary supports bf16, fp16 or fp32 tensors of one dtype')
     half, axes = 0, len(sections)
@@ -121,31 +121,32 @@ def rotary_axes(query, key, positions, sections, *, interleaved=False, theta=DEF
         raise ValueError('positions must be an int64 (axes, batch, length) tensor')
     qs, ps, ks, k_heads = query.stride(), positions.stride(), (0, 0, 0, 1), 0
     if key is None:
-        _lib.require_gpu(query, positions)
+        device = _lib.gpu_index(query, positions)
     else:
         key_batch, key_tokens, k_heads, key_width = key.shape
         if key_batch != batch or key_tokens != tokens or key_width != width:
             raise ValueError('query and key rows must have one batch, length and width')
         ks = key.stride()
-        _lib.require_gpu(query, key, positions)
+        device = _lib.gpu_index(query, key, positions)
     if qs[3] != 1 or ks[3] != 1 or q_heads < 1 or (key is not None and k_heads < 1):
         raise ValueError('rows must be unit-stride, at least one per token')
     if inv_freq is None:
-        turns = _turns(half, theta, device)
+        turns = _turns(half, theta, query)
     else:
         if inv_freq.shape != (half,):
             raise ValueError('inv_freq must have one entry per frequency')
-        turns = inv_freq.to(device=device, dtype=torch.float64) / (2 * math.pi)
+        turns = inv_freq.to(device=query.device, dtype=torch.float64) / (2 * math.pi)
     if inplace:
         for t in (query,) if key is None else (query, key):
             if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
                 raise ValueError('rows that share memory cannot be rotated in place')
         q_out, k_out, qos, kos = query, key, qs, ks
     else:
-        q_out, qos = torch.empty((batch, tokens, q_heads, width), device=device, dtype=dtype), (tokens * q_heads * width, q_heads * width, width)
-        k_out, kos = None, (0, 0, 0)
+        q_out, k_out, kos = query.new_empty((batch, tokens, q_heads, width)), None, (0, 0, 0)
+        qos = (tokens * q_heads * width, q_heads * width, width)
         if key is not None:
-            k_out, kos = torch.empty((batch, tokens, k_heads, width), device=device, dtype=dtype), (tokens * k_heads * width, k_heads * width, width)
+            k_out = query.new_empty((batch, tokens, k_heads, width))
+            kos = (tokens * k_heads * width, k_heads * width, width)
     if batch == 0 or tokens == 0:
         return q_out, k_out
     a = _lib.RotaryAxesArgs(
@@ -153,7 +154,5 @@ def rotary_axes(query, key, positions, sections, *, interleaved=False, theta=DEF
         scaling, turns.data_ptr(), positions.data_ptr(), ps[0], ps[1], ps[2],
         query.data_ptr(), None if key is None else key.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
         q_out.data_ptr(), None if key is None else k_out.data_ptr(), qos[0], qos[1], qos[2], kos[0], kos[1], kos[2])
-    with _lib.on_device(device):
-        status = _lib.library().q3t_rotary_axes(a, _lib.stream_handle(device))
-    _lib.check(status, 'rotary axes')
+    _lib.launch(_lib.library().q3t_rotary_axes, a, device, 'rotary axes')
     return q_out, k_out
