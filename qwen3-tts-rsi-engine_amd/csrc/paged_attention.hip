@@ -130,6 +130,9 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
+// LDS reads above are issued before anything below: left alone, the compiler waits for each one alone.
+Q3T_DEVICE void together() { __builtin_amdgcn_sched_barrier(0); }
+
 // The products of a wave's tile of 16 keys, by type.  Lane (g, c) = (lane / 16, lane % 16) holds
 // column c; of S^T the keys 4 g ... 4 g + 3.
 template <typename T, int D> struct Tile;
@@ -204,12 +207,22 @@ template <typename T, int D> struct Tile {
     }
     // tile t of the stage at byte `stage` of the ring
     Q3T_DEVICE f32x4_t scores(uint32_t stage, int t) const {
+        U4 k[D / 32];
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk) k[kk] = lds_read16(key_at[kk] + stage + t * 16 * S::row);
+        together();
         f32x4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < D / 32; ++kk) s = Half<T>::scores(lds_read16(key_at[kk] + stage + t * 16 * S::row), q[kk], s);
+        for (int kk = 0; kk < D / 32; ++kk) s = Half<T>::scores(k[kk], q[kk], s);
         return s;
     }
-    Q3T_DEVICE void values(uint32_t stage, int t, const float (&w)[4]) {
+    uint2 v[D / 16];  // the next value fragments
+    Q3T_DEVICE void read_values(uint32_t stage, int t) {
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) v[d] = lds_read_tr16(value_at[d] + stage + t * 16 * S::row);
+        together();
+    }
+    Q3T_DEVICE void values(const float (&w)[4]) {
         uint2 part[3];
         float x[4] = {w[0], w[1], w[2], w[3]};
 #pragma unroll
@@ -222,10 +235,9 @@ template <typename T, int D> struct Tile {
         }
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
-            const uint2 v = lds_read_tr16(value_at[d] + stage + t * 16 * S::row);
-            first[d] = Half<T>::values(v, part[0], first[d]);
+            first[d] = Half<T>::values(v[d], part[0], first[d]);
 #pragma unroll
-            for (int i = 1; i < Half<T>::parts; ++i) rest[d] = Half<T>::values(v, part[i], rest[d]);
+            for (int i = 1; i < Half<T>::parts; ++i) rest[d] = Half<T>::values(v[d], part[i], rest[d]);
         }
     }
     // Elements of column c into its row of D floats, four to a chunk, chunk k at k ^ c.
@@ -268,24 +280,35 @@ template <int D> struct Tile<float, D> {
         value_at = ring + (S::keys + 4 * g) * S::row + c * 16;
     }
     Q3T_DEVICE f32x4_t scores(uint32_t stage, int t) const {
-        f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+        f32x4_t k[D / 16], s = {0.f, 0.f, 0.f, 0.f}, s2 = s;  // two chains: one waits for its last product
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            const f32x4_t k = read(key_at[kk] + stage + t * 16 * S::row);
+        for (int kk = 0; kk < D / 16; ++kk) k[kk] = read(key_at[kk] + stage + t * 16 * S::row);
+        together();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[kk][e], s, 0, 0, 0);
-        }
-        return s;
+        for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[kk][e], q[kk][e], s, 0, 0, 0);
+                s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(k[kk][e + 1], q[kk][e + 1], s2, 0, 0, 0);
+            }
+        return s + s2;
     }
-    Q3T_DEVICE void values(uint32_t stage, int t, const float (&w)[4]) {
+    f32x4_t v[D / 16];
+    Q3T_DEVICE void read_values(uint32_t stage, int t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < D / 64; ++j) {
-                const f32x4_t v = read(value_at + stage + (16 * t + i) * S::row + j * 256);
+            for (int j = 0; j < D / 64; ++j) v[i * (D / 64) + j] = read(value_at + stage + (16 * t + i) * S::row + j * 256);
+        together();
+    }
+    Q3T_DEVICE void values(const float (&w)[4]) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[4 * j + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], w[i], acc[4 * j + e], 0, 0, 0);
-            }
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[4 * j + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i * (D / 64) + j][e], w[i], acc[4 * j + e], 0, 0, 0);
     }
     Q3T_DEVICE void store(uint32_t to, int g, int c) const {
 #pragma unroll
@@ -634,13 +657,16 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
                 highest = fmaxf(highest, v[t][i]);
             }
         }
+        x.read_values(stage, 0);  // on their way during the softmax
         if (__builtin_amdgcn_ballot_w64(highest > m + threshold)) {
             highest = fmaxf(highest, xor16(highest));
             highest = fmaxf(highest, xor32(highest));
             highest = fmaxf(highest, m);
-            const float alpha = fexp2((m - (highest == -INFINITY ? 0.f : highest)) * unit);
-            l *= alpha;
-            x.rescale(alpha);
+            if (__builtin_amdgcn_ballot_w64(m != -INFINITY)) {  // something has been added up
+                const float alpha = fexp2((m - (highest == -INFINITY ? 0.f : highest)) * unit);
+                l *= alpha;
+                x.rescale(alpha);
+            }
             m = highest;
         }
         const float from = m == -INFINITY ? 0.f : m;
@@ -650,7 +676,8 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = fexp2((v[t][i] - from) * unit + Products::shift);
             l += (w[0] + w[1]) + (w[2] + w[3]);
-            x.values(stage, t, w);
+            if (t > 0) x.read_values(stage, t);
+            x.values(w);
         }
     };
     auto finish = [&](const Run &r, uint32_t column, uint32_t d, const State &sum) {
