@@ -740,9 +740,15 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
             s.ml[wave][c][1] = l;
         }
         if (lane == 0) s.slot[wave] = slot;
+        const bool whole = r.parts == 1;
+        // The first of two parts is done last in its share, and the other first in the next one: where that
+        // one is there already, it is merged at once and nothing is published.
+        int32_t *counter = p.counters + r.b * p.heads + r.head;
+        if (tid == kThreads - 1 && r.parts == 2 && r.begins)
+            s.count = (uint32_t)__hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if ((uint32_t)c < columns) x.store(slot, g, c);
         lds_barrier();
-        const bool whole = r.parts == 1;
+        const bool two = r.parts == 2 && r.begins && uniform(s.count) == 1;
         float *state = p.states + (2 * blockIdx.x + r.begins) * (uint64_t)state_size;
         for (uint32_t item = tid; item < columns * (D / 4); item += kThreads) {
             const uint32_t column = item / (D / 4), chunk = item % (D / 4);
@@ -755,12 +761,18 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
                 own.l += s.ml[w][column][1] * e;
                 own.a += __builtin_bit_cast(f32x4_t, lds_read16(s.slot[w] + column * D * 4 + (chunk ^ column) * 16)) * e;
             }
-            if (whole) finish(r, column, chunk * 4, own);
+            if (two) {
+                State other;
+                other.collect(p.states + 2 * (r.first + 1) * (uint64_t)state_size, p.columns * D, column, chunk * 4, D);
+                own.add(other, unit);
+            }
+            if (whole || two) finish(r, column, chunk * 4, own);
             else own.publish(state, p.columns * D, column, chunk * 4, D);
         }
-        if (!whole) wait_loads<0>();  // the state has been stored
+        if (!whole && !two) wait_loads<0>();  // the state has been stored
         lds_barrier();
-        if (whole) continue;
+        if (two && tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (whole || two) continue;
 
         // Parts beyond kTogether are merged in two steps: kTogether neighbours' last to arrive merges
         // theirs into the first one's state, and the last of those merges them.
@@ -827,7 +839,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         };
         bool last = r.parts <= kTogether;
         uint32_t begin = last ? 0 : part / kTogether * kTogether, step = 1, count = min(kTogether, r.parts - begin);
-        while (arrive(last ? p.counters + r.b * p.heads + r.head : p.counters + kPairs + slot_of(begin), count)) {
+        while (arrive(last ? counter : p.counters + kPairs + slot_of(begin), count)) {
             merge(begin, step, count, last);
             if (last) break;
             wait_loads<0>();
