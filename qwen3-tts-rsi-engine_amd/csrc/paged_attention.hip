@@ -6,16 +6,16 @@
 // in one pass over the keys, with a running maximum m that moves when it is passed by more than a
 // threshold.  Every key and value row is read once, so HBM bounds a launch of many keys (2 to 16
 // operations per byte), and the chain arguments - positions - page numbers - rows - merge one of few.
-//   * Work: a workgroup of four waves takes an equal share of the rounds of all (request, KV head)
-//     pairs (paged_index.hpp), whatever the requests' lengths; it finds its place by adding up
-//     all requests' rounds.  A pair that lies in several shares leaves its parts' states in the
+//   * Work: a workgroup takes an equal share of the stages of all (request, KV head) pairs
+//     (paged_index.hpp), whatever the requests' lengths; its waves find their place by adding up all
+//     requests' stages.  A pair that lies in several shares leaves its parts' states in the
 //     workspace, and the workgroup that arrives last merges them, in the parts' order.
-//   * A wave takes every fourth stage of 16 (rows of 128 bytes: 32) keys of a pair.  A stage's rows
-//     go straight from memory to the wave's own two LDS slots, one stage ahead of the one that is
-//     scored, over the ends of pairs: no barrier but where a pair ends.  The page numbers of up to 64
-//     stages come the same way, while the stages before them are read.  Where pages hold whole
-//     stages a stage's rows are one range of memory; for other page sizes each lane works out the
-//     address of its own row.
+//   * Of a run of a pair's stages of 16 (rows of 128 bytes: 32) keys each of the workgroup's W waves takes
+//     every W-th.  A stage's rows go straight from memory to the wave's own two LDS slots, one stage
+//     ahead of the one that is scored, over the ends of runs: no barrier but where a run ends.  The
+//     page numbers of up to 64 stages come the same way, while the stages before them are read.
+//     Where pages hold whole stages a stage's rows are one range of memory; for other page sizes
+//     each lane works out the address of its own row.
 //   * The rows of a KV head's query heads are the columns of 16x16 products, S^T = K . Q^T and
 //     O^T += V^T . P^T.  The matrix cores idle (under a twentieth of their rate), so the weights are
 //     not rounded to the cache's type: bf16 weights go in three parts (all 24 bits of their
@@ -31,13 +31,11 @@
 namespace q3t {
 namespace paged {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kColumns = 16;           // query heads of a workgroup: columns of a product
 constexpr uint32_t kLeastStages = 8;   // stages that are not shared out
 constexpr uint32_t kRunCost = 8;       // stages that the end of a run costs as much as
 constexpr int kCounters = 65536;       // counter words in front of a decode workspace: of the pairs,
-constexpr int kPairs = kCounters - 1024;  // then of the state slots
-constexpr int kWorkgroups = 512;       // at most
+constexpr int kPairs = kCounters - 1024;  // then of the state slots, two for each of up to 512 workgroups
 constexpr uint32_t kTogether = 16;     // parts that are merged in one step
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -66,20 +64,25 @@ struct Shape {
     static constexpr int log_keys = keys == 32 ? 5 : 4;
     static constexpr bool f32 = sizeof(T) == 4;
     static_assert(kColumns * D * 4 <= stage, "a free slot holds a wave's accumulators");
-    static constexpr int per_cu = row == 512 ? 1 : 2;      // workgroups that fit a CU's LDS
     // chunk c of key (value) row r sits at c ^ swizzle: the products' reads meet distinct banks
     static Q3T_DEVICE int key_swizzle(int r) { return chunks == 8 ? (r >> 1) & 7 : r & 15; }
     static Q3T_DEVICE int value_swizzle(int r) { return f32 ? 0 : chunks == 8 ? (2 * (r >> 1)) & 7 : (2 * r) & 15; }
 };
 
-template <typename T, int D, bool MASK>
+// Workgroups of W waves, as many as fit the LDS of 256 CUs.
+template <typename T, int D, int W> struct Workgroups {
+    static constexpr int per_cu = Shape<T, D>::row * W > 256 * 4 ? 1 : 2;
+    static constexpr int count = 256 * per_cu;
+};
+
+template <typename T, int D, bool MASK, int W>
 struct Lds {
-    alignas(1024) char ring[kWaves][2][Shape<T, D>::stage];
+    alignas(1024) char ring[W][2][Shape<T, D>::stage];
     alignas(16) char query[2][kColumns * Shape<T, D>::row];  // of this run's pair and the next's
-    uint32_t ids[kWaves][2][64];
-    alignas(16) uint32_t maskw[MASK ? kWaves : 1][2][MASK ? Shape<T, D>::keys : 4];
-    float ml[kWaves][kColumns][2];
-    uint32_t slot[kWaves];  // each wave's free slot
+    uint32_t ids[W][2][64];
+    alignas(16) uint32_t maskw[MASK ? W : 1][2][MASK ? Shape<T, D>::keys : 4];
+    float ml[W][kColumns][2];
+    uint32_t slot[W];  // each wave's free slot
     uint32_t count;
 };
 
@@ -378,7 +381,7 @@ struct State {
     }
 };
 
-// Stages of a wave in one run, every fourth from key `key` on below `end`, up to the number of
+// Stages of a wave in one run, every W-th from key `key` on below `end`, up to the number of
 // stages whose page numbers fit its 64 words.
 struct Batch {
     uint32_t b, kv_head, length, key, end;
@@ -406,13 +409,13 @@ Q3T_DEVICE uint32_t scan(uint32_t x) {
 
 // WHOLE: a stage's keys share a page (page sizes that are multiples of a stage), so their rows are one
 // range of memory.
-template <typename T, int D, bool MASK, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, (Shape<T, D>::per_cu))
+template <typename T, int D, bool MASK, bool WHOLE, int W>
+__global__ void __launch_bounds__(64 * W, (W / 4 * Workgroups<T, D, W>::per_cu))
 paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     typedef Shape<T, D> S;
     typedef Tile<T, D> Products;
-    constexpr int LOADS = 2 * S::loads;
-    __shared__ Lds<T, D, MASK> s;
+    constexpr int LOADS = 2 * S::loads, kThreads = 64 * W;
+    __shared__ Lds<T, D, MASK, W> s;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = (int)uniform(tid >> 6);
 
@@ -476,7 +479,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     auto kv_head = [&](uint32_t head) { return p.blocks == 1 ? head : head / p.blocks; };
     Cursor ahead = at;
     int32_t runs = -1;
-    constexpr uint32_t kStep = kWaves * S::keys, kBatch = (WHOLE ? 64 : 64 / S::keys) * kStep;  // keys
+    constexpr uint32_t kStep = W * S::keys, kBatch = (WHOLE ? 64 : 64 / S::keys) * kStep;  // keys
     Batch batches = {0u, 0u, 0u, 0u, 0u, -1};  // the next one, whose page numbers are on their way
     auto next_batch = [&]() {
         if (batches.key + kBatch < batches.end) {
@@ -490,7 +493,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
             batches.b = run.b;
             batches.kv_head = kv_head(run.head);
             batches.length = length;
-            batches.key = (run.lo + ((wave - run.lo) & (kWaves - 1))) * S::keys;  // every fourth stage is the wave's
+            batches.key = (run.lo + ((wave - run.lo) & (W - 1))) * S::keys;  // every W-th stage is the wave's
             batches.end = min(run.hi * S::keys, length);
             batches.run = runs;
             if (batches.key < batches.end) return;
@@ -588,7 +591,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         }
     };
 
-    if (wave == kWaves - 1) load_query(at.b, at.head, 0);
+    if (wave == W - 1) load_query(at.b, at.head, 0);
     next_batch();
     Batch now = batches;  // the batch whose rows are being loaded, its page numbers in half `half`
     uint32_t index = 0, half = 0;
@@ -692,7 +695,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     for (int32_t order = 0; at.left > 0; ++order) {
         const Run r = next_run(at, stages_of(request_length(at.b)), p.heads, sh);
         const uint32_t columns = columns_of(r.head);
-        if (wave == kWaves - 1 && at.left > 0) load_query(at.b, at.head, (order + 1) & 1);
+        if (wave == W - 1 && at.left > 0) load_query(at.b, at.head, (order + 1) & 1);
         x.load_query(queries + (order & 1) * kColumns * S::row, g, c, (uint32_t)c < columns);
         x.clear();
         m = -INFINITY;
@@ -723,9 +726,10 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
             score(s0);
             s0 = s1;
             ++n;
-            // Of two workgroups on a CU the older one's loads go first, and the younger one (the later
-            // half, as they are dealt out) would end after it: it goes first on every second stage.
-            if (blockIdx.x >= kWorkgroups / 2) {
+            // Of two waves on a SIMD the older one's loads go first, and the younger one (of the later half
+            // of the workgroups, as they are dealt out, or of a workgroup's waves) would end after it: it
+            // goes first on every second stage.
+            if (W == 8 ? wave >= 4 : blockIdx.x >= 256) {
                 if (n & 1) __builtin_amdgcn_s_setprio(2);
                 else __builtin_amdgcn_s_setprio(0);
             }
@@ -753,10 +757,12 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         for (uint32_t item = tid; item < columns * (D / 4); item += kThreads) {
             const uint32_t column = item / (D / 4), chunk = item % (D / 4);
             State own = {};
-            own.m = fmaxf(fmaxf(s.ml[0][column][0], s.ml[1][column][0]), fmaxf(s.ml[2][column][0], s.ml[3][column][0]));
+            own.m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < W; ++w) own.m = fmaxf(own.m, s.ml[w][column][0]);
             const float from = own.m == -INFINITY ? 0.f : own.m;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
+            for (int w = 0; w < W; ++w) {
                 const float e = fexp2((s.ml[w][column][0] - from) * unit);
                 own.l += s.ml[w][column][1] * e;
                 own.a += __builtin_bit_cast(f32x4_t, lds_read16(s.slot[w] + column * D * 4 + (chunk ^ column) * 16)) * e;
@@ -852,24 +858,45 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     }
 }
 
+// Eight waves a workgroup instead of four: half as many shares, so half as many cut pairs, but more
+// waves with nothing to do in a short one.  us, four / eight: 128 requests of 100..4095 keys 180 / 174.5, 4
+// of 16000 53.5 / 50.9, 64 of 64..1023 33.4 / 31.6, 32 of 100..2000 31.8 / 31.1; 8 of 100..2000 14.3 / 16.6,
+// 128 of 32..511 32.5 / 37.8, 64 of 64 9.3 / 10.6, 200 of 10..400 27 / 43.  The host sees capacities, not
+// lengths: eight from 768 keys a request and 24576 stages in all, for up to 1024 pairs, where short
+// requests cost little.
+constexpr int64_t kLongRequest = 768, kManyStages = 24576, kFewPairs = 1024;
+
 template <typename T, int D>
 struct Launch {
+    typedef Shape<T, D> S;
+    static int64_t stages(const q3t_paged_args *a, int64_t pairs) { return pairs * ((a->ctx + S::keys - 1) / S::keys + kRunCost); }
+    // rows of a stage as one range: whole pages, rows that do not overlap, 32-bit offsets
+    static bool whole(const q3t_paged_args *a) {
+        const int64_t es = sizeof(T), most = ((int64_t)1 << 30) / S::keys;
+        return a->page_size % S::keys == 0 && a->kp_stride_t * es >= S::row && a->vp_stride_t * es >= S::row &&
+               a->kp_stride_t * es < most && a->vp_stride_t * es < most;
+    }
+    static bool eight(const q3t_paged_args *a, int64_t pairs) {
+        return S::row < 512 && whole(a) && a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs) >= kManyStages;
+    }
     static int64_t workgroups(const q3t_paged_args *a, int64_t pairs) {
-        const int64_t stages = (a->ctx + Shape<T, D>::keys - 1) / Shape<T, D>::keys;
-        const int64_t pieces = pairs * ((stages + kLeastStages - 1) / kLeastStages), most = kWorkgroups / 2 * Shape<T, D>::per_cu;
+        const int64_t stages = (a->ctx + S::keys - 1) / S::keys, pieces = pairs * ((stages + kLeastStages - 1) / kLeastStages);
+        const int64_t most = eight(a, pairs) ? Workgroups<T, D, 8>::count : Workgroups<T, D, 4>::count;
         return pieces < most ? pieces : most;
     }
-    static int64_t stages(const q3t_paged_args *a, int64_t pairs) { return pairs * ((a->ctx + Shape<T, D>::keys - 1) / Shape<T, D>::keys + kRunCost); }
-    static void run(const int64_t *positions, uint32_t batch, uint32_t ctx, const Params &p, uint32_t blocks, hipStream_t s) {
-        auto launch = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, s, positions, batch, ctx, p);
+    static void run(const q3t_paged_args *a, int64_t pairs, const Params &p, uint32_t blocks, hipStream_t s) {
+        auto launch = [&](auto kernel, int waves) {
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves), 0, s, a->positions, (uint32_t)a->batch, (uint32_t)a->ctx, p);
         };
-        // rows of a stage as one range: whole pages, rows that do not overlap, 32-bit offsets
-        typedef Shape<T, D> S;
-        const bool whole = p.by_page.d % S::keys == 0 && p.kp_st * 16ull >= S::row && p.vp_st * 16ull >= S::row &&
-                           p.kp_st < (1u << 26) / S::keys && p.vp_st < (1u << 26) / S::keys;
-        if (p.mask) whole ? launch(paged_kernel<T, D, true, true>) : launch(paged_kernel<T, D, true, false>);
-        else whole ? launch(paged_kernel<T, D, false, true>) : launch(paged_kernel<T, D, false, false>);
+        auto masked = [&](auto mask) {
+            constexpr bool MASK = decltype(mask)::value;
+            if constexpr (S::row < 512)
+                if (eight(a, pairs)) return launch(paged_kernel<T, D, MASK, true, 8>, 8);
+            if (whole(a)) launch(paged_kernel<T, D, MASK, true, 4>, 4);
+            else launch(paged_kernel<T, D, MASK, false, 4>, 4);
+        };
+        if (a->mask) masked(std::true_type{});
+        else masked(std::false_type{});
     }
 };
 // f on the Launch of a call's type and width
@@ -965,6 +992,6 @@ extern "C" int q3t_paged_attention(const q3t_paged_args *a, void *stream) {
     p.by_page = divisor((uint32_t)a->page_size);
     p.by_grid = divisor((uint32_t)z.workgroups);
     p.scale = a->mask ? a->scale : a->scale * kLog2e;
-    with(a, [&](auto l) { l.run(a->positions, (uint32_t)a->batch, (uint32_t)a->ctx, p, (uint32_t)z.workgroups, (hipStream_t)stream); });
+    with(a, [&](auto l) { l.run(a, z.pairs, p, (uint32_t)z.workgroups, (hipStream_t)stream); });
     return launch_status();
 }

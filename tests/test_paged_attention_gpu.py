@@ -42,9 +42,25 @@ def test_many_requests_share_the_card(pkg, device, lengths):
     assert_within(run(pkg, p), *expected(p))
 
 
-def test_table_wider_than_the_requests_need(pkg, device):
-    """Entries past a request's pages are not looked at (they hold -7 here)."""
-    p = problem(device, RAGGED, table_width=4000, seed=5)
+@pytest.mark.parametrize('masked', [False, True])
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (BF16, 64), (F16, 128), (F16, 64), (F32, 128), (F32, 64)], ids=str)
+@pytest.mark.parametrize('heads', [(16, 8), (8, 1), (20, 1)], ids=str)
+def test_table_wider_than_the_requests_need(pkg, device, masked, dtype, width, heads):
+    """Tables of 32000 rows a request, for which the launch takes larger workgroups; entries past a
+    request's pages are not looked at (they hold -7 here)."""
+    p = problem(device, RAGGED + [2100, 900], q_heads=heads[0], kv_heads=heads[1], width=width, dtype=dtype, table_width=1000,
+                page=32, seed=5)
+    mask = None
+    if masked:
+        mask = torch.ones(len(p.lengths), 1, 1, 32000, dtype=torch.bool, device=device)
+        mask[:, :, :, 3::7] = False
+        mask[5] = False
+    assert_within(run(pkg, p, mask=mask), *expected(p, mask=mask))
+
+
+@pytest.mark.parametrize('lengths', [[4000] * 70 + [1, 0, 17], [900] * 90, [30000, 31000, 5, 64]], ids=['70 long', '90x900', 'two'])
+def test_launches_that_fill_the_card(pkg, device, lengths):
+    p = problem(device, lengths, q_heads=16, kv_heads=8, page=64, seed=27)
     assert_within(run(pkg, p), *expected(p))
 
 
