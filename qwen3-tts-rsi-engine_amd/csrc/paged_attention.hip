@@ -83,7 +83,8 @@ struct Lds {
     alignas(16) uint32_t maskw[MASK ? W : 1][2][MASK ? Shape<T, D>::keys : 4];
     float ml[W][kColumns][2];
     uint32_t slot[W];  // each wave's free slot
-    uint32_t count;
+    uint32_t there;    // the count of a pair of two parts, ahead of the waves' merge
+    uint32_t count;    // parts that have arrived
 };
 
 #define Q3T_LDS __attribute__((address_space(3)))
@@ -98,7 +99,7 @@ Q3T_DEVICE uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_read
                  OPCODE " %1, " ADDRESS POLICY "\n\t"                                              \
                  OPCODE " %2, " ADDRESS " offset:1024" POLICY "\n\t"                               \
                  OPCODE " %3, " ADDRESS " offset:2048" POLICY "\n\t"                               \
-                 OPCODE " %4, " ADDRESS " offset:3072" POLICY                                      \
+                 OPCODE " %4, " ADDRESS " offset:3*1024" POLICY                                      \
                  :: "s"(base), "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]) __VA_ARGS__ : "memory", "m0")
 // from a pointer per lane
 Q3T_DEVICE void load_rows(const uint64_t *p, uint32_t base) { Q3T_LOAD4("global_load_lds_dwordx4", "off", " nt"); }
@@ -749,10 +750,10 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         // one is there already, it is merged at once and nothing is published.
         int32_t *counter = p.counters + r.b * p.heads + r.head;
         if (tid == kThreads - 1 && r.parts == 2 && r.begins)
-            s.count = (uint32_t)__hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s.there = (uint32_t)__hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if ((uint32_t)c < columns) x.store(slot, g, c);
         lds_barrier();
-        const bool two = r.parts == 2 && r.begins && uniform(s.count) == 1;
+        const bool two = r.parts == 2 && r.begins && uniform(s.there) == 1;
         float *state = p.states + (2 * blockIdx.x + r.begins) * (uint64_t)state_size;
         for (uint32_t item = tid; item < columns * (D / 4); item += kThreads) {
             const uint32_t column = item / (D / 4), chunk = item % (D / 4);
@@ -786,7 +787,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         auto slot_of = [&](uint32_t i) { return 2 * (r.first + i) + (i == 0); };  // part i's state
         auto arrive = [&](int32_t *counter, uint32_t expected) {
             if (tid == 0) s.count = (uint32_t)__hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __syncthreads();  // (and there are more barriers before the next count)
+            __syncthreads();  // (the waves' merge or a merge of parts, with barriers, lies before the next count)
             const bool last = uniform(s.count) == expected - 1;
             if (last && tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             return last;
