@@ -425,7 +425,9 @@ int q3t_paged_write(const q3t_paged_write_args *args, void *stream);
  * (packed_attention.py:75-84) over pages instead of slots.
  *
  * dtype Q3T_BF16, Q3T_F16 or Q3T_F32; head_dim 64 or 128; pool bases and strides, query rows:
- * 16-byte multiples.
+ * 16-byte multiples.  batch * kv_heads, each KV head counted once for every 16 query heads of it: 64512 at
+ * most.  No stride is negative; those of the output, the mask and the table stay below 2^32 elements, the
+ * others below 2^36 bytes.
  */
 typedef struct q3t_paged_args {
     int64_t batch, q_heads, kv_heads, head_dim, dtype;
@@ -468,8 +470,8 @@ int q3t_paged_attention(const q3t_paged_args *args, void *stream);
  *   y[i] = x[i] cos - x[i + half] sin,  y[i + half] = x[i + half] cos + x[i] sin
  * with cos and sin multiplied by `scaling`; elements past 2 * half are copied.  Angles are formed
  * in 64 bits and reduced before cos and sin, products and sums in float32, and each element is
- * rounded once (q3t_rotary, given cos/sin rows, rounds as torch-eager does).  Outputs may be the
- * inputs themselves.  turns: device, `half` doubles, frequency / (2 pi).
+ * rounded once (q3t_rotary, given cos/sin rows, rounds as torch-eager does).  An output may be
+ * its input itself, by the same strides; otherwise rows overlap no output row.  turns: device, `half` doubles, frequency / (2 pi).
  * Replaces: the talker's rotary_emb and apply_multimodal_rotary_pos_emb on unequal axes
  * (continuous.py:193, packed_attention.py:66-69).
  */

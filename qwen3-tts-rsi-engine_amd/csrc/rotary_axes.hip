@@ -234,7 +234,8 @@ extern "C" int q3t_rotary_axes(const q3t_rotary_axes_args *a, void *stream) {
     p.rotated = (uint32_t)(half / v);
     p.tail = (uint32_t)(2 * half);
     // what is not rotated needs no copy where every output is its input
-    const bool in_place = p.q.x == p.q.y && p.k.x == p.k.y;
+    auto same = [](const Rows &r) { return r.x == r.y && r.x_sb == r.y_sb && r.x_ss == r.y_ss && r.x_sh == r.y_sh; };
+    const bool in_place = same(p.q) && same(p.k);
     p.units = p.rotated + (in_place ? 0u : (uint32_t)((a->width - 2 * half) / v));
     p.axes = (uint32_t)a->axes;
     p.interleaved = a->interleaved != 0;

@@ -80,12 +80,48 @@ _TURNS = {}
 
 def _turns(half, theta, like):
     """Full turns per position of every frequency, theta**(-i/half) / 2 pi, in float64."""
+    theta = float(theta)
     key = (like.get_device(), half, theta)
     turns = _TURNS.get(key)
-    if turns is None:  # cached so that captured graphs never see a host copy
-        exponent = torch.arange(half, dtype=torch.float64) / half
-        turns = _TURNS[key] = (float(theta) ** -exponent / (2 * math.pi)).to(like.device)
+    if turns is None:
+        if not 0 < theta < math.inf:
+            raise ValueError('theta must be positive')
+        # kept, but a graph being captured forms its own: it takes no host copy, and its memory is its own
+        with torch.cuda.device(like.device):
+            capturing = torch.cuda.is_current_stream_capturing()
+        exponent = torch.arange(half, dtype=torch.float64, device=like.device if capturing else None) / half
+        turns = (theta ** -exponent / (2 * math.pi)).to(like.device)
+        if not capturing:
+            _TURNS[key] = turns
     return turns
+
+
+def _dims(t):
+    """(stride, size) of the dimensions of rows t that have more than one entry, outermost first."""
+    return sorted(((s, n) for n, s in zip(t.shape[:-1], t.stride()) if n > 1), reverse=True)
+
+
+def _extent(dims, row):
+    """Elements from the first to the last of rows of ``row`` elements."""
+    return sum((n - 1) * s for s, n in dims) + row
+
+
+def _share_memory(x, y=None):
+    """Whether rows of x overlap each other, or rows of y; True as well where no nesting of the
+    dimensions (each stride passes all that lies within it) shows that they do not."""
+    row, dims = x.shape[-1], _dims(x)
+    if y is None:
+        return any(s < _extent(dims[i + 1:], row) for i, (s, _) in enumerate(dims))
+    others, apart = _dims(y), (y.data_ptr() - x.data_ptr()) // x.element_size()
+    while True:
+        ends = _extent(dims, row), apart + _extent(others, row)
+        if apart >= ends[0] or ends[1] <= 0:
+            return False
+        if not dims or not others or dims[0][0] != others[0][0]:
+            return True
+        dims, others, stride = dims[1:], others[1:], dims[0][0]
+        if max(_extent(dims, row), apart + _extent(others, row)) - min(0, apart) > stride:
+            return True
 
 
 def rotary_axes(query, key, positions, sections, *, interleaved=False, theta=DEFAULT_THETA, inv_freq=None,
@@ -103,7 +139,7 @@ def rotary_axes(query, key, positions, sections, *, interleaved=False, theta=DEF
     is rounded once (``rotary``, given cos/sin rows, rounds as torch-eager does).
 
     Returns (query, key) rotated: new contiguous tensors, or with ``inplace`` the given ones,
-    rotated where they are."""
+    rotated where they are (their rows must not overlap).  Inference only, as ``rotary``."""
     if query.ndim != 4 or (key is not None and key.ndim != 4):
         raise ValueError('expected BSND query and key rows')
     batch, tokens, q_heads, width = query.shape
@@ -135,11 +171,10 @@ def rotary_axes(query, key, positions, sections, *, interleaved=False, theta=DEF
     else:
         if inv_freq.shape != (half,):
             raise ValueError('inv_freq must have one entry per frequency')
-        turns = inv_freq.to(device=query.device, dtype=torch.float64) / (2 * math.pi)
+        turns = (inv_freq.to(device=query.device, dtype=torch.float64) / (2 * math.pi)).contiguous()
     if inplace:
-        for t in (query,) if key is None else (query, key):
-            if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
-                raise ValueError('rows that share memory cannot be rotated in place')
+        if _share_memory(query) or (key is not None and (_share_memory(key) or _share_memory(query, key))):
+            raise ValueError('rows that share memory cannot be rotated in place')
         q_out, k_out, qos, kos = query, key, qs, ks
     else:
         q_out, k_out, kos = query.new_empty((batch, tokens, q_heads, width)), None, (0, 0, 0)

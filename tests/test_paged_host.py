@@ -2,6 +2,7 @@
 C entry points, before anything is launched, the index arithmetic compiled by the host compiler,
 and the arena's page accounting."""
 import ctypes
+import importlib
 import random
 import subprocess
 from pathlib import Path
@@ -299,3 +300,57 @@ def test_arena_hands_out_every_page_once(pkg):
     for bad in (dict(pages=0), dict(pages=3, page_size=0)):
         with pytest.raises(ValueError):
             pkg.PagedArena(_reference(), **bad)
+
+
+def test_a_prefill_cache_of_other_layers_is_refused(pkg):
+    arena = pkg.PagedArena(_reference(), pages=4)
+    rows = torch.zeros(1, 8, 3, 128, dtype=torch.bfloat16)
+    cache = SimpleNamespace(layers=[SimpleNamespace(keys=rows, values=rows)])
+    with pytest.raises(ValueError, match='layers'):
+        arena.load(arena.page_table([[0]]), cache, torch.tensor([3], dtype=torch.int32))
+
+
+def _places(t):
+    return torch.arange(100000).as_strided(t.shape, t.stride(), t.storage_offset()).flatten().tolist()
+
+
+@pytest.mark.parametrize('seed', range(20))
+def test_rows_that_share_memory_are_found(pkg, seed):
+    """No overlap is missed, whatever the strides."""
+    share = importlib.import_module(pkg.__name__ + '.rotary')._share_memory
+    rng = torch.Generator().manual_seed(seed)
+    memory = torch.zeros(20000, dtype=torch.float16)
+    number = lambda low, high: int(torch.randint(low, high + 1, (1,), generator=rng))
+    apart = 0
+    for _ in range(300):
+        width, strides = number(1, 4), [number(0, 40) for _ in range(3)]
+        views = []
+        for _ in range(2):
+            shape = [number(1, 3) for _ in range(3)]
+            if number(0, 2) == 0:
+                strides = [number(0, 40) for _ in range(3)]
+            views.append(memory.as_strided(shape + [width], strides + [1], number(0, 60)))
+        x, y = views
+        for t in views:
+            if len(set(_places(t))) < t.numel():
+                assert share(t)
+        if set(_places(x)) & set(_places(y)):
+            assert share(x, y)
+        elif not share(x, y):
+            apart += 1
+    assert apart > 30  # some were told apart
+
+
+def test_rows_of_one_projection_do_not_share_memory(pkg):
+    share = importlib.import_module(pkg.__name__ + '.rotary')._share_memory
+    fused = torch.zeros(3, 5, 28, 16)
+    per_head = torch.zeros(3, 5, 8, 3, 16)
+    bnsd = torch.zeros(3, 24, 5, 16).transpose(1, 2)
+    for q, k in ((fused[:, :, :16], fused[:, :, 16:24]), (fused[:, :, 8:24], fused[:, :, :8]), (fused[:1, :, :16], fused[:1, :, 16:20]),
+                 (fused[:, :1, :16], fused[:, :1, 27:]), (per_head[:, :, :, 0], per_head[:, :, :, 1]),
+                 (per_head[:, :, :, 2], per_head[:, :, :, 0]), (bnsd[:, :, :16], bnsd[:, :, 16:]), (fused, bnsd),
+                 (fused[..., :8], fused[..., 8:])):
+        assert not share(q) and not share(k) and not share(q, k) and not share(k, q)
+    for q, k in ((fused, fused), (fused[:, :, :16], fused[:, :, 15:24]), (fused[..., :8], fused[..., 4:12]), (fused, fused[1:])):
+        assert share(q, k) and share(k, q)
+    assert share(fused[:, :, :1].expand(3, 5, 4, 16)) and share(torch.zeros(200).as_strided((1, 4, 4, 16), (0, 16, 15, 1)))

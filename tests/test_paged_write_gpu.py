@@ -104,6 +104,23 @@ def test_layouts(pkg, device):
     _check(pkg, list(flat), _pools(device, 16, 4, 8, 64, dtype), table, positions)
 
 
+@pytest.mark.parametrize('tokens', [1, 3])
+def test_more_requests_than_a_grid_is_wide(pkg, device, tokens):
+    batch = 70001
+    keys, values = _rows(device, batch, 1, tokens, 4, BF16)
+    pools = _pools(device, batch + 5, 1, 4, 4, BF16)
+    table = torch.randperm(batch + 5, generator=torch.Generator().manual_seed(9))[:batch].to(torch.int32)[:, None].to(device)
+    positions = torch.arange(batch, device=device) % 3
+    want = [pool.clone() for pool in pools]
+    for t in range(tokens):
+        fits = positions + t < 4
+        for pool, rows in zip(want, (keys, values)):
+            pool[table[fits, 0].long(), 0, positions[fits] + t] = rows[fits, 0, t]
+    pkg.paged_write(keys, values, *pools, table, positions)
+    for pool, expected in zip(pools, want):
+        assert torch.equal(_bits(pool), _bits(expected))
+
+
 def test_special_values_are_copied_as_they_are(pkg, device):
     rows = torch.tensor([0x7fc1, 0xff81, 0x0001, 0x8000] * 16, dtype=torch.int32).to(torch.int16).view(BF16)
     rows = rows.view(1, 1, 1, 64).to(device)

@@ -5,6 +5,7 @@ float32 (pi u), by a few units of sincospi (4 u) and, from the float64 angle, by
 2 pi; a product and a sum round by u each: |x1| + |x2| times (8 + 3) u + 2 pi |turns| 2^-52, and half a
 step of the output, eps/2 |y| (and half the smallest subnormal, for fp16).  ``scaling`` multiplies both
 and rounds once more (u)."""
+import importlib
 import math
 
 import pytest
@@ -146,6 +147,20 @@ def test_in_place(pkg, device, sections):
         pkg.rotary_axes(q[:, :, :1].expand(3, 5, 16, 128), k, positions, sections, inplace=True)
 
 
+@pytest.mark.parametrize('views', [lambda f: (f[:, :, :16], f[:, :, 8:16]), lambda f: (f, f), lambda f: (f[:, :, :16], f[:, :, 15:20]),
+                                   lambda f: (f[:, :, :1].expand(3, 5, 16, 128), None)], ids=['part', 'same', 'one row', 'expanded'])
+def test_in_place_refuses_rows_that_overlap(pkg, device, views):
+    fused = _rows(device, 3, 5, 28, 128, BF16)
+    before = fused.clone()
+    q, k = views(fused)
+    positions = _positions(device, 3, 3, 5, 700)
+    with pytest.raises(ValueError):
+        pkg.rotary_axes(q, k, positions, (24, 20, 20), inplace=True)
+    assert torch.equal(fused, before)
+    got = pkg.rotary_axes(q, k, positions, (24, 20, 20))  # (fresh outputs: any views are fine)
+    assert torch.equal(got[0], pkg.rotary_axes(q.contiguous(), None, positions, (24, 20, 20))[0])
+
+
 def test_no_rows(pkg, device):
     q = torch.empty(0, 5, 4, 128, device=device)
     got, none = pkg.rotary_axes(q, None, torch.empty(3, 0, 5, dtype=torch.int64, device=device), (24, 20, 20))
@@ -180,6 +195,27 @@ def test_captured_call_follows_its_positions(pkg, device):
         graph.replay()
         torch.cuda.synchronize(device)
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_first_call_of_a_theta_under_capture(pkg, device):
+    """A graph forms the frequencies of a theta that no call has had, and leaves nothing for later calls."""
+    q = _rows(device, 4, 1, 16, 128, BF16)
+    positions = _positions(device, 3, 4, 1, 100)
+    table = importlib.import_module(pkg.__name__ + '.rotary')._TURNS
+    kept = dict(table)
+    graph = torch.cuda.CUDAGraph()
+    with torch.inference_mode(), torch.cuda.graph(graph):
+        out, _ = pkg.rotary_axes(q, None, positions, (24, 20, 20), theta=54321.5)
+    assert table.keys() == kept.keys()
+    for step in range(4):
+        positions.add_(step * 1000)
+        graph.replay()
+        torch.cuda.synchronize(device)
+        assert_within(out.cpu().double(), *rotated64(q, positions, (24, 20, 20), theta=54321.5))
+        _check(pkg, q, q, positions, (24, 20, 20), theta=54321.5)
+    for theta in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            pkg.rotary_axes(q, None, positions, (24, 20, 20), theta=theta)
 
 
 def test_a_layers_step(pkg, device):
