@@ -89,7 +89,8 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     0 ... positions[b] of request b, which its row of ``page_table`` (B, width) int32 finds in
     key_pages/value_pages (pages, Hkv, page_size, D), by any strides with unit-stride rows.
     Returns (B, 1, Hq, D); bf16, fp16 or fp32, head_dim 64 or 128, any number of query heads
-    that is a multiple of the KV heads.
+    that is a multiple of the KV heads.  Rows of the pools start at multiples of 16 bytes, and
+    there are at most 64512 requests times KV heads (times blocks of 16 query heads of one).
 
     ``mask``: SDPA-style, broadcastable to (B, 1, 1, K) with K at most ``width * page_size``:
     bool (True attends) or additive (bf16 / fp16 / fp32, added to the scaled scores in float32).
@@ -129,6 +130,8 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     else:
         _check_out(out, (batch, 1, q_heads, head_dim), dtype, query.device, 'paged attention')
         os = out.stride()
+        if any(n > 1 and s == 0 for n, s in zip(out.shape, os)):
+            raise ValueError('paged attention: rows of out must not share memory')
     if batch == 0:
         return out
     if query.data_ptr() % 16 or (qs[0] | qs[2]) * query.element_size() % 16:
@@ -211,6 +214,8 @@ class PagedArena:
         """Copy the rows of a prefill cache (``cache.layers[i].keys`` / ``.values``, (B, kv_heads,
         length, head_dim)) into the pages of their requests: row b's first ``lengths[b]`` (int32,
         device) positions, to positions 0 on."""
+        if len(cache.layers) != len(self.keys):
+            raise ValueError('the cache and the arena must have the same layers')
         start = torch.zeros(page_table.shape[0], device=page_table.device, dtype=torch.int64)
         for layer, keys, values in zip(cache.layers, self.keys, self.values):
             paged_write(layer.keys, layer.values, keys, values, page_table, start, lengths)

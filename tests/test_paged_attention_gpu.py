@@ -36,7 +36,7 @@ def test_one_request_of_any_length(pkg, device, length, dtype, width):
 
 
 @pytest.mark.parametrize('lengths', [[1] * 700, [70] * 300, [5] + [1500] * 3 + [0] * 5 + [64] * 200, [9000, 3, 1, 9000],
-                                     list(range(0, 520))], ids=['700x1', '300x70', 'mixed', 'two long', 'ramp'])
+                                     list(range(0, 520)), [i % 37 for i in range(9001)]], ids=['700x1', '300x70', 'mixed', 'two long', 'ramp', '9001'])
 def test_many_requests_share_the_card(pkg, device, lengths):
     p = problem(device, lengths, q_heads=4, kv_heads=2, seed=4)
     assert_within(run(pkg, p), *expected(p))
@@ -226,6 +226,8 @@ def test_refuses_what_it_cannot_read(pkg, device):
         odd = pool if pool.shape == p.key_pages.shape else pool.expand_as(pool)
         with pytest.raises(ValueError):
             pkg.paged_attention(p.query, odd, odd, p.table, p.positions)
+    with pytest.raises(ValueError):
+        run(pkg, p, out=torch.zeros(2, 1, 1, 128, dtype=BF16, device=device).expand(p.query.shape))
     wide = problem(device, [20], q_heads=8, kv_heads=8, width=96, seed=17)
     with pytest.raises(ValueError):
         run(pkg, wide)
