@@ -429,11 +429,22 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     const uint32_t each = (batch + 63) / 64;  // requests of a lane, one after the other
     uint32_t lengths = length_at(lane);       // of requests window + lane
     uint32_t stages = 0, pieces = 0, window = 0;
-    for (uint32_t i = 0; i < each; ++i) {
-        const uint32_t b = lane * each + i, r = stages_of(each == 1 ? lengths : length_at(b));
-        if (b >= batch) break;
+    auto count = [&](uint32_t r) {
         stages += r;
         pieces += (r + kLeastStages - 1) / kLeastStages;
+    };
+    if (each == 1) {
+        if ((uint32_t)lane < batch) count(stages_of(lengths));
+    } else {
+        constexpr uint32_t kFlight = 8;  // positions on their way at once (4096 requests: one 118 us, eight 116)
+        for (uint32_t i = 0; i < each; i += kFlight) {
+            uint32_t r[kFlight];
+#pragma unroll
+            for (uint32_t j = 0; j < kFlight; ++j) r[j] = stages_of(length_at(min(lane * each + i + j, batch - 1)));
+#pragma unroll
+            for (uint32_t j = 0; j < kFlight; ++j)
+                if (i + j < each && lane * each + i + j < batch) count(r[j]);
+        }
     }
     const uint32_t stages_to = scan(stages), pieces_to = scan(pieces);
     auto last_lane = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); };
