@@ -7,6 +7,7 @@ library is missing or a call is rejected, the wrappers raise.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -138,6 +139,16 @@ class RotaryAxesArgs(ctypes.Structure):
     ]
 
 
+def packer(structure):
+    """A function from the fields of ``structure``, in order, arrays spread out and null pointers 0, to
+    its bytes: 0.2 us where the constructor of one of 28 fields takes 1.1."""
+    codes = {c_i64: "q", c_vp: "P", ctypes.c_int32: "i", ctypes.c_float: "f"}
+    form = "".join(codes.get(kind) or f"{kind._length_}{codes[kind._type_]}" for _, kind in structure._fields_)
+    form = struct.Struct("@" + form)
+    assert form.size == ctypes.sizeof(structure)
+    return form.pack
+
+
 # Every exported entry point with its ctypes signature.
 SIGNATURES = {
     "q3t_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -226,7 +237,7 @@ def gpu_index(*tensors: torch.Tensor) -> int:
     """The index of the ROCm device that holds all tensors (``require_gpu`` for calls whose host time
     counts)."""
     index = tensors[0].get_device()
-    if index < 0 or tensors[0].device.type != "cuda":
+    if index < 0 or not tensors[0].is_cuda:
         raise ValueError("expected tensors on a ROCm GPU device")
     for t in tensors:
         if t.get_device() != index:
@@ -254,10 +265,24 @@ class on_device:
             self.guard.__exit__(*error)
 
 
-def launch(entry, args, index: int, what: str) -> None:
-    """An entry point of an argument structure and a stream, on device ``index``."""
+_packed = {}
+
+
+def packed(name: str):
+    """The entry point ``name``, taking the bytes of its argument structure (``packer``)."""
+    entry = _packed.get(name)
+    if entry is None:
+        entry = library()[name]  # a function object of its own, besides library()'s attribute
+        entry.restype, argtypes = SIGNATURES[name]
+        entry.argtypes = [c_vp] * len(argtypes)
+        _packed[name] = entry
+    return entry
+
+
+def launch(name: str, args: bytes, index: int, what: str) -> None:
+    """The entry point ``name`` of an argument structure and a stream, on device ``index``."""
     with on_device(index) as stream:
-        status = entry(args, stream)
+        status = packed(name)(args, stream)
     if status != Q3T_OK:
         check(status, what)
 

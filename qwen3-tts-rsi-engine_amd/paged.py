@@ -27,6 +27,8 @@ from transformers.cache_utils import Cache
 from . import _lib
 from .attention import _check_out, workspace
 
+_pack_attention = _lib.packer(_lib.PagedArgs)
+_pack_write = _lib.packer(_lib.PagedWriteArgs)
 _TYPES = {torch.bfloat16: _lib.Q3T_BF16, torch.float16: _lib.Q3T_F16, torch.float32: _lib.Q3T_F32}
 
 
@@ -76,12 +78,12 @@ def paged_write(keys, values, key_pages, value_pages, page_table, positions, len
         _lib.gpu_index(keys, lengths)
     if batch == 0 or tokens == 0:
         return
-    a = _lib.PagedWriteArgs(
+    _lib.launch('q3t_paged_write', _pack_write(
         batch, heads, tokens, width, keys.element_size(), keys.data_ptr(), values.data_ptr(),
         ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], key_pages.data_ptr(), value_pages.data_ptr(),
         kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], pages, page_size,
-        page_table.data_ptr(), table_width, ts, positions.data_ptr(), None if lengths is None else lengths.data_ptr())
-    _lib.launch(_lib.library().q3t_paged_write, a, device, 'paged write')
+        page_table.data_ptr(), table_width, ts, positions.data_ptr(), 0 if lengths is None else lengths.data_ptr()),
+        device, 'paged write')
 
 
 def paged_attention(query, key_pages, value_pages, page_table, positions, *, scale=None, mask=None, out=None):
@@ -112,7 +114,7 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
         raise ValueError('rows must be unit-stride along head_dim')
     device = _lib.gpu_index(query, key_pages, value_pages, page_table, positions)
     ctx = table_width * page_size
-    mask_fields = (None, 0, 0, 0)
+    mask_fields = (0, 0, 0, 0)
     if mask is not None:
         if mask.dtype not in _lib.DTYPE_CODES:
             raise ValueError('attention mask must be bool, bf16, fp16 or fp32')
@@ -137,19 +139,17 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     if query.data_ptr() % 16 or (qs[0] | qs[2]) * query.element_size() % 16:
         query = query.clone(memory_format=torch.contiguous_format)  # rows that 16-byte loads do not fit
         qs = query.stride()
-    a = _lib.PagedArgs(
+    fields = (
         batch, q_heads, kv_heads, head_dim, _TYPES[dtype], ctx, head_dim ** -0.5 if scale is None else scale, 0,
         query.data_ptr(), qs[0], qs[2], key_pages.data_ptr(), value_pages.data_ptr(),
         kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], pages, page_size,
         page_table.data_ptr(), table_width, ts, positions.data_ptr(), *mask_fields, out.data_ptr(), os[0], os[2])
-    lib = _lib.library()
-    need = lib.q3t_paged_workspace_bytes(a)
+    need = _lib.packed('q3t_paged_workspace_bytes')(_pack_attention(*fields, 0, 0))
     if need < 0:
         raise ValueError('paged attention: unsupported shape or dtype')
     with _lib.on_device(device) as stream:
         ws = workspace(query.device, need, stream)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        status = lib.q3t_paged_attention(a, stream)
+        status = _lib.packed('q3t_paged_attention')(_pack_attention(*fields, ws.data_ptr(), ws.numel()), stream)
     if status != _lib.Q3T_OK:
         _lib.check(status, 'paged attention')
     return out

@@ -74,6 +74,7 @@ def rope_tables(positions, head_dim, theta=DEFAULT_THETA, scaling=1.0, dtype=tor
     return cos, sin
 
 
+_pack_axes = _lib.packer(_lib.RotaryAxesArgs)
 _ROTARY_TYPES = {torch.bfloat16: _lib.Q3T_BF16, torch.float16: _lib.Q3T_F16, torch.float32: _lib.Q3T_F32}
 _TURNS = {}
 
@@ -184,10 +185,10 @@ def rotary_axes(query, key, positions, sections, *, interleaved=False, theta=DEF
             kos = (tokens * k_heads * width, k_heads * width, width)
     if batch == 0 or tokens == 0:
         return q_out, k_out
-    a = _lib.RotaryAxesArgs(
-        batch, tokens, q_heads, k_heads, width, _ROTARY_TYPES[dtype], axes, (_lib.c_i64 * 4)(*sections), bool(interleaved),
+    _lib.launch('q3t_rotary_axes', _pack_axes(
+        batch, tokens, q_heads, k_heads, width, _ROTARY_TYPES[dtype], axes, *sections, *(0,) * (4 - axes), bool(interleaved),
         scaling, turns.data_ptr(), positions.data_ptr(), ps[0], ps[1], ps[2],
-        query.data_ptr(), None if key is None else key.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
-        q_out.data_ptr(), None if key is None else k_out.data_ptr(), qos[0], qos[1], qos[2], kos[0], kos[1], kos[2])
-    _lib.launch(_lib.library().q3t_rotary_axes, a, device, 'rotary axes')
+        query.data_ptr(), 0 if key is None else key.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
+        q_out.data_ptr(), 0 if key is None else k_out.data_ptr(), qos[0], qos[1], qos[2], kos[0], kos[1], kos[2]),
+        device, 'rotary axes')
     return q_out, k_out
