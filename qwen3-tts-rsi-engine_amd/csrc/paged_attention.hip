@@ -32,11 +32,19 @@ namespace q3t {
 namespace paged {
 
 constexpr int kColumns = 16;           // query heads of a workgroup: columns of a product
-constexpr uint32_t kLeastStages = 8;   // stages that are not shared out
-constexpr uint32_t kRunCost = 8;       // stages that the end of a run costs as much as
+// Stages that are not shared out: two of each wave of four.  us with 4 / 8 / 16: one request of 300 keys 9.5 /
+// 10.2 / 10.2, of 100 8.8 / 7.7 / -, of 4000 13.4 / 12.9 / -, 4 of 300..1000 11.1 / 10.7 / -, 3 of 5000..9000
+// with one KV head 22.5 / 20.8 / 20.8, 8 of 100..2000 14.0 / 14.0 / 15.0.
+constexpr uint32_t kLeastStages = 8;
+// Stages that the end of a run of W waves costs as much as.  us with 1 / 8 / 24 for four waves: 200 requests of
+// 10..400 keys 44 / 27.2 / 28.3, 128 of 32..511 42 / 32.9 / 34.6; with 8 / 16 / 24 for eight: 64 of 64..1023
+// 31.6 / 30.8 / 31.2, 128 of 100..4095 174.8 / 174.4 / 176.2.
+constexpr uint32_t run_cost(int waves) { return 2 * waves; }
 constexpr int kCounters = 65536;       // counter words in front of a decode workspace: of the pairs,
 constexpr int kPairs = kCounters - 1024;  // then of the state slots, two for each of up to 512 workgroups
-constexpr uint32_t kTogether = 16;     // parts that are merged in one step
+// Parts that are merged in one step.  us with 4 / 16 / all: one request of 65000 keys 35.6 / 33.9 / 49.4, 8 of
+// 100..2000 15.9 / 14.0 / 14.1.
+constexpr uint32_t kTogether = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -101,7 +109,8 @@ Q3T_DEVICE uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_read
                  OPCODE " %3, " ADDRESS " offset:2048" POLICY "\n\t"                               \
                  OPCODE " %4, " ADDRESS " offset:3*1024" POLICY                                      \
                  :: "s"(base), "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]) __VA_ARGS__ : "memory", "m0")
-// from a pointer per lane
+// Rows are read once: the non-temporal policy (64 requests of 64..1023 keys without it 35.1 us, with it 32.8;
+// 128 of 100..4095 194.9, 176.2).  From a pointer per lane:
 Q3T_DEVICE void load_rows(const uint64_t *p, uint32_t base) { Q3T_LOAD4("global_load_lds_dwordx4", "off", " nt"); }
 // from an offset per lane into a resource; past its range zeros are written without a memory access
 #define Q3T_RSRC , "s"(rsrc)
@@ -449,7 +458,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     const uint32_t stages_to = scan(stages), pieces_to = scan(pieces);
     auto last_lane = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); };
     const Sharing sh = sharing(batch * p.heads, last_lane(stages_to) * p.heads, last_lane(pieces_to) * p.heads,
-                               kLeastStages, kRunCost, p.by_grid);
+                               kLeastStages, run_cost(W), p.by_grid);
     Cursor at = {};
     at.x = blockIdx.x * sh.share;
     if (at.x >= sh.total) return;
@@ -738,10 +747,11 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
             score(s0);
             s0 = s1;
             ++n;
-            // Of two waves on a SIMD the older one's loads go first, and the younger one (of the later half
-            // of the workgroups, as they are dealt out, or of a workgroup's waves) would end after it: it
-            // goes first on every second stage.
-            if (W == 8 ? wave >= 4 : blockIdx.x >= 256) {
+            // Of two workgroups on a CU the older one's loads go first, and the younger one (of the later half, as
+            // they are dealt out) would end after it: it goes first on every second stage (200 requests of
+            // 10..400 keys 28.0 -> 27.2 us).  Not in one workgroup of eight waves, where all wait for the
+            // last (64 of 64..1023 with it 33.0, without 31.6).
+            if (W == 4 && blockIdx.x >= 256) {
                 if (n & 1) __builtin_amdgcn_s_setprio(2);
                 else __builtin_amdgcn_s_setprio(0);
             }
@@ -871,8 +881,8 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 }
 
 // Eight waves a workgroup instead of four: half as many shares, so half as many cut pairs, but more
-// waves with nothing to do in a short one.  us, four / eight: 128 requests of 100..4095 keys 180 / 174.5, 4
-// of 16000 53.5 / 50.9, 64 of 64..1023 33.4 / 31.6, 32 of 100..2000 31.8 / 31.1; 8 of 100..2000 14.3 / 16.6,
+// waves with nothing to do in a short one.  us, four / eight: 128 requests of 100..4095 keys 180 / 174, 4
+// of 16000 53.5 / 49.9, 64 of 64..1023 33.4 / 30.8, 32 of 100..2000 31.8 / 30.6; 8 of 100..2000 14.3 / 16.6,
 // 128 of 32..511 32.5 / 37.8, 64 of 64 9.3 / 10.6, 200 of 10..400 27 / 43.  The host sees capacities, not
 // lengths: eight from 768 keys a request and 24576 stages in all, for up to 1024 pairs, where short
 // requests cost little.
@@ -881,7 +891,7 @@ constexpr int64_t kLongRequest = 768, kManyStages = 24576, kFewPairs = 1024;
 template <typename T, int D>
 struct Launch {
     typedef Shape<T, D> S;
-    static int64_t stages(const q3t_paged_args *a, int64_t pairs) { return pairs * ((a->ctx + S::keys - 1) / S::keys + kRunCost); }
+    static int64_t stages(const q3t_paged_args *a, int64_t pairs, int waves) { return pairs * ((a->ctx + S::keys - 1) / S::keys + run_cost(waves)); }
     // rows of a stage as one range: whole pages, rows that do not overlap, 32-bit offsets
     static bool whole(const q3t_paged_args *a) {
         const int64_t es = sizeof(T), most = ((int64_t)1 << 30) / S::keys;
@@ -889,7 +899,7 @@ struct Launch {
                a->kp_stride_t * es < most && a->vp_stride_t * es < most;
     }
     static bool eight(const q3t_paged_args *a, int64_t pairs) {
-        return S::row < 512 && whole(a) && a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs) >= kManyStages;
+        return S::row < 512 && whole(a) && a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
     }
     static int64_t workgroups(const q3t_paged_args *a, int64_t pairs) {
         const int64_t stages = (a->ctx + S::keys - 1) / S::keys, pieces = pairs * ((stages + kLeastStages - 1) / kLeastStages);
@@ -939,7 +949,7 @@ static int sizes_of(const q3t_paged_args *a, Sizes &z) {
     z.pairs = a->batch * a->kv_heads * z.blocks;
     z.columns = z.group < kColumns ? z.group : kColumns;
     if (z.pairs > kPairs) return Q3T_EUNSUPPORTED;  // a counter each
-    if (with(a, [&](auto l) { return l.stages(a, z.pairs); }) >= INT32_MAX / 2) return Q3T_EUNSUPPORTED;
+    if (with(a, [&](auto l) { return l.stages(a, z.pairs, 8); }) >= INT32_MAX / 2) return Q3T_EUNSUPPORTED;
     z.workgroups = with(a, [&](auto l) { return l.workgroups(a, z.pairs); });
     z.workspace = kCounters * 4 + 2 * z.workgroups * z.columns * (a->head_dim + 2) * 4;
     return Q3T_OK;
