@@ -881,12 +881,13 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 }
 
 // Eight waves a workgroup instead of four: half as many shares, so half as many cut pairs, but more
-// waves with nothing to do in a short one.  us, four / eight: 128 requests of 100..4095 keys 180 / 174, 4
-// of 16000 53.5 / 49.9, 64 of 64..1023 33.4 / 30.8, 32 of 100..2000 31.8 / 30.6; 8 of 100..2000 14.3 / 16.6,
-// 128 of 32..511 32.5 / 37.8, 64 of 64 9.3 / 10.6, 200 of 10..400 27 / 43.  The host sees capacities, not
-// lengths: eight from 768 keys a request and 24576 stages in all, for up to 1024 pairs, where short
-// requests cost little.
-constexpr int64_t kLongRequest = 768, kManyStages = 24576, kFewPairs = 1024;
+// waves with nothing to do in a short one.  us, four / eight: 128 requests of 100..4095 keys 180 / 174, 64
+// of 64..1023 33.4 / 30.8, 64 of 64..700 26.2 / 24.7, 40 of 64..1023 25.5 / 23.4, one of 65000 33.1 / 31.7, 8 of
+// 1000..4000 24.7 / 24.3; 96 of 64..600 31.0 / 31.4, 24 of 64..1023 18.7 / 19.0, 8 of 100..2000 14.1 / 14.7, 64 of
+// 512 27.0 / 28.2, 128 of 32..511 32.7 / 34.6, 512 of 20..200 32.8 / 41.6.  The host sees capacities, not
+// lengths: eight from 640 keys a request and 15000 stages and run ends in all, for up to 1024 pairs, where
+// short requests cost little.
+constexpr int64_t kLongRequest = 640, kManyStages = 15000, kFewPairs = 1024;
 
 template <typename T, int D>
 struct Launch {
