@@ -32,10 +32,10 @@ namespace q3t {
 namespace paged {
 
 constexpr int kColumns = 16;           // query heads of a workgroup: columns of a product
-// Stages that are not shared out: two of each wave of four.  us with 4 / 8 / 16: one request of 300 keys 9.5 /
-// 10.2 / 10.2, of 100 8.8 / 7.7 / -, of 4000 13.4 / 12.9 / -, 4 of 300..1000 11.1 / 10.7 / -, 3 of 5000..9000
-// with one KV head 22.5 / 20.8 / 20.8, 8 of 100..2000 14.0 / 14.0 / 15.0.
-constexpr uint32_t kLeastStages = 8;
+// Stages that are not shared out: two of each wave of four, or a whole short request for eight.  us with 4 / 8 /
+// 16 for four waves: one request of 300 keys 9.5 / 10.2 / 10.2, of 100 8.8 / 7.7 / -, of 4000 13.4 / 12.9 / -, 4
+// of 300..1000 11.1 / 10.7 / -, 3 of 5000..9000 with one KV head 22.5 / 20.8 / 20.8, 8 of 100..2000 14.0 / 14.0 / 15.0.
+constexpr uint32_t least_stages(int waves) { return waves == 8 ? 32 : 8; }
 // Stages that the end of a run of W waves costs as much as.  us with 1 / 8 / 24 for four waves: 200 requests of
 // 10..400 keys 44 / 27.2 / 28.3, 128 of 32..511 42 / 32.9 / 34.6; with 8 / 16 / 24 for eight: 64 of 64..1023
 // 31.6 / 30.8 / 31.2, 128 of 100..4095 174.8 / 174.4 / 176.2.
@@ -425,6 +425,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     typedef Shape<T, D> S;
     typedef Tile<T, D> Products;
     constexpr int LOADS = 2 * S::loads, kThreads = 64 * W;
+    constexpr uint32_t kLeast = least_stages(W);
     __shared__ Lds<T, D, MASK, W> s;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = (int)uniform(tid >> 6);
@@ -440,7 +441,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     uint32_t stages = 0, pieces = 0, window = 0;
     auto count = [&](uint32_t r) {
         stages += r;
-        pieces += (r + kLeastStages - 1) / kLeastStages;
+        pieces += (r + kLeast - 1) / kLeast;
     };
     if (each == 1) {
         if ((uint32_t)lane < batch) count(stages_of(lengths));
@@ -458,7 +459,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     const uint32_t stages_to = scan(stages), pieces_to = scan(pieces);
     auto last_lane = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); };
     const Sharing sh = sharing(batch * p.heads, last_lane(stages_to) * p.heads, last_lane(pieces_to) * p.heads,
-                               kLeastStages, run_cost(W), p.by_grid);
+                               kLeast, run_cost(W), p.by_grid);
     Cursor at = {};
     at.x = blockIdx.x * sh.share;
     if (at.x >= sh.total) return;
@@ -472,7 +473,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
             return (uint32_t)j;
         };
         uint32_t from = 0;
-        at.b = holder(sh.unit > 1 ? pieces_to * kLeastStages : stages_to + sh.cost * min((lane + 1) * each, batch), from);
+        at.b = holder(sh.unit > 1 ? pieces_to * kLeast : stages_to + sh.cost * min((lane + 1) * each, batch), from);
         if (each > 1) {
             window = at.b * each;
             while (true) {  // (once, for up to 4096 requests)
@@ -880,14 +881,19 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     }
 }
 
-// Eight waves a workgroup instead of four: half as many shares, so half as many cut pairs, but more
-// waves with nothing to do in a short one.  us, four / eight: 128 requests of 100..4095 keys 180 / 174, 64
-// of 64..1023 33.4 / 30.8, 64 of 64..700 26.2 / 24.7, 40 of 64..1023 25.5 / 23.4, one of 65000 33.1 / 31.7, 8 of
-// 1000..4000 24.7 / 24.3; 96 of 64..600 31.0 / 31.4, 24 of 64..1023 18.7 / 19.0, 8 of 100..2000 14.1 / 14.7, 64 of
-// 512 27.0 / 28.2, 128 of 32..511 32.7 / 34.6, 512 of 20..200 32.8 / 41.6.  The host sees capacities, not
-// lengths: eight from 640 keys a request and 15000 stages and run ends in all, for up to 1024 pairs, where
-// short requests cost little.
+// Eight waves a workgroup instead of four, by what the host sees: capacities, not lengths.
+//   * Many stages: half as many shares, so half as many cut pairs, but more waves with nothing to do in a
+//     short one.  us, four / eight: 128 requests of 100..4095 keys 180 / 174, 64 of 64..1023 33.4 / 30.8, 64 of
+//     64..700 26.2 / 24.7, 40 of 64..1023 25.5 / 23.4, one of 65000 33.1 / 31.7, 8 of 1000..4000 24.7 / 24.3; 96 of
+//     64..600 31.0 / 31.4, 24 of 64..1023 18.7 / 19.0, 8 of 100..2000 14.1 / 14.7, 64 of 512 27.0 / 28.2, 128 of
+//     32..511 32.7 / 34.6, 512 of 20..200 32.8 / 41.6.  From 640 keys a request and 15000 stages and run
+//     ends in all, for up to 1024 pairs, where short requests cost little.
+//   * Few short pairs: one workgroup attends a whole pair, and no states pass through memory.  us, four /
+//     eight, 8 KV heads: one request of 100 keys 7.7 / 7.2, of 300 10.2 / 8.7, of 400 10.3 / 9.6, of 500 10.4 /
+//     10.4, of 600 10.2 / 11.5; 8 of 300 10.5 / 9.8, 16 of 400 13.1 / 11.4, 32 of 300 16.4 / 12.4, 32 of 500 17.9 /
+//     16.6, 48 of 200 16.4 / 15.8, 64 of 64 9.0 / 10.0.  Up to 448 keys and a pair for each CU.
 constexpr int64_t kLongRequest = 640, kManyStages = 15000, kFewPairs = 1024;
+constexpr int64_t kShortRequest = 448, kOnePairEach = 256;
 
 template <typename T, int D>
 struct Launch {
@@ -900,11 +906,15 @@ struct Launch {
                a->kp_stride_t * es < most && a->vp_stride_t * es < most;
     }
     static bool eight(const q3t_paged_args *a, int64_t pairs) {
-        return S::row < 512 && whole(a) && a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
+        const bool many = a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
+        const bool few = a->ctx <= kShortRequest && pairs <= kOnePairEach;
+        return S::row < 512 && whole(a) && (many || few);
     }
     static int64_t workgroups(const q3t_paged_args *a, int64_t pairs) {
-        const int64_t stages = (a->ctx + S::keys - 1) / S::keys, pieces = pairs * ((stages + kLeastStages - 1) / kLeastStages);
-        const int64_t most = eight(a, pairs) ? Workgroups<T, D, 8>::count : Workgroups<T, D, 4>::count;
+        const bool wide = eight(a, pairs);
+        const int64_t least = least_stages(wide ? 8 : 4), stages = (a->ctx + S::keys - 1) / S::keys;
+        const int64_t pieces = pairs * ((stages + least - 1) / least);
+        const int64_t most = wide ? Workgroups<T, D, 8>::count : Workgroups<T, D, 4>::count;
         return pieces < most ? pieces : most;
     }
     static void run(const q3t_paged_args *a, int64_t pairs, const Params &p, uint32_t blocks, hipStream_t s) {

@@ -64,6 +64,21 @@ def test_launches_that_fill_the_card(pkg, device, lengths):
     assert_within(run(pkg, p), *expected(p))
 
 
+@pytest.mark.parametrize('masked', [False, True])
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (BF16, 64), (F16, 128), (F16, 64), (F32, 64)], ids=str)
+@pytest.mark.parametrize('heads', [(16, 8), (20, 1)], ids=str)
+def test_short_requests_of_a_workgroup_each(pkg, device, masked, dtype, width, heads):
+    """Tables of 448 rows, of which a workgroup attends any number for itself."""
+    p = problem(device, [0, 1, 15, 16, 17, 127, 128, 129, 130, 255, 257, 300, 385, 447, 448], q_heads=heads[0], kv_heads=heads[1],
+                width=width, dtype=dtype, table_width=14, page=32, seed=28)
+    mask = None
+    if masked:
+        mask = torch.ones(len(p.lengths), 1, 1, 448, dtype=torch.bool, device=device)
+        mask[:, :, :, 2::5] = False
+        mask[4] = False
+    assert_within(run(pkg, p, mask=mask), *expected(p, mask=mask))
+
+
 @pytest.mark.parametrize('dtype', [BF16, F32], ids=str)
 def test_positions_outside_the_table_attend_nothing(pkg, device, dtype):
     p = problem(device, [40, 41, 42, 43, 44], dtype=dtype, seed=6)
