@@ -891,9 +891,11 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 //   * Few short pairs: one workgroup attends a whole pair, and no states pass through memory.  us, four /
 //     eight, 8 KV heads: one request of 100 keys 7.7 / 7.2, of 300 10.2 / 8.7, of 400 10.3 / 9.6, of 500 10.4 /
 //     10.4, of 600 10.2 / 11.5; 8 of 300 10.5 / 9.8, 16 of 400 13.1 / 11.4, 32 of 300 16.4 / 12.4, 32 of 500 17.9 /
-//     16.6, 48 of 200 16.4 / 15.8, 64 of 64 9.0 / 10.0.  Up to 448 keys and a pair for each CU.
+//     16.6, 48 of 200 16.4 / 15.8, 64 of 64 9.0 / 10.0.  With enough pairs for half of the CUs, longer ones too:
+//     24 of 1..700 17.3 / 14.7, 16 of 600 15.9 / 14.8, 32 of 600 20.3 / 18.8, 32 of 800 22.6 / 22.5, 32 of 1000 26.6 /
+//     27.0; 12 of 1..700 12.4 / 12.8.  Up to 448 keys and a pair for each CU; up to 800 for half as many on.
 constexpr int64_t kLongRequest = 640, kManyStages = 15000, kFewPairs = 1024;
-constexpr int64_t kShortRequest = 448, kOnePairEach = 256;
+constexpr int64_t kShortRequest = 448, kMiddleRequest = 800, kCUs = 256;
 
 template <typename T, int D>
 struct Launch {
@@ -907,7 +909,7 @@ struct Launch {
     }
     static bool eight(const q3t_paged_args *a, int64_t pairs) {
         const bool many = a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
-        const bool few = a->ctx <= kShortRequest && pairs <= kOnePairEach;
+        const bool few = pairs <= kCUs && a->ctx <= (pairs >= kCUs / 2 ? kMiddleRequest : kShortRequest);
         return S::row < 512 && whole(a) && (many || few);
     }
     static int64_t workgroups(const q3t_paged_args *a, int64_t pairs) {

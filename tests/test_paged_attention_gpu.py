@@ -64,6 +64,12 @@ def test_launches_that_fill_the_card(pkg, device, lengths):
     assert_within(run(pkg, p), *expected(p))
 
 
+@pytest.mark.parametrize('lengths', [[800] * 16, [n % 801 for n in range(0, 24 * 331, 331)]], ids=['equal', 'ragged'])
+def test_pairs_for_more_than_half_of_the_card(pkg, device, lengths):
+    p = problem(device, lengths, q_heads=16, kv_heads=8, table_width=50, page=16, seed=29)
+    assert_within(run(pkg, p), *expected(p))
+
+
 @pytest.mark.parametrize('masked', [False, True])
 @pytest.mark.parametrize('dtype,width', [(BF16, 128), (BF16, 64), (F16, 128), (F16, 64), (F32, 64)], ids=str)
 @pytest.mark.parametrize('heads', [(16, 8), (20, 1)], ids=str)
