@@ -32,10 +32,11 @@ namespace q3t {
 namespace paged {
 
 constexpr int kColumns = 16;           // query heads of a workgroup: columns of a product
-// Stages that are not shared out: two of each wave of four, or a whole short request for eight.  us with 4 / 8 /
-// 16 for four waves: one request of 300 keys 9.5 / 10.2 / 10.2, of 100 8.8 / 7.7 / -, of 4000 13.4 / 12.9 / -, 4
-// of 300..1000 11.1 / 10.7 / -, 3 of 5000..9000 with one KV head 22.5 / 20.8 / 20.8, 8 of 100..2000 14.0 / 14.0 / 15.0.
-constexpr uint32_t least_stages(int waves) { return waves == 8 ? 32 : 8; }
+// Stages that are not shared out, as a power of two: two of each wave, but a short request's all where it has a
+// workgroup of eight waves (below).  us with 4 / 8 / 16 for four waves: one request of 300 keys 9.5 / 10.2 /
+// 10.2, of 100 8.8 / 7.7 / -, of 4000 13.4 / 12.9 / -, 4 of 300..1000 11.1 / 10.7 / -, 8 of 100..2000 14.0 / 14.0 /
+// 15.0; with 16 / 32 for eight: one of 300 10.3 / 8.8, one of 1000 with one KV head and 16 others 11.8 / 13.7.
+constexpr uint32_t kLogLeast4 = 3, kLogLeast8 = 4, kLogLeastShort = 5;
 // Stages that the end of a run of W waves costs as much as.  us with 1 / 8 / 24 for four waves: 200 requests of
 // 10..400 keys 44 / 27.2 / 28.3, 128 of 32..511 42 / 32.9 / 34.6; with 8 / 16 / 24 for eight: 64 of 64..1023
 // 31.6 / 30.8 / 31.2, 128 of 100..4095 174.8 / 174.4 / 176.2.
@@ -57,7 +58,7 @@ struct Params {
     uint32_t o_sb, o_sh, m_sb, m_st, table_sb;                      // elements
     int32_t mask_dtype, vec_out;
     uint32_t pages, group, heads, blocks;       // heads: pairs of a request; blocks: of a KV head
-    uint32_t columns;                                  // of a state
+    uint32_t columns, log_least;                       // of a state; of eight waves
     Divisor by_page, by_grid;
     float scale;                                       // unmasked: times log2(e)
 };
@@ -425,7 +426,6 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     typedef Shape<T, D> S;
     typedef Tile<T, D> Products;
     constexpr int LOADS = 2 * S::loads, kThreads = 64 * W;
-    constexpr uint32_t kLeast = least_stages(W);
     __shared__ Lds<T, D, MASK, W> s;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = (int)uniform(tid >> 6);
@@ -436,12 +436,13 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         return pos >= 0 && pos < (int64_t)ctx ? (uint32_t)pos + 1 : 0u;
     };
     auto stages_of = [&](uint32_t length) { return max(1u, (length + S::keys - 1) >> S::log_keys); };
+    const uint32_t log_least = W == 4 ? kLogLeast4 : p.log_least, least = 1u << log_least;
     const uint32_t each = (batch + 63) / 64;  // requests of a lane, one after the other
     uint32_t lengths = length_at(lane);       // of requests window + lane
     uint32_t stages = 0, pieces = 0, window = 0;
     auto count = [&](uint32_t r) {
         stages += r;
-        pieces += (r + kLeast - 1) / kLeast;
+        pieces += (r + least - 1) >> log_least;
     };
     if (each == 1) {
         if ((uint32_t)lane < batch) count(stages_of(lengths));
@@ -459,7 +460,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     const uint32_t stages_to = scan(stages), pieces_to = scan(pieces);
     auto last_lane = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); };
     const Sharing sh = sharing(batch * p.heads, last_lane(stages_to) * p.heads, last_lane(pieces_to) * p.heads,
-                               kLeast, run_cost(W), p.by_grid);
+                               least, run_cost(W), p.by_grid);
     Cursor at = {};
     at.x = blockIdx.x * sh.share;
     if (at.x >= sh.total) return;
@@ -473,7 +474,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
             return (uint32_t)j;
         };
         uint32_t from = 0;
-        at.b = holder(sh.unit > 1 ? pieces_to * kLeast : stages_to + sh.cost * min((lane + 1) * each, batch), from);
+        at.b = holder(sh.unit > 1 ? pieces_to * least : stages_to + sh.cost * min((lane + 1) * each, batch), from);
         if (each > 1) {
             window = at.b * each;
             while (true) {  // (once, for up to 4096 requests)
@@ -894,8 +895,14 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 //     16.6, 48 of 200 16.4 / 15.8, 64 of 64 9.0 / 10.0.  With enough pairs for half of the CUs, longer ones too:
 //     24 of 1..700 17.3 / 14.7, 16 of 600 15.9 / 14.8, 32 of 600 20.3 / 18.8, 32 of 800 22.6 / 22.5, 32 of 1000 26.6 /
 //     27.0; 12 of 1..700 12.4 / 12.8.  Up to 448 keys and a pair for each CU; up to 800 for half as many on.
+//   * Groups of more than 8 query heads, whose states are large: half as many parts.  us, four / eight: 16
+//     heads on one KV head, one request of 1000 keys 12.6 / 11.7, of 8000 18.8 / 16.4, of 60000 31.6 / 21.0, 8 of
+//     2000 16.5 / 13.2, 128 of 64..1023 20.5 / 19.1, 32 of 4000 26.1 / 22.3; 256 of 100..1000 24.8 / 25.2, 512 of
+//     20..200 20.1 / 20.4, 300 of 10..60 10.1 / 13.9.  From 192 keys on.  Groups of 8 lose as often (one of
+//     1000 and two KV heads 10.7 / 11.8, of 4000 and four 14.4 / 13.1).
 constexpr int64_t kLongRequest = 640, kManyStages = 15000, kFewPairs = 1024;
 constexpr int64_t kShortRequest = 448, kMiddleRequest = 800, kCUs = 256;
+constexpr int64_t kWideGroup = 8, kWideRequest = 192;
 
 template <typename T, int D>
 struct Launch {
@@ -907,14 +914,20 @@ struct Launch {
         return a->page_size % S::keys == 0 && a->kp_stride_t * es >= S::row && a->vp_stride_t * es >= S::row &&
                a->kp_stride_t * es < most && a->vp_stride_t * es < most;
     }
+    static bool few(const q3t_paged_args *a, int64_t pairs) {
+        return pairs <= kCUs && a->ctx <= (pairs >= kCUs / 2 ? kMiddleRequest : kShortRequest);
+    }
     static bool eight(const q3t_paged_args *a, int64_t pairs) {
         const bool many = a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
-        const bool few = pairs <= kCUs && a->ctx <= (pairs >= kCUs / 2 ? kMiddleRequest : kShortRequest);
-        return S::row < 512 && whole(a) && (many || few);
+        const bool wide = a->q_heads / a->kv_heads > kWideGroup && a->ctx >= kWideRequest;
+        return S::row < 512 && whole(a) && (many || few(a, pairs) || wide);
+    }
+    static uint32_t log_least(const q3t_paged_args *a, int64_t pairs) {
+        return !eight(a, pairs) ? kLogLeast4 : few(a, pairs) ? kLogLeastShort : kLogLeast8;
     }
     static int64_t workgroups(const q3t_paged_args *a, int64_t pairs) {
         const bool wide = eight(a, pairs);
-        const int64_t least = least_stages(wide ? 8 : 4), stages = (a->ctx + S::keys - 1) / S::keys;
+        const int64_t least = (int64_t)1 << log_least(a, pairs), stages = (a->ctx + S::keys - 1) / S::keys;
         const int64_t pieces = pairs * ((stages + least - 1) / least);
         const int64_t most = wide ? Workgroups<T, D, 8>::count : Workgroups<T, D, 4>::count;
         return pieces < most ? pieces : most;
@@ -1024,6 +1037,7 @@ extern "C" int q3t_paged_attention(const q3t_paged_args *a, void *stream) {
     p.group = (uint32_t)z.group; p.blocks = (uint32_t)z.blocks;
     p.heads = (uint32_t)(a->kv_heads * z.blocks);
     p.columns = (uint32_t)z.columns;
+    p.log_least = with(a, [&](auto l) { return l.log_least(a, z.pairs); });
     p.by_page = divisor((uint32_t)a->page_size);
     p.by_grid = divisor((uint32_t)z.workgroups);
     p.scale = a->mask ? a->scale : a->scale * kLog2e;

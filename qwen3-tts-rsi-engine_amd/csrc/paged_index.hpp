@@ -40,13 +40,13 @@ Q3T_BOTH uint32_t divide(uint32_t n, const Divisor &v) {
 //     merge, the output), and the shares are equal.
 
 struct Sharing {
-    uint32_t unit, cost;  // places of a pair: a multiple of unit, and cost more
+    uint32_t unit, cost;  // places of a pair: a multiple of unit (a power of two), and cost more
     uint32_t share;       // places of a workgroup
     uint32_t total;       // places in all
 };
 
 // From the number of pairs, their stages (fewer than 2^30 together), and their pieces of `least`
-// stages.
+// stages, a power of two.
 Q3T_BOTH Sharing sharing(uint32_t pairs, uint32_t stages, uint32_t pieces, uint32_t least, uint32_t cost, const Divisor &workgroups) {
     if (pieces <= workgroups.d) return {least, 0u, least, pieces * least};
     const uint32_t total = stages + cost * pairs;
@@ -54,7 +54,7 @@ Q3T_BOTH Sharing sharing(uint32_t pairs, uint32_t stages, uint32_t pieces, uint3
 }
 
 Q3T_BOTH uint32_t places(uint32_t stages, const Sharing &s) {
-    return (s.unit == 1 ? stages : (stages + s.unit - 1) / s.unit * s.unit) + s.cost;
+    return ((stages + s.unit - 1) & ~(s.unit - 1)) + s.cost;
 }
 
 // Where a workgroup is on the line: place x, `left` places to go, at place `off` of pair (b, head).

@@ -64,6 +64,21 @@ def test_launches_that_fill_the_card(pkg, device, lengths):
     assert_within(run(pkg, p), *expected(p))
 
 
+@pytest.mark.parametrize('masked', [False, True])
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (F16, 128), (BF16, 64), (F32, 64)], ids=str)
+@pytest.mark.parametrize('heads', [(16, 1), (22, 2), (48, 1)], ids=str)
+def test_large_groups_over_long_requests(pkg, device, masked, dtype, width, heads):
+    """Many parts of states of up to 16 rows, merged in two steps."""
+    lengths = [9000, 3, 0, 20001, 190, 700]
+    p = problem(device, lengths, q_heads=heads[0], kv_heads=heads[1], width=width, dtype=dtype, page=32, seed=30)
+    mask = None
+    if masked:
+        mask = torch.ones(len(lengths), 1, 1, 20001, dtype=torch.bool, device=device)
+        mask[:, :, :, 5::11] = False
+        mask[3, :, :, 4000:8000] = False
+    assert_within(run(pkg, p, mask=mask), *expected(p, mask=mask))
+
+
 @pytest.mark.parametrize('lengths', [[800] * 16, [n % 801 for n in range(0, 24 * 331, 331)]], ids=['equal', 'ragged'])
 def test_pairs_for_more_than_half_of_the_card(pkg, device, lengths):
     p = problem(device, lengths, q_heads=16, kv_heads=8, table_width=50, page=16, seed=29)
