@@ -10,9 +10,12 @@
 // only what is left after whole turns goes on to sincospi in 32: an angle kept in 32 bits would
 // be off by radians at far positions.  Products and sums are float32, and each element is rounded
 // once, to nearest even.
-// Bound by HBM (every row read and written once: 16396 tokens of 32 heads of 128, 269 MB, 49 us, 5.5
-// TB/s; one row of a thread on its way at a time 60), by the launch for a decode step (64 tokens 3.5
-// us); the first rows are on their way while the angles are formed.
+// Bound by HBM (every row read and written once: 16396 tokens of 32 heads of 128, 269 MB, 57 us, 4.7
+// TB/s, and 49 where the outputs' memory is in the caches; one row of a thread on its way at a time 65, four
+// 57), by the launch for a decode step (64 tokens 3.5 us); the first rows are on their way while the
+// angles are formed.  Rows are loaded with the non-temporal policy and stored with the plain one: whoever
+// reads the outputs next finds more of them in the caches (with a copy of both outputs behind it 97 us;
+// plain loads 120, non-temporal stores too 109).
 #include "paged_index.hpp"
 #include "q3t_common.hpp"
 
@@ -115,7 +118,16 @@ __global__ void __launch_bounds__(kThreads) rotary_axes_kernel(Params p) {
         it.y = r.y + b * r.y_sb + s * r.y_ss + h * r.y_sh + element * sizeof(T);
         return it;
     };
+    typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
     typedef std::conditional_t<VEC, U4, T> Word;
+    auto load_word = [](const char *x) {
+        if constexpr (VEC) {
+            const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(x));
+            return U4{v[0], v[1], v[2], v[3]};
+        } else {
+            return *reinterpret_cast<const T *>(x);
+        }
+    };
     const uint32_t items = count * p.heads * p.units, apart = p.half * sizeof(T);
     Item it[kFlight];
     Word a[kFlight], b[kFlight];
@@ -125,8 +137,8 @@ __global__ void __launch_bounds__(kThreads) rotary_axes_kernel(Params p) {
             const uint32_t i = first_item + j * kThreads;
             if (i >= items) break;
             it[j] = item_of(i);
-            a[j] = *reinterpret_cast<const Word *>(it[j].x);
-            if (it[j].unit < p.rotated) b[j] = *reinterpret_cast<const Word *>(it[j].x + apart);
+            a[j] = load_word(it[j].x);
+            if (it[j].unit < p.rotated) b[j] = load_word(it[j].x + apart);
         }
     };
     load(threadIdx.x);
