@@ -14,12 +14,14 @@
 //     (paged_index.hpp), whatever the requests' lengths; its waves find their place by adding up all
 //     requests' stages.  A pair that lies in several shares leaves its parts' states in the
 //     workspace, and the workgroup that arrives last merges them, in the parts' order.
+//     Where no pair can have more than one share a workgroup takes the pair of its own number, and its page
+//     numbers are on their way together with the position.
 //   * Of a run of a pair's stages of 16 (rows of 128 bytes: 32) keys each of the workgroup's W waves takes
 //     every W-th.  A stage's rows go straight from memory to the wave's own two LDS slots, one stage
 //     ahead of the one that is scored, over the ends of runs: no barrier but where a run ends.  The
 //     page numbers of up to 64 stages come the same way, while the stages before them are read.
-//     Where pages hold whole stages a stage's rows are one range of memory; for other page sizes
-//     each lane works out the address of its own row.
+//     Where pages hold whole stages (or halves of 16 keys) the rows are one range of memory (two); for other
+//     page sizes each lane works out the address of its own row.
 //   * The rows of a KV head's query heads are the columns of 16x16 products, S^T = K . Q^T and
 //     O^T += V^T . P^T.  The matrix cores idle (under a twentieth of their rate), so the weights are
 //     not rounded to the cache's type: bf16 weights go in three parts (all 24 bits of their
@@ -63,6 +65,7 @@ struct Params {
     int32_t mask_dtype, vec_out;
     uint32_t pages, group, heads, blocks;       // heads: pairs of a request; blocks: of a KV head
     uint32_t columns, log_least;                       // of a state; of eight waves
+    uint32_t single;                                   // eight waves: no pair can have more than one share
     Divisor by_page, by_grid;
     float scale;                                       // unmasked: times log2(e)
 };
@@ -117,10 +120,17 @@ Q3T_DEVICE uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_read
 // Rows are read once: the non-temporal policy (64 requests of 64..1023 keys without it 35.1 us, with it 32.8;
 // 128 of 100..4095 194.9, 176.2).  From a pointer per lane:
 Q3T_DEVICE void load_rows(const uint64_t *p, uint32_t base) { Q3T_LOAD4("global_load_lds_dwordx4", "off", " nt"); }
-// from an offset per lane into a resource; past its range zeros are written without a memory access
+// from an offset per lane into a resource; past its range zeros are written without a memory access: four
+// loads, or two
 #define Q3T_RSRC , "s"(rsrc)
 Q3T_DEVICE void load_rows(i32x4_t rsrc, const uint32_t *p, uint32_t base) {
     Q3T_LOAD4("buffer_load_dwordx4", "%5, 0 offen", " nt lds", Q3T_RSRC);
+}
+Q3T_DEVICE void load_half(i32x4_t rsrc, const uint32_t *p, uint32_t base) {
+    asm volatile("s_mov_b32 m0, %0\n\t" Q3T_VMEM_SGPR_WAIT
+                 "buffer_load_dwordx4 %1, %3, 0 offen nt lds\n\t"
+                 "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 nt lds"
+                 :: "s"(base), "v"(p[0]), "v"(p[1]), "s"(rsrc) : "memory", "m0");
 }
 #undef Q3T_RSRC
 #undef Q3T_LOAD4
@@ -422,14 +432,15 @@ Q3T_DEVICE uint32_t scan(uint32_t x) {
     return x;
 }
 
-// WHOLE: a stage's keys share a page (page sizes that are multiples of a stage), so their rows are one
-// range of memory.
-template <typename T, int D, bool MASK, bool WHOLE, int W>
+// RANGES: ranges of memory that a stage's rows are in, in pages that hold whole ones; 0: any page size.
+template <typename T, int D, bool MASK, int RANGES, int W>
 __global__ void __launch_bounds__(64 * W, (W / 4 * Workgroups<T, D, W>::per_cu))
 paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     typedef Shape<T, D> S;
     typedef Tile<T, D> Products;
     constexpr int LOADS = 2 * S::loads, kThreads = 64 * W;
+    constexpr bool WHOLE = RANGES > 0;
+    constexpr uint32_t kRows = S::keys / (WHOLE ? RANGES : S::keys);  // of a page number
     __shared__ Lds<T, D, MASK, W> s;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = (int)uniform(tid >> 6);
@@ -441,35 +452,37 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     };
     auto stages_of = [&](uint32_t length) { return max(1u, (length + S::keys - 1) >> S::log_keys); };
     const uint32_t log_least = W == 4 ? kLogLeast4 : p.log_least, least = 1u << log_least;
-    const uint32_t each = (batch + 63) / 64;  // requests of a lane, one after the other
-    uint32_t lengths = length_at(lane);       // of requests window + lane
-    uint32_t stages = 0, pieces = 0, window = 0;
-    auto count = [&](uint32_t r) {
-        stages += r;
-        pieces += (r + least - 1) >> log_least;
-    };
-    if (each == 1) {
-        if ((uint32_t)lane < batch) count(stages_of(lengths));
-    } else {
-        constexpr uint32_t kFlight = 8;  // positions on their way at once (4096 requests: one 118 us, eight 116)
-        for (uint32_t i = 0; i < each; i += kFlight) {
-            uint32_t r[kFlight];
-#pragma unroll
-            for (uint32_t j = 0; j < kFlight; ++j) r[j] = stages_of(length_at(min(lane * each + i + j, batch - 1)));
-#pragma unroll
-            for (uint32_t j = 0; j < kFlight; ++j)
-                if (i + j < each && lane * each + i + j < batch) count(r[j]);
-        }
-    }
-    const uint32_t stages_to = scan(stages), pieces_to = scan(pieces);
-    auto last_lane = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); };
-    const Sharing sh = sharing(batch * p.heads, last_lane(stages_to) * p.heads, last_lane(pieces_to) * p.heads,
-                               least, run_cost(W), p.by_grid);
+    uint32_t lengths, window = 0;  // of requests window + lane
+    Sharing sh;
     Cursor at = {};
-    at.x = blockIdx.x * sh.share;
-    if (at.x >= sh.total) return;
-    at.left = min(sh.share, sh.total - at.x);
-    {
+    auto find_share = [&]() {
+        const uint32_t each = (batch + 63) / 64;  // requests of a lane, one after the other
+        uint32_t stages = 0, pieces = 0;
+        lengths = length_at(lane);
+        auto count = [&](uint32_t r) {
+            stages += r;
+            pieces += (r + least - 1) >> log_least;
+        };
+        if (each == 1) {
+            if ((uint32_t)lane < batch) count(stages_of(lengths));
+        } else {
+            constexpr uint32_t kFlight = 8;  // positions on their way at once (4096 requests: one 118 us, eight 116)
+            for (uint32_t i = 0; i < each; i += kFlight) {
+                uint32_t r[kFlight];
+#pragma unroll
+                for (uint32_t j = 0; j < kFlight; ++j) r[j] = stages_of(length_at(min(lane * each + i + j, batch - 1)));
+#pragma unroll
+                for (uint32_t j = 0; j < kFlight; ++j)
+                    if (i + j < each && lane * each + i + j < batch) count(r[j]);
+            }
+        }
+        const uint32_t stages_to = scan(stages), pieces_to = scan(pieces);
+        auto last_lane = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); };
+        sh = sharing(batch * p.heads, last_lane(stages_to) * p.heads, last_lane(pieces_to) * p.heads,
+                     least, run_cost(W), p.by_grid);
+        at.x = blockIdx.x * sh.share;
+        if (at.x >= sh.total) return false;
+        at.left = min(sh.share, sh.total - at.x);
         // the lane whose requests hold the share's first place, then the request
         auto holder = [&](uint32_t to, uint32_t &from) {  // `from`: the first place of the lane found
             const uint64_t below = __builtin_amdgcn_ballot_w64(to * p.heads <= at.x - from);
@@ -495,7 +508,17 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         at.off = (at.x - from) - at.head * length;
         if (at.off >= stages_here) end_pair(at, length, p.heads);
         at = Cursor{uniform(at.x), uniform(at.left), uniform(at.b), uniform(at.head), uniform(at.off)};
-        if (at.left == 0) return;
+        return at.left > 0;
+    };
+    const bool single = W == 8 && p.single;
+    if (single) {
+        sh = {least, 0u, least, batch * p.heads * least};
+        const uint32_t b = blockIdx.x / p.heads;
+        at = Cursor{blockIdx.x * least, least, b, blockIdx.x - b * p.heads, 0u};
+        window = b;
+        lengths = length_at(b + lane);
+    } else if (!find_share()) {
+        return;
     }
     auto request_length = [&](uint32_t b) {
         return b - window < 64 ? (uint32_t)__builtin_amdgcn_readlane((int)lengths, (int)(b - window)) : uniform(length_at(b));
@@ -506,7 +529,8 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     auto kv_head = [&](uint32_t head) { return p.blocks == 1 ? head : head / p.blocks; };
     Cursor ahead = at;
     int32_t runs = -1;
-    constexpr uint32_t kStep = W * S::keys, kBatch = (WHOLE ? 64 : 64 / S::keys) * kStep;  // keys
+    constexpr uint32_t kIds = S::keys / kRows;                        // page numbers of a stage
+    constexpr uint32_t kStep = W * S::keys, kBatch = 64 / kIds * kStep;  // keys
     Batch batches = {0u, 0u, 0u, 0u, 0u, -1};  // the next one, whose page numbers are on their way
     auto next_batch = [&]() {
         if (batches.key + kBatch < batches.end) {
@@ -531,10 +555,10 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     const uint32_t ids = uniform(lds_at(&s.ids[wave][0][0]));
     const uint32_t maskw = MASK ? uniform(lds_at(&s.maskw[wave][0][0])) : 0u;
     const uint32_t mask_size = !MASK ? 0 : p.mask_dtype == Q3T_F32 ? 4 : p.mask_dtype == Q3T_BOOL ? 1 : 2;
-    // The batch's page numbers: lane i's is stage i's (WHOLE), or that of key i % keys of stage i / keys;
-    // past the request's end that of its last key.
+    // The batch's page numbers: lane i's is that of range (WHOLE) or key i % kIds of stage i / kIds; past the
+    // request's end that of its last key.
     auto load_ids = [&](uint32_t half) {
-        const uint32_t key = batches.key + (WHOLE ? lane * kStep : lane / S::keys * kStep + lane % S::keys);
+        const uint32_t key = batches.key + lane / kIds * kStep + lane % kIds * kRows;
         const uint32_t at_page = divide(min(key, batches.length - 1), p.by_page);
         load_lds4(reinterpret_cast<uint64_t>(p.table + (uint64_t)batches.b * p.table_sb + at_page), uniform(ids + half * 256));
     };
@@ -545,14 +569,15 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     if constexpr (WHOLE) {
 #pragma unroll
         for (int i = 0; i < S::loads; ++i) {
-            const int r = row_of(i);
-            key_offset[i] = (uint32_t)(r * p.kp_st + (chunk_of(i) ^ S::key_swizzle(r))) * 16 - 1024 * (i & 3);
-            value_offset[i] = (uint32_t)(r * p.vp_st + (chunk_of(i) ^ S::value_swizzle(r))) * 16 - 1024 * (i & 3);
+            const int r = row_of(i) % kRows;  // of its range (the swizzles repeat every 16 rows)
+            const uint32_t ahead = 1024 * (RANGES == 1 ? i & 3 : i & 1);
+            key_offset[i] = (uint32_t)(r * p.kp_st + (chunk_of(i) ^ S::key_swizzle(r))) * 16 - ahead;
+            value_offset[i] = (uint32_t)(r * p.vp_st + (chunk_of(i) ^ S::value_swizzle(r))) * 16 - ahead;
         }
     }
     // stage `index` of a batch into ring slot n % 2
     auto load_stage = [&](const Batch &bt, uint32_t index, uint32_t half, uint32_t n) {
-        const uint32_t key0 = bt.key + index * kStep, at_ids = ids + half * 256 + index * (WHOLE ? 4 : 4 * S::keys);
+        const uint32_t key0 = bt.key + index * kStep, at_ids = ids + half * 256 + index * (4 * kIds);
         if constexpr (MASK) {
             const uint32_t key = min(key0 + lane, bt.length - 1);
             const uint64_t byte = ((uint64_t)bt.b * p.m_sb + (uint64_t)key * p.m_st) * mask_size;
@@ -561,24 +586,37 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         }
         const uint32_t base = uniform(ring + (n & 1) * S::stage);
         Stage st = {bt.b, key0, 0u, bt.run};
-        const uint32_t rest = bt.length - key0;  // keys from key0 on
         if constexpr (WHOLE) {
-            // the stage's rows that exist, none on no page
-            const uint32_t id = uniform(*(Q3T_LDS const uint32_t *)(uintptr_t)at_ids);
-            const uint32_t row = key0 - divide(key0, p.by_page) * p.by_page.d;
-            const uint32_t count = id < p.pages ? min((uint32_t)S::keys, rest) : 0u;
-            st.exists = count == 32 ? ~0u : (1u << count) - 1;
-            auto range = [&](const char *pool, uint32_t page_stride, uint32_t head_stride, uint32_t row_stride) {
-                const uint64_t from = reinterpret_cast<uint64_t>(pool) +
-                                      (count ? ((uint64_t)id * page_stride + (uint64_t)row * row_stride + (uint64_t)bt.kv_head * head_stride) * 16 : 0);
-                return scalar_rsrc(reinterpret_cast<const void *>(from), count ? (count - 1) * row_stride * 16 + S::row : 0u);
+            i32x4_t keys[RANGES], values[RANGES];
+#pragma unroll
+            for (int n = 0; n < RANGES; ++n) {
+                // the range's rows that exist, none on no page
+                const uint32_t id = uniform(*(Q3T_LDS const uint32_t *)(uintptr_t)(at_ids + 4 * n));
+                const uint32_t key = key0 + kRows * n, row = key - divide(key, p.by_page) * p.by_page.d;
+                const uint32_t count = id < p.pages && bt.length > key ? min(kRows, bt.length - key) : 0u;
+                st.exists |= (count == 32 ? ~0u : (1u << count) - 1) << kRows * n % 32;
+                auto range = [&](const char *pool, uint32_t page_stride, uint32_t head_stride, uint32_t row_stride) {
+                    const uint64_t from = reinterpret_cast<uint64_t>(pool) +
+                                          (count ? ((uint64_t)id * page_stride + (uint64_t)row * row_stride + (uint64_t)bt.kv_head * head_stride) * 16 : 0);
+                    return scalar_rsrc(reinterpret_cast<const void *>(from), count ? (count - 1) * row_stride * 16 + S::row : 0u);
+                };
+                keys[n] = range(p.kp, p.kp_sp, p.kp_sh, p.kp_st);
+                values[n] = range(p.vp, p.vp_sp, p.vp_sh, p.vp_st);
+            }
+            auto load = [&](const i32x4_t *ranges, const uint32_t *offset, uint32_t to) {
+                if constexpr (RANGES == 1) {
+#pragma unroll
+                    for (int i = 0; i < S::loads; i += 4) load_rows(ranges[0], offset + i, to + i * 1024);
+                } else {
+                    static_assert(S::loads == 2 * RANGES, "two loads a range");
+#pragma unroll
+                    for (int n = 0; n < RANGES; ++n) load_half(ranges[n], offset + 2 * n, to + n * 2048);
+                }
             };
-            const i32x4_t keys = range(p.kp, p.kp_sp, p.kp_sh, p.kp_st), values = range(p.vp, p.vp_sp, p.vp_sh, p.vp_st);
-#pragma unroll
-            for (int i = 0; i < S::loads; i += 4) load_rows(keys, key_offset + i, base + i * 1024);
-#pragma unroll
-            for (int i = 0; i < S::loads; i += 4) load_rows(values, value_offset + i, base + (S::loads + i) * 1024);
+            load(keys, key_offset, base);
+            load(values, value_offset, base + S::loads * 1024);
         } else {
+            const uint32_t rest = bt.length - key0;  // keys from key0 on
             const uint32_t mine = *(Q3T_LDS const uint32_t *)(uintptr_t)(at_ids + lane % S::keys * 4);
             st.exists = (uint32_t)__builtin_amdgcn_ballot_w64(lane < S::keys && (uint32_t)lane < rest && mine < p.pages);
             const uint64_t kh = (uint64_t)bt.kv_head * p.kp_sh, vh = (uint64_t)bt.kv_head * p.vp_sh;
@@ -619,12 +657,18 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     };
 
     if (wave == W - 1) load_query(at.b, at.head, 0);
+    if (single) {  // the first batch's page numbers, whatever the length
+        batches.b = at.b;
+        batches.key = wave * S::keys;
+        batches.length = ctx;
+        load_ids(0);
+    }
     next_batch();
     Batch now = batches;  // the batch whose rows are being loaded, its page numbers in half `half`
     uint32_t index = 0, half = 0;
     Stage s0 = {0u, 0u, 0u, -1};
     if (now.run >= 0) {
-        load_ids(0);
+        if (!single) load_ids(0);
         next_batch();
         if (batches.run >= 0) load_ids(1);
         wait_loads<0>();
@@ -892,42 +936,52 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 //     64..700 26.2 / 24.7, 40 of 64..1023 25.5 / 23.4, one of 65000 33.1 / 31.7, 8 of 1000..4000 24.7 / 24.3; 96 of
 //     64..600 31.0 / 31.4, 24 of 64..1023 18.7 / 19.0, 8 of 100..2000 14.1 / 14.7, 64 of 512 27.0 / 28.2, 128 of
 //     32..511 32.7 / 34.6, 512 of 20..200 32.8 / 41.6.  From 640 keys a request and 15000 stages and run
-//     ends in all, for up to 1024 pairs, where short requests cost little.
+//     ends in all, for up to 1024 pairs, where short requests cost little.  Not rows of 128 bytes: 64 of
+//     64..2047 33.5 / 36.9, 128 of 100..4000 94.6 / 95.6, 32 of 100..1500 17.9 / 17.9.
 //   * Few short pairs: one workgroup attends a whole pair, and no states pass through memory.  us, four /
-//     eight, 8 KV heads: one request of 100 keys 7.7 / 7.2, of 300 10.2 / 8.7, of 400 10.3 / 9.6, of 500 10.4 /
-//     10.4, of 600 10.2 / 11.5; 8 of 300 10.5 / 9.8, 16 of 400 13.1 / 11.4, 32 of 300 16.4 / 12.4, 32 of 500 17.9 /
-//     16.6, 48 of 200 16.4 / 15.8, 64 of 64 9.0 / 10.0.  With enough pairs for half of the CUs, longer ones too:
+//     eight, 8 KV heads: one request of 100 keys 7.7 / 7.1, of 300 10.2 / 8.5, of 400 10.3 / 9.2, of 500 10.5 /
+//     10.1, of 600 10.2 / 11.5; 8 of 300 10.5 / 9.0, 16 of 400 13.1 / 10.8, 32 of 300 16.4 / 11.5, 32 of 500 17.9 /
+//     15.6, 48 of 200 16.4 / 15.8, 64 of 64 9.0 / 10.0.  With enough pairs for half of the CUs, longer ones too:
 //     24 of 1..700 17.3 / 14.7, 16 of 600 15.9 / 14.8, 32 of 600 20.3 / 18.8, 32 of 800 22.6 / 22.5, 32 of 1000 26.6 /
-//     27.0; 12 of 1..700 12.4 / 12.8.  Up to 448 keys and a pair for each CU; up to 800 for half as many on.
+//     27.0; 12 of 1..700 12.4 / 12.8.  Up to 512 keys and a pair for each CU; up to 800 for half as many on.  Rows of
+//     128 bytes: one of 440 9.1 / 7.5, 32 of 440 12.2 / 9.5, 32 of 1000 17.5 / 15.6, 24 of 100..1000 12.3 / 11.2, 32
+//     of 100..1500 17.9 / 22.4; one of 1000 9.9 / 10.9: up to 1024.  There two ranges a stage (pages of an odd
+//     number of 16 rows) gain as much here (one of 440 9.8 / 8.1), but elsewhere less than the per-lane form:
+//     64 of 64..2047 per lane 32.9, two ranges 37.4.
 //   * Groups of more than 8 query heads, whose states are large: half as many parts.  us, four / eight: 16
 //     heads on one KV head, one request of 1000 keys 12.6 / 11.7, of 8000 18.8 / 16.4, of 60000 31.6 / 21.0, 8 of
 //     2000 16.5 / 13.2, 128 of 64..1023 20.5 / 19.1, 32 of 4000 26.1 / 22.3; 256 of 100..1000 24.8 / 25.2, 512 of
 //     20..200 20.1 / 20.4, 300 of 10..60 10.1 / 13.9.  From 192 keys on.  Groups of 8 lose as often (one of
-//     1000 and two KV heads 10.7 / 11.8, of 4000 and four 14.4 / 13.1).
+//     1000 and two KV heads 10.7 / 11.8, of 4000 and four 14.4 / 13.1).  Rows of 128 bytes from 2500 keys on: one
+//     of 1000 9.9 / 11.3, 8 of 2000 10.9 / 11.7, 32 of 4000 17.3 / 14.4, one of 8000 13.9 / 12.4.
 constexpr int64_t kLongRequest = 640, kManyStages = 15000, kFewPairs = 1024;
-constexpr int64_t kShortRequest = 448, kMiddleRequest = 800, kCUs = 256;
-constexpr int64_t kWideGroup = 8, kWideRequest = 192;
+constexpr int64_t kShortRequest = 512, kMiddleRequest = 800, kMiddleNarrow = 1024, kCUs = 256;
+constexpr int64_t kWideGroup = 8, kWideRequest = 192, kWideNarrow = 2500;
 
 template <typename T, int D>
 struct Launch {
     typedef Shape<T, D> S;
     static int64_t stages(const q3t_paged_args *a, int64_t pairs, int waves) { return pairs * ((a->ctx + S::keys - 1) / S::keys + run_cost(waves)); }
-    // rows of a stage as one range: whole pages, rows that do not overlap, 32-bit offsets
-    static bool whole(const q3t_paged_args *a) {
+    // Ranges of memory that a stage's rows are in: whole pages, rows that do not overlap, 32-bit offsets; else 0.
+    static int ranges(const q3t_paged_args *a) {
         const int64_t es = sizeof(T), most = ((int64_t)1 << 30) / S::keys;
-        return a->page_size % S::keys == 0 && a->kp_stride_t * es >= S::row && a->vp_stride_t * es >= S::row &&
-               a->kp_stride_t * es < most && a->vp_stride_t * es < most;
+        if (a->kp_stride_t * es < S::row || a->vp_stride_t * es < S::row || a->kp_stride_t * es >= most || a->vp_stride_t * es >= most)
+            return 0;
+        return a->page_size % S::keys == 0 ? 1 : a->page_size % 16 == 0 ? 2 : 0;
     }
     static bool few(const q3t_paged_args *a, int64_t pairs) {
-        return pairs <= kCUs && a->ctx <= (pairs >= kCUs / 2 ? kMiddleRequest : kShortRequest);
+        return pairs <= kCUs && a->ctx <= (pairs < kCUs / 2 ? kShortRequest : S::row == 128 ? kMiddleNarrow : kMiddleRequest);
     }
     static bool eight(const q3t_paged_args *a, int64_t pairs) {
-        const bool many = a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
-        const bool wide = a->q_heads / a->kv_heads > kWideGroup && a->ctx >= kWideRequest;
-        return S::row < 512 && whole(a) && (many || few(a, pairs) || wide);
+        const bool many = S::row > 128 && a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
+        const bool wide = a->q_heads / a->kv_heads > kWideGroup && a->ctx >= (S::row == 128 ? kWideNarrow : kWideRequest);
+        return S::row < 512 && (ranges(a) == 1 ? many || wide || few(a, pairs) : ranges(a) == 2 && few(a, pairs));
     }
     static uint32_t log_least(const q3t_paged_args *a, int64_t pairs) {
         return !eight(a, pairs) ? kLogLeast4 : few(a, pairs) ? kLogLeastShort : kLogLeast8;
+    }
+    static bool single(const q3t_paged_args *a, int64_t pairs) {
+        return eight(a, pairs) && few(a, pairs) && a->ctx <= (int64_t)S::keys << kLogLeastShort;
     }
     static int64_t workgroups(const q3t_paged_args *a, int64_t pairs) {
         const bool wide = eight(a, pairs);
@@ -943,9 +997,11 @@ struct Launch {
         auto masked = [&](auto mask) {
             constexpr bool MASK = decltype(mask)::value;
             if constexpr (S::row < 512)
-                if (eight(a, pairs)) return launch(paged_kernel<T, D, MASK, true, 8>, 8);
-            if (whole(a)) launch(paged_kernel<T, D, MASK, true, 4>, 4);
-            else launch(paged_kernel<T, D, MASK, false, 4>, 4);
+                if (eight(a, pairs) && ranges(a) == 1) return launch(paged_kernel<T, D, MASK, 1, 8>, 8);
+            if constexpr (S::keys == 32)
+                if (eight(a, pairs)) return launch(paged_kernel<T, D, MASK, 2, 8>, 8);
+            if (ranges(a) == 1) launch(paged_kernel<T, D, MASK, 1, 4>, 4);
+            else launch(paged_kernel<T, D, MASK, 0, 4>, 4);
         };
         if (a->mask) masked(std::true_type{});
         else masked(std::false_type{});
@@ -1042,6 +1098,7 @@ extern "C" int q3t_paged_attention(const q3t_paged_args *a, void *stream) {
     p.heads = (uint32_t)(a->kv_heads * z.blocks);
     p.columns = (uint32_t)z.columns;
     p.log_least = with(a, [&](auto l) { return l.log_least(a, z.pairs); });
+    p.single = with(a, [&](auto l) { return l.single(a, z.pairs); });
     p.by_page = divisor((uint32_t)a->page_size);
     p.by_grid = divisor((uint32_t)z.workgroups);
     p.scale = a->mask ? a->scale : a->scale * kLog2e;

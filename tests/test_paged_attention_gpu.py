@@ -79,6 +79,21 @@ def test_large_groups_over_long_requests(pkg, device, masked, dtype, width, head
     assert_within(run(pkg, p, mask=mask), *expected(p, mask=mask))
 
 
+@pytest.mark.parametrize('masked', [False, True])
+@pytest.mark.parametrize('dtype', [BF16, F16], ids=str)
+@pytest.mark.parametrize('page', [16, 32, 48])
+@pytest.mark.parametrize('lengths', [[0, 1, 16, 17, 31, 33, 47, 49, 200, 255, 500], [n % 960 for n in range(1, 17 * 271, 271)]], ids=['few', 'more'])
+def test_narrow_rows_in_pages_of_half_a_stage(pkg, device, lengths, page, dtype, masked):
+    p = problem(device, lengths, q_heads=16, kv_heads=8, width=64, dtype=dtype, page=page, seed=31)
+    ctx = p.table.shape[1] * page
+    mask = None
+    if masked:
+        mask = torch.ones(len(p.lengths), 1, 1, ctx, dtype=torch.bool, device=device)
+        mask[:, :, :, 1::6] = False
+        mask[8] = False
+    assert_within(run(pkg, p, mask=mask), *expected(p, mask=mask))
+
+
 @pytest.mark.parametrize('lengths', [[800] * 16, [n % 801 for n in range(0, 24 * 331, 331)]], ids=['equal', 'ragged'])
 def test_pairs_for_more_than_half_of_the_card(pkg, device, lengths):
     p = problem(device, lengths, q_heads=16, kv_heads=8, table_width=50, page=16, seed=29)
