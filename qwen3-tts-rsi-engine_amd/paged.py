@@ -128,7 +128,7 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
             raise ValueError('the mask must be broadcastable to (batch, 1, 1, keys)') from None
         mask_fields = (mask.data_ptr(), _lib.DTYPE_CODES[mask.dtype], rows.stride(0), rows.stride(3))
     if out is None:
-        out, os = query.new_empty((batch, 1, q_heads, head_dim)), (q_heads * head_dim, 0, head_dim)
+        out, os = torch.empty_like(query, memory_format=torch.contiguous_format), (q_heads * head_dim, 0, head_dim)
     else:
         _check_out(out, (batch, 1, q_heads, head_dim), dtype, query.device, 'paged attention')
         os = out.stride()

@@ -178,10 +178,10 @@ def rotary_axes(query, key, positions, sections, *, interleaved=False, theta=DEF
             raise ValueError('rows that share memory cannot be rotated in place')
         q_out, k_out, qos, kos = query, key, qs, ks
     else:
-        q_out, k_out, kos = query.new_empty((batch, tokens, q_heads, width)), None, (0, 0, 0)
+        q_out, k_out, kos = torch.empty_like(query, memory_format=torch.contiguous_format), None, (0, 0, 0)
         qos = (tokens * q_heads * width, q_heads * width, width)
         if key is not None:
-            k_out = query.new_empty((batch, tokens, k_heads, width))
+            k_out = torch.empty_like(key, memory_format=torch.contiguous_format)
             kos = (tokens * k_heads * width, k_heads * width, width)
     if batch == 0 or tokens == 0:
         return q_out, k_out
