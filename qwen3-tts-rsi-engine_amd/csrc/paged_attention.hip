@@ -349,18 +349,13 @@ template <int D> struct Tile<float, D> {
     }
 };
 
-// Four mask terms from four words, each holding its element at byte (low + i step) % 4.
-Q3T_DEVICE void mask_terms(const U4 &words, uint32_t low, uint32_t step, int dtype, float (&x)[4]) {
-    const uint32_t w[4] = {words.x, words.y, words.z, words.w};
-    auto each = [&](auto term) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = term(w[i] >> (8 * ((low + i * step) & 3u)));
-    };
+// The mask term whose element lies in a word's low bytes.
+Q3T_DEVICE float mask_term(uint32_t e, int dtype) {
     switch (dtype) {
-        case Q3T_BF16: each([](uint32_t e) { return bf16_to_float(e & 0xffffu); }); break;
-        case Q3T_F16: each([](uint32_t e) { return (float)__builtin_bit_cast(_Float16, (uint16_t)e); }); break;
-        case Q3T_F32: each([](uint32_t e) { return __uint_as_float(e); }); break;
-        default: each([](uint32_t e) { return e & 0xffu ? 0.0f : -INFINITY; });  // bool: true attends
+        case Q3T_BF16: return bf16_to_float(e & 0xffffu);
+        case Q3T_F16: return (float)__builtin_bit_cast(_Float16, (uint16_t)e);
+        case Q3T_F32: return __uint_as_float(e);
+        default: return e & 0xffu ? 0.0f : -INFINITY;  // bool: true attends
     }
 }
 
@@ -685,30 +680,43 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     float m, l;
     uint32_t n = 0;
     x.place(ring, g, c);
+    constexpr uint32_t kAllKeys = (uint32_t)((1ull << S::keys) - 1);
     auto score = [&](const Stage &st) {
         const uint32_t stage = (n & 1) * S::stage;
-        float v[S::keys / 16][4];
-        bool hidden[S::keys / 16][4] = {}, any = false;
         // Keys that do not exist.  Their value rows are zeroed, unless they are rows past a range, for
         // which the loads left zeros.
-        if (MASK || st.exists != (uint32_t)((1ull << S::keys) - 1)) {
+        bool zero_rows = !WHOLE && st.exists != kAllKeys;
+        U4 terms[MASK ? S::keys / 16 : 1];
+        if constexpr (MASK) {
+            // lane k's term is that of key k, from its word; then, through LDS, each lane takes its own four
+            const uint32_t k = lane % S::keys, words = maskw + (n & 1) * S::keys * 4;
+            const uint32_t low = (uint32_t)reinterpret_cast<uint64_t>(p.mask) + (st.b * p.m_sb + (st.key0 + k) * p.m_st) * mask_size;
+            float term = mask_term(*(Q3T_LDS const uint32_t *)(uintptr_t)(words + 4 * k) >> (8 * (low & 3u)), p.mask_dtype);
+            if (!(st.exists >> k & 1u)) term = -INFINITY;
+            *(Q3T_LDS float *)(uintptr_t)(words + 4 * k) = term;
+            zero_rows = __builtin_amdgcn_ballot_w64(term == -INFINITY) != 0;
+            asm volatile("" ::: "memory");
 #pragma unroll
-            for (int t = 0; t < S::keys / 16; ++t) {
-                if constexpr (MASK) {
-                    const uint32_t step = p.m_st * mask_size;
-                    const uint32_t low = (uint32_t)reinterpret_cast<uint64_t>(p.mask) + st.b * p.m_sb * mask_size +
-                                         (st.key0 + 16 * t + 4 * g) * step;
-                    mask_terms(lds_read16(maskw + ((n & 1) * S::keys + 16 * t + 4 * g) * 4), low, step, p.mask_dtype, v[t]);
-                }
-                const uint32_t exists = st.exists >> (16 * t + 4 * g);
+            for (int t = 0; t < S::keys / 16; ++t) terms[t] = lds_read16(words + (16 * t + 4 * g) * 4);
+        }
+        f32x4_t scores[S::keys / 16];
+#pragma unroll
+        for (int t = 0; t < S::keys / 16; ++t) scores[t] = x.scores(stage, t);
+        float v[S::keys / 16][4], highest = -INFINITY;
+        bool hidden[S::keys / 16][4] = {};
+        if (MASK || st.exists != kAllKeys) {
+#pragma unroll
+            for (int t = 0; t < S::keys / 16; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    hidden[t][i] = !(exists & (1u << i));
-                    if constexpr (MASK) hidden[t][i] = hidden[t][i] || v[t][i] == -INFINITY;
-                    any = any || hidden[t][i];
+                    if constexpr (MASK) {
+                        v[t][i] = __uint_as_float(i == 0 ? terms[t].x : i == 1 ? terms[t].y : i == 2 ? terms[t].z : terms[t].w);
+                        hidden[t][i] = v[t][i] == -INFINITY;
+                    } else {
+                        hidden[t][i] = !(st.exists >> (16 * t + 4 * g) & (1u << i));
+                    }
                 }
-            }
-            if ((!WHOLE || MASK) && __builtin_amdgcn_ballot_w64(any)) {
+            if ((!WHOLE || MASK) && zero_rows) {
                 const U4 zero = {0u, 0u, 0u, 0u};
 #pragma unroll
                 for (int t = 0; t < S::keys / 16; ++t)
@@ -720,17 +728,14 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
                 asm volatile("" ::: "memory");
             }
         }
-        float highest = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < S::keys / 16; ++t) {
-            const f32x4_t st4 = x.scores(stage, t);
+        for (int t = 0; t < S::keys / 16; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float scaled = MASK ? st4[i] * p.scale + v[t][i] : st4[i] * p.scale;
+                const float scaled = MASK ? scores[t][i] * p.scale + v[t][i] : scores[t][i] * p.scale;
                 v[t][i] = hidden[t][i] ? -INFINITY : scaled;
                 highest = fmaxf(highest, v[t][i]);
             }
-        }
         x.read_values(stage, 0);  // on their way during the softmax
         if (__builtin_amdgcn_ballot_w64(highest > m + threshold)) {
             highest = fmaxf(highest, xor16(highest));
