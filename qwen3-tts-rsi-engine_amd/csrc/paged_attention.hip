@@ -7,9 +7,9 @@
 // threshold.  Every key and value row is read once, so HBM bounds a launch of many keys (2 to 16
 // operations per byte), and the chain arguments - positions - page numbers - rows - merge one of few.
 // us per launch in a graph, rows not in the caches (TB/s of them): 128 requests of 100..4095 keys, 8 KV heads of
-// 128, bf16 175 (6.0, the rate of a large read); 64 of 64..1023 30.5 (4.9); one of 65000, 4 heads, fp16 32.6 (4.1);
-// 32 of 30..2047 under a mask, 4 heads 22.9 (3.2); 21 of 1..700 in float32 under a mask, 12 heads of 64 20.5
-// (2.7); one of 300 8.4.  The first rows are there after 5.8 us.
+// 128, bf16 175 (6.0, the rate of a large read); 64 of 64..1023 30.8 (4.8); one of 65000, 4 heads, fp16 32.7 (4.1);
+// 32 of 30..2047 under a mask, 4 heads 22.9 (3.2); 21 of 1..700 in float32 under a mask, 12 heads of 64 20.2
+// (2.7); one of 300 8.5.  The first rows are there after 5.8 us.
 //   * Work: a workgroup takes an equal share of the stages of all (request, KV head) pairs
 //     (paged_index.hpp), whatever the requests' lengths; its waves find their place by adding up all
 //     requests' stages.  A pair that lies in several shares leaves its parts' states in the
@@ -941,7 +941,8 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 //     64..700 26.2 / 24.7, 40 of 64..1023 25.5 / 23.4, one of 65000 33.1 / 31.7, 8 of 1000..4000 24.7 / 24.3; 96 of
 //     64..600 31.0 / 31.4, 24 of 64..1023 18.7 / 19.0, 8 of 100..2000 14.1 / 14.7, 64 of 512 27.0 / 28.2, 128 of
 //     32..511 32.7 / 34.6, 512 of 20..200 32.8 / 41.6.  From 640 keys a request and 15000 stages and run
-//     ends in all, for up to 1024 pairs, where short requests cost little.  Not rows of 128 bytes: 64 of
+//     ends in all, for up to 1024 pairs, where short requests cost little (under a mask: 64 of 64..1023 34.6 /
+//     33.2, 32 of 30..2047 33.8 / 32.9, with 4 KV heads of 8 query heads 21.5 / 22.7).  Not rows of 128 bytes: 64 of
 //     64..2047 33.5 / 36.9, 128 of 100..4000 94.6 / 95.6, 32 of 100..1500 17.9 / 17.9.
 //   * Few short pairs: one workgroup attends a whole pair, and no states pass through memory.  us, four /
 //     eight, 8 KV heads: one request of 100 keys 7.7 / 7.1, of 300 10.2 / 8.5, of 400 10.3 / 9.2, of 500 10.5 /
