@@ -65,7 +65,6 @@ struct Params {
     int32_t mask_dtype, vec_out;
     uint32_t pages, group, heads, blocks;       // heads: pairs of a request; blocks: of a KV head
     uint32_t columns, log_least;                       // of a state; of eight waves
-    uint32_t single;                                   // eight waves: no pair can have more than one share
     Divisor by_page, by_grid;
     float scale;                                       // unmasked: times log2(e)
 };
@@ -428,7 +427,9 @@ Q3T_DEVICE uint32_t scan(uint32_t x) {
 }
 
 // RANGES: ranges of memory that a stage's rows are in, in pages that hold whole ones; 0: any page size.
-template <typename T, int D, bool MASK, int RANGES, int W>
+// SINGLE: no pair can have more than one share (without the code for others 64 requests of 64 keys take 8.2 us
+// instead of 9.0; as a branch of one instance it cost 1024 of 20..200 98 -> 105).
+template <typename T, int D, bool MASK, int RANGES, int W, bool SINGLE>
 __global__ void __launch_bounds__(64 * W, (W / 4 * Workgroups<T, D, W>::per_cu))
 paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     typedef Shape<T, D> S;
@@ -505,11 +506,11 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         at = Cursor{uniform(at.x), uniform(at.left), uniform(at.b), uniform(at.head), uniform(at.off)};
         return at.left > 0;
     };
-    const bool single = W == 8 && p.single;
-    if (single) {
-        sh = {least, 0u, least, batch * p.heads * least};
+    if constexpr (SINGLE) {
+        constexpr uint32_t kRoom = 1u << kLogLeastShort;  // holds any such pair's stages
+        sh = {kRoom, 0u, kRoom, batch * p.heads * kRoom};
         const uint32_t b = blockIdx.x / p.heads;
-        at = Cursor{blockIdx.x * least, least, b, blockIdx.x - b * p.heads, 0u};
+        at = Cursor{blockIdx.x * kRoom, kRoom, b, blockIdx.x - b * p.heads, 0u};
         window = b;
         lengths = length_at(b + lane);
     } else if (!find_share()) {
@@ -652,7 +653,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     };
 
     if (wave == W - 1) load_query(at.b, at.head, 0);
-    if (single) {  // the first batch's page numbers, whatever the length
+    if constexpr (SINGLE) {  // the first batch's page numbers, whatever the length
         batches.b = at.b;
         batches.key = wave * S::keys;
         batches.length = ctx;
@@ -663,7 +664,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     uint32_t index = 0, half = 0;
     Stage s0 = {0u, 0u, 0u, -1};
     if (now.run >= 0) {
-        if (!single) load_ids(0);
+        if (!SINGLE) load_ids(0);
         next_batch();
         if (batches.run >= 0) load_ids(1);
         wait_loads<0>();
@@ -821,15 +822,15 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
             s.ml[wave][c][1] = l;
         }
         if (lane == 0) s.slot[wave] = slot;
-        const bool whole = r.parts == 1;
+        const bool whole = SINGLE || r.parts == 1;
         // The first of two parts is done last in its share, and the other first in the next one: where that
         // one is there already, it is merged at once and nothing is published.
         int32_t *counter = p.counters + r.b * p.heads + r.head;
-        if (tid == kThreads - 1 && r.parts == 2 && r.begins)
+        if (!whole && tid == kThreads - 1 && r.parts == 2 && r.begins)
             s.there = (uint32_t)__hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if ((uint32_t)c < columns) x.store(slot, g, c);
         lds_barrier();
-        const bool two = r.parts == 2 && r.begins && uniform(s.there) == 1;
+        const bool two = !whole && r.parts == 2 && r.begins && uniform(s.there) == 1;
         float *state = p.states + (2 * blockIdx.x + r.begins) * (uint64_t)state_size;
         for (uint32_t item = tid; item < columns * (D / 4); item += kThreads) {
             const uint32_t column = item / (D / 4), chunk = item % (D / 4);
@@ -954,6 +955,9 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 //     of 100..1500 17.9 / 22.4; one of 1000 9.9 / 10.9: up to 1024.  There two ranges a stage (pages of an odd
 //     number of 16 rows) gain as much here (one of 440 9.8 / 8.1), but elsewhere less than the per-lane form:
 //     64 of 64..2047 per lane 32.9, two ranges 37.4.
+//     Beyond that four waves attend a whole pair of up to 256 keys (one batch of page numbers), for as many pairs as
+//     there are workgroups: 64 of 64 9.0 -> 8.2, 48 of 200 16.3 -> 12.9, 40 of 30..120 9.5 -> 8.9, 64 of 250 16.0.  Not
+//     rows of 512 bytes (one of 200 12.0 -> 14.4) or 128 (7.4 -> 7.7).
 //   * Groups of more than 8 query heads, whose states are large: half as many parts.  us, four / eight: 16
 //     heads on one KV head, one request of 1000 keys 12.6 / 11.7, of 8000 18.8 / 16.4, of 60000 31.6 / 21.0, 8 of
 //     2000 16.5 / 13.2, 128 of 64..1023 20.5 / 19.1, 32 of 4000 26.1 / 22.3; 256 of 100..1000 24.8 / 25.2, 512 of
@@ -962,6 +966,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 //     of 1000 9.9 / 11.3, 8 of 2000 10.9 / 11.7, 32 of 4000 17.3 / 14.4, one of 8000 13.9 / 12.4.
 constexpr int64_t kLongRequest = 640, kManyStages = 15000, kFewPairs = 1024;
 constexpr int64_t kShortRequest = 512, kMiddleRequest = 800, kMiddleNarrow = 1024, kCUs = 256;
+constexpr int64_t kSmallRequest = 256;
 constexpr int64_t kWideGroup = 8, kWideRequest = 192, kWideNarrow = 2500;
 
 template <typename T, int D>
@@ -983,11 +988,15 @@ struct Launch {
         const bool wide = a->q_heads / a->kv_heads > kWideGroup && a->ctx >= (S::row == 128 ? kWideNarrow : kWideRequest);
         return S::row < 512 && (ranges(a) == 1 ? many || wide || few(a, pairs) : ranges(a) == 2 && few(a, pairs));
     }
+    static bool small(const q3t_paged_args *a, int64_t pairs) {
+        return S::row == 256 && ranges(a) == 1 && !eight(a, pairs) && pairs <= Workgroups<T, D, 4>::count && a->ctx <= kSmallRequest;
+    }
     static uint32_t log_least(const q3t_paged_args *a, int64_t pairs) {
-        return !eight(a, pairs) ? kLogLeast4 : few(a, pairs) ? kLogLeastShort : kLogLeast8;
+        if (eight(a, pairs)) return few(a, pairs) ? kLogLeastShort : kLogLeast8;
+        return small(a, pairs) ? kLogLeastShort : kLogLeast4;
     }
     static bool single(const q3t_paged_args *a, int64_t pairs) {
-        return eight(a, pairs) && few(a, pairs) && a->ctx <= (int64_t)S::keys << kLogLeastShort;
+        return small(a, pairs) || (eight(a, pairs) && few(a, pairs) && a->ctx <= (int64_t)S::keys << kLogLeastShort);
     }
     static int64_t workgroups(const q3t_paged_args *a, int64_t pairs) {
         const bool wide = eight(a, pairs);
@@ -1002,12 +1011,19 @@ struct Launch {
         };
         auto masked = [&](auto mask) {
             constexpr bool MASK = decltype(mask)::value;
-            if constexpr (S::row < 512)
-                if (eight(a, pairs) && ranges(a) == 1) return launch(paged_kernel<T, D, MASK, 1, 8>, 8);
-            if constexpr (S::keys == 32)
-                if (eight(a, pairs)) return launch(paged_kernel<T, D, MASK, 2, 8>, 8);
-            if (ranges(a) == 1) launch(paged_kernel<T, D, MASK, 1, 4>, 4);
-            else launch(paged_kernel<T, D, MASK, 0, 4>, 4);
+            if constexpr (S::row < 512) {
+                const bool wide = eight(a, pairs);
+                if (single(a, pairs)) {
+                    if constexpr (S::keys == 32)
+                        if (ranges(a) == 2) return launch(paged_kernel<T, D, MASK, 2, 8, true>, 8);
+                    if constexpr (S::row == 256)
+                        if (!wide) return launch(paged_kernel<T, D, MASK, 1, 4, true>, 4);
+                    return launch(paged_kernel<T, D, MASK, 1, 8, true>, 8);
+                }
+                if (wide) return launch(paged_kernel<T, D, MASK, 1, 8, false>, 8);
+            }
+            if (ranges(a) == 1) launch(paged_kernel<T, D, MASK, 1, 4, false>, 4);
+            else launch(paged_kernel<T, D, MASK, 0, 4, false>, 4);
         };
         if (a->mask) masked(std::true_type{});
         else masked(std::false_type{});
@@ -1104,7 +1120,6 @@ extern "C" int q3t_paged_attention(const q3t_paged_args *a, void *stream) {
     p.heads = (uint32_t)(a->kv_heads * z.blocks);
     p.columns = (uint32_t)z.columns;
     p.log_least = with(a, [&](auto l) { return l.log_least(a, z.pairs); });
-    p.single = with(a, [&](auto l) { return l.single(a, z.pairs); });
     p.by_page = divisor((uint32_t)a->page_size);
     p.by_grid = divisor((uint32_t)z.workgroups);
     p.scale = a->mask ? a->scale : a->scale * kLog2e;
