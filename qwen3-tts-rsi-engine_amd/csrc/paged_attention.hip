@@ -38,11 +38,11 @@ namespace q3t {
 namespace paged {
 
 constexpr int kColumns = 16;           // query heads of a workgroup: columns of a product
-// Stages that are not shared out, as a power of two: two of each wave, but a short request's all where it has a
-// workgroup of eight waves (below).  us with 4 / 8 / 16 for four waves: one request of 300 keys 9.5 / 10.2 /
-// 10.2, of 100 8.8 / 7.7 / -, of 4000 13.4 / 12.9 / -, 4 of 300..1000 11.1 / 10.7 / -, 8 of 100..2000 14.0 / 14.0 /
-// 15.0; with 16 / 32 for eight: one of 300 10.3 / 8.8, one of 1000 with one KV head and 16 others 11.8 / 13.7.
-constexpr uint32_t kLogLeast4 = 3, kLogLeast8 = 4, kLogLeastShort = 5;
+// Stages that are not shared out, as a power of two: two of each wave; all of a pair that a workgroup has to
+// itself (below).  us with 4 / 8 / 16 for four waves: one request of 4000 keys 13.4 / 12.9 / -, 4 of 300..1000 11.3 /
+// 10.8 / -, 3 of 5000..9000 with one KV head 22.5 / 20.8 / 20.8, 8 of 100..2000 14.0 / 14.0 / 15.0; with 16 / 32 for
+// eight: one of 1000 with one KV head and 16 others 11.8 / 13.7.
+constexpr uint32_t kLogLeast4 = 3, kLogLeast8 = 4, kLogLeastSingle = 6;
 // Stages that the end of a run of W waves costs as much as.  us with 1 / 8 / 24 for four waves: 200 requests of
 // 10..400 keys 44 / 27.2 / 28.3, 128 of 32..511 42 / 32.9 / 34.6; with 8 / 16 / 24 for eight: 64 of 64..1023
 // 31.6 / 30.8 / 31.2, 128 of 100..4095 174.8 / 174.4 / 176.2.
@@ -507,7 +507,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
         return at.left > 0;
     };
     if constexpr (SINGLE) {
-        constexpr uint32_t kRoom = 1u << kLogLeastShort;  // holds any such pair's stages
+        constexpr uint32_t kRoom = 1u << kLogLeastSingle;  // holds any such pair's stages
         sh = {kRoom, 0u, kRoom, batch * p.heads * kRoom};
         const uint32_t b = blockIdx.x / p.heads;
         at = Cursor{blockIdx.x * kRoom, kRoom, b, blockIdx.x - b * p.heads, 0u};
@@ -936,37 +936,33 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     }
 }
 
-// Eight waves a workgroup instead of four, by what the host sees: capacities, not lengths.
-//   * Many stages: half as many shares, so half as many cut pairs, but more waves with nothing to do in a
-//     short one.  us, four / eight: 128 requests of 100..4095 keys 180 / 174, 64 of 64..1023 33.4 / 30.8, 64 of
-//     64..700 26.2 / 24.7, 40 of 64..1023 25.5 / 23.4, one of 65000 33.1 / 31.7, 8 of 1000..4000 24.7 / 24.3; 96 of
-//     64..600 31.0 / 31.4, 24 of 64..1023 18.7 / 19.0, 8 of 100..2000 14.1 / 14.7, 64 of 512 27.0 / 28.2, 128 of
-//     32..511 32.7 / 34.6, 512 of 20..200 32.8 / 41.6.  From 640 keys a request and 15000 stages and run
-//     ends in all, for up to 1024 pairs, where short requests cost little (under a mask: 64 of 64..1023 34.6 /
-//     33.2, 32 of 30..2047 33.8 / 32.9, with 4 KV heads of 8 query heads 21.5 / 22.7).  Not rows of 128 bytes: 64 of
-//     64..2047 33.5 / 36.9, 128 of 100..4000 94.6 / 95.6, 32 of 100..1500 17.9 / 17.9.
-//   * Few short pairs: one workgroup attends a whole pair, and no states pass through memory.  us, four /
-//     eight, 8 KV heads: one request of 100 keys 7.7 / 7.1, of 300 10.2 / 8.5, of 400 10.3 / 9.2, of 500 10.5 /
-//     10.1, of 600 10.2 / 11.5; 8 of 300 10.5 / 9.0, 16 of 400 13.1 / 10.8, 32 of 300 16.4 / 11.5, 32 of 500 17.9 /
-//     15.6, 48 of 200 16.4 / 15.8, 64 of 64 9.0 / 10.0.  With enough pairs for half of the CUs, longer ones too:
-//     24 of 1..700 17.3 / 14.7, 16 of 600 15.9 / 14.8, 32 of 600 20.3 / 18.8, 32 of 800 22.6 / 22.5, 32 of 1000 26.6 /
-//     27.0; 12 of 1..700 12.4 / 12.8.  Up to 512 keys and a pair for each CU; up to 800 for half as many on.  Rows of
-//     128 bytes: one of 440 9.1 / 7.5, 32 of 440 12.2 / 9.5, 32 of 1000 17.5 / 15.6, 24 of 100..1000 12.3 / 11.2, 32
-//     of 100..1500 17.9 / 22.4; one of 1000 9.9 / 10.9: up to 1024.  There two ranges a stage (pages of an odd
-//     number of 16 rows) gain as much here (one of 440 9.8 / 8.1), but elsewhere less than the per-lane form:
-//     64 of 64..2047 per lane 32.9, two ranges 37.4.
-//     Beyond that four waves attend a whole pair of up to 256 keys (one batch of page numbers), for as many pairs as
-//     there are workgroups: 64 of 64 9.0 -> 8.2, 48 of 200 16.3 -> 12.9, 40 of 30..120 9.5 -> 8.9, 64 of 250 16.0.  Not
-//     rows of 512 bytes (one of 200 12.0 -> 14.4) or 128 (7.4 -> 7.7).
-//   * Groups of more than 8 query heads, whose states are large: half as many parts.  us, four / eight: 16
+// What a launch does, by what the host sees: capacities, not lengths.
+//   * Few short pairs, a workgroup each: nothing to find or share, and no states pass through memory.  Eight waves
+//     for a pair a CU, us shared out / a workgroup each (8 KV heads of 128, bf16): one request of 100 keys 7.7 / 6.0,
+//     of 300 10.2 / 7.5, of 600 10.6 / 9.9, of 700 10.5 / 10.5, 8 of 300 10.5 / 8.4, 8 of 600 12.5 / 11.9, 8 of
+//     100..700 11.2 / 11.5; from half of the CUs on longer ones too: 32 of 1..700 17.9 / 14.3, 20 of 900 21.7 / 17.2,
+//     24 of 100..1000 18.0 / 16.3, 32 of 1000 26.6 / 24.9, but 32 of 30..2047 with 4 KV heads 22.5 / 27.7.  Up to
+//     700 keys, or 1024; twice that for rows of 128 bytes (one of 1000 9.4 / 8.6, 32 of 100..1800 18.3 / 16.0, 24 of
+//     2000 25.0 / 20.3; where a stage's rows are not one range one of 1000 9.7 / 11.1, so 700 stays).
+//     Four waves for as many pairs as there are workgroups (rows of 256 bytes): 64 of 64 9.0 / 7.5, 48 of 100..400
+//     19.0 / 15.4, 64 of 10..500 21.1 / 17.7, 40 of 600 27.5 / 23.5, 64 of 700 35.7 / 33.1, 64 of 10..750 23.7 / 22.3;
+//     40 of 64..1023 23.4 / 25.1.  Up to 768 keys.
+//   * Many stages: eight waves, half as many shares, so half as many cut pairs, but more waves with nothing to
+//     do in a short one.  us, four / eight: 128 requests of 100..4095 keys 180 / 174, 64 of 64..1023 33.4 / 30.8, 40 of
+//     64..1023 25.5 / 23.4, one of 65000 33.1 / 31.7, 8 of 1000..4000 24.7 / 24.3; 8 of 100..2000 14.1 / 14.7, 512 of
+//     20..200 32.8 / 41.6.  From 769 keys a request and 15000 stages and run ends in all, for up to 1024 pairs,
+//     where short requests cost little (under a mask: 64 of 64..1023 34.6 / 33.2, 32 of 30..2047 33.8 / 32.9, with 4
+//     KV heads of 8 query heads 21.5 / 22.7).  Not rows of 128 bytes: 64 of 64..2047 33.5 / 36.9, 128 of
+//     100..4000 94.6 / 95.6.
+//   * Groups of more than 8 query heads, whose states are large: eight waves, half as many parts.  us, four / eight: 16
 //     heads on one KV head, one request of 1000 keys 12.6 / 11.7, of 8000 18.8 / 16.4, of 60000 31.6 / 21.0, 8 of
 //     2000 16.5 / 13.2, 128 of 64..1023 20.5 / 19.1, 32 of 4000 26.1 / 22.3; 256 of 100..1000 24.8 / 25.2, 512 of
 //     20..200 20.1 / 20.4, 300 of 10..60 10.1 / 13.9.  From 192 keys on.  Groups of 8 lose as often (one of
 //     1000 and two KV heads 10.7 / 11.8, of 4000 and four 14.4 / 13.1).  Rows of 128 bytes from 2500 keys on: one
 //     of 1000 9.9 / 11.3, 8 of 2000 10.9 / 11.7, 32 of 4000 17.3 / 14.4, one of 8000 13.9 / 12.4.
-constexpr int64_t kLongRequest = 640, kManyStages = 15000, kFewPairs = 1024;
-constexpr int64_t kShortRequest = 512, kMiddleRequest = 800, kMiddleNarrow = 1024, kCUs = 256;
-constexpr int64_t kSmallRequest = 256;
+constexpr int64_t kLongRequest = 769, kManyStages = 15000, kFewPairs = 1024;
+constexpr int64_t kShortRequest = 700, kMiddleRequest = 1024, kCUs = 256;
+constexpr int64_t kSmallRequest = 768;
 constexpr int64_t kWideGroup = 8, kWideRequest = 192, kWideNarrow = 2500;
 
 template <typename T, int D>
@@ -980,23 +976,24 @@ struct Launch {
             return 0;
         return a->page_size % S::keys == 0 ? 1 : a->page_size % 16 == 0 ? 2 : 0;
     }
+    // one workgroup of eight waves, or of four, for each pair
     static bool few(const q3t_paged_args *a, int64_t pairs) {
-        return pairs <= kCUs && a->ctx <= (pairs < kCUs / 2 ? kShortRequest : S::row == 128 ? kMiddleNarrow : kMiddleRequest);
+        constexpr int64_t narrow = 256 / S::row;
+        return S::row < 512 && pairs <= kCUs &&
+               a->ctx <= (pairs >= kCUs / 2 ? kMiddleRequest * narrow : kShortRequest * (ranges(a) == 1 ? narrow : 1));
     }
+    static bool small(const q3t_paged_args *a, int64_t pairs) {
+        return S::row == 256 && ranges(a) == 1 && !eight(a, pairs) && pairs > kCUs && pairs <= Workgroups<T, D, 4>::count &&
+               a->ctx <= kSmallRequest;
+    }
+    static bool single(const q3t_paged_args *a, int64_t pairs) { return few(a, pairs) || small(a, pairs); }
     static bool eight(const q3t_paged_args *a, int64_t pairs) {
         const bool many = S::row > 128 && a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
         const bool wide = a->q_heads / a->kv_heads > kWideGroup && a->ctx >= (S::row == 128 ? kWideNarrow : kWideRequest);
-        return S::row < 512 && (ranges(a) == 1 ? many || wide || few(a, pairs) : ranges(a) == 2 && few(a, pairs));
-    }
-    static bool small(const q3t_paged_args *a, int64_t pairs) {
-        return S::row == 256 && ranges(a) == 1 && !eight(a, pairs) && pairs <= Workgroups<T, D, 4>::count && a->ctx <= kSmallRequest;
+        return few(a, pairs) || (S::row < 512 && ranges(a) == 1 && (many || wide));
     }
     static uint32_t log_least(const q3t_paged_args *a, int64_t pairs) {
-        if (eight(a, pairs)) return few(a, pairs) ? kLogLeastShort : kLogLeast8;
-        return small(a, pairs) ? kLogLeastShort : kLogLeast4;
-    }
-    static bool single(const q3t_paged_args *a, int64_t pairs) {
-        return small(a, pairs) || (eight(a, pairs) && few(a, pairs) && a->ctx <= (int64_t)S::keys << kLogLeastShort);
+        return single(a, pairs) ? kLogLeastSingle : eight(a, pairs) ? kLogLeast8 : kLogLeast4;
     }
     static int64_t workgroups(const q3t_paged_args *a, int64_t pairs) {
         const bool wide = eight(a, pairs);
@@ -1012,15 +1009,14 @@ struct Launch {
         auto masked = [&](auto mask) {
             constexpr bool MASK = decltype(mask)::value;
             if constexpr (S::row < 512) {
-                const bool wide = eight(a, pairs);
-                if (single(a, pairs)) {
+                if (few(a, pairs)) {
                     if constexpr (S::keys == 32)
                         if (ranges(a) == 2) return launch(paged_kernel<T, D, MASK, 2, 8, true>, 8);
-                    if constexpr (S::row == 256)
-                        if (!wide) return launch(paged_kernel<T, D, MASK, 1, 4, true>, 4);
-                    return launch(paged_kernel<T, D, MASK, 1, 8, true>, 8);
+                    return ranges(a) == 1 ? launch(paged_kernel<T, D, MASK, 1, 8, true>, 8) : launch(paged_kernel<T, D, MASK, 0, 8, true>, 8);
                 }
-                if (wide) return launch(paged_kernel<T, D, MASK, 1, 8, false>, 8);
+                if constexpr (S::row == 256)
+                    if (small(a, pairs)) return launch(paged_kernel<T, D, MASK, 1, 4, true>, 4);
+                if (eight(a, pairs)) return launch(paged_kernel<T, D, MASK, 1, 8, false>, 8);
             }
             if (ranges(a) == 1) launch(paged_kernel<T, D, MASK, 1, 4, false>, 4);
             else launch(paged_kernel<T, D, MASK, 0, 4, false>, 4);

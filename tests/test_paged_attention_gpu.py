@@ -80,6 +80,23 @@ def test_large_groups_over_long_requests(pkg, device, masked, dtype, width, head
 
 
 @pytest.mark.parametrize('masked', [False, True])
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (F32, 64), (BF16, 64)], ids=str)
+@pytest.mark.parametrize('page', [16, 24, 64])
+@pytest.mark.parametrize('lengths,rows', [([n % 749 for n in range(1, 40 * 173, 173)], 768), ([n % 1009 for n in range(3, 20 * 277, 277)], 960),
+                                          ([690, 3, 0, 64, 65, 512, 513], 696)], ids=['40', '20', 'few'])
+def test_a_workgroup_for_each_pair(pkg, device, lengths, rows, page, dtype, width, masked):
+    """Launches at the capacities up to which no pair is cut."""
+    lengths = [min(n, rows // page * page) for n in lengths]
+    p = problem(device, lengths, q_heads=16, kv_heads=8, width=width, dtype=dtype, page=page, table_width=rows // page, seed=32)
+    mask = None
+    if masked:
+        mask = torch.zeros(len(lengths), 1, 1, rows // page * page, device=device)
+        mask[:, :, :, 3::9] = -math.inf
+        mask[4] = -math.inf
+    assert_within(run(pkg, p, mask=mask), *expected(p, mask=mask))
+
+
+@pytest.mark.parametrize('masked', [False, True])
 @pytest.mark.parametrize('dtype', [BF16, F16], ids=str)
 @pytest.mark.parametrize('page', [16, 32, 48])
 @pytest.mark.parametrize('lengths', [[0, 1, 16, 17, 31, 33, 47, 49, 200, 255, 500], [n % 960 for n in range(1, 17 * 271, 271)]], ids=['few', 'more'])
