@@ -7,9 +7,9 @@
 // threshold.  Every key and value row is read once, so HBM bounds a launch of many keys (2 to 16
 // operations per byte), and the chain arguments - positions - page numbers - rows - merge one of few.
 // us per launch in a graph, rows not in the caches (TB/s of them): 128 requests of 100..4095 keys, 8 KV heads of
-// 128, bf16 175 (6.0, the rate of a large read); 64 of 64..1023 30.8 (4.8); one of 65000, 4 heads, fp16 32.7 (4.1);
-// 32 of 30..2047 under a mask, 4 heads 22.9 (3.2); 21 of 1..700 in float32 under a mask, 12 heads of 64 20.2
-// (2.7); one of 300 8.5.  The first rows are there after 5.8 us.
+// 128, bf16 175 (6.0, the rate of a large read); 64 of 64..1023 30.7 (4.9); one of 65000, 4 heads, fp16 32.7 (4.1);
+// 32 of 30..2047 under a mask, 4 heads 22.3 (3.3); 21 of 1..700 in float32 under a mask, 12 heads of 64 18.0
+// (3.1); one of 300 7.6.  The first rows are there after 5.8 us.
 //   * Work: a workgroup takes an equal share of the stages of all (request, KV head) pairs
 //     (paged_index.hpp), whatever the requests' lengths; its waves find their place by adding up all
 //     requests' stages.  A pair that lies in several shares leaves its parts' states in the
