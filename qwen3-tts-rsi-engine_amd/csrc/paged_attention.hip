@@ -86,7 +86,7 @@ struct Shape {
 
 // Workgroups of W waves, as many as fit the LDS of 256 CUs.
 template <typename T, int D, int W> struct Workgroups {
-    static constexpr int per_cu = Shape<T, D>::row * W > 256 * 4 ? 1 : 2;
+    static constexpr int per_cu = 2 * W * Shape<T, D>::stage > 64 * 1024 ? 1 : 2;
     static constexpr int count = 256 * per_cu;
 };
 
@@ -986,7 +986,12 @@ struct Launch {
         return S::row == 256 && ranges(a) == 1 && !eight(a, pairs) && pairs > kCUs && pairs <= Workgroups<T, D, 4>::count &&
                a->ctx <= kSmallRequest;
     }
-    static bool single(const q3t_paged_args *a, int64_t pairs) { return few(a, pairs) || small(a, pairs); }
+    static bool single(const q3t_paged_args *a, int64_t pairs) {
+        // a pair is one piece, and there is a workgroup for it
+        static_assert(S::row == 512 || kMiddleRequest * 256 / S::row <= (int64_t)S::keys << kLogLeastSingle, "");
+        static_assert(kSmallRequest <= (int64_t)S::keys << kLogLeastSingle && kCUs <= Workgroups<T, D, 8>::count, "");
+        return few(a, pairs) || small(a, pairs);
+    }
     static bool eight(const q3t_paged_args *a, int64_t pairs) {
         const bool many = S::row > 128 && a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
         const bool wide = a->q_heads / a->kv_heads > kWideGroup && a->ctx >= (S::row == 128 ? kWideNarrow : kWideRequest);
