@@ -26,7 +26,8 @@ signature compatibility):
   mask's values are read once, outside graph capture, and the result is kept per mask
   tensor;
 * a one-token step over a ``PagedCache`` rotates q and k, writes the new rows into their pages
-  and attends them with ``paged_attention`` under the layer's mask, if any;
+  and attends them with ``paged_attention`` under the layer's mask, if any
+  (``PagedCache.step``);
 * every other call rotates q/k with ``rotary`` (bf16-exact to torch eager), lets the cache
   update and calls ``attention`` (the npu_attention.attention drop-in).
 
@@ -41,7 +42,7 @@ from __future__ import annotations
 import torch
 
 from .attention import attention, decode_step, plan_shape, prefill_attention
-from .paged import PagedCache, paged_attention
+from .paged import PagedCache
 from .prefill import prefill_rope_write
 from .rotary import rotary
 from .slots import PredictorCache, PrefillCache, SlotCache
@@ -255,9 +256,8 @@ class PackedAttention(torch.nn.Module):
         if isinstance(past_key_values, PagedCache):
             if reference.training or getattr(reference, 'sliding_window', None) is not None:
                 raise ValueError('Paged attention is inference-only and without a sliding window')
-            pages = past_key_values.update(key, value, reference.layer_idx)
-            output = paged_attention(query.transpose(1, 2), *pages, past_key_values.page_table,
-                                     past_key_values.positions, scale=reference.scaling, mask=attention_mask)
+            output = past_key_values.step(query.transpose(1, 2), key, value, reference.layer_idx,
+                                          scale=reference.scaling, mask=attention_mask)
             return reference.o_proj(output.reshape(*shape, -1)), None
         if past_key_values is not None:
             key, value = past_key_values.update(key, value, reference.layer_idx,

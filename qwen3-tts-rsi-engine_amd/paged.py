@@ -99,6 +99,12 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     With it a request has K keys at most, else ``width * page_size``; a position outside
     those attends nothing.  A key under -inf (or False), or on no page of the pool, does not
     exist, whatever its rows hold; a request that attends nothing gets zero rows."""
+    return _attend(_attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out))
+
+
+def _attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out):
+    """An attention launch whose arguments have been checked, for ``_attend``: (query, out, device index, fields,
+    bytes of workspace); nothing has been launched on the pools yet."""
     if query.ndim != 4 or query.shape[1] != 1:
         raise ValueError('paged attention takes one token per request, (batch, 1, heads, head_dim)')
     batch, _, q_heads, head_dim = query.shape
@@ -116,7 +122,7 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     ctx = table_width * page_size
     mask_fields = (0, 0, 0, 0)
     if mask is not None:
-        if mask.dtype not in _lib.DTYPE_CODES:
+        if getattr(mask, 'dtype', None) not in _lib.DTYPE_CODES:
             raise ValueError('attention mask must be bool, bf16, fp16 or fp32')
         if not 1 <= mask.ndim <= 4 or not 1 <= mask.shape[-1] <= ctx or any(n != 1 for n in mask.shape[-3:-1]):
             raise ValueError('the mask must be broadcastable to (batch, 1, 1, keys), its keys within the page table')
@@ -127,6 +133,8 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
         except RuntimeError:
             raise ValueError('the mask must be broadcastable to (batch, 1, 1, keys)') from None
         mask_fields = (mask.data_ptr(), _lib.DTYPE_CODES[mask.dtype], rows.stride(0), rows.stride(3))
+        if max(mask_fields[2:]) >= 1 << 32:
+            raise ValueError('paged attention: mask strides must be below 2^32 elements')
     if out is None:
         out, os = torch.empty_like(query, memory_format=torch.contiguous_format), (q_heads * head_dim, 0, head_dim)
     else:
@@ -135,7 +143,7 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
         if any(n > 1 and s == 0 for n, s in zip(out.shape, os)):
             raise ValueError('paged attention: rows of out must not share memory')
     if batch == 0:
-        return out
+        return query, out, device, None, 0
     if query.data_ptr() % 16 or (qs[0] | qs[2]) * query.element_size() % 16:
         query = query.clone(memory_format=torch.contiguous_format)  # rows that 16-byte loads do not fit
         qs = query.stride()
@@ -147,6 +155,14 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     need = _lib.packed('q3t_paged_workspace_bytes')(_pack_attention(*fields, 0, 0))
     if need < 0:
         raise ValueError('paged attention: unsupported shape or dtype')
+    return query, out, device, fields, need
+
+
+def _attend(call):
+    """Launches what ``_attention_call`` has checked; the caller keeps its tensors."""
+    query, out, device, fields, need = call
+    if fields is None:
+        return out
     with _lib.on_device(device) as stream:
         ws = workspace(query.device, need, stream)
         status = _lib.packed('q3t_paged_attention')(_pack_attention(*fields, ws.data_ptr(), ws.numel()), stream)
@@ -223,8 +239,8 @@ class PagedArena:
 
 class PagedCache(Cache):
     """HF ``Cache`` over a paged arena for one-token steps: ``update`` writes request b's row at
-    ``positions[b]`` and returns the layer's pools, which ``PackedAttention`` reads with
-    ``paged_attention``.  ``page_table`` and ``positions`` are read at every step as they are
+    ``positions[b]`` and returns the layer's pools; ``step`` attends over them too, as
+    ``PackedAttention`` calls it.  ``page_table`` and ``positions`` are read at every step as they are
     then, so a captured step follows changes of their contents."""
 
     def __init__(self, arena, page_table, positions):
@@ -239,6 +255,14 @@ class PagedCache(Cache):
         key_pages, value_pages = self.arena.keys[layer_idx], self.arena.values[layer_idx]
         paged_write(keys, values, key_pages, value_pages, self.page_table, self.positions)
         return key_pages, value_pages
+
+    def step(self, query, keys, values, layer_idx, *, scale=None, mask=None):
+        """A layer's step: ``update`` with keys/values (B, Hkv, 1, D), then ``paged_attention`` of query
+        (B, 1, Hq, D).  A call that the attention refuses writes nothing."""
+        call = _attention_call(query, self.arena.keys[layer_idx], self.arena.values[layer_idx], self.page_table,
+                               self.positions, scale, mask, None)
+        self.update(keys, values, layer_idx)
+        return _attend(call)
 
     def get_seq_length(self, layer_idx=0):
         return 0  # the lengths are per request and live on the device: positions + 1

@@ -1,0 +1,88 @@
+"""What the paged cache's wrappers check and pass on, without a GPU: the device check is taken as
+passed, and launches are recorded instead of made."""
+import importlib
+from contextlib import contextmanager
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture
+def launches(pkg, monkeypatch):
+    """The calls that would have been launched: ('write',) or ('attend', argument structure)."""
+    lib, seen = pkg._lib, []
+    paged = importlib.import_module(pkg.__name__ + '.paged')
+    real = lib.packed
+
+    @contextmanager
+    def on_device(index):
+        yield 0
+
+    def packed(name):
+        if name != 'q3t_paged_attention':
+            return real(name)
+        return lambda args, stream: seen.append(('attend', lib.PagedArgs.from_buffer_copy(args))) or 0
+
+    monkeypatch.setattr(lib, 'gpu_index', lambda *tensors: 0)
+    monkeypatch.setattr(lib, 'on_device', on_device)
+    monkeypatch.setattr(lib, 'packed', packed)
+    monkeypatch.setattr(lib, 'launch', lambda name, *rest: seen.append(('write',)))
+    monkeypatch.setattr(paged, 'workspace', lambda device, size, stream: torch.empty(size, dtype=torch.uint8))
+    return seen
+
+
+def _tensors(batch=2, q_heads=16, kv_heads=8, width=128, page=16, pages=9, table=4, dtype=BF16):
+    return dict(query=torch.zeros(batch, 1, q_heads, width, dtype=dtype),
+                key_pages=torch.zeros(pages, kv_heads, page, width, dtype=dtype),
+                value_pages=torch.zeros(pages, kv_heads, page, width, dtype=dtype),
+                page_table=torch.zeros(batch, table, dtype=torch.int32), positions=torch.zeros(batch, dtype=torch.int64))
+
+
+def _cache(pkg, batch=2, width=128, table=4):
+    module = torch.nn.Linear(2, 2).bfloat16()
+    reference = SimpleNamespace(parameters=module.parameters, layers=[None],
+                                config=SimpleNamespace(num_key_value_heads=8, head_dim=width))
+    arena = pkg.PagedArena(reference, pages=9, page_size=16)
+    return pkg.PagedCache(arena, torch.zeros(batch, table, dtype=torch.int32), torch.zeros(batch, dtype=torch.int64))
+
+
+def _step(cache, batch=2, width=128, **kwargs):
+    rows = torch.zeros(batch, 8, 1, width, dtype=BF16)
+    return cache.step(torch.zeros(batch, 1, 16, width, dtype=BF16), rows, rows, 0, **kwargs)
+
+
+def test_a_step_writes_and_then_attends(pkg, launches):
+    out = _step(_cache(pkg), scale=0.25)
+    assert out.shape == (2, 1, 16, 128)
+    assert [call[0] for call in launches] == ['write', 'attend']
+    assert launches[1][1].scale == 0.25 and launches[1][1].ctx == 64
+
+
+@pytest.mark.parametrize('mask', [
+    torch.zeros(2, 1, 1, 65, dtype=BF16), torch.zeros(2, 1, 1, 64, dtype=torch.float64), torch.zeros(2, 1, 1, 64, dtype=torch.int64),
+    torch.zeros(2, 16, 1, 64, dtype=BF16), torch.zeros(3, 1, 1, 64, dtype=BF16), torch.zeros(2, 64, dtype=BF16), (0.0,) * 64,
+    torch.zeros(2, 1, 1, 0, dtype=BF16),
+], ids=['long', 'float64', 'int64', 'heads', 'batch', 'rows', 'tuple', 'none'])
+def test_a_refused_step_writes_nothing(pkg, launches, mask):
+    with pytest.raises(ValueError):
+        _step(_cache(pkg), mask=mask)
+    assert launches == []
+
+
+def test_a_step_under_a_mask_of_far_rows_writes_nothing(pkg, launches):
+    """Rows of a mask 2^32 elements apart (memory that is never touched)."""
+    mask = torch.empty((1 << 32) + 64, dtype=torch.bool).as_strided((2, 1, 1, 64), (1 << 32, 1, 1, 1))
+    with pytest.raises(ValueError):
+        _step(_cache(pkg), mask=mask)
+    assert launches == []
+
+
+def test_a_step_of_unsupported_sizes_writes_nothing(pkg, launches):
+    with pytest.raises(ValueError):
+        _step(_cache(pkg, width=96), width=96)
+    with pytest.raises(ValueError):  # rows of two tokens
+        _cache(pkg).step(torch.zeros(2, 2, 16, 128, dtype=BF16), *[torch.zeros(2, 8, 2, 128, dtype=BF16)] * 2, 0)
+    assert launches == []

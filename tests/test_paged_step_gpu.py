@@ -1,0 +1,36 @@
+"""Steps of ``PackedAttention`` over a ``PagedCache`` that are refused, or take an unusual mask."""
+import pytest
+import torch
+
+from tests._talker import Talker
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+def _layer(pkg, device, table_width=4):
+    model = Talker(layers=1, hidden=256, seed=3, dtype=BF16).to(device).eval()
+    pkg.install_packed_attention(model, native_gqa=True, text_only_rope=True, triton_talker_rope=True)
+    arena = pkg.PagedArena(model, pages=9, page_size=16)
+    arena.packed.normal_()
+    table = arena.page_table([arena.allocate(3), arena.allocate(3)], width=table_width)
+    return model, arena, pkg.PagedCache(arena, table, torch.tensor([40, 20], device=device))
+
+
+def _step(model, cache, hidden, mask):
+    tables = model.rotary_emb(hidden, cache.positions.expand(3, -1)[..., None])
+    with torch.inference_mode():
+        return model.layers[0](hidden, attention_mask=mask, past_key_values=cache, position_embeddings=tables)[0]
+
+
+@pytest.mark.parametrize('shape,dtype', [((2, 1, 1, 65), BF16), ((2, 1, 1, 64), torch.float64), ((2, 16, 1, 64), BF16),
+                                         ((3, 1, 1, 64), BF16), ((2, 64), BF16)], ids=str)
+def test_a_refused_step_leaves_the_pages(pkg, device, shape, dtype):
+    model, arena, cache = _layer(pkg, device)
+    before = arena.packed.clone()
+    with pytest.raises(ValueError):
+        _step(model, cache, torch.randn(2, 1, 256, device=device, dtype=BF16), torch.zeros(shape, dtype=dtype, device=device))
+    torch.cuda.synchronize(device)
+    same = torch.equal(arena.packed, before)
+    assert same
