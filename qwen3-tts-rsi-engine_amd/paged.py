@@ -96,8 +96,9 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
 
     ``mask``: SDPA-style, broadcastable to (B, 1, 1, K) with K at most ``width * page_size``:
     bool (True attends) or additive (bf16 / fp16 / fp32, added to the scaled scores in float32).
-    With it a request has K keys at most, else ``width * page_size``; a position outside
-    those attends nothing.  A key under -inf (or False), or on no page of the pool, does not
+    A mask that ends in K > 1 gives a request K keys at most; without one, or with one term for all
+    keys (a last dimension of 1), it has ``width * page_size``.  A position outside those attends
+    nothing.  A key under -inf (or False), or on no page of the pool, does not
     exist, whatever its rows hold; a request that attends nothing gets zero rows."""
     return _attend(_attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out))
 
@@ -127,7 +128,8 @@ def _attention_call(query, key_pages, value_pages, page_table, positions, scale,
         if not 1 <= mask.ndim <= 4 or not 1 <= mask.shape[-1] <= ctx or any(n != 1 for n in mask.shape[-3:-1]):
             raise ValueError('the mask must be broadcastable to (batch, 1, 1, keys), its keys within the page table')
         _lib.gpu_index(query, mask)
-        ctx = mask.shape[-1]
+        if mask.shape[-1] > 1:  # else one term for all keys
+            ctx = mask.shape[-1]
         try:
             rows = mask.expand(batch, 1, 1, ctx)
         except RuntimeError:
@@ -241,7 +243,10 @@ class PagedCache(Cache):
     """HF ``Cache`` over a paged arena for one-token steps: ``update`` writes request b's row at
     ``positions[b]`` and returns the layer's pools; ``step`` attends over them too, as
     ``PackedAttention`` calls it.  ``page_table`` and ``positions`` are read at every step as they are
-    then, so a captured step follows changes of their contents."""
+    then, so a captured step follows changes of their contents.
+
+    The lengths live on the device, so ``get_seq_length`` is 0: pass the model ``position_ids``, and as
+    its mask None (a request then attends its keys up to its position) or one over the table's rows."""
 
     def __init__(self, arena, page_table, positions):
         super().__init__(layers=[])
@@ -258,7 +263,12 @@ class PagedCache(Cache):
 
     def step(self, query, keys, values, layer_idx, *, scale=None, mask=None):
         """A layer's step: ``update`` with keys/values (B, Hkv, 1, D), then ``paged_attention`` of query
-        (B, 1, Hq, D).  A call that the attention refuses writes nothing."""
+        (B, 1, Hq, D).  A call that the attention refuses writes nothing.
+
+        The mask must end in the key dimension: the one that transformers' ``create_causal_mask``
+        builds ends in a single key, since it cannot know the lengths, and is refused."""
+        if getattr(mask, 'shape', ())[-1:] == (1,) and self.page_table.shape[1] * self.arena.page_size > 1:
+            raise ValueError('the mask of a paged step must end in the key dimension')
         call = _attention_call(query, self.arena.keys[layer_idx], self.arena.values[layer_idx], self.page_table,
                                self.positions, scale, mask, None)
         self.update(keys, values, layer_idx)

@@ -86,3 +86,53 @@ def test_a_step_of_unsupported_sizes_writes_nothing(pkg, launches):
     with pytest.raises(ValueError):  # rows of two tokens
         _cache(pkg).step(torch.zeros(2, 2, 16, 128, dtype=BF16), *[torch.zeros(2, 8, 2, 128, dtype=BF16)] * 2, 0)
     assert launches == []
+
+
+@pytest.mark.parametrize('shape', [(2, 1, 1, 1), (1, 1, 1, 1), (1, 1), (1,)], ids=str)
+@pytest.mark.parametrize('dtype', [torch.bool, BF16, torch.float32], ids=str)
+def test_a_mask_of_one_term_is_for_all_keys(pkg, launches, shape, dtype):
+    pkg.paged_attention(**_tensors(), mask=torch.ones(shape, dtype=dtype))
+    a = launches[0][1]
+    assert a.ctx == 64 and a.mask and a.mask_stride_t == 0 and a.mask_stride_b == (1 if shape[0] == 2 else 0)
+
+
+def test_a_mask_of_several_keys_bounds_them(pkg, launches):
+    pkg.paged_attention(**_tensors(), mask=torch.ones(2, 1, 1, 2, dtype=torch.bool))
+    pkg.paged_attention(**_tensors(), mask=torch.ones(2, 1, 1, 64, dtype=torch.bool))
+    pkg.paged_attention(**_tensors())
+    assert [call[1].ctx for call in launches] == [2, 64, 64]
+    assert launches[0][1].mask_stride_t == launches[1][1].mask_stride_t == 1
+
+
+@pytest.mark.parametrize('dtype', [torch.bool, BF16], ids=str)
+def test_a_step_refuses_a_mask_of_one_key(pkg, launches, dtype):
+    for shape in ((2, 1, 1, 1), (1, 1, 1, 1), (1,)):
+        with pytest.raises(ValueError, match='key dimension'):
+            _step(_cache(pkg), mask=torch.ones(shape, dtype=dtype))
+    assert launches == []
+
+
+def test_a_step_over_one_key_takes_its_mask(pkg, launches):
+    cache = _cache(pkg)
+    cache.arena.page_size = 1
+    cache.arena.keys, cache.arena.values = [[torch.zeros(9, 8, 1, 128, dtype=BF16)] for _ in range(2)]
+    cache.page_table = torch.zeros(2, 1, dtype=torch.int32)
+    _step(cache, mask=torch.ones(2, 1, 1, 1, dtype=torch.bool))
+    assert [call[0] for call in launches] == ['write', 'attend'] and launches[1][1].ctx == 1
+
+
+@pytest.mark.parametrize('implementation', ['eager', 'sdpa'])
+def test_masks_that_transformers_builds_are_refused(pkg, launches, implementation):
+    from transformers import Qwen3Config
+    from transformers.masking_utils import create_causal_mask
+    config = Qwen3Config(hidden_size=256, num_attention_heads=2, num_key_value_heads=1, head_dim=128, num_hidden_layers=1)
+    config._attn_implementation = implementation
+    cache = _cache(pkg)
+    padded = torch.ones(2, 40, dtype=torch.int64)
+    padded[0, :7] = 0
+    mask = create_causal_mask(config=config, inputs_embeds=torch.zeros(2, 1, 256, dtype=BF16), attention_mask=padded,
+                              past_key_values=cache, position_ids=torch.tensor([[39], [39]]))
+    assert mask is not None
+    with pytest.raises(ValueError):
+        _step(cache, mask=mask)
+    assert launches == []

@@ -1,7 +1,10 @@
 """Steps of ``PackedAttention`` over a ``PagedCache`` that are refused, or take an unusual mask."""
+import math
+
 import pytest
 import torch
 
+from tests._paged import assert_within, expected, problem, run
 from tests._talker import Talker
 
 pytestmark = pytest.mark.gpu
@@ -25,7 +28,8 @@ def _step(model, cache, hidden, mask):
 
 
 @pytest.mark.parametrize('shape,dtype', [((2, 1, 1, 65), BF16), ((2, 1, 1, 64), torch.float64), ((2, 16, 1, 64), BF16),
-                                         ((3, 1, 1, 64), BF16), ((2, 64), BF16)], ids=str)
+                                         ((3, 1, 1, 64), BF16), ((2, 64), BF16), ((2, 1, 1, 1), BF16),
+                                         ((2, 1, 1, 1), torch.bool), ((1, 1, 1, 1), torch.float32)], ids=str)
 def test_a_refused_step_leaves_the_pages(pkg, device, shape, dtype):
     model, arena, cache = _layer(pkg, device)
     before = arena.packed.clone()
@@ -34,3 +38,19 @@ def test_a_refused_step_leaves_the_pages(pkg, device, shape, dtype):
     torch.cuda.synchronize(device)
     same = torch.equal(arena.packed, before)
     assert same
+
+
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (torch.float16, 64), (torch.float32, 64)], ids=str)
+@pytest.mark.parametrize('kind', [torch.bool, BF16, torch.float32], ids=str)
+@pytest.mark.parametrize('table_width', [None, 300])
+def test_a_mask_of_one_term_is_for_all_keys(pkg, device, dtype, width, kind, table_width):
+    """SDPA's meaning of a last dimension of 1: a request is shown all of its keys, or none."""
+    p = problem(device, [1, 40, 300, 17, 0], width=width, dtype=dtype, seed=40, table_width=table_width)
+    ctx = p.table.shape[1] * p.page
+    shown = torch.tensor([True, True, True, False, True], device=device)[:, None, None, None]
+    mask = shown if kind == torch.bool else torch.where(shown, 1.5, -math.inf).to(kind)
+    out = run(pkg, p, mask=mask)
+    assert (out[3] == 0).all() and (out[4] == 0).all()
+    assert_within(out, *expected(p, mask=mask.expand(5, 1, 1, ctx)))
+    for one in (mask[:1], mask[0, 0, 0], mask[:1].expand(5, 1, 1, 1)):
+        assert_within(run(pkg, p, mask=one), *expected(p, mask=one.expand(5, 1, 1, ctx)))
