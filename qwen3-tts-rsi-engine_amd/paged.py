@@ -49,6 +49,20 @@ def _check_pools(key_pages, value_pages, page_table, positions, batch):
     return ks, vs, ts[0], width
 
 
+def _rows_overlap(row, count, stride, other_count, other_stride):
+    """Whether any two rows of ``row`` elements at i * stride + j * other_stride, i < count, j < other_count,
+    share one."""
+    (inner, inner_count), (outer, outer_count) = sorted(((stride, count), (other_stride, other_count)))
+    if inner_count > 1 and inner < row:
+        return True
+    if outer_count == 1 or outer >= (inner_count - 1) * inner + row:
+        return False
+    # a row i outer strides on lies between two rows of the inner dimension, or past their last
+    return outer < row or inner_count > 1 and any(
+        i * outer % inner < row and i * outer // inner < inner_count
+        or -i * outer % inner < row and -(-i * outer // inner) < inner_count for i in range(1, outer_count))
+
+
 def paged_write(keys, values, key_pages, value_pages, page_table, positions, lengths=None):
     """Write the rows keys/values (B, Hkv, T, D) of every request into its pages, from row
     ``positions[b]`` on; one launch for both, bit-exact.
@@ -142,7 +156,7 @@ def _attention_call(query, key_pages, value_pages, page_table, positions, scale,
     else:
         _check_out(out, (batch, 1, q_heads, head_dim), dtype, query.device, 'paged attention')
         os = out.stride()
-        if any(n > 1 and s == 0 for n, s in zip(out.shape, os)):
+        if _rows_overlap(head_dim, batch, os[0], q_heads, os[2]):
             raise ValueError('paged attention: rows of out must not share memory')
     if batch == 0:
         return query, out, device, None, 0

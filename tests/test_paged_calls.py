@@ -1,6 +1,7 @@
 """What the paged cache's wrappers check and pass on, without a GPU: the device check is taken as
 passed, and launches are recorded instead of made."""
 import importlib
+import random
 from contextlib import contextmanager
 from types import SimpleNamespace
 
@@ -136,3 +137,31 @@ def test_masks_that_transformers_builds_are_refused(pkg, launches, implementatio
     with pytest.raises(ValueError):
         _step(cache, mask=mask)
     assert launches == []
+
+
+def test_overlapping_rows_are_told_from_others(pkg):
+    overlap = importlib.import_module(pkg.__name__ + '.paged')._rows_overlap
+    rng, found = random.Random(0), [0, 0]
+    for _ in range(20000):
+        row, counts = rng.randrange(1, 6), [rng.randrange(1, 6) for _ in range(2)]
+        strides = [rng.choice([0, rng.randrange(0, 12), rng.randrange(0, 60)]) for _ in range(2)]
+        places = [i * strides[0] + j * strides[1] + e for i in range(counts[0]) for j in range(counts[1]) for e in range(row)]
+        want = len(set(places)) < len(places)
+        assert overlap(row, counts[0], strides[0], counts[1], strides[1]) == want, (row, counts, strides)
+        found[want] += 1
+    assert min(found) > 1000
+
+
+@pytest.mark.parametrize('strides,refused', [
+    ((2048, 128), False), ((128, 256), False), ((4096, 256), False), ((2048 + 64, 128), False), ((128, 384), False),
+    ((192, 384), False), ((0, 128), True), ((2048, 0), True), ((2048, 64), True), ((1024, 128), True), ((64, 256), True),
+    ((2047, 128), True), ((384, 192), True),
+], ids=str)
+def test_outputs_whose_rows_share_memory_are_refused(pkg, launches, strides, refused):
+    out = torch.zeros(20000, dtype=BF16).as_strided((2, 1, 16, 128), (strides[0], 128, strides[1], 1))
+    if refused:
+        with pytest.raises(ValueError, match='share memory'):
+            pkg.paged_attention(**_tensors(), out=out)
+        assert launches == []
+    else:
+        assert pkg.paged_attention(**_tensors(), out=out) is out and len(launches) == 1
