@@ -26,6 +26,7 @@ from transformers.cache_utils import Cache
 
 from . import _lib
 from .attention import _check_out, workspace
+from .rotary import _share_memory
 
 _pack_attention = _lib.packer(_lib.PagedArgs)
 _pack_write = _lib.packer(_lib.PagedWriteArgs)
@@ -71,7 +72,8 @@ def paged_write(keys, values, key_pages, value_pages, page_table, positions, len
     page_table (B, width) int32; positions (B,) int64; lengths (B,) int32: only the first
     ``lengths[b]`` of the T rows belong to request b (a right-padded batch).  bf16, fp16 or
     fp32.  Rows outside the table's ``width * page_size`` rows, or on no page of the pool, are
-    skipped on the device; everything else of the pools stays as it was."""
+    skipped on the device; everything else of the pools stays as it was.  keys/values must not
+    overlap the rows that are written."""
     if keys.ndim != 4 or values.shape != keys.shape:
         raise ValueError('Expected matching BNSD K/V')
     batch, heads, tokens, width = keys.shape
@@ -106,7 +108,8 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     key_pages/value_pages (pages, Hkv, page_size, D), by any strides with unit-stride rows.
     Returns (B, 1, Hq, D); bf16, fp16 or fp32, head_dim 64 or 128, any number of query heads
     that is a multiple of the KV heads.  Rows of the pools start at multiples of 16 bytes, and
-    there are at most 64512 requests times KV heads (times blocks of 16 query heads of one).
+    there are at most 64512 requests times KV heads (times blocks of 16 query heads of one).  ``out``
+    may be the query itself; other tensors of the call it must not overlap.
 
     ``mask``: SDPA-style, broadcastable to (B, 1, 1, K) with K at most ``width * page_size``:
     bool (True attends) or additive (bf16 / fp16 / fp32, added to the scaled scores in float32).
@@ -158,6 +161,9 @@ def _attention_call(query, key_pages, value_pages, page_table, positions, scale,
         os = out.stride()
         if _rows_overlap(head_dim, batch, os[0], q_heads, os[2]):
             raise ValueError('paged attention: rows of out must not share memory')
+        same = out.data_ptr() == query.data_ptr() and all(n == 1 or o == s for n, o, s in zip(out.shape, os, qs))
+        if not same and _share_memory(query, out):
+            raise ValueError('paged attention: out must be the query itself, row by row, or lie apart from it')
     if batch == 0:
         return query, out, device, None, 0
     if query.data_ptr() % 16 or (qs[0] | qs[2]) * query.element_size() % 16:

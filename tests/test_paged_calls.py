@@ -165,3 +165,19 @@ def test_outputs_whose_rows_share_memory_are_refused(pkg, launches, strides, ref
         assert launches == []
     else:
         assert pkg.paged_attention(**_tensors(), out=out) is out and len(launches) == 1
+
+
+def test_outputs_over_other_rows_of_the_query_are_refused(pkg, launches):
+    room = torch.zeros(2, 1, 40, 128, dtype=BF16)
+    call = _tensors()
+    call['query'] = room[:, :, 8:24]
+    for out in (room[:, :, 7:23], room[:, :, 9:25], room[:, :, :16], room[:, :, 23:39], room.view(-1)[8 * 128:][:4096].view(2, 1, 16, 128)):
+        with pytest.raises(ValueError, match='query itself'):
+            pkg.paged_attention(**call, out=out)
+    assert launches == []
+    for out in (room[:, :, 8:24], room[:, :, 24:], torch.zeros(2, 1, 16, 128, dtype=BF16)):
+        assert pkg.paged_attention(**call, out=out) is out
+    one = _tensors(batch=1)
+    view = one['query'].as_strided((1, 1, 16, 128), (7, 11, 128, 1))  # strides of single entries mean nothing
+    assert pkg.paged_attention(**one, out=view) is view
+    assert len(launches) == 4

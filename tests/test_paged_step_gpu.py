@@ -54,3 +54,13 @@ def test_a_mask_of_one_term_is_for_all_keys(pkg, device, dtype, width, kind, tab
     assert_within(out, *expected(p, mask=mask.expand(5, 1, 1, ctx)))
     for one in (mask[:1], mask[0, 0, 0], mask[:1].expand(5, 1, 1, 1)):
         assert_within(run(pkg, p, mask=one), *expected(p, mask=one.expand(5, 1, 1, ctx)))
+
+
+@pytest.mark.parametrize('dtype', [BF16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize('heads', [(16, 8), (20, 1)], ids=str)
+@pytest.mark.parametrize('lengths', [[100, 3, 0, 333], [9000, 17, 4000]], ids=['short', 'cut'])
+def test_the_output_may_be_the_query(pkg, device, dtype, heads, lengths):
+    p = problem(device, lengths, q_heads=heads[0], kv_heads=heads[1], dtype=dtype, seed=41)
+    want = run(pkg, p)
+    assert run(pkg, p, out=p.query) is p.query
+    assert torch.equal(p.query, want)
