@@ -64,3 +64,33 @@ def test_the_output_may_be_the_query(pkg, device, dtype, heads, lengths):
     want = run(pkg, p)
     assert run(pkg, p, out=p.query) is p.query
     assert torch.equal(p.query, want)
+
+
+@pytest.mark.parametrize('masked', [False, True])
+@pytest.mark.parametrize('below', [5.0, 23.0, 25.0, 40.0, 80.0])
+@pytest.mark.parametrize('dtype', [BF16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize('lengths', [[100, 40], [5000, 2000]], ids=['short', 'cut'])
+def test_infinite_values_under_small_weights_show(pkg, device, dtype, lengths, below, masked):
+    """An attended infinity is an infinity of the output down to float32's smallest weights (e^-87), and NaN a
+    NaN; other elements keep their values.  All scores are 0 but one key's, ``below`` higher."""
+    p = problem(device, lengths, q_heads=4, kv_heads=2, dtype=dtype, seed=42)
+    p.query.zero_()
+    p.query[..., 0] = 8.0
+    for b, n in enumerate(lengths):
+        at = p.table[b, :-(-n // 16)].long()
+        p.key_pages[at] = 0
+        p.key_pages[at[1], :, 3, 0] = below * 128 ** 0.5 / 8.0
+    mask = torch.zeros(2, 1, 1, p.table.shape[1] * 16, device=device) if masked else None
+    clean, tol = expected(p, mask=mask)
+    assert_within(run(pkg, p, mask=mask), clean, tol)
+    first, last = int(p.table[0, 0]), int(p.table[0, (lengths[0] - 1) // 16])
+    p.value_pages[first, 0, 4, 17] = math.inf
+    p.value_pages[last, 0, 0, 18] = -math.inf
+    p.value_pages[first, 0, 5, 19] = math.inf
+    p.value_pages[last, 0, 1, 19] = -math.inf
+    p.value_pages[last, 0, 2, 20] = math.nan
+    out = run(pkg, p, mask=mask).cpu()
+    for h in (0, 1):
+        assert out[0, 0, h, 17] == math.inf and out[0, 0, h, 18] == -math.inf and out[0, 0, h, 19:21].isnan().all()
+        out[0, 0, h, 17:21], clean[0, 0, h, 17:21] = 0, 0
+    assert_within(out, clean, tol)
