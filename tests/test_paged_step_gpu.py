@@ -72,14 +72,15 @@ def test_the_output_may_be_the_query(pkg, device, dtype, heads, lengths):
 @pytest.mark.parametrize('lengths', [[100, 40], [5000, 2000]], ids=['short', 'cut'])
 def test_infinite_values_under_small_weights_show(pkg, device, dtype, lengths, below, masked):
     """An attended infinity is an infinity of the output down to float32's smallest weights (e^-87), and NaN a
-    NaN; other elements keep their values.  All scores are 0 but one key's, ``below`` higher."""
+    NaN; other elements keep their values.  All scores are 0 but those of row 3 of every page, ``below`` higher:
+    each stage of a wave has the maximum."""
     p = problem(device, lengths, q_heads=4, kv_heads=2, dtype=dtype, seed=42)
     p.query.zero_()
     p.query[..., 0] = 8.0
     for b, n in enumerate(lengths):
         at = p.table[b, :-(-n // 16)].long()
         p.key_pages[at] = 0
-        p.key_pages[at[1], :, 3, 0] = below * 128 ** 0.5 / 8.0
+        p.key_pages[at, :, 3, 0] = below * 128 ** 0.5 / 8.0
     mask = torch.zeros(2, 1, 1, p.table.shape[1] * 16, device=device) if masked else None
     clean, tol = expected(p, mask=mask)
     assert_within(run(pkg, p, mask=mask), clean, tol)
