@@ -110,6 +110,8 @@ def _extent(dims, row):
 def _share_memory(x, y=None):
     """Whether rows of x overlap each other, or rows of y; True as well where no nesting of the
     dimensions (each stride passes all that lies within it) shows that they do not."""
+    if x.numel() == 0 or (y is not None and y.numel() == 0):
+        return False
     row, dims = x.shape[-1], _dims(x)
     if y is None:
         return any(s < _extent(dims[i + 1:], row) for i, (s, _) in enumerate(dims))

@@ -181,3 +181,17 @@ def test_outputs_over_other_rows_of_the_query_are_refused(pkg, launches):
     view = one['query'].as_strided((1, 1, 16, 128), (7, 11, 128, 1))  # strides of single entries mean nothing
     assert pkg.paged_attention(**one, out=view) is view
     assert len(launches) == 4
+
+
+def test_empty_tensors_share_no_memory(pkg, launches):
+    """Empty tensors have one address, null: calls in place on them do nothing."""
+    query, key = torch.zeros(3, 5, 16, 128), torch.zeros(3, 5, 8, 128)
+    for at in ((slice(0), slice(None)), (slice(None), slice(0))):
+        q, k = query[at], key[at]
+        positions = torch.zeros(3, *q.shape[:2], dtype=torch.int64)
+        out = pkg.rotary_axes(q, k, positions, (24, 20, 20), inv_freq=torch.ones(64), inplace=True)
+        assert out[0] is q and out[1] is k
+    call = _tensors(batch=0)
+    for out in (torch.zeros(0, 1, 16, 128, dtype=BF16), torch.zeros(5, 1, 32, 128, dtype=BF16)[:0, :, :16]):
+        assert pkg.paged_attention(**call, out=out) is out
+    assert launches == []
