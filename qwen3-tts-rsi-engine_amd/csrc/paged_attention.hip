@@ -4,12 +4,17 @@
 //   s_j = scale q . k_j (+ mask_j),  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
 //
 // in one pass over the keys, with a running maximum m that moves when it is passed by more than a
-// threshold.  Every key and value row is read once, so HBM bounds a launch of many keys (2 to 16
-// operations per byte), and the chain arguments - positions - page numbers - rows - merge one of few.
+// threshold.  Every key and value row is read once for 16 query heads of its KV head, so HBM bounds a launch of
+// many keys (2 to 16 operations per byte), and the chain arguments - positions - page numbers - rows - merge one of few.
 // us per launch in a graph, rows not in the caches (TB/s of them): 128 requests of 100..4095 keys, 8 KV heads of
 // 128, bf16 175 (6.0, the rate of a large read); 64 of 64..1023 30.7 (4.9); one of 65000, 4 heads, fp16 32.7 (4.1);
 // 32 of 30..2047 under a mask, 4 heads 22.3 (3.3); 21 of 1..700 in float32 under a mask, 12 heads of 64 18.0
 // (3.1); one of 300 7.6.  The first rows are there after 5.8 us.
+// float32 rows of 128: 64 of 64..1023 54.0 (5.5), 128 of 100..2000 192 (5.9), one of 30000 49.3 (5.0), one of 300
+// 11.6.  Pages that hold no whole stages: 128 of 100..2000 in bf16 in pages of 16 / 24 / 100 96.0 / 101 / 98.7.
+// Each further block of 16 query heads of a KV head reads that head's rows again, from memory: 64 requests of 2000
+// keys, 2 KV heads of 128 in bf16, with 16 / 20 / 32 / 48 query heads each 30.3 / 47.4 / 46.8 / 67.6 us (135 / 263 / 264 /
+// 381 MB fetched); 8 requests of 4000 18.2 / 19.1 / 19.6 / 25.9.
 //   * Work: a workgroup takes an equal share of the stages of all (request, KV head) pairs
 //     (paged_index.hpp), whatever the requests' lengths; its waves find their place by adding up all
 //     requests' stages.  A pair that lies in several shares leaves its parts' states in the
@@ -20,8 +25,11 @@
 //     every W-th.  A stage's rows go straight from memory to the wave's own two LDS slots, one stage
 //     ahead of the one that is scored, over the ends of runs: no barrier but where a run ends.  The
 //     page numbers of up to 64 stages come the same way, while the stages before them are read.
-//     Where pages hold whole stages (or halves of 16 keys) the rows are one range of memory (two); for other
-//     page sizes each lane works out the address of its own row.
+//     Where pages hold whole stages the rows are one range of memory; for other page sizes each lane works out
+//     the address of its own row.  In pages of halves of a stage of 32 (16 rows of 128 bytes each) they are two
+//     ranges where a pair has a workgroup to itself, and single rows elsewhere, where ranges gain nothing (us, rows /
+//     ranges, 64 columns in fp16, pages of 16: 128 requests of 100..4000 keys 89.7 / 90.2, 64 of 64..2047 32.8 / 33.0, 200 of
+//     10..400 25.8 / 26.1).
 //   * The rows of a KV head's query heads are the columns of 16x16 products, S^T = K . Q^T and
 //     O^T += V^T . P^T.  The matrix cores idle (under a twentieth of their rate), so the weights are
 //     not rounded to the cache's type: bf16 weights go in three parts (all 24 bits of their
@@ -943,7 +951,11 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
     }
 }
 
-// What a launch does, by what the host sees: capacities, not lengths.
+// What a launch does, by what the host sees: capacities, not lengths.  The figures are of tables as wide as the longest
+// request; requests in a wider table run as the table's width has it.  us, 8 KV heads of 128 in bf16, exact / 1024 /
+// 4096 / 32000 rows: one request of 300 keys 7.6 / 10.3 / 10.3 / 9.7, 8 of 300 8.3 / 10.9 / 10.1 / 10.2, 32 of 300 10.7 /
+// 10.7 / 12.0 / 12.0, 64 of 64 8.0 / 11.9 / 11.9 / 12.0, 48 of 100..400 15.4 / 18.6 / 18.7 / 18.6, 64 of 64..1023 31.7 / 30.6 /
+// 30.5 / 30.5.
 //   * Few short pairs, a workgroup each: nothing to find or share, and no states pass through memory.  Eight waves
 //     for a pair a CU, us shared out / a workgroup each (8 KV heads of 128, bf16): one request of 100 keys 7.7 / 6.0,
 //     of 300 10.2 / 7.5, of 600 10.6 / 9.9, of 700 10.5 / 10.5, 8 of 300 10.5 / 8.4, 8 of 600 12.5 / 11.9, 8 of
@@ -958,9 +970,10 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, Params p) {
 //     do in a short one.  us, four / eight: 128 requests of 100..4095 keys 180 / 174, 64 of 64..1023 33.4 / 30.8, 40 of
 //     64..1023 25.5 / 23.4, one of 65000 33.1 / 31.7, 8 of 1000..4000 24.7 / 24.3; 8 of 100..2000 14.1 / 14.7, 512 of
 //     20..200 32.8 / 41.6.  From 769 keys a request and 15000 stages and run ends in all, for up to 1024 pairs,
-//     where short requests cost little (under a mask: 64 of 64..1023 34.6 / 33.2, 32 of 30..2047 33.8 / 32.9, with 4
-//     KV heads of 8 query heads 21.5 / 22.7).  Not rows of 128 bytes: 64 of 64..2047 33.5 / 36.9, 128 of
-//     100..4000 94.6 / 95.6.
+//     where short requests cost little.  Under a mask too: 64 of 64..1023 33.3 / 31.8, 32 of 30..2047 33.2 / 32.1, 128 of
+//     100..2000 with 4 KV heads 57.7 / 53.8, 8 of 1000..4000 25.1 / 25.1; the rule costs 1 to 3% in the smallest masked
+//     launches that it takes (32 of 30..2047 with 4 KV heads of 4 query heads 21.6 / 21.9, of 8 21.9 / 22.4).  Not
+//     rows of 128 bytes: 64 of 64..2047 33.5 / 36.9, 128 of 100..4000 94.6 / 95.6.
 //   * Groups of more than 8 query heads, whose states are large: eight waves, half as many parts.  us, four / eight: 16
 //     heads on one KV head, one request of 1000 keys 12.6 / 11.7, of 8000 18.8 / 16.4, of 60000 31.6 / 21.0, 8 of
 //     2000 16.5 / 13.2, 128 of 64..1023 20.5 / 19.1, 32 of 4000 26.1 / 22.3; 256 of 100..1000 24.8 / 25.2, 512 of

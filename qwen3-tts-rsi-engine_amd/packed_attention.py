@@ -33,7 +33,8 @@ signature compatibility):
 
 ``fused_qk_norm=True`` (an extension, off by default) also moves the module's q_norm /
 k_norm (RMSNorm over head_dim, packed_attention.py:42-45) into that fused launch: the raw
-projection rows go in, and the per-layer chain of norm kernels disappears.  The norm's fp32
+projection rows go in, and the per-layer chain of norm kernels disappears (every other path,
+the step over a ``PagedCache`` among them, runs the module's norms).  The norm's fp32
 row sums then follow the kernel's order, so normalised rows can differ from the module's in
 the last bf16 bit (the reference's own norm runs with yet another order on its device).
 """
