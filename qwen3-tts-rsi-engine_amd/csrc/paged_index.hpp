@@ -13,7 +13,8 @@
 namespace q3t {
 
 // Division of 0 <= n < 2^31 by a divisor in [1, 2^31) as a multiplication, an addition and a
-// shift (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994): with 2^(l-1) < d <= 2^l and m = floor(2^32 (2^l - d) / d) + 1, floor(n / d) is
+// shift (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994): with
+// 2^(l-1) < d <= 2^l and m = floor(2^32 (2^l - d) / d) + 1, floor(n / d) is
 // (floor(m n / 2^32) + n) >> l (the sum stays below 2^32 since floor(m n / 2^32) <= n < 2^31).
 struct Divisor {
     uint32_t d, m, l;

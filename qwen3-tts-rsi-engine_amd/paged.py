@@ -115,8 +115,8 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     bool (True attends) or additive (bf16 / fp16 / fp32, added to the scaled scores in float32).
     A mask that ends in K > 1 gives a request K keys at most; without one, or with one term for all
     keys (a last dimension of 1), it has ``width * page_size``.  A position outside those attends
-    nothing.  A key under -inf (or False), or on no page of the pool, does not
-    exist, whatever its rows hold; a request that attends nothing gets zero rows."""
+    nothing.  A key under -inf (or False), or on no page of the pool, does not exist, whatever its
+    rows hold; a request that attends nothing gets zero rows."""
     return _attend(_attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out))
 
 
