@@ -95,3 +95,18 @@ def test_infinite_values_under_small_weights_show(pkg, device, dtype, lengths, b
         assert out[0, 0, h, 17] == math.inf and out[0, 0, h, 18] == -math.inf and out[0, 0, h, 19:21].isnan().all()
         out[0, 0, h, 17:21], clean[0, 0, h, 17:21] = 0, 0
     assert_within(out, clean, tol)
+
+
+@pytest.mark.parametrize('masked', [False, True])
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (torch.float16, 128), (torch.float16, 64), (torch.float32, 64)], ids=str)
+@pytest.mark.parametrize('lengths', [[100, 40], [5000, 2000]], ids=['short', 'cut'])
+def test_an_attended_key_that_is_nan_shows(pkg, device, dtype, width, lengths, masked):
+    """Its score is NaN, and with it all of its head's outputs; other heads and requests keep their values."""
+    p = problem(device, lengths, q_heads=4, kv_heads=2, width=width, dtype=dtype, seed=43)
+    mask = torch.zeros(2, 1, 1, p.table.shape[1] * 16, device=device) if masked else None
+    clean, tol = expected(p, mask=mask)
+    p.key_pages[int(p.table[0, (lengths[0] - 1) // 16]), 1, 2, 9] = math.nan
+    out = run(pkg, p, mask=mask).cpu()
+    assert out[0, 0, 2:].isnan().all()
+    out[0, 0, 2:], clean[0, 0, 2:] = 0, 0
+    assert_within(out, clean, tol)
