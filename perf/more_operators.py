@@ -135,7 +135,8 @@ def _quantised(x, store):
         return (x.float() * (127 / largest)[..., None]).round().to(torch.int8), largest / 127
     part, exponent = torch.frexp(largest)  # part in [1/2, 1)
     exponent = exponent - torch.where(part <= 0.875, 9, 8)
-    return torch.ldexp(x.float(), -exponent[..., None]).to(torch.float8_e4m3fn), torch.ldexp(torch.ones_like(largest), exponent)
+    power = lambda n: (n + 127 << 23).to(torch.int32).view(torch.float32)  # 2^n, exactly
+    return (x.float() * power(-exponent)[..., None]).to(torch.float8_e4m3fn), power(exponent)
 
 
 def _quantised_pool(x, store):
@@ -362,6 +363,11 @@ def work(case):
 
 # ---- in 64 bits ----------------------------------------------------------------------------
 
+def _power64(n):
+    """2^n in float64, exactly."""
+    return (n.long() + 1023 << 52).view(torch.float64)
+
+
 def _values64(pool, scales, index):
     """Rows of a pool, by an index of its pages, heads and rows, as float64."""
     if scales is None:
@@ -414,11 +420,11 @@ def _exact_store(s):
                 out[b, :, :count] = torch.round(x * 127 / a) * (a / 127)
                 continue
             _, above = torch.frexp(a / 448 * (1 - 2.0 ** -50))  # the smallest power of two at or over a / 448 (not the next for a power)
-            step = torch.ldexp(torch.ones_like(a), above)
+            step = _power64(above)
             y = x / step
             # e4m3: four significant bits, whole multiples of 2^-9 below 2^-6
             _, above = torch.frexp(y.abs().clamp(min=2.0 ** -6))
-            unit = torch.ldexp(torch.ones_like(y), above - 4)
+            unit = _power64(above - 4)
             out[b, :, :count] = torch.round(y / unit) * unit * step
         found.append(out)
     return tuple(found)
