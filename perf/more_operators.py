@@ -132,7 +132,8 @@ def _quantised(x, store):
     """x's rows in 8 bits, and their scales, in float32 arithmetic throughout."""
     largest = x.float().abs().amax(-1).clamp(min=2.0 ** -100)
     if store == 'int8':
-        return (x.float() * (127 / largest)[..., None]).round().to(torch.int8), largest / 127
+        inverse = torch.full_like(largest, 127.0) / largest  # (127 / largest would be 127 times the reciprocal)
+        return (x.float() * inverse[..., None]).round().to(torch.int8), largest / 127
     part, exponent = torch.frexp(largest)  # part in [1/2, 1)
     exponent = exponent - torch.where(part <= 0.875, 9, 8)
     power = lambda n: (n + 127 << 23).to(torch.int32).view(torch.float32)  # 2^n, exactly
