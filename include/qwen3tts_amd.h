@@ -38,6 +38,8 @@ extern "C" {
 #define Q3T_F16 1
 #define Q3T_F32 2
 #define Q3T_BOOL 3  /* masks only: nonzero = attend, as a torch bool SDPA mask */
+#define Q3T_I8 4    /* paged pools only, with scales */
+#define Q3T_E4M3 5  /* paged pools only, with scales: OCP 8-bit floats of 4 exponent and 3 mantissa bits */
 
 /* Human-readable text for a status returned by any entry point.  The reference's wrappers
    raise ValueError with such a text before launching (kv_triton_ascend.py:40-53); the
@@ -458,6 +460,70 @@ typedef struct q3t_paged_args {
 int64_t q3t_paged_workspace_bytes(const q3t_paged_args *args);
 
 int q3t_paged_attention(const q3t_paged_args *args, void *stream);
+
+/* ---- paged cache in 8 bits, and prefixes that requests share ------------------------------ */
+
+/*
+ * Pools of 8-bit elements (Q3T_I8 or Q3T_E4M3): every key (value) row of head_dim elements has a
+ * float32 scale, (pages, kv_heads, page_size) by strides (p, h, t) in elements, and stands for
+ * scale * element.  Of a row x with a = max(2^-100, max |x|), in float32 arithmetic:
+ *   Q3T_I8    scale = a / 127, elements round(x * (127 / a)), ties to even;
+ *   Q3T_E4M3  scale = the smallest power of two with a <= 448 scale, elements x / scale rounded to
+ *             the nearest e4m3 value, ties to even (a value's step follows its own size, so that a scale of
+ *             more bits would gain nothing, and x / scale is exact).
+ * A row that holds an infinity or a NaN has the scale NaN and elements 0: it stands for NaN.
+ */
+typedef struct q3t_paged_scales {
+    int64_t format; /* Q3T_I8 or Q3T_E4M3 */
+    float *key_scales, *value_scales;
+    int64_t ks_stride_p, ks_stride_h, ks_stride_t;
+    int64_t vs_stride_p, vs_stride_h, vs_stride_t;
+} q3t_paged_scales;
+
+/*
+ * q3t_paged_write into pools of 8 bits: `args` as there, elem_size and dtype (Q3T_BF16, Q3T_F16 or Q3T_F32)
+ * being the new rows', the pools' strides in elements of one byte.  head_dim 64 or 128; pool bases and
+ * strides are multiples of 16 bytes.
+ */
+int q3t_paged_write_quantized(const q3t_paged_write_args *args, int64_t dtype, const q3t_paged_scales *scales, void *stream);
+
+/*
+ * Rows out of a paged cache, the inverse of the writes: with j = positions[b] + t,
+ *   keys  [b, h, t, :] = key_pages  [page_table[b, j / page_size], h, j % page_size, :]
+ *   values[b, h, t, :] = value_pages[page_table[b, j / page_size], h, j % page_size, :]
+ * for t < min(tokens, lengths[b]) (lengths == NULL: all tokens).  Rows past those, rows whose j lies
+ * outside [0, table_width * page_size) and rows on no page are zeros.  scales == NULL: the pools have the
+ * rows' type, and elements of elem_size bytes are copied; else the pools have 8 bits (head_dim 64 or 128, bases and
+ * strides multiples of 16 bytes), and elements are scale * element in float32, rounded to dtype.
+ * The counterpart of q3t_copy_strided out of a slot (SlotArena.move, continuous.py:124-128).
+ */
+typedef struct q3t_paged_read_args {
+    int64_t batch, heads, tokens, width, dtype; /* dtype: Q3T_BF16, Q3T_F16 or Q3T_F32 */
+    void *keys, *values;                        /* rows (b, h, t), unit-stride elements */
+    int64_t k_stride_b, k_stride_h, k_stride_t;
+    int64_t v_stride_b, v_stride_h, v_stride_t;
+    const void *key_pages, *value_pages;
+    int64_t kp_stride_p, kp_stride_h, kp_stride_t;
+    int64_t vp_stride_p, vp_stride_h, vp_stride_t;
+    int64_t pages, page_size;
+    const int32_t *page_table; /* device (batch, table_width) */
+    int64_t table_width, table_stride_b;
+    const int64_t *positions;  /* device (batch): j of each request's row t = 0 */
+    const int32_t *lengths;    /* optional device (batch) */
+} q3t_paged_read_args;
+
+int q3t_paged_read(const q3t_paged_read_args *args, const q3t_paged_scales *scales, void *stream);
+
+/*
+ * q3t_paged_attention over pools of 8 bits (scales != NULL), the queries and the output having dtype; and for
+ * a batch whose requests begin with the same pages (shared_pages > 0): the first shared_pages entries of every
+ * request's row of page_table are taken to be those of request 0's row, and the keys on them are read
+ * once for many requests.  Everything else is as q3t_paged_attention has it: a request attends its
+ * keys 0 ... positions[b], also where that ends within the shared pages, under its own mask.
+ * shared_pages * page_size is below ctx.
+ */
+int64_t q3t_paged_workspace_bytes_with(const q3t_paged_args *args, const q3t_paged_scales *scales, int64_t shared_pages);
+int q3t_paged_attention_with(const q3t_paged_args *args, const q3t_paged_scales *scales, int64_t shared_pages, void *stream);
 
 /* ---- rotary positions with several axes --------------------------------------------------- */
 

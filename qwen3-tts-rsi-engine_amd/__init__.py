@@ -12,7 +12,7 @@ Modules
                   prefill_attention
                                                          (npu_attention.py, SDPA dispatch)
   slots           SlotArena / SlotCache / PredictorCache (continuous.py, predictor.py)
-  paged           paged_write / paged_attention / PagedArena / PagedCache: the cache in pages
+  paged           paged_write / paged_read / paged_attention / PagedArena / PagedCache: the cache in pages
   packed_attention PackedAttention / install_packed_attention / restore_modules
   prefill         varlen prefill of packed prompts       (prefill_graph.py)
   scheduler       integer slot state of continuous batching (continuous.py tick/admit)
@@ -31,7 +31,7 @@ from .prefill import prefill_rope_write, prefill_step
 from .packed_attention import PackedAttention, install_packed_attention, restore_modules
 from .scheduler import SlotScheduler, DecodeBatch
 from .slots import SlotArena, SlotCache, PredictorCache, PrefillCache, grow_arena
-from .paged import PagedArena, PagedCache, paged_attention, paged_write
+from .paged import PagedArena, PagedCache, paged_attention, paged_read, paged_write
 from .slot_graph import SlotGraph
 from .prefill_graph import PrefillGraph, pad_prefill_batch
 
@@ -43,7 +43,7 @@ __all__ = [
     "prefill_attention", "prefill_rope_write", "prefill_step", "PackedAttention",
     "install_packed_attention", "restore_modules", "SlotScheduler", "DecodeBatch", "SlotArena",
     "SlotCache", "PredictorCache", "PrefillCache", "grow_arena", "SlotGraph", "PrefillGraph",
-    "pad_prefill_batch", "rotary_axes", "paged_write", "paged_attention", "PagedArena", "PagedCache", "library",
+    "pad_prefill_batch", "rotary_axes", "paged_write", "paged_read", "paged_attention", "PagedArena", "PagedCache", "library",
 ]
 
 library = _lib.library

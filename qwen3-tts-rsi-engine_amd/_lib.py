@@ -20,7 +20,7 @@ Q3T_EINVAL = -1
 Q3T_EUNSUPPORTED = -2
 Q3T_EWORKSPACE = -3
 
-Q3T_BF16, Q3T_F16, Q3T_F32, Q3T_BOOL = 0, 1, 2, 3
+Q3T_BF16, Q3T_F16, Q3T_F32, Q3T_BOOL, Q3T_I8, Q3T_E4M3 = 0, 1, 2, 3, 4, 5
 DTYPE_CODES = {torch.bfloat16: Q3T_BF16, torch.float16: Q3T_F16, torch.float32: Q3T_F32,
                torch.bool: Q3T_BOOL}
 
@@ -122,6 +122,20 @@ class PagedArgs(ctypes.Structure):
     ]
 
 
+class PagedReadArgs(ctypes.Structure):
+    """Mirror of ``q3t_paged_read_args``."""
+    _fields_ = [(name if name != "elem_size" else "dtype", kind) for name, kind in PagedWriteArgs._fields_]
+
+
+class PagedScales(ctypes.Structure):
+    """Mirror of ``q3t_paged_scales``."""
+    _fields_ = [
+        ("format", c_i64), ("key_scales", c_vp), ("value_scales", c_vp),
+        ("ks_stride_p", c_i64), ("ks_stride_h", c_i64), ("ks_stride_t", c_i64),
+        ("vs_stride_p", c_i64), ("vs_stride_h", c_i64), ("vs_stride_t", c_i64),
+    ]
+
+
 class RotaryAxesArgs(ctypes.Structure):
     """Mirror of ``q3t_rotary_axes_args``."""
     _fields_ = [
@@ -176,6 +190,10 @@ SIGNATURES = {
     "q3t_paged_write": (ctypes.c_int, [ctypes.POINTER(PagedWriteArgs), c_vp]),
     "q3t_paged_workspace_bytes": (c_i64, [ctypes.POINTER(PagedArgs)]),
     "q3t_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedArgs), c_vp]),
+    "q3t_paged_write_quantized": (ctypes.c_int, [ctypes.POINTER(PagedWriteArgs), c_i64, ctypes.POINTER(PagedScales), c_vp]),
+    "q3t_paged_read": (ctypes.c_int, [ctypes.POINTER(PagedReadArgs), ctypes.POINTER(PagedScales), c_vp]),
+    "q3t_paged_workspace_bytes_with": (c_i64, [ctypes.POINTER(PagedArgs), ctypes.POINTER(PagedScales), c_i64]),
+    "q3t_paged_attention_with": (ctypes.c_int, [ctypes.POINTER(PagedArgs), ctypes.POINTER(PagedScales), c_i64, c_vp]),
     "q3t_rotary_axes": (ctypes.c_int, [ctypes.POINTER(RotaryAxesArgs), c_vp]),
 }
 
@@ -279,10 +297,10 @@ def packed(name: str):
     return entry
 
 
-def launch(name: str, args: bytes, index: int, what: str) -> None:
-    """The entry point ``name`` of an argument structure and a stream, on device ``index``."""
+def launch(name: str, args: bytes, index: int, what: str, *more) -> None:
+    """The entry point ``name`` of an argument structure, ``more`` and a stream, on device ``index``."""
     with on_device(index) as stream:
-        status = packed(name)(args, stream)
+        status = packed(name)(args, *more, stream)
     if status != Q3T_OK:
         check(status, what)
 

@@ -1,0 +1,310 @@
+// Rows into a paged cache of 8-bit elements, and rows out of a paged cache.
+//
+// Written: with a = max(2^-100, max |x|) of a row, int8 elements round(x * (127 / a)) and the scale a / 127;
+// e4m3 elements x / s and the scale s, the smallest power of two with a <= 448 s.  A row with an infinity or a NaN gets
+// the scale NaN.  Read: scale * element, or the elements of an unquantised pool.
+// Both are bound by HBM where rows are many and by the launch where they are few.
+#include "paged_index.hpp"
+#include "q3t_common.hpp"
+
+#include <type_traits>
+
+namespace q3t {
+namespace paged_quantized {
+
+constexpr int kThreads = 256;
+
+struct Rows {  // one of keys and values
+    char *rows, *pages;                         // of the call, of the pool
+    float *scales;
+    int64_t r_sb, r_sh, r_st, p_sp, p_sh, p_st;  // bytes
+    int64_t s_sp, s_sh, s_st;                   // elements
+};
+struct Params {
+    Rows x[2];
+    const int64_t *positions;
+    const int32_t *lengths, *table;
+    int64_t table_sb, rows;  // rows: table_width * page_size
+    uint32_t batch, heads, tokens, units, pages;
+    Divisor by_units, by_heads, by_page;
+};
+
+// Place of row t of request b: page and row of it, page -1 for a row that it has not.
+struct Place { int32_t page; uint32_t row; };
+Q3T_DEVICE Place place(const Params &p, uint32_t b, uint32_t t) {
+    const int64_t start = p.positions[b];
+    const uint32_t used = p.lengths ? (uint32_t)max(0, min(p.lengths[b], (int32_t)p.tokens)) : p.tokens;
+    // (start + t overflows for no start that is left)
+    if (t >= used || start >= p.rows || start < -(int64_t)p.tokens || start + t < 0 || start + t >= p.rows) return {-1, 0u};
+    const uint32_t j = (uint32_t)(start + t), entry = divide(j, p.by_page);
+    const int32_t page = p.table[b * p.table_sb + entry];
+    return {(uint32_t)page < p.pages ? page : -1, j - entry * p.by_page.d};
+}
+
+template <typename T> struct Eight { alignas(16) T x[8]; };
+
+// Eight elements of a row in float32; VEC: by 16-byte loads.
+template <typename T, bool VEC>
+Q3T_DEVICE void load8(const char *from, float (&x)[8]) {
+    Eight<T> e;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<U4 *>(&e)[i] = reinterpret_cast<const U4 *>(from)[i];
+    } else {
+        for (int i = 0; i < 8; ++i) e.x[i] = reinterpret_cast<const T *>(from)[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)e.x[i];
+}
+
+Q3T_DEVICE uint32_t dpp_max(uint32_t x, uint32_t y) { return x > y ? x : y; }
+template <int CTRL> Q3T_DEVICE uint32_t dpp_u(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, false);
+}
+
+// The largest |x| of a row of L lanes of eight elements, as bits: NaN above infinity above the rest.
+template <int L> Q3T_DEVICE uint32_t row_largest(const float (&x)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = dpp_max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    m = dpp_max(m, dpp_u<kDppXor1>(m));
+    m = dpp_max(m, dpp_u<kDppXor2>(m));
+    m = dpp_max(m, dpp_u<kDppHalfMirror>(m));
+    if (L == 16) m = dpp_max(m, xor8u(m));
+    return m;
+}
+
+// A row's scale and the lane's eight elements.
+template <bool E4M3> Q3T_DEVICE uint2 quantise(const float (&x)[8], uint32_t largest, float &scale) {
+    const bool finite = largest < 0x7f800000u;
+    const uint32_t a = dpp_max(largest, 0x0d800000u);  // 2^-100
+    float inverse;
+    if constexpr (E4M3) {
+        // a = m 2^E: s = 2^(E - 8) where m <= 1.75, else 2^(E - 7); the carry out of the mantissa says which
+        const uint32_t exponent = ((a + 0x1fffffu) >> 23) - 8;
+        scale = __uint_as_float(exponent << 23);
+        inverse = __uint_as_float((254 - exponent) << 23);
+    } else {
+        scale = __uint_as_float(a) / 127.f;
+        inverse = 127.f / __uint_as_float(a);
+    }
+    if (!finite) scale = __uint_as_float(0x7fc00000u);
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (E4M3) {
+            w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inverse, x[4 * i + 1] * inverse, 0, false);
+            w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inverse, x[4 * i + 3] * inverse, (int)w[i], true);
+        } else {
+            w[i] = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[i] |= ((uint32_t)(int)__builtin_rintf(x[4 * i + k] * inverse) & 0xffu) << 8 * k;
+        }
+        if (!finite) w[i] = 0;
+    }
+    return uint2{w[0], w[1]};
+}
+
+// A thread takes eight elements of one row of the keys and of the values; L of them have a row.
+template <typename T, int L, bool E4M3, bool VEC>
+__global__ void __launch_bounds__(kThreads) write_kernel(Params p) {
+    for (uint32_t b = blockIdx.y; b < p.batch; b += gridDim.y) {
+        const uint32_t i = blockIdx.x * kThreads + threadIdx.x, row = i / L, unit = i % L;
+        const uint32_t t = divide(row, p.by_heads), h = row - t * p.heads;
+        const Place at = place(p, b, t);
+        if (at.page < 0) continue;  // (the same for all lanes of a row)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const Rows &r = p.x[n];
+            float x[8], scale;
+            load8<T, VEC>(r.rows + b * r.r_sb + h * r.r_sh + t * r.r_st + unit * 8 * sizeof(T), x);
+            const uint2 w = quantise<E4M3>(x, row_largest<L>(x), scale);
+            *reinterpret_cast<uint2 *>(r.pages + at.page * r.p_sp + h * r.p_sh + at.row * r.p_st + unit * 8) = w;
+            if (unit == 0) r.scales[at.page * r.s_sp + h * r.s_sh + at.row * r.s_st] = scale;
+        }
+    }
+}
+
+// Eight elements, from their bytes.
+template <bool E4M3> Q3T_DEVICE void elements(uint2 w, float (&x)[8]) {
+    const uint32_t u[2] = {w.x, w.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (E4M3) {
+            const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)u[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)u[i], true);
+            x[4 * i] = lo[0]; x[4 * i + 1] = lo[1]; x[4 * i + 2] = hi[0]; x[4 * i + 3] = hi[1];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[4 * i + k] = (float)(int8_t)(u[i] >> 8 * k);
+        }
+    }
+}
+
+template <typename T> Q3T_DEVICE T rounded(float x) { return (T)x; }
+template <> Q3T_DEVICE __bf16 rounded<__bf16>(float x) { return __builtin_bit_cast(__bf16, (uint16_t)float_to_bf16(x)); }
+
+template <typename T, int L, bool E4M3, bool VEC>
+__global__ void __launch_bounds__(kThreads) read_kernel(Params p) {
+    for (uint32_t b = blockIdx.y; b < p.batch; b += gridDim.y) {
+        const uint32_t i = blockIdx.x * kThreads + threadIdx.x, row = i / L, unit = i % L;
+        const uint32_t t = divide(row, p.by_heads), h = row - t * p.heads;
+        if (t >= p.tokens) continue;
+        const Place at = place(p, b, t);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const Rows &r = p.x[n];
+            Eight<T> e = {};
+            if (at.page >= 0) {
+                float x[8];
+                elements<E4M3>(*reinterpret_cast<const uint2 *>(r.pages + at.page * r.p_sp + h * r.p_sh + at.row * r.p_st + unit * 8), x);
+                const float scale = r.scales[at.page * r.s_sp + h * r.s_sh + at.row * r.s_st];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) e.x[k] = rounded<T>(x[k] * scale);
+            }
+            char *to = r.rows + b * r.r_sb + h * r.r_sh + t * r.r_st + unit * 8 * sizeof(T);
+            if constexpr (VEC) {
+#pragma unroll
+                for (int k = 0; k < (int)sizeof(e) / 16; ++k) reinterpret_cast<U4 *>(to)[k] = reinterpret_cast<U4 *>(&e)[k];
+            } else {
+                for (int k = 0; k < 8; ++k) reinterpret_cast<T *>(to)[k] = e.x[k];
+            }
+        }
+    }
+}
+
+// Units of V bytes out of pools of the rows' own type.
+template <int V> struct Unit { typedef uint32_t T __attribute__((ext_vector_type(V / 4))); };
+template <> struct Unit<4> { typedef uint32_t T; };
+template <> struct Unit<2> { typedef uint16_t T; };
+
+template <int V>
+__global__ void __launch_bounds__(kThreads) copy_kernel(Params p) {
+    typedef typename Unit<V>::T T;
+    for (uint32_t b = blockIdx.y; b < p.batch; b += gridDim.y) {
+        const uint32_t i = blockIdx.x * kThreads + threadIdx.x, row = divide(i, p.by_units);
+        const uint32_t t = divide(row, p.by_heads), h = row - t * p.heads;
+        const int64_t unit = (int64_t)(i - row * p.units) * V;
+        if (t >= p.tokens) continue;
+        const Place at = place(p, b, t);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const Rows &r = p.x[n];
+            T v = {};
+            if (at.page >= 0) v = *reinterpret_cast<const T *>(r.pages + at.page * r.p_sp + h * r.p_sh + at.row * r.p_st + unit);
+            *reinterpret_cast<T *>(r.rows + b * r.r_sb + h * r.r_sh + t * r.r_st + unit) = v;
+        }
+    }
+}
+
+// The fields that writes and reads share; Q3T_OK, or the status to return.
+template <typename A>
+static int common(const A *a, int64_t es, int64_t held, const q3t_paged_scales *s, Params &p) {
+    if (!a || a->batch < 0 || a->heads < 1 || a->tokens < 0 || a->width < 1 || a->pages < 1 || a->page_size < 1 || a->table_width < 1)
+        return Q3T_EINVAL;
+    if (s && s->format != Q3T_I8 && s->format != Q3T_E4M3) return Q3T_EUNSUPPORTED;
+    if (s && a->width != 64 && a->width != 128) return Q3T_EUNSUPPORTED;
+    if (a->batch == 0 || a->tokens == 0) return Q3T_OK;
+    if (!a->keys || !a->values || !a->key_pages || !a->value_pages || !a->page_table || !a->positions) return Q3T_EINVAL;
+    if (s && (!s->key_scales || !s->value_scales || !aligned(s->key_scales, 4) || !aligned(s->value_scales, 4))) return Q3T_EINVAL;
+    if (a->pages > INT32_MAX || a->table_width > INT32_MAX / a->page_size || a->batch > INT32_MAX || a->width > 1 << 20)
+        return Q3T_EUNSUPPORTED;
+    p.x[0] = {(char *)a->keys, (char *)a->key_pages, s ? s->key_scales : nullptr, a->k_stride_b * es, a->k_stride_h * es,
+              a->k_stride_t * es, a->kp_stride_p * held, a->kp_stride_h * held, a->kp_stride_t * held,
+              s ? s->ks_stride_p : 0, s ? s->ks_stride_h : 0, s ? s->ks_stride_t : 0};
+    p.x[1] = {(char *)a->values, (char *)a->value_pages, s ? s->value_scales : nullptr, a->v_stride_b * es, a->v_stride_h * es,
+              a->v_stride_t * es, a->vp_stride_p * held, a->vp_stride_h * held, a->vp_stride_t * held,
+              s ? s->vs_stride_p : 0, s ? s->vs_stride_h : 0, s ? s->vs_stride_t : 0};
+    p.positions = a->positions; p.lengths = a->lengths; p.table = a->page_table;
+    p.table_sb = a->table_stride_b;
+    p.rows = a->table_width * a->page_size;
+    p.batch = (uint32_t)a->batch; p.heads = (uint32_t)a->heads; p.tokens = (uint32_t)a->tokens;
+    p.pages = (uint32_t)a->pages;
+    p.by_heads = divisor(p.heads);
+    p.by_page = divisor((uint32_t)a->page_size);
+    if (!aligned(a->page_table, 4) || !aligned(a->positions, 8) || (a->lengths && !aligned(a->lengths, 4))) return Q3T_EINVAL;
+    for (const Rows &r : p.x) {
+        const int64_t at = r.p_sp | r.p_sh | r.p_st | (int64_t)(uintptr_t)r.pages;
+        if (s ? at % 16 : at % es) return Q3T_EINVAL;
+        if ((r.r_sb | r.r_sh | r.r_st | (int64_t)(uintptr_t)r.rows) % es) return Q3T_EINVAL;
+    }
+    return Q3T_OK;
+}
+
+// What every row of the call, and every pool row, is a multiple of, in bytes.
+static int64_t strides(const Params &p, bool pools) {
+    int64_t all = 0;
+    for (const Rows &r : p.x) {
+        all |= r.r_sb | r.r_sh | r.r_st | (int64_t)(uintptr_t)r.rows;
+        if (pools) all |= r.p_sp | r.p_sh | r.p_st | (int64_t)(uintptr_t)r.pages;
+    }
+    return all;
+}
+
+// Launches `kernel` for `units` units of a row; Q3T_OK, or the status to return.
+template <typename K>
+static int launch(K kernel, Params &p, uint32_t units, void *stream) {
+    p.units = units;
+    p.by_units = divisor(units);
+    // units of a request stay below 2^31, and threads of a launch below 2^32
+    if (p.heads > INT32_MAX / units || p.tokens > (INT32_MAX - 2 * kThreads) / (p.heads * units)) return Q3T_EUNSUPPORTED;
+    const int64_t blocks = ((int64_t)p.tokens * p.heads * units + kThreads - 1) / kThreads, most = ((int64_t)1 << 24) - 1;
+    if (blocks > most) return Q3T_EUNSUPPORTED;
+    int64_t across = p.batch < 65535 ? p.batch : 65535;
+    if (across > most / blocks) across = most / blocks;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks, (uint32_t)across), dim3(kThreads), 0, (hipStream_t)stream, p);
+    return launch_status();
+}
+
+// f(type, lanes of a row, e4m3, vectors) for a call's rows
+template <typename F>
+static int with(int64_t dtype, int64_t width, int64_t format, bool vec, F f) {
+    auto by_vec = [&](auto t, auto l, auto e) { return vec ? f(t, l, e, std::true_type{}) : f(t, l, e, std::false_type{}); };
+    auto by_format = [&](auto t, auto l) { return format == Q3T_E4M3 ? by_vec(t, l, std::true_type{}) : by_vec(t, l, std::false_type{}); };
+    auto by_width = [&](auto t) {
+        return width == 64 ? by_format(t, std::integral_constant<int, 8>{}) : by_format(t, std::integral_constant<int, 16>{});
+    };
+    if (dtype == Q3T_F32) return by_width(float{});
+    return dtype == Q3T_BF16 ? by_width(__bf16{}) : by_width(_Float16{});
+}
+
+}  // namespace paged_quantized
+}  // namespace q3t
+
+using namespace q3t;
+
+extern "C" int q3t_paged_write_quantized(const q3t_paged_write_args *a, int64_t dtype, const q3t_paged_scales *s, void *stream) {
+    using namespace paged_quantized;
+    if (!a || !s) return Q3T_EINVAL;
+    if (dtype != Q3T_BF16 && dtype != Q3T_F16 && dtype != Q3T_F32) return Q3T_EUNSUPPORTED;
+    if (a->elem_size != (dtype == Q3T_F32 ? 4 : 2)) return Q3T_EINVAL;
+    Params p = {};
+    const int status = common(a, a->elem_size, 1, s, p);
+    if (status != Q3T_OK || a->batch == 0 || a->tokens == 0) return status;
+    return with(dtype, a->width, s->format, strides(p, false) % 16 == 0, [&](auto t, auto l, auto e, auto vec) {
+        return launch(write_kernel<decltype(t), decltype(l)::value, decltype(e)::value, decltype(vec)::value>, p, decltype(l)::value, stream);
+    });
+}
+
+extern "C" int q3t_paged_read(const q3t_paged_read_args *a, const q3t_paged_scales *s, void *stream) {
+    using namespace paged_quantized;
+    if (!a) return Q3T_EINVAL;
+    if (a->dtype != Q3T_BF16 && a->dtype != Q3T_F16 && a->dtype != Q3T_F32) return Q3T_EUNSUPPORTED;
+    const int64_t es = a->dtype == Q3T_F32 ? 4 : 2;
+    Params p = {};
+    const int status = common(a, es, s ? 1 : es, s, p);
+    if (status != Q3T_OK || a->batch == 0 || a->tokens == 0) return status;
+    if (s)
+        return with(a->dtype, a->width, s->format, strides(p, false) % 16 == 0, [&](auto t, auto l, auto e, auto vec) {
+            return launch(read_kernel<decltype(t), decltype(l)::value, decltype(e)::value, decltype(vec)::value>, p, decltype(l)::value, stream);
+        });
+    const int64_t all = strides(p, true) | a->width * es;  // the widest unit that divides the row, every stride and every pointer
+    int64_t v = 16;
+    while (v > es && all % v) v >>= 1;
+    const uint32_t units = (uint32_t)(a->width * es / v);
+    switch (v) {
+        case 16: return launch(copy_kernel<16>, p, units, stream);
+        case 8: return launch(copy_kernel<8>, p, units, stream);
+        case 4: return launch(copy_kernel<4>, p, units, stream);
+        default: return launch(copy_kernel<2>, p, units, stream);
+    }
+}

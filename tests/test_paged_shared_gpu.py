@@ -1,0 +1,222 @@
+"""``paged_attention`` of requests that share their first pages, against the definition in float64."""
+import math
+
+import pytest
+import torch
+
+from tests._paged import assert_within
+from tests._paged_more import HELD, expected, problem, run
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _behind(prefix, own):
+    """Lengths of requests of ``own`` keys behind ``prefix`` shared ones."""
+    return [prefix + n for n in own]
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize('width', [64, 128])
+@pytest.mark.parametrize('heads', [(16, 8), (8, 8), (32, 4), (16, 1), (20, 1), (28, 4), (3, 3)], ids=str)
+def test_types_widths_and_head_layouts(pkg, device, dtype, width, heads):
+    p = problem(device, _behind(208, [1, 15, 16, 17, 40, 100, 333]), shared=13, q_heads=heads[0], kv_heads=heads[1], width=width,
+                dtype=dtype, seed=1)
+    assert_within(run(pkg, p), *expected(p))
+
+
+@pytest.mark.parametrize('page', [1, 5, 8, 16, 24, 32, 64, 100, 256])
+@pytest.mark.parametrize('dtype,width,layout', [(BF16, 128, 'nhd'), (F32, 64, 'hnd'), (F16, 64, 'hnd')], ids=str)
+def test_page_sizes_and_layouts(pkg, device, page, dtype, width, layout):
+    shared = max(1, 300 // page)
+    p = problem(device, _behind(shared * page, [1, 15, 16, 17, 40, 100, 333]), shared=shared, page=page, dtype=dtype, width=width,
+                layout=layout, seed=2)
+    assert_within(run(pkg, p), *expected(p))
+
+
+@pytest.mark.parametrize('shared', [1, 2, 3, 4, 7, 8, 9, 31, 64, 129, 600])
+@pytest.mark.parametrize('batch', [1, 2, 5, 33])
+def test_lengths_of_the_prefix(pkg, device, shared, batch):
+    p = problem(device, _behind(16 * shared, [1 + 7 * b % 50 for b in range(batch)]), shared=shared, q_heads=8, kv_heads=4, seed=3)
+    assert_within(run(pkg, p), *expected(p))
+
+
+@pytest.mark.parametrize('batch', [8, 16, 17, 40, 64, 100, 200])
+@pytest.mark.parametrize('heads', [(16, 8), (8, 1), (3, 3)], ids=str)
+@pytest.mark.parametrize('dtype', [BF16, F32], ids=str)
+def test_many_requests(pkg, device, batch, heads, dtype):
+    p = problem(device, _behind(640, [b % 90 for b in range(batch)]), shared=20, page=32, q_heads=heads[0], kv_heads=heads[1], dtype=dtype,
+                seed=4)
+    assert_within(run(pkg, p), *expected(p))
+
+
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (F16, 128), (F32, 64)], ids=str)
+@pytest.mark.parametrize('own', [[1, 2000, 0, 300, 5], [1] * 24], ids=['ragged', 'one'])
+def test_long_prefixes(pkg, device, dtype, width, own):
+    p = problem(device, _behind(9000, own), shared=90, page=100, q_heads=8, kv_heads=2, width=width, dtype=dtype, seed=5)
+    assert_within(run(pkg, p), *expected(p))
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize('batch', [9, 50])
+def test_requests_that_end_within_the_shared_pages(pkg, device, dtype, batch):
+    """And such that attend nothing, as padded requests of a captured batch."""
+    lengths = ([0, 1, 15, 16, 17, 100, 159, 160, 161] * 6)[:batch]
+    p = problem(device, lengths, shared=10, dtype=dtype, seed=6)
+    out = run(pkg, p)
+    assert (out[0] == 0).all()
+    assert_within(out, *expected(p))
+    p.positions.fill_(-1)
+    assert (run(pkg, p) == 0).all()
+    p.positions[3], p.positions[4] = 2 ** 62, -2 ** 62
+    p.positions[5] = p.table.shape[1] * 16
+    assert (run(pkg, p) == 0).all()
+
+
+@pytest.mark.parametrize('width,dtype,heads', [(128, BF16, (16, 8)), (64, F32, (8, 8)), (128, F16, (24, 2))], ids=str)
+@pytest.mark.parametrize('kind', [torch.bool, BF16, F16, F32], ids=str)
+@pytest.mark.parametrize('batch', [7, 40])
+def test_masks(pkg, device, width, dtype, heads, kind, batch):
+    """Keys hidden from some requests and from all, requests that are left nothing, hidden rows that hold NaN."""
+    lengths = ([330, 340, 600, 321, 400, 0, 100] * 6)[:batch]
+    p = problem(device, lengths, shared=20, page=16, width=width, dtype=dtype, q_heads=heads[0], kv_heads=heads[1], seed=7)
+    ctx = p.table.shape[1] * 16
+    shown = torch.rand(batch, 1, 1, ctx, generator=torch.Generator().manual_seed(8)) < 0.7
+    shown[3] = False
+    shown[4, ..., :320] = False
+    shown[1, ..., 320:] = False
+    shown[..., 64:129] = False  # from all requests
+    for pool in (p.key_pages, p.value_pages):
+        pool[int(p.table[0, 5])] = math.nan
+    mask = shown if kind == torch.bool else torch.where(shown, torch.rand(shown.shape), -math.inf).to(kind)
+    mask = mask.to(device)
+    out = run(pkg, p, mask=mask)
+    assert (out[3] == 0).all() and (out[5] == 0).all()
+    want = expected(p, mask=mask)
+    assert_within(out, *want)
+    strided = torch.full((batch, 1, 1, ctx, 3), 9, device=device).to(mask.dtype)[..., 1].copy_(mask)
+    assert torch.equal(run(pkg, p, mask=strided), out)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32], ids=str)
+def test_a_value_hidden_from_some_requests_alone(pkg, device, dtype):
+    """A NaN or an infinity among the shared values shows where it is attended, and nowhere else."""
+    p = problem(device, _behind(320, [5] * 20), shared=20, q_heads=4, kv_heads=2, dtype=dtype, seed=9)
+    mask = torch.ones(20, 1, 1, p.table.shape[1] * 16, dtype=torch.bool, device=device)
+    mask[::2, ..., 40] = False
+    clean, tol = expected(p, mask=mask)
+    page, row = int(p.table[0, 2]), 40 % 16
+    p.value_pages[page, 1, row, 9], p.value_pages[page, 1, row, 10] = math.nan, math.inf
+    out = run(pkg, p, mask=mask).cpu()
+    assert out[1::2, 0, 2:, 9].isnan().all() and (out[1::2, 0, 2:, 10] == math.inf).all()
+    out[1::2, 0, 2:, 9:11], clean[1::2, 0, 2:, 9:11] = 0, 0
+    assert_within(out, clean, tol)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32], ids=str)
+def test_masks_of_few_keys_and_of_one_term(pkg, device, dtype):
+    """A mask that ends within the shared pages, and one term for all keys."""
+    p = problem(device, _behind(160, [16, 40, 16]), shared=10, dtype=dtype, seed=10)  # rows for every position below
+    for keys in (2, 16, 100, 160, 161, 176):
+        mask = torch.ones(3, 1, 1, keys, dtype=torch.bool, device=device)
+        p.positions = torch.tensor([keys - 1, keys // 2, keys], device=device)
+        out = run(pkg, p, mask=mask)
+        assert (out[2] == 0).all()
+        assert_within(out, *expected(p, mask=mask))
+    p.positions = torch.tensor([164, 199, 160], device=device)
+    one = torch.tensor([True, False, True], device=device)[:, None, None, None]
+    out = run(pkg, p, mask=one)
+    assert (out[1] == 0).all()
+    assert_within(out, *expected(p, mask=one.expand(3, 1, 1, p.table.shape[1] * 16)))
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize('below', [5.0, 40.0, 80.0])
+def test_infinite_shared_values_under_small_weights_show(pkg, device, dtype, below):
+    p = problem(device, _behind(320, [40] * 10), shared=20, q_heads=4, kv_heads=2, dtype=dtype, seed=11)
+    p.query.zero_()
+    p.query[..., 0] = 8.0
+    p.key_pages.nan_to_num_(0.0).zero_()
+    p.key_pages[p.table[0, :20].long(), :, 3, 0] = below * 128 ** 0.5 / 8.0
+    clean, tol = expected(p)
+    assert_within(run(pkg, p), clean, tol)
+    p.value_pages[int(p.table[0, 0]), 0, 4, 17] = math.inf
+    p.value_pages[int(p.table[0, 19]), 0, 0, 18] = -math.inf
+    p.value_pages[int(p.table[0, 7]), 0, 0, 19] = math.nan
+    out = run(pkg, p).cpu()
+    assert (out[:, 0, :2, 17] == math.inf).all() and (out[:, 0, :2, 18] == -math.inf).all() and out[:, 0, :2, 19].isnan().all()
+    out[:, 0, :2, 17:20], clean[:, 0, :2, 17:20] = 0, 0
+    assert_within(out, clean, tol)
+
+
+def test_shared_pages_outside_the_pool_do_not_exist(pkg, device):
+    p = problem(device, _behind(320, [5, 40, 1, 17]), shared=20, seed=12)
+    p.table[:, 3], p.table[:, 7], p.table[2, 20] = -1, 2 ** 31 - 1, -5
+    assert_within(run(pkg, p), *expected(p))
+    p.table[:, :20] = -1
+    assert_within(run(pkg, p), *expected(p))
+
+
+def test_the_first_rows_entries_are_everybodys(pkg, device):
+    p = problem(device, _behind(160, [5, 40, 1, 17] * 4), shared=10, seed=13)
+    want = run(pkg, p)
+    p.table[1:, :10] = -9
+    assert torch.equal(run(pkg, p), want)
+
+
+@pytest.mark.parametrize('held', HELD, ids=str)
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (F16, 64), (F32, 128)], ids=str)
+@pytest.mark.parametrize('batch', [3, 40])
+def test_pools_of_8_bits(pkg, device, held, dtype, width, batch):
+    p = problem(device, _behind(480, [b % 50 for b in range(batch)]), shared=20, page=24, held=held, dtype=dtype, width=width, seed=14)
+    assert_within(run(pkg, p), *expected(p))
+
+
+def test_out_strides_scales_and_the_query_itself(pkg, device):
+    p = problem(device, _behind(320, [5, 40, 1, 17, 200]), shared=20, seed=15)
+    want = run(pkg, p)
+    out = torch.zeros(5, 1, 40, 130, device=device, dtype=BF16)[:, :, 3:35:2, 1:129]
+    assert run(pkg, p, out=out) is out and torch.equal(out, want)
+    assert_within(run(pkg, p, scale=0.3), *expected(p, scale=0.3))
+    assert run(pkg, p, out=p.query) is p.query and torch.equal(p.query, want)
+
+
+@pytest.mark.parametrize('batch', [6, 40])
+def test_captured_and_replayed(pkg, device, batch):
+    """Two graphs, replayed in turn as positions change, with eager calls between."""
+    problems = [problem(device, _behind(640, [(b * k) % 90 + 1 for b in range(batch)]), shared=20, page=32, seed=16 + k) for k in (1, 2)]
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    for p in problems:
+        run(pkg, p)
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            outs.append(run(pkg, p))
+        torch.cuda.current_stream().wait_stream(side)
+        graphs.append(graph)
+    for n in range(4):
+        for p, graph, out in zip(problems, graphs, outs):
+            p.positions -= n
+            p.query.normal_()
+            graph.replay()
+            eager = run(pkg, p)
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager)
+            assert_within(out, *expected(p))
+
+
+def test_on_two_streams_at_once(pkg, device):
+    problems = [problem(device, _behind(1600, [(b * k) % 90 + 1 for b in range(30)]), shared=50, page=32, seed=20 + k) for k in (1, 2)]
+    want = [run(pkg, p) for p in problems]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in problems]
+    outs = [[], []]
+    for _ in range(10):
+        for p, stream, out in zip(problems, streams, outs):
+            with torch.cuda.stream(stream):
+                out.append(run(pkg, p))
+    torch.cuda.synchronize()
+    for w, out in zip(want, outs):
+        assert all(torch.equal(w, o) for o in out)
