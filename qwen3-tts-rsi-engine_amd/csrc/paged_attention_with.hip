@@ -4,8 +4,7 @@
 //   s_j = scale ks_j (q . k_j) (+ mask_j),  out = sum_j exp(s_j - m) vs_j v_j / sum_j exp(s_j - m)
 //
 // A workgroup takes one query head of a request, its waves every fourth key, with a running maximum.
-#include "paged_index.hpp"
-#include "q3t_common.hpp"
+#include "paged_with.hpp"
 
 namespace q3t {
 namespace paged_with {
@@ -80,10 +79,12 @@ __global__ void __launch_bounds__(64 * kWaves) simple_kernel(Params p) {
     else ((uint16_t *)a.out)[at] = (uint16_t)float_to_bf16(y);
 }
 
-static int check(const q3t_paged_args *a, const q3t_paged_scales *s, int64_t shared_pages) {
-    const int64_t need = q3t_paged_workspace_bytes(a);
-    if (need < 0) return Q3T_EINVAL;
+// The sizes of a launch; Q3T_OK, or the status to return.
+static int check(const q3t_paged_args *a, const q3t_paged_scales *s, int64_t shared_pages, paged::Sizes &z) {
+    if (!a) return Q3T_EINVAL;
     if (s && s->format != Q3T_I8 && s->format != Q3T_E4M3) return Q3T_EUNSUPPORTED;
+    const int status = s && s->format == Q3T_I8 ? paged::sizes_int8(a, z) : paged::sizes_e4m3(a, z);
+    if (status != Q3T_OK) return status;
     if (shared_pages < 0 || shared_pages > a->table_width || shared_pages * a->page_size >= a->ctx) return Q3T_EINVAL;
     return Q3T_OK;
 }
@@ -94,14 +95,17 @@ static int check(const q3t_paged_args *a, const q3t_paged_scales *s, int64_t sha
 using namespace q3t;
 
 extern "C" int64_t q3t_paged_workspace_bytes_with(const q3t_paged_args *a, const q3t_paged_scales *s, int64_t shared_pages) {
-    return paged_with::check(a, s, shared_pages) == Q3T_OK ? q3t_paged_workspace_bytes(a) : -1;
+    paged::Sizes z;
+    return paged_with::check(a, s, shared_pages, z) == Q3T_OK ? z.workspace : -1;
 }
 
 extern "C" int q3t_paged_attention_with(const q3t_paged_args *a, const q3t_paged_scales *s, int64_t shared_pages, void *stream) {
     using namespace paged_with;
-    const int status = check(a, s, shared_pages);
-    if (status != Q3T_OK) return status;
-    if (a->batch == 0) return Q3T_OK;
+    paged::Sizes z;
+    const int status = check(a, s, shared_pages, z);
+    if (status != Q3T_OK || a->batch == 0) return status;
+    if (s && shared_pages == 0)
+        return (s->format == Q3T_I8 ? paged::attend_int8 : paged::attend_e4m3)(a, z, s, paged::Behind{}, (hipStream_t)stream);
     if (!a->query || !a->key_pages || !a->value_pages || !a->page_table || !a->positions || !a->out) return Q3T_EINVAL;
     if (s && (!s->key_scales || !s->value_scales || !aligned(s->key_scales, 4) || !aligned(s->value_scales, 4))) return Q3T_EINVAL;
     if (a->mask && (a->mask_dtype < Q3T_BF16 || a->mask_dtype > Q3T_BOOL)) return Q3T_EINVAL;
@@ -116,7 +120,7 @@ extern "C" int q3t_paged_attention_with(const q3t_paged_args *a, const q3t_paged
     if (!aligned(a->query, 16) || !aligned(a->key_pages, 16) || !aligned(a->value_pages, 16) || !aligned(a->out, es) ||
         !aligned(a->page_table, 4) || !aligned(a->positions, 8) || (a->mask && !aligned(a->mask, mask_size)))
         return Q3T_EINVAL;
-    if (!a->workspace || a->workspace_bytes < q3t_paged_workspace_bytes(a)) return Q3T_EWORKSPACE;
+    if (!a->workspace || a->workspace_bytes < z.workspace) return Q3T_EWORKSPACE;
     Params p = {};
     p.a = *a;
     if (s) p.s = *s;

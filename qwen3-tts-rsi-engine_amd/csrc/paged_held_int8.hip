@@ -1,0 +1,21 @@
+// The attention over pages of int8 rows (paged_attention_with.hip).
+#include "paged_with.hpp"
+
+namespace q3t {
+namespace paged {
+
+// f on the Launch of a call's type and width
+constexpr auto with = [](const q3t_paged_args *a, auto f) {
+    const bool wide = a->head_dim == 128;
+    if (a->dtype == Q3T_F32) return wide ? f(Launch<Held<float, false>, 128>{}) : f(Launch<Held<float, false>, 64>{});
+    if (a->dtype == Q3T_BF16) return wide ? f(Launch<Held<__bf16, false>, 128>{}) : f(Launch<Held<__bf16, false>, 64>{});
+    return wide ? f(Launch<Held<_Float16, false>, 128>{}) : f(Launch<Held<_Float16, false>, 64>{});
+};
+
+int sizes_int8(const q3t_paged_args *a, Sizes &z) { return sizes_of(a, z, with); }
+int attend_int8(const q3t_paged_args *a, const Sizes &z, const q3t_paged_scales *s, const Behind &behind, hipStream_t stream) {
+    return attend_with(a, z, s, behind, stream, with);
+}
+
+}  // namespace paged
+}  // namespace q3t
