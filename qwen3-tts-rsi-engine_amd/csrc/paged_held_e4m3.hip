@@ -13,8 +13,8 @@ constexpr auto with = [](const q3t_paged_args *a, auto f) {
 };
 
 int sizes_e4m3(const q3t_paged_args *a, Sizes &z) { return sizes_of(a, z, with); }
-int attend_e4m3(const q3t_paged_args *a, const Sizes &z, const q3t_paged_scales *s, const Behind &behind, hipStream_t stream) {
-    return attend_with(a, z, s, behind, stream, with);
+int attend_e4m3(const q3t_paged_args *a, const Sizes &z, const q3t_paged_scales *s, hipStream_t stream) {
+    return attend_with(a, z, s, stream, with);
 }
 
 }  // namespace paged
