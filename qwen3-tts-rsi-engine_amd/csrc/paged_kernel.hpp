@@ -64,6 +64,8 @@ struct MoreParams : Params {
     uint32_t skip;                                     // keys of the prefix
     uint32_t parts, columns_all;                       // states of a query head over the prefix; query heads of a KV head in the batch
     const float *prefix, *prefix_ml;                   // (part, KV head, request and query head): D values; maximum and sum
+    const uint32_t *odd;                               // one that is not zero: these states are not to be used
+    uint32_t odds, skip_pages;
 };
 
 template <typename T, int D>
@@ -586,6 +588,16 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
     __shared__ Lds<T, D, MASK, W> s;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = (int)uniform(tid >> 6);
+    if constexpr (MORE && !HELD) {
+        uint32_t odd = 0;
+        for (uint32_t i = lane; i < p.odds; i += 64) odd |= p.odd[i];
+        if (__builtin_amdgcn_ballot_w64(odd != 0)) {  // the prefix' keys as all others
+            ctx += p.skip;
+            p.table -= p.skip_pages;
+            if constexpr (MASK) p.mask -= (uint64_t)p.skip * p.m_st * (p.mask_dtype == Q3T_F32 ? 4 : p.mask_dtype == Q3T_BOOL ? 1 : 2);
+            p.skip = p.parts = 0;
+        }
+    }
 
     // ---- the share: every wave adds up all requests' stages and pieces for itself ---------------
     auto length_at = [&](uint32_t b) {
@@ -654,7 +666,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
         return at.left > 0;
     };
     if constexpr (SINGLE) {
-        constexpr uint32_t kRoom = 1u << kLogLeastSingle;  // holds any such pair's stages
+        constexpr uint32_t kRoom = 1u << (MORE ? 21 : kLogLeastSingle);  // holds any such pair's stages
         sh = {kRoom, 0u, kRoom, batch * p.heads * kRoom};
         const uint32_t b = blockIdx.x / p.heads;
         at = Cursor{blockIdx.x * kRoom, kRoom, b, blockIdx.x - b * p.heads, 0u};
@@ -972,10 +984,19 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
         if constexpr (MORE) {
             const uint32_t h = kv_head(r.head), kv_heads = p.heads / p.blocks;
             const uint64_t row = (uint64_t)h * p.columns_all + r.b * p.group + first_head(r.head) - h * p.group + column;
-            for (uint32_t i = 0; i < p.parts; ++i) {
-                const uint64_t at = (uint64_t)i * kv_heads * p.columns_all + row;
-                const f32x2_t ml = *reinterpret_cast<const f32x2_t *>(p.prefix_ml + 2 * at);
-                sum.add(State{ml[0], ml[1], *reinterpret_cast<const f32x4_t *>(p.prefix + at * D + d)}, unit);
+            constexpr uint32_t kFlight = 4;  // states on their way at once
+            for (uint32_t i = 0; i < p.parts; i += kFlight) {
+                f32x2_t ml[kFlight];
+                f32x4_t a[kFlight];
+#pragma unroll
+                for (uint32_t j = 0; j < kFlight; ++j) {
+                    const uint64_t at = (uint64_t)min(i + j, p.parts - 1) * kv_heads * p.columns_all + row;
+                    ml[j] = *reinterpret_cast<const f32x2_t *>(p.prefix_ml + 2 * at);
+                    a[j] = *reinterpret_cast<const f32x4_t *>(p.prefix + at * D + d);
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < kFlight; ++j)
+                    if (i + j < p.parts) sum.add(State{ml[j][0], ml[j][1], a[j]}, unit);
             }
         }
         float y[4];

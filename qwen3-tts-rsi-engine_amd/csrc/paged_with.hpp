@@ -77,7 +77,10 @@ static int shared_attend(const q3t_paged_args *a, int64_t keys, hipStream_t stre
     p.parts = (uint32_t)plan.parts;
     p.columns_all = (uint32_t)plan.columns;
     p.prefix = states;
-    p.prefix_ml = states + plan.parts * a->kv_heads * plan.columns * a->head_dim;
+    p.prefix_ml = states + plan.states * a->head_dim;
+    p.odd = (const uint32_t *)(p.prefix_ml + 2 * plan.states);
+    p.odds = (uint32_t)plan.workgroups;
+    p.skip_pages = (uint32_t)(keys / a->page_size);
     with(&b, [&](auto l) { l.run(&b, z.pairs, p, (uint32_t)z.workgroups, stream); });
     return launch_status();
 }
