@@ -6,7 +6,7 @@
 //   * A workgroup takes one KV head, a block of CW * CT * 16 columns and a part of the keys.  CW waves share a stage of
 //     keys in LDS, each with CT tiles of 16 columns in registers; KW such groups take the stages in turn and are merged
 //     at the end.
-//   * Stages come straight from memory to LDS, two ahead of the one that is multiplied.
+//   * Stages come straight from memory to LDS, ahead of the one that is multiplied.
 //   * The weights go into the second product in one part of the type's own bits (half a step of 2^-8 in bf16, as the
 //     prefill's weights have; float32 is multiplied as such): here, unlike in the attention of one request, the matrix
 //     cores are the bound.  Their sum is that of the rounded weights, by a product with ones, so that what rounding takes
@@ -33,8 +33,9 @@ struct PrefixParams {
     uint32_t heads, columns, blocks;    // KV heads; columns of one, and their blocks
     uint32_t parts, keys, chunk;        // parts of `chunk` keys
     uint32_t pages, ctx;
+    int32_t flip, zero;                 // unmasked: the scale is below zero, is zero
     Divisor by_page, by_group;
-    float scale;                        // unmasked: times log2(e)
+    float scale;                        // unmasked: its size times log2(e), 1 for none
 };
 
 // The products of a wave's CT tiles of 16 columns with a stage's keys.
@@ -46,9 +47,13 @@ template <typename T, int D, int CT> struct Wide {
     f32x4_t acc[CT][D / 16], sum[CT];
     uint32_t key_at[D / 32], value_at[D / 16];
 
-    Q3T_DEVICE void load_query(int ct, const char *row, int g, bool live) {
+    Q3T_DEVICE void load_query(int ct, const char *row, int g, bool live, bool flip) {
+        const uint32_t sign = flip ? 0x80008000u : 0u;
 #pragma unroll
-        for (int kk = 0; kk < D / 32; ++kk) q[ct][kk] = live ? load16(row + (4 * kk + g) * 16) : U4{0u, 0u, 0u, 0u};
+        for (int kk = 0; kk < D / 32; ++kk) {
+            const U4 x = live ? load16(row + (4 * kk + g) * 16) : U4{0u, 0u, 0u, 0u};
+            q[ct][kk] = U4{x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign};
+        }
     }
     // The query rows have come: no wait for them is left to the loop, where it would hold up the stages.
     Q3T_DEVICE void settle() {
@@ -77,14 +82,15 @@ template <typename T, int D, int CT> struct Wide {
         for (int d = 0; d < D / 16; ++d)
             value_at[d] = (keys + r) * S::row + (((2 * d + ((c >> 1) & 1)) ^ S::value_swizzle(r)) & (S::chunks - 1)) * 16 + 8 * (c & 1);
     }
-    U4 v[D / 16];  // a stage's value fragments
-    Q3T_DEVICE void scores(uint32_t stage, f32x4_t (&s)[CT][tiles]) {
-        U4 k[tiles][D / 32];
+    U4 k[tiles][D / 32], v[D / 16], p[CT];  // a stage's fragments of keys and values, its weights
+    Q3T_DEVICE void read_keys(uint32_t stage) {
 #pragma unroll
         for (int t = 0; t < tiles; ++t)
 #pragma unroll
             for (int kk = 0; kk < D / 32; ++kk) k[t][kk] = lds_read16(key_at[kk] + stage + t * 16 * S::row);
         together();
+    }
+    Q3T_DEVICE void scores(f32x4_t (&s)[CT][tiles]) const {
 #pragma unroll
         for (int t = 0; t < tiles; ++t)
 #pragma unroll
@@ -109,19 +115,19 @@ template <typename T, int D, int CT> struct Wide {
         return U4{Half<T>::round2(w[0][0], w[0][1]), Half<T>::round2(w[0][2], w[0][3]), Half<T>::round2(w[1][0], w[1][1]),
                   Half<T>::round2(w[1][2], w[1][3])};
     }
-    Q3T_DEVICE void sums(const float (&w)[CT][tiles][4]) {
-        const uint32_t one = std::is_same<T, __bf16>::value ? 0x3f803f80u : 0x3c003c00u;
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) sum[ct] = Half<T>::scores(U4{one, one, one, one}, pack(w[ct]), sum[ct]);
+    // (worked out here, not where they are used)
+    Q3T_DEVICE void weights(int ct, const float (&w)[tiles][4]) {
+        p[ct] = pack(w);
+        asm volatile("" : "+v"(p[ct].x), "+v"(p[ct].y), "+v"(p[ct].z), "+v"(p[ct].w));
     }
-    Q3T_DEVICE void values(const float (&w)[CT][tiles][4]) {
-        U4 p[CT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) p[ct] = pack(w[ct]);
+    Q3T_DEVICE void values() {
+        const uint32_t one = std::is_same<T, __bf16>::value ? 0x3f803f80u : 0x3c003c00u;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d)
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) acc[ct][d] = Half<T>::scores(v[d], p[ct], acc[ct][d]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) sum[ct] = Half<T>::scores(U4{one, one, one, one}, p[ct], sum[ct]);
     }
     Q3T_DEVICE float total(int ct) const { return sum[ct][0]; }
     // the values' dims, as they are stored: 16 bytes of acc[][a] from dim
@@ -143,10 +149,12 @@ template <int D, int CT> struct Wide<float, D, CT> {
     float sum[CT];
     uint32_t key_at[D / 16], value_at;
 
-    Q3T_DEVICE void load_query(int ct, const char *row, int g, bool live) {
+    Q3T_DEVICE void load_query(int ct, const char *row, int g, bool live, bool flip) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-            q[ct][kk] = __builtin_bit_cast(f32x4_t, live ? load16(row + (4 * kk + g) * 16) : U4{0u, 0u, 0u, 0u});
+        for (int kk = 0; kk < D / 16; ++kk) {
+            const f32x4_t x = __builtin_bit_cast(f32x4_t, live ? load16(row + (4 * kk + g) * 16) : U4{0u, 0u, 0u, 0u});
+            q[ct][kk] = flip ? -x : x;
+        }
     }
     Q3T_DEVICE void settle() {
 #pragma unroll
@@ -170,12 +178,14 @@ template <int D, int CT> struct Wide<float, D, CT> {
         for (int kk = 0; kk < D / 16; ++kk) key_at[kk] = c * S::row + ((4 * kk + g) ^ S::key_swizzle(c)) * 16;
         value_at = (keys + 4 * g) * S::row + c * 16;
     }
-    f32x4_t v[4 * (D / 64)];
-    Q3T_DEVICE void scores(uint32_t stage, f32x4_t (&s)[CT][tiles]) {
-        f32x4_t k[D / 16];
+    f32x4_t k[D / 16], v[4 * (D / 64)];
+    float p[CT][4];
+    Q3T_DEVICE void read_keys(uint32_t stage) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) k[kk] = __builtin_bit_cast(f32x4_t, lds_read16(key_at[kk] + stage));
         together();
+    }
+    Q3T_DEVICE void scores(f32x4_t (&s)[CT][tiles]) const {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) s[ct][0] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -192,11 +202,15 @@ template <int D, int CT> struct Wide<float, D, CT> {
             for (int j = 0; j < D / 64; ++j) v[i * (D / 64) + j] = __builtin_bit_cast(f32x4_t, lds_read16(value_at + stage + i * S::row + j * 256));
         together();
     }
-    Q3T_DEVICE void sums(const float (&w)[CT][tiles][4]) {
+    Q3T_DEVICE void weights(int ct, const float (&w)[tiles][4]) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) sum[ct] += (w[ct][0][0] + w[ct][0][1]) + (w[ct][0][2] + w[ct][0][3]);
+        for (int i = 0; i < 4; ++i) {
+            p[ct][i] = w[0][i];
+            asm volatile("" : "+v"(p[ct][i]));
+        }
+        sum[ct] += (w[0][0] + w[0][1]) + (w[0][2] + w[0][3]);
     }
-    Q3T_DEVICE void values(const float (&w)[CT][tiles][4]) {
+    Q3T_DEVICE void values() {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -205,7 +219,7 @@ template <int D, int CT> struct Wide<float, D, CT> {
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int ct = 0; ct < CT; ++ct)
-                        acc[ct][4 * j + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i * (D / 64) + j][e], w[ct][0][i], acc[ct][4 * j + e], 0, 0, 0);
+                        acc[ct][4 * j + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i * (D / 64) + j][e], p[ct][i], acc[ct][4 * j + e], 0, 0, 0);
     }
     Q3T_DEVICE float total(int ct) const {
         const float l = sum[ct] + xor16(sum[ct]);
@@ -224,129 +238,114 @@ template <int D, int CT> struct Wide<float, D, CT> {
     static Q3T_DEVICE float visible(float w) { return w; }
 };
 
-// Loads into LDS from scalar addresses and an offset per lane.
-Q3T_DEVICE void load_rows_from(const uint64_t *from, const uint32_t *offset, uint32_t base) {
+// Loads into LDS from an address per lane (load_rows and load_half, for rows that several workgroups read).
+Q3T_DEVICE void load_shared(const uint64_t *p, uint32_t base) {
     asm volatile("s_mov_b32 m0, %0\n\t" Q3T_VMEM_SGPR_WAIT
-                 "global_load_lds_dwordx4 %1, %5\n\t"
-                 "global_load_lds_dwordx4 %2, %6 offset:1024\n\t"
-                 "global_load_lds_dwordx4 %3, %7 offset:2048\n\t"
-                 "global_load_lds_dwordx4 %4, %8 offset:3*1024"
-                 :: "s"(base), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3]), "s"(from[0]), "s"(from[1]),
-                    "s"(from[2]), "s"(from[3]) : "memory", "m0");
+                 "global_load_lds_dwordx4 %1, off\n\t"
+                 "global_load_lds_dwordx4 %2, off offset:1024\n\t"
+                 "global_load_lds_dwordx4 %3, off offset:2048\n\t"
+                 "global_load_lds_dwordx4 %4, off offset:3*1024"
+                 :: "s"(base), "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]) : "memory", "m0");
 }
-Q3T_DEVICE void load_half_from(const uint64_t *from, const uint32_t *offset, uint32_t base) {
+Q3T_DEVICE void load_shared_half(const uint64_t *p, uint32_t base) {
     asm volatile("s_mov_b32 m0, %0\n\t" Q3T_VMEM_SGPR_WAIT
-                 "global_load_lds_dwordx4 %1, %3\n\t"
-                 "global_load_lds_dwordx4 %2, %4 offset:1024"
-                 :: "s"(base), "v"(offset[0]), "v"(offset[1]), "s"(from[0]), "s"(from[1]) : "memory", "m0");
+                 "global_load_lds_dwordx4 %1, off\n\t"
+                 "global_load_lds_dwordx4 %2, off offset:1024"
+                 :: "s"(base), "v"(p[0]), "v"(p[1]) : "memory", "m0");
 }
 
-constexpr uint32_t kWindow = 1024;  // page numbers that a workgroup holds
+constexpr uint32_t kEntries = 1024;  // pages that a workgroup knows: those of its part
 
 template <typename T, int D, int CW, int KW, int CT>
 struct PrefixLds {
     typedef Wide<T, D, CT> X;
-    static constexpr int stage = 2 * X::keys * Shape<T, D>::row, buffers = 2 * KW * stage > 64 * 1024 ? 2 : 3;
+    static constexpr int stage = 2 * X::keys * Shape<T, D>::row, buffers = CW == 1 ? 2 : 4;
     union {
         alignas(1024) char ring[buffers][KW][stage];
         alignas(1024) f32x4_t merge[KW == 1 ? 1 : KW - 1][CW][CT][D / 16][64];  // the groups' states, each in the first group's order
     };
     float ml[KW][CW][CT][2][64];
-    uint32_t ids[kWindow];
+    uint64_t pages[kEntries][2];     // addresses of the head's first key and value row on a page, kBias short; odd for no page
     uint32_t odd;                    // values that are not finite were found
     uint32_t least;                  // keys that all live columns see
+    uint32_t holes;                  // entries that are no page
 };
 
 // CW waves share the columns, KW groups of them the stages.
-// WHOLE: a load's rows lie in one page.
+// WHOLE: a stage lies in one page, or pages of whole loads in a stage.
 template <typename T, int D, bool MASK, bool WHOLE, int CW, int KW, int CT>
 __global__ void __launch_bounds__(64 * CW * KW, (CW * KW / 4 * (sizeof(PrefixLds<T, D, CW, KW, CT>) <= 80 * 1024 ? 2 : 1)))
 prefix_kernel(PrefixParams p) {
     typedef Shape<T, D> S;
     typedef Wide<T, D, CT> X;
     typedef PrefixLds<T, D, CW, KW, CT> L;
-    constexpr int SK = X::keys, TILES = X::tiles, AHEAD = L::buffers - 1, kThreads = 64 * CW * KW;
+    constexpr int SK = X::keys, TILES = X::tiles, B = L::buffers, kThreads = 64 * CW * KW;
     constexpr int LOADS = L::stage / 1024 / CW;  // of a wave's share of a stage: keys' rows in the first half, values' in the second
-    constexpr int kRows = 1024 / S::row;         // of a load
     constexpr uint32_t kAll = (uint32_t)((1ull << SK) - 1);
+    static_assert(CW == 1 || KW == 2, "");
     static_assert(sizeof(f32x4_t) * (KW - 1) * CW * CT * (D / 16) * 64 <= sizeof(char) * L::buffers * KW * L::stage, "");
     __shared__ L s;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = (int)uniform(tid >> 6), cw = wave % CW, group = wave / CW;
 
     // all column blocks of a KV head's part follow each other on one XCD
-    const uint32_t unit = blockIdx.x / (8 * p.blocks) * 8 + blockIdx.x % 8, block = blockIdx.x / 8 % p.blocks;
-    if (unit >= p.heads * p.parts) return;
-    const uint32_t part = unit / p.heads, head = unit - part * p.heads;
+    const uint32_t task = blockIdx.x / (8 * p.blocks) * 8 + blockIdx.x % 8, block = blockIdx.x / 8 % p.blocks;
+    if (task >= p.heads * p.parts) return;
+    const uint32_t part = task / p.heads, head = task - part * p.heads;
     const uint32_t begin = part * p.chunk, end = min(p.keys, begin + p.chunk);
 
     // ---- stages ----
     const uint32_t ring = uniform(lds_at(&s.ring[0][0][0]));
-    uint32_t window = ~0u;  // first entry of the window
-    auto buffer = [&](uint32_t n) { return ring + ((n % L::buffers) * KW + group) * L::stage; };
+    const uint32_t entry0 = divide(begin, p.by_page);
+    auto buffer = [&](uint32_t n) { return ring + (n % B * KW + group) * L::stage; };
     const uint32_t sets = (end - begin + KW * SK - 1) / (KW * SK);  // of a stage for every group
     // row and chunk of the lane's 16 bytes of load i of the wave's share
     auto row_of = [&](int i) { return ((cw * LOADS + i) * 64 + lane) / S::chunks % SK; };
     auto is_value = [&](int i) { return cw * LOADS + i >= L::stage / 2048; };
-    // WHOLE: the lane's place from the first row of load i on; else the chunk that it takes of its row
-    uint32_t offset[LOADS];
+    // the lane's place in load i: entry and offset from those of the stage's first row (WHOLE), or the chunk of its row
+    uint32_t entry_of[LOADS], offset[LOADS];
+    constexpr uint32_t kBias = 4096;  // (the loads' offsets move both of their addresses: load i's is 1024 i short)
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        const int r = row_of(i);
-        offset[i] = lane % S::chunks ^ (is_value(i) ? S::value_swizzle(r) : S::key_swizzle(r));
-        if constexpr (WHOLE) offset[i] = (lane / S::chunks * (is_value(i) ? p.vp_st : p.kp_st) + offset[i]) * 16;
+        const uint32_t r = row_of(i), chunk = lane % S::chunks ^ (is_value(i) ? S::value_swizzle(r) : S::key_swizzle(r));
+        const uint32_t ahead = p.by_page.d < (uint32_t)SK ? r / p.by_page.d : 0;
+        entry_of[i] = ahead;
+        offset[i] = chunk * 16 + kBias - 1024 * (LOADS == 2 ? i : i & 3);
+        if constexpr (WHOLE) offset[i] += (r - ahead * p.by_page.d) * (is_value(i) ? p.vp_st : p.kp_st) * 16;
     }
+    const uint32_t pages = uniform(lds_at(&s.pages[0][0]));
+    const uint32_t last_entry = divide(end - 1, p.by_page) - entry0;
+    uint32_t holes = 0;
     auto load = [&](uint32_t n) {
-        const uint32_t first = begin + n * KW * SK, last = min(end, first + KW * SK) - 1;
-        const uint32_t from = divide(first, p.by_page), to = divide(last, p.by_page);
-        if (window == ~0u || to - window >= kWindow) {  // (the same for all waves)
-            if (window != ~0u) __syncthreads();
-            window = from;
-            const uint32_t entries = min(kWindow, divide(end - 1, p.by_page) - from + 1);
-            for (uint32_t i = tid; i < entries; i += kThreads) s.ids[i] = (uint32_t)p.table[from + i];
-            __syncthreads();
-        }
-        const uint32_t key0 = first + group * SK;
-        const uint32_t mine = min(key0 + lane % SK, end - 1);
-        const uint32_t my_entry = divide(mine, p.by_page), my_id = s.ids[my_entry - window];
-        const bool there = (uint32_t)lane < SK && key0 + lane < end && my_id < p.pages;
-        const uint32_t exists = (uint32_t)__builtin_amdgcn_ballot_w64(there);
-        const uint32_t base = uniform(buffer(n) + cw * LOADS * 1024);
-        // (the loads' offsets move both of their addresses)
-        auto short_of = [&](int i) { return (uint64_t)(1024 * (LOADS == 2 ? i : i & 3)); };
-        auto place = [&](int i, uint32_t id, uint32_t row) {
-            const bool value = is_value(i);
-            const uint64_t o = value ? (uint64_t)id * p.vp_sp + (uint64_t)row * p.vp_st + (uint64_t)head * p.vp_sh
-                                     : (uint64_t)id * p.kp_sp + (uint64_t)row * p.kp_st + (uint64_t)head * p.kp_sh;
-            return reinterpret_cast<uint64_t>(value ? p.vp : p.kp) + o * 16 - short_of(i);
-        };
+        const uint32_t key0 = begin + (n * KW + group) * SK;
         uint64_t at[LOADS];
         if constexpr (WHOLE) {
-            // lane r has the page of the stage's row r and its place there
-            const uint32_t my_row = mine - my_entry * p.by_page.d;
+            const uint32_t entry = divide(key0, p.by_page) - entry0;
+            const uint32_t row = p.by_page.d < (uint32_t)SK ? 0 : key0 - divide(key0, p.by_page) * p.by_page.d;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int r = (cw * LOADS + i) * kRows % SK;
-                const bool there = exists >> r & 1u;  // else: rows that are not looked at, from the first on
-                at[i] = place(i, there ? (uint32_t)__builtin_amdgcn_readlane((int)my_id, r) : 0u,
-                              there ? (uint32_t)__builtin_amdgcn_readlane((int)my_row, r) : 0u);
+                // (past the end, the part's last page: its rows are not looked at)
+                const uint64_t from = *(Q3T_LDS const uint64_t *)(uintptr_t)(pages + min(entry + entry_of[i], last_entry) * 16 + (is_value(i) ? 8 : 0));
+                at[i] = (from & ~(uint64_t)1) + (offset[i] + row * (is_value(i) ? p.vp_st : p.kp_st) * 16);
             }
-            if constexpr (LOADS == 2) load_half_from(at, offset, base);
-            else
-#pragma unroll
-                for (int i = 0; i < LOADS; i += 4) load_rows_from(at + i, offset + i, base + i * 1024);
         } else {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const uint32_t key = min(key0 + row_of(i), end - 1), entry = divide(key, p.by_page);
-                uint32_t id = s.ids[entry - window];
-                if (id >= p.pages) id = 0;
-                at[i] = place(i, id, key - entry * p.by_page.d) + offset[i] * 16;
+                const uint64_t from = *(Q3T_LDS const uint64_t *)(uintptr_t)(pages + (entry - entry0) * 16 + (is_value(i) ? 8 : 0));
+                at[i] = (from & ~(uint64_t)1) + (uint64_t)(key - entry * p.by_page.d) * (is_value(i) ? p.vp_st : p.kp_st) * 16 + offset[i];
             }
-            if constexpr (LOADS == 2) load_half(at, base);
-            else
+        }
+        const uint32_t base = uniform(buffer(n) + cw * LOADS * 1024);
+        if constexpr (LOADS == 2) load_shared_half(at, base);
+        else
 #pragma unroll
-                for (int i = 0; i < LOADS; i += 4) load_rows(at + i, base + i * 1024);
+            for (int i = 0; i < LOADS; i += 4) load_shared(at + i, base + i * 1024);
+        const uint32_t count = key0 < end ? min((uint32_t)SK, end - key0) : 0u;
+        uint32_t exists = (uint32_t)((1ull << count) - 1);
+        if (holes) {
+            const uint32_t key = min(key0 + lane % SK, end - 1);
+            exists &= (uint32_t)__builtin_amdgcn_ballot_w64(!(s.pages[divide(key, p.by_page) - entry0][0] & 1));
         }
         return exists;
     };
@@ -354,9 +353,18 @@ prefix_kernel(PrefixParams p) {
     // ---- columns ----
     if (tid == 0) {
         s.least = p.keys;
-        s.odd = 0;
+        s.odd = s.holes = 0;
     }
     __syncthreads();
+    for (uint32_t i = tid; i <= last_entry; i += kThreads) {
+        const uint32_t id = (uint32_t)p.table[entry0 + i], none = id >= p.pages;
+        auto first = [&](const char *pool, uint32_t page_stride, uint32_t head_stride) {
+            return reinterpret_cast<uint64_t>(pool) + ((uint64_t)(none ? 0 : id) * page_stride + (uint64_t)head * head_stride) * 16 - kBias + none;
+        };
+        s.pages[i][0] = first(p.kp, p.kp_sp, p.kp_sh);
+        s.pages[i][1] = first(p.vp, p.vp_sp, p.vp_sh);
+        if (none) s.holes = 1;
+    }
     X x;
     uint32_t column[CT], seen[CT], request[CT];  // keys that a column sees (one that attends nothing: all of them, for no state)
     bool live[CT];
@@ -370,54 +378,44 @@ prefix_kernel(PrefixParams p) {
         live[ct] = pos >= 0 && pos < (int64_t)p.ctx;
         seen[ct] = live[ct] && pos < (int64_t)p.keys ? (uint32_t)pos + 1 : p.keys;
         if (seen[ct] < p.keys) atomicMin(&s.least, seen[ct]);
-        x.load_query(ct, p.q + ((uint64_t)request[ct] * p.q_sb + (uint64_t)(head * p.by_group.d + (real ? i : 0)) * p.q_sh) * 16, g, real);
+        x.load_query(ct, p.q + ((uint64_t)request[ct] * p.q_sb + (uint64_t)(head * p.by_group.d + (real ? i : 0)) * p.q_sh) * 16, g, real && !p.zero, p.flip);
     }
     x.place(g, c);
     x.clear();
     x.settle();
     __syncthreads();
     const uint32_t least = uniform(s.least);
+    holes = uniform(s.holes);
 
-    float m[CT];
+    float m[CT], w[CT][TILES][4];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) m[ct] = -INFINITY;
-    const float unit_of = MASK ? kLog2e : 1.f;  // scores are natural under a mask, else in log2 units
-    const float threshold = MASK ? X::threshold / kLog2e : X::threshold;
+    // exponents are unit (v - m) in log2 units: v the products themselves, or, under a mask, the natural scores
+    const float unit = MASK ? kLog2e : p.scale, threshold = X::threshold / unit;
     bool odd = false;
-    uint32_t exists[AHEAD] = {};  // keys of the stages that are on their way
-    for (int32_t step = -AHEAD; step < (int32_t)sets; ++step) {
-        const uint32_t n = (uint32_t)step, key0 = begin + (n * KW + group) * SK, here = exists[0], at = buffer(n);
-        const bool partial = MASK || key0 + SK > least, hide = partial || here != kAll;
-        if (step >= 0) {
-        if (AHEAD == 1 || n + 1 == sets) wait_loads<0>();
-        else wait_loads<LOADS>();
-        // Value rows of keys that do not exist become zeros: zero times NaN would be NaN.  Where some column does not see
-        // all keys, values that are not finite are looked for, for the same reason.
-        if (hide) {
+    auto partial = [&](uint32_t key0) { return MASK || key0 + SK > least; };
+    // Stage n, whose loads of this wave have ended.  Value rows of keys that do not exist become zeros: zero times NaN would
+    // be NaN.  Where some column does not see all keys, values that are not finite are looked for, for the same reason.
+    auto arrived = [&](uint32_t n, uint32_t here) {
+        const uint32_t key0 = begin + (n * KW + group) * SK, at = buffer(n);
+        if (here == kAll && !partial(key0)) return;
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                if (!is_value(i)) continue;
-                const uint32_t to = at + (cw * LOADS + i) * 1024 + lane * 16;
-                if (!(here >> row_of(i) & 1u)) lds_write16(to, U4{0u, 0u, 0u, 0u});
-                else if (partial && !X::finite(lds_read16(to))) odd = true;
-            }
+        for (int i = 0; i < LOADS; ++i) {
+            if (!is_value(i)) continue;
+            const uint32_t to = at + (cw * LOADS + i) * 1024 + lane * 16;
+            if (!(here >> row_of(i) & 1u)) lds_write16(to, U4{0u, 0u, 0u, 0u});
+            else if (partial(key0) && !X::finite(lds_read16(to))) odd = true;
         }
-        lds_barrier();  // the stage is there for all waves, and all have left the one before
-        }
+    };
+    auto scores = [&] {
+        f32x4_t score[CT][TILES];
+        x.scores(score);
 #pragma unroll
-        for (int i = 0; i + 1 < AHEAD; ++i) exists[i] = exists[i + 1];
-        exists[AHEAD - 1] = n + AHEAD < sets ? load(n + AHEAD) : 0u;
-        if (step < 0) continue;
-
-        float w[CT][TILES][4];
-        {
-            f32x4_t score[CT][TILES];
-            x.scores(at, score);
-#pragma unroll
-            for (int k = 0; k < CT * TILES * 4; ++k) w[k / (TILES * 4)][k / 4 % TILES][k % 4] = score[k / (TILES * 4)][k / 4 % TILES][k % 4] * p.scale;
-        }
-        x.read_values(at);  // on their way during the softmax
-        if (hide) {
+        for (int k = 0; k < CT * TILES * 4; ++k) w[k / (TILES * 4)][k / 4 % TILES][k % 4] = score[k / (TILES * 4)][k / 4 % TILES][k % 4];
+    };
+    auto softmax = [&](uint32_t n, uint32_t here) {
+        const uint32_t key0 = begin + (n * KW + group) * SK;
+        if (here != kAll || partial(key0)) {
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -438,7 +436,7 @@ prefix_kernel(PrefixParams p) {
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t k = 16 * t + 4 * g + i;
                         const bool hidden = !(here >> k & 1u) || key0 + k >= seen[ct] || term[i] == -INFINITY;
-                        w[ct][t][i] = hidden ? -INFINITY : w[ct][t][i] + term[i];
+                        w[ct][t][i] = hidden ? -INFINITY : MASK ? w[ct][t][i] * p.scale + term[i] : w[ct][t][i];
                     }
                 }
         }
@@ -457,23 +455,77 @@ prefix_kernel(PrefixParams p) {
                 float top = fmaxf(highest[ct], m[ct]);
                 top = fmaxf(top, xor16(top));
                 top = fmaxf(top, xor32(top));
-                x.rescale(ct, fexp2((m[ct] - (top == -INFINITY ? 0.f : top)) * unit_of));
+                x.rescale(ct, fexp2((m[ct] - (top == -INFINITY ? 0.f : top)) * unit));
                 m[ct] = top;
             }
         }
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-            const float from = m[ct] == -INFINITY ? 0.f : m[ct];
+            const float from = X::shift - (m[ct] == -INFINITY ? 0.f : m[ct]) * unit;
 #pragma unroll
             for (int k = 0; k < TILES * 4; ++k) {
                 float &e = w[ct][k / 4][k % 4];
-                const float v = X::visible(fexp2((e - from) * unit_of + X::shift));
+                const float v = X::visible(fexp2(__builtin_fmaf(e, unit, from)));
                 // (the smallest weight is for keys that are seen)
                 e = X::visible(0.f) != 0.f && e == -INFINITY ? 0.f : v;
             }
+            x.weights(ct, w[ct]);
         }
-        x.sums(w);
-        x.values(w);
+    };
+
+    if constexpr (CW == 1) {
+        // each wave has stages of its own, and no barriers
+        uint32_t here = load(0);
+        for (uint32_t n = 0; n < sets; ++n) {
+            wait_loads<0>();
+            arrived(n, here);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the other buffer's reads have returned, too)
+            const uint32_t next = n + 1 < sets ? load(n + 1) : 0u;
+            x.read_keys(buffer(n));
+            scores();
+            x.read_values(buffer(n));  // on their way during the softmax
+            softmax(n, here);
+            x.values();
+            here = next;
+        }
+    } else {
+        // Two groups of waves in turn: while one multiplies, the values of its last stage and the scores of the next, the other one
+        // works out its weights, so that matrix cores and vector units are both busy.  Buffer n - 1 is free once its values have been
+        // read, and stage n + 3 goes there.
+        uint32_t exists[B];  // of stages n ... n + 3
+#pragma unroll
+        for (int n = 0; n < B - 1; ++n) exists[n] = (uint32_t)n < sets ? load(n) : 0u;
+        // the loads of stages up to n have ended, of those up to `issued` that are on their way
+        auto wait_for = [&](uint32_t n, uint32_t issued) {
+            const uint32_t behind = min(issued, sets - 1) - n;
+            if (behind == 0) wait_loads<0>();
+            else if (behind == 1) wait_loads<LOADS>();
+            else wait_loads<2 * LOADS>();
+        };
+        wait_for(0, B - 2);
+        arrived(0, exists[0]);
+        lds_barrier();
+        if (group) lds_barrier();
+        for (uint32_t n = 0; n < sets; ++n) {
+            __builtin_amdgcn_s_setprio(1);
+            x.read_keys(buffer(n));
+            if (n) x.values();
+            scores();
+            __builtin_amdgcn_s_setprio(0);
+            lds_barrier();
+            exists[B - 1] = n + B - 1 < sets ? load(n + B - 1) : 0u;
+            x.read_values(buffer(n));
+            softmax(n, exists[0]);
+            if (n + 1 < sets) {
+                wait_for(n + 1, n + B - 1);
+                arrived(n + 1, exists[1]);
+            }
+#pragma unroll
+            for (int i = 0; i + 1 < B; ++i) exists[i] = exists[i + 1];
+            lds_barrier();
+        }
+        x.values();
+        if (!group) lds_barrier();
     }
 
     // ---- the groups' states, into the first one's ----
@@ -482,7 +534,7 @@ prefix_kernel(PrefixParams p) {
     for (int ct = 0; ct < CT; ++ct) l[ct] = x.total(ct);
     if (odd) s.odd = 1;
     lds_barrier();  // all have left the last stage
-    if (tid == 0) p.odd[unit * p.blocks + block] = s.odd;
+    if (tid == 0) p.odd[task * p.blocks + block] = s.odd;
     if constexpr (KW > 1) {
         if (group > 0) {
 #pragma unroll
@@ -500,7 +552,7 @@ prefix_kernel(PrefixParams p) {
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
                 const float om = s.ml[n][cw][ct][0][lane], top = fmaxf(m[ct], om), from = top == -INFINITY ? 0.f : top;
-                const float e0 = fexp2((m[ct] - from) * unit_of), e1 = fexp2((om - from) * unit_of);
+                const float e0 = fexp2((m[ct] - from) * unit), e1 = fexp2((om - from) * unit);
                 l[ct] = l[ct] * e0 + s.ml[n][cw][ct][1][lane] * e1;
                 m[ct] = top;
 #pragma unroll
@@ -512,7 +564,7 @@ prefix_kernel(PrefixParams p) {
     for (int ct = 0; ct < CT; ++ct) {
         if (column[ct] >= p.columns) continue;
         const bool none = !live[ct] || l[ct] == 0.f;
-        if (g == 0) *reinterpret_cast<f32x2_t *>(p.ml + 2 * (rows + column[ct])) = none ? f32x2_t{-INFINITY, 0.f} : f32x2_t{m[ct], l[ct]};
+        if (g == 0) *reinterpret_cast<f32x2_t *>(p.ml + 2 * (rows + column[ct])) = none ? f32x2_t{-INFINITY, 0.f} : f32x2_t{MASK ? m[ct] : m[ct] * unit, l[ct]};
 #pragma unroll
         for (int a = 0; a < D / 16; ++a)
             *reinterpret_cast<f32x4_t *>(p.states + (rows + column[ct]) * D + X::dim(a, g)) = none ? f32x4_t{0.f, 0.f, 0.f, 0.f} : x.four(ct, a);
@@ -543,6 +595,8 @@ static PrefixPlan prefix_plan(const q3t_paged_args *a, int64_t keys) {
     z.chunk = (keys + parts - 1) / parts;
     if (z.chunk < kLeastChunk) z.chunk = kLeastChunk;
     z.chunk = (z.chunk + step - 1) / step * step;
+    const int64_t most = (kEntries - 2) * a->page_size / step * step;  // whose page numbers a workgroup holds
+    if (z.chunk > most) z.chunk = most;
     z.parts = (keys + z.chunk - 1) / z.chunk;
     z.states = z.parts * a->kv_heads * z.columns;
     z.workgroups = z.parts * a->kv_heads * z.blocks;
@@ -571,10 +625,17 @@ static int prefix_run(const q3t_paged_args *a, const PrefixPlan &z, int64_t keys
     x.by_page = p.by_page;
     x.by_group = divisor(p.group);
     x.scale = p.scale;
+    if (!mask) {
+        x.flip = p.scale < 0.f;
+        x.zero = p.scale == 0.f;
+        x.scale = x.zero ? 1.f : p.scale < 0.f ? -p.scale : p.scale;
+    }
     const int64_t units = a->kv_heads * z.parts;
     const dim3 grid((uint32_t)((units + 7) / 8 * 8 * z.blocks));
-    // (a lane's offset within a load has 32 bits)
-    const bool whole = a->page_size % (1024 / (a->head_dim * (int64_t)sizeof(T))) == 0 && (p.kp_st | p.vp_st) < 1 << 20;
+    // (offsets within a page have 32 bits)
+    const int64_t stage = sizeof(T) == 4 ? 16 : 32, rows = 1024 / (a->head_dim * (int64_t)sizeof(T));
+    const bool whole = (a->page_size % stage == 0 || (stage % a->page_size == 0 && a->page_size % rows == 0)) &&
+                       (int64_t)(p.kp_st > p.vp_st ? p.kp_st : p.vp_st) * a->page_size < (1 << 27) - 1024;
     auto shape = [&](auto d, auto masked, auto in_one) {
         constexpr int D = decltype(d)::value;
         constexpr bool MASK = decltype(masked)::value, WHOLE = decltype(in_one)::value;
