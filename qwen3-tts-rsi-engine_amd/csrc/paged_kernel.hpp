@@ -980,25 +980,31 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
             x.values(w);
         }
     };
-    auto finish = [&](const Run &r, uint32_t column, uint32_t d, State sum) {
+    // The states over the prefix of four elements of a column, every `step`-th part from `from` on.
+    auto prefix_state = [&](const Run &r, uint32_t column, uint32_t d, uint32_t from, uint32_t step) {
+        State sum = {};
+        sum.m = -INFINITY;
         if constexpr (MORE) {
             const uint32_t h = kv_head(r.head), kv_heads = p.heads / p.blocks;
             const uint64_t row = (uint64_t)h * p.columns_all + r.b * p.group + first_head(r.head) - h * p.group + column;
             constexpr uint32_t kFlight = 4;  // states on their way at once
-            for (uint32_t i = 0; i < p.parts; i += kFlight) {
+            for (uint32_t i = from; i < p.parts; i += kFlight * step) {
                 f32x2_t ml[kFlight];
                 f32x4_t a[kFlight];
 #pragma unroll
                 for (uint32_t j = 0; j < kFlight; ++j) {
-                    const uint64_t at = (uint64_t)min(i + j, p.parts - 1) * kv_heads * p.columns_all + row;
+                    const uint64_t at = (uint64_t)min(i + j * step, p.parts - 1) * kv_heads * p.columns_all + row;
                     ml[j] = *reinterpret_cast<const f32x2_t *>(p.prefix_ml + 2 * at);
                     a[j] = *reinterpret_cast<const f32x4_t *>(p.prefix + at * D + d);
                 }
 #pragma unroll
                 for (uint32_t j = 0; j < kFlight; ++j)
-                    if (i + j < p.parts) sum.add(State{ml[j][0], ml[j][1], a[j]}, unit);
+                    if (i + j * step < p.parts) sum.add(State{ml[j][0], ml[j][1], a[j]}, unit);
             }
         }
+        return sum;
+    };
+    auto finish = [&](const Run &r, uint32_t column, uint32_t d, const State &sum) {
         float y[4];
         const float inverse = sum.l == 0.f ? 0.f : 1.f / sum.l;
 #pragma unroll
@@ -1007,6 +1013,10 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
         store_out<Q>(p.out + ((uint64_t)r.b * p.o_sb + (uint64_t)(first_head(r.head) + column) * p.o_sh + d) * sizeof(Q), y, p.vec_out);
     };
     const uint32_t state_size = p.columns * (D + 2);
+    uint32_t p_parts = 0;
+    if constexpr (MORE) p_parts = p.parts;
+    // (a thread's place behind a wave's states, where groups of threads have some each)
+    static_assert(!MORE || HELD || kThreads / (D / 4) * D * 4 / 2 + 64 * 32 <= S::stage, "");
 
     for (int32_t order = 0; at.left > 0; ++order) {
         const Run r = next_run(at, stages_of(request_length(at.b)), p.heads, sh);
@@ -1067,11 +1077,28 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
         int32_t *counter = p.counters + r.b * p.heads + r.head;
         if (!whole && tid == kThreads - 1 && r.parts == 2 && r.begins)
             s.there = (uint32_t)__hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // The pair's first part takes in the states over the prefix: all threads have some of them on their way while the waves'
+        // own are stored, behind those in the free slots.
+        const uint32_t items = columns * (D / 4);
+        const bool prefix = MORE && p_parts && r.begins;
+        const uint32_t prefix_groups = prefix ? max(1u, min(p_parts, kThreads / items)) : 0u;
+        auto prefix_place = [&](uint32_t t) { return s.slot[t >> 6] + columns * D * 4 + (t & 63) * 32; };
+        State before = {};
+        const uint32_t prefix_group = prefix_groups > 1 ? tid / items : 0u;
+        if (prefix_groups > 1 && prefix_group < prefix_groups) {
+            const uint32_t item = tid - prefix_group * items;
+            before = prefix_state(r, item / (D / 4), item % (D / 4) * 4, prefix_group, prefix_groups);
+        }
         if ((uint32_t)c < columns) x.store(slot, g, c);
+        if (prefix_groups > 1) {
+            const uint32_t to = slot + columns * D * 4 + lane * 32;
+            lds_write16(to, __builtin_bit_cast(U4, before.a));
+            lds_write16(to + 16, U4{__float_as_uint(before.m), __float_as_uint(before.l), 0u, 0u});
+        }
         lds_barrier();
         const bool two = !whole && r.parts == 2 && r.begins && uniform(s.there) == 1;
         float *state = p.states + (2 * blockIdx.x + r.begins) * (uint64_t)state_size;
-        for (uint32_t item = tid; item < columns * (D / 4); item += kThreads) {
+        for (uint32_t item = tid; item < items; item += kThreads) {
             const uint32_t column = item / (D / 4), chunk = item % (D / 4);
             State own = {};
             own.m = -INFINITY;
@@ -1083,6 +1110,15 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
                 const float e = fexp2((s.ml[w][column][0] - from) * unit);
                 own.l += s.ml[w][column][1] * e;
                 own.a += __builtin_bit_cast(f32x4_t, lds_read16(s.slot[w] + column * D * 4 + (chunk ^ column) * 16)) * e;
+            }
+            if (prefix) {
+                if (prefix_groups == 1) own.add(prefix_state(r, column, chunk * 4, 0, 1), unit);
+                else
+                    for (uint32_t o = 0; o < prefix_groups; ++o) {
+                        const uint32_t from = prefix_place(item + o * items);
+                        const U4 ml = lds_read16(from + 16);
+                        own.add(State{__uint_as_float(ml.x), __uint_as_float(ml.y), __builtin_bit_cast(f32x4_t, lds_read16(from))}, unit);
+                    }
             }
             if (two) {
                 State other;
@@ -1237,7 +1273,9 @@ struct Launch {
         return few(a, pairs) || small(a, pairs);
     }
     static bool eight(const q3t_paged_args *a, int64_t pairs) {
-        const bool many = S::row > 128 && a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
+        // (float32 queries of 8-bit rows of 128: one workgroup of four waves is all that a CU's LDS holds; 128 requests of
+        // 100..4095 keys four / eight 143 / 107 us, but with bf16 queries 64 of 64..1023 22.9 / 26.2)
+        const bool many = (S::row > 128 || (S::held && Workgroups<T, D, 4>::per_cu == 1)) && a->ctx >= kLongRequest && pairs <= kFewPairs && stages(a, pairs, 4) >= kManyStages;
         const bool wide = a->q_heads / a->kv_heads > kWideGroup && a->ctx >= (S::row == 128 ? kWideNarrow : kWideRequest);
         return few(a, pairs) || (S::row < 512 && ranges(a) == 1 && (many || wide));
     }

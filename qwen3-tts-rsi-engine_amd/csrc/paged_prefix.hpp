@@ -29,7 +29,7 @@ struct PrefixParams {
     uint32_t *odd;                      // of each workgroup: its states are not to be used, nor any other
     uint32_t q_sb, q_sh, kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;  // 16 bytes
     uint32_t m_sb, m_st;                // elements
-    int32_t mask_dtype;
+    int32_t mask_dtype, mask_vec;       // four terms at once: unit strides, aligned, keys a multiple of 4
     uint32_t heads, columns, blocks;    // KV heads; columns of one, and their blocks
     uint32_t parts, keys, chunk;        // parts of `chunk` keys
     uint32_t pages, ctx;
@@ -316,9 +316,10 @@ prefix_kernel(PrefixParams p) {
     const uint32_t pages = uniform(lds_at(&s.pages[0][0]));
     const uint32_t last_entry = divide(end - 1, p.by_page) - entry0;
     uint32_t holes = 0;
-    auto load = [&](uint32_t n) {
+    uint64_t at[LOADS];  // of the next stage's loads
+    // works them out, and says which of stage n's keys exist
+    auto locate = [&](uint32_t n) {
         const uint32_t key0 = begin + (n * KW + group) * SK;
-        uint64_t at[LOADS];
         if constexpr (WHOLE) {
             const uint32_t entry = divide(key0, p.by_page) - entry0;
             const uint32_t row = p.by_page.d < (uint32_t)SK ? 0 : key0 - divide(key0, p.by_page) * p.by_page.d;
@@ -336,11 +337,6 @@ prefix_kernel(PrefixParams p) {
                 at[i] = (from & ~(uint64_t)1) + (uint64_t)(key - entry * p.by_page.d) * (is_value(i) ? p.vp_st : p.kp_st) * 16 + offset[i];
             }
         }
-        const uint32_t base = uniform(buffer(n) + cw * LOADS * 1024);
-        if constexpr (LOADS == 2) load_shared_half(at, base);
-        else
-#pragma unroll
-            for (int i = 0; i < LOADS; i += 4) load_shared(at + i, base + i * 1024);
         const uint32_t count = key0 < end ? min((uint32_t)SK, end - key0) : 0u;
         uint32_t exists = (uint32_t)((1ull << count) - 1);
         if (holes) {
@@ -350,14 +346,38 @@ prefix_kernel(PrefixParams p) {
         return exists;
     };
 
+    auto load = [&](uint32_t n) {
+        const uint32_t base = uniform(buffer(n) + cw * LOADS * 1024);
+        if constexpr (LOADS == 2) load_shared_half(at, base);
+        else
+#pragma unroll
+            for (int i = 0; i < LOADS; i += 4) load_shared(at + i, base + i * 1024);
+    };
+
     // ---- columns ----
+    X x;
+    uint32_t column[CT], seen[CT], request[CT];  // keys that a column sees (one that attends nothing: all of them, for no state)
+    bool live[CT];
+    // what all of it starts with, on its way together: positions, query rows, page numbers
+    int64_t position[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        column[ct] = (block * CW * CT + cw * CT + ct) * kColumns + c;
+        const bool real = column[ct] < p.columns;
+        request[ct] = real ? divide(column[ct], p.by_group) : 0;
+        const uint32_t i = column[ct] - request[ct] * p.by_group.d;
+        position[ct] = p.positions[request[ct]];
+        if (!real) position[ct] = -1;
+        x.load_query(ct, p.q + ((uint64_t)request[ct] * p.q_sb + (uint64_t)(head * p.by_group.d + (real ? i : 0)) * p.q_sh) * 16, g, real && !p.zero, p.flip);
+    }
+    const uint32_t first_id = (uint32_t)p.table[entry0 + min((uint32_t)tid, last_entry)];
     if (tid == 0) {
         s.least = p.keys;
         s.odd = s.holes = 0;
     }
     __syncthreads();
     for (uint32_t i = tid; i <= last_entry; i += kThreads) {
-        const uint32_t id = (uint32_t)p.table[entry0 + i], none = id >= p.pages;
+        const uint32_t id = i == (uint32_t)tid ? first_id : (uint32_t)p.table[entry0 + i], none = id >= p.pages;
         auto first = [&](const char *pool, uint32_t page_stride, uint32_t head_stride) {
             return reinterpret_cast<uint64_t>(pool) + ((uint64_t)(none ? 0 : id) * page_stride + (uint64_t)head * head_stride) * 16 - kBias + none;
         };
@@ -365,20 +385,11 @@ prefix_kernel(PrefixParams p) {
         s.pages[i][1] = first(p.vp, p.vp_sp, p.vp_sh);
         if (none) s.holes = 1;
     }
-    X x;
-    uint32_t column[CT], seen[CT], request[CT];  // keys that a column sees (one that attends nothing: all of them, for no state)
-    bool live[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-        column[ct] = (block * CW * CT + cw * CT + ct) * kColumns + c;
-        const bool real = column[ct] < p.columns;
-        request[ct] = real ? divide(column[ct], p.by_group) : 0;
-        const uint32_t i = column[ct] - request[ct] * p.by_group.d;
-        const int64_t pos = real ? p.positions[request[ct]] : -1;
-        live[ct] = pos >= 0 && pos < (int64_t)p.ctx;
-        seen[ct] = live[ct] && pos < (int64_t)p.keys ? (uint32_t)pos + 1 : p.keys;
+        live[ct] = position[ct] >= 0 && position[ct] < (int64_t)p.ctx;
+        seen[ct] = live[ct] && position[ct] < (int64_t)p.keys ? (uint32_t)position[ct] + 1 : p.keys;
         if (seen[ct] < p.keys) atomicMin(&s.least, seen[ct]);
-        x.load_query(ct, p.q + ((uint64_t)request[ct] * p.q_sb + (uint64_t)(head * p.by_group.d + (real ? i : 0)) * p.q_sh) * 16, g, real && !p.zero, p.flip);
     }
     x.place(g, c);
     x.clear();
@@ -407,6 +418,57 @@ prefix_kernel(PrefixParams p) {
             else if (partial(key0) && !X::finite(lds_read16(to))) odd = true;
         }
     };
+    // The mask's words of stage n, four keys of a column at once where they lie so, and the terms in them.
+    uint32_t words[CT][TILES][4] = {};
+    float terms[MASK ? CT : 1][TILES][4] = {};
+    auto fetch_terms = [&](uint32_t n) {
+        if constexpr (MASK) {
+            const uint32_t key0 = begin + (n * KW + group) * SK;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    uint32_t (&to)[4] = words[ct][t];
+                    const uint32_t key = key0 + 16 * t + 4 * g;
+                    const uint64_t row = (uint64_t)request[ct] * p.m_sb;
+                    if (p.mask_vec) {
+                        const uint64_t at = row + min(key, end - 4);
+                        if (p.mask_dtype == Q3T_F32) {
+                            const U4 x = load16(p.mask + at * 4);
+                            to[0] = x.x; to[1] = x.y; to[2] = x.z; to[3] = x.w;
+                        } else if (p.mask_dtype == Q3T_BOOL) {
+                            to[0] = *reinterpret_cast<const uint32_t *>(p.mask + at);
+                        } else {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(p.mask + at * 2);
+                            to[0] = x.x; to[1] = x.y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint64_t at = row + (uint64_t)min(key + i, end - 1) * p.m_st;
+                            to[i] = p.mask_dtype == Q3T_F32 ? reinterpret_cast<const uint32_t *>(p.mask)[at]
+                                  : p.mask_dtype == Q3T_BOOL ? reinterpret_cast<const uint8_t *>(p.mask)[at]
+                                                             : reinterpret_cast<const uint16_t *>(p.mask)[at];
+                        }
+                    }
+                }
+        }
+    };
+    auto read_terms = [&] {
+        if constexpr (MASK) {
+            const int of_word = !p.mask_vec || p.mask_dtype == Q3T_F32 ? 1 : p.mask_dtype == Q3T_BOOL ? 4 : 2;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t (&from)[4] = words[ct][t];
+                        const uint32_t e = of_word == 1 ? from[i] : of_word == 4 ? from[0] >> 8 * i : from[i / 2] >> 16 * (i & 1);
+                        terms[ct][t][i] = mask_term(e, p.mask_dtype);
+                    }
+        }
+    };
     auto scores = [&] {
         f32x4_t score[CT][TILES];
         x.scores(score);
@@ -421,17 +483,9 @@ prefix_kernel(PrefixParams p) {
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
                     float term[4] = {};
-                    if constexpr (MASK) {
+                    if constexpr (MASK)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t key = min(key0 + 16 * t + 4 * g + i, end - 1);
-                            const uint64_t element = (uint64_t)request[ct] * p.m_sb + (uint64_t)key * p.m_st;
-                            const uint32_t e = p.mask_dtype == Q3T_F32 ? reinterpret_cast<const uint32_t *>(p.mask)[element]
-                                             : p.mask_dtype == Q3T_BOOL ? reinterpret_cast<const uint8_t *>(p.mask)[element]
-                                                                        : reinterpret_cast<const uint16_t *>(p.mask)[element];
-                            term[i] = mask_term(e, p.mask_dtype);
-                        }
-                    }
+                        for (int i = 0; i < 4; ++i) term[i] = terms[ct][t][i];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t k = 16 * t + 4 * g + i;
@@ -475,12 +529,20 @@ prefix_kernel(PrefixParams p) {
 
     if constexpr (CW == 1) {
         // each wave has stages of its own, and no barriers
-        uint32_t here = load(0);
+        uint32_t here = locate(0);
+        load(0);
+        fetch_terms(0);
         for (uint32_t n = 0; n < sets; ++n) {
             wait_loads<0>();
+            read_terms();
             arrived(n, here);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the other buffer's reads have returned, too)
-            const uint32_t next = n + 1 < sets ? load(n + 1) : 0u;
+            uint32_t next = 0;
+            if (n + 1 < sets) {
+                next = locate(n + 1);
+                load(n + 1);
+                fetch_terms(n + 1);
+            }
             x.read_keys(buffer(n));
             scores();
             x.read_values(buffer(n));  // on their way during the softmax
@@ -490,40 +552,48 @@ prefix_kernel(PrefixParams p) {
         }
     } else {
         // Two groups of waves in turn: while one multiplies, the values of its last stage and the scores of the next, the other one
-        // works out its weights, so that matrix cores and vector units are both busy.  Buffer n - 1 is free once its values have been
-        // read, and stage n + 3 goes there.
-        uint32_t exists[B];  // of stages n ... n + 3
-#pragma unroll
-        for (int n = 0; n < B - 1; ++n) exists[n] = (uint32_t)n < sets ? load(n) : 0u;
-        // the loads of stages up to n have ended, of those up to `issued` that are on their way
-        auto wait_for = [&](uint32_t n, uint32_t issued) {
-            const uint32_t behind = min(issued, sets - 1) - n;
-            if (behind == 0) wait_loads<0>();
-            else if (behind == 1) wait_loads<LOADS>();
-            else wait_loads<2 * LOADS>();
-        };
-        wait_for(0, B - 2);
+        // works out its weights, so that matrix cores and vector units are both busy.  Four buffers: of the stages whose values and
+        // whose keys are read, and of two that are on their way.
+        static_assert(B == 4, "");
+        uint32_t exists[4];  // of stages n ... n + 3
+        exists[0] = locate(0);
+        load(0);
+        exists[1] = exists[2] = exists[3] = 0;
+        if (sets > 1) {
+            exists[1] = locate(1);
+            load(1);
+            wait_loads<LOADS>();
+        } else {
+            wait_loads<0>();
+        }
+        if (sets > 2) exists[2] = locate(2);
         arrived(0, exists[0]);
         lds_barrier();
         if (group) lds_barrier();
         for (uint32_t n = 0; n < sets; ++n) {
             __builtin_amdgcn_s_setprio(1);
+            // (the terms' words are waited for below, and what is on its way before them: the next stage, which is needed then)
+            if (MASK) fetch_terms(n);
+            else if (n + 2 < sets) load(n + 2);
+            if (n) x.read_values(buffer(n - 1));
             x.read_keys(buffer(n));
             if (n) x.values();
             scores();
+            if (!MASK && n + 3 < sets) exists[3] = locate(n + 3);
             __builtin_amdgcn_s_setprio(0);
             lds_barrier();
-            exists[B - 1] = n + B - 1 < sets ? load(n + B - 1) : 0u;
-            x.read_values(buffer(n));
+            read_terms();
             softmax(n, exists[0]);
-            if (n + 1 < sets) {
-                wait_for(n + 1, n + B - 1);
-                arrived(n + 1, exists[1]);
-            }
+            if (MASK && n + 2 < sets) load(n + 2);
+            if (n + 2 < sets) wait_loads<LOADS>();
+            else wait_loads<0>();
+            if (n + 1 < sets) arrived(n + 1, exists[1]);
+            if (MASK && n + 3 < sets) exists[3] = locate(n + 3);
 #pragma unroll
-            for (int i = 0; i + 1 < B; ++i) exists[i] = exists[i + 1];
+            for (int i = 0; i < 3; ++i) exists[i] = exists[i + 1];
             lds_barrier();
         }
+        x.read_values(buffer(sets - 1));
         x.values();
         if (!group) lds_barrier();
     }
@@ -579,7 +649,7 @@ struct PrefixPlan {
 
 // By sizes alone: tiles for the columns that there are, and as many parts as fill the card with a chunk of kLeastChunk keys at least (a
 // state is written and read again for every part).
-constexpr int64_t kLeastChunk = 256;
+constexpr int64_t kLeastChunk = 64;
 
 template <typename T>
 static PrefixPlan prefix_plan(const q3t_paged_args *a, int64_t keys) {
@@ -618,6 +688,8 @@ static int prefix_run(const q3t_paged_args *a, const PrefixPlan &z, int64_t keys
     x.q_sb = p.q_sb; x.q_sh = p.q_sh;
     x.kp_sp = p.kp_sp; x.kp_sh = p.kp_sh; x.kp_st = p.kp_st; x.vp_sp = p.vp_sp; x.vp_sh = p.vp_sh; x.vp_st = p.vp_st;
     x.m_sb = p.m_sb; x.m_st = p.m_st; x.mask_dtype = p.mask_dtype;
+    const int64_t mask_size = a->mask_dtype == Q3T_F32 ? 4 : a->mask_dtype == Q3T_BOOL ? 1 : 2;
+    x.mask_vec = p.m_st == 1 && p.m_sb % 4 == 0 && aligned(mask, 4 * mask_size) && keys % 4 == 0;
     x.heads = (uint32_t)a->kv_heads; x.columns = (uint32_t)z.columns; x.blocks = (uint32_t)z.blocks;
     x.parts = (uint32_t)z.parts; x.keys = (uint32_t)keys; x.chunk = (uint32_t)z.chunk;
     x.pages = p.pages;

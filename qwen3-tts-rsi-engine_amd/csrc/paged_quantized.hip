@@ -29,11 +29,13 @@ struct Params {
     Divisor by_units, by_heads, by_page;
 };
 
-// Place of row t of request b: page and row of it, page -1 for a row that it has not.
+// Rows of a request that the call has.
+Q3T_DEVICE uint32_t used_rows(const Params &p, uint32_t b) {
+    return p.lengths ? (uint32_t)max(0, min(p.lengths[b], (int32_t)p.tokens)) : p.tokens;
+}
+// Place of row t of request b, whose first row is at `start`: page and row of it, page -1 for a row that it has not.
 struct Place { int32_t page; uint32_t row; };
-Q3T_DEVICE Place place(const Params &p, uint32_t b, uint32_t t) {
-    const int64_t start = p.positions[b];
-    const uint32_t used = p.lengths ? (uint32_t)max(0, min(p.lengths[b], (int32_t)p.tokens)) : p.tokens;
+Q3T_DEVICE Place place(const Params &p, uint32_t b, int64_t start, uint32_t used, uint32_t t) {
     // (start + t overflows for no start that is left)
     if (t >= used || start >= p.rows || start < -(int64_t)p.tokens || start + t < 0 || start + t >= p.rows) return {-1, 0u};
     const uint32_t j = (uint32_t)(start + t), entry = divide(j, p.by_page);
@@ -41,20 +43,33 @@ Q3T_DEVICE Place place(const Params &p, uint32_t b, uint32_t t) {
     return {(uint32_t)page < p.pages ? page : -1, j - entry * p.by_page.d};
 }
 
+// The call's rows are read and written once: the non-temporal policy.  The pools' are not, which what follows reads (16 prompts of
+// up to 1024 rows in int8 written and read back 32.5 us; all with the policy 37.3, none 37.1).
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
 template <typename T> struct Eight { alignas(16) T x[8]; };
 
-// Eight elements of a row in float32; VEC: by 16-byte loads.
-template <typename T, bool VEC>
-Q3T_DEVICE void load8(const char *from, float (&x)[8]) {
-    Eight<T> e;
+// Eight elements of a row; VEC: by 16-byte accesses.
+template <bool VEC, typename T>
+Q3T_DEVICE void load8(const char *from, Eight<T> &e) {
     if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<U4 *>(&e)[i] = reinterpret_cast<const U4 *>(from)[i];
+        for (int i = 0; i < (int)sizeof(e) / 16; ++i)
+            reinterpret_cast<u32x4_t *>(&e)[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(from) + i);
     } else {
         for (int i = 0; i < 8; ++i) e.x[i] = reinterpret_cast<const T *>(from)[i];
     }
+}
+template <bool VEC, typename T>
+Q3T_DEVICE void store8(char *to, const Eight<T> &e) {
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)e.x[i];
+        for (int i = 0; i < (int)sizeof(e) / 16; ++i)
+            __builtin_nontemporal_store(reinterpret_cast<const u32x4_t *>(&e)[i], reinterpret_cast<u32x4_t *>(to) + i);
+    } else {
+        for (int i = 0; i < 8; ++i) reinterpret_cast<T *>(to)[i] = e.x[i];
+    }
 }
 
 Q3T_DEVICE uint32_t dpp_max(uint32_t x, uint32_t y) { return x > y ? x : y; }
@@ -62,20 +77,56 @@ template <int CTRL> Q3T_DEVICE uint32_t dpp_u(uint32_t x) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, false);
 }
 
-// The largest |x| of a row of L lanes of eight elements, as bits: NaN above infinity above the rest.
-template <int L> Q3T_DEVICE uint32_t row_largest(const float (&x)[8]) {
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+Q3T_DEVICE uint32_t pairs_max(uint32_t x, uint32_t y) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, x), __builtin_bit_cast(u16x2_t, y)));
+}
+
+// The largest |x| of a row of L lanes of eight elements, as float32's bits: NaN above infinity above the rest.  Types of 16
+// bits are compared as such, two at once.
+template <int L, typename T> Q3T_DEVICE uint32_t row_largest(const Eight<T> &e) {
+    const uint32_t *bits = reinterpret_cast<const uint32_t *>(&e);
+    auto over_lanes = [](uint32_t m, auto max) {
+        m = max(m, dpp_u<kDppXor1>(m));
+        m = max(m, dpp_u<kDppXor2>(m));
+        m = max(m, dpp_u<kDppHalfMirror>(m));
+        return L == 16 ? max(m, xor8u(m)) : m;
+    };
     uint32_t m = 0;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = dpp_max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-    m = dpp_max(m, dpp_u<kDppXor1>(m));
-    m = dpp_max(m, dpp_u<kDppXor2>(m));
-    m = dpp_max(m, dpp_u<kDppHalfMirror>(m));
-    if (L == 16) m = dpp_max(m, xor8u(m));
-    return m;
+        for (int i = 0; i < 8; ++i) m = dpp_max(m, bits[i] & 0x7fffffffu);
+        return over_lanes(m, dpp_max);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = pairs_max(m, bits[i] & 0x7fff7fffu);
+        m = over_lanes(m, pairs_max);
+        m = dpp_max(m & 0xffffu, m >> 16);
+        if constexpr (std::is_same<T, _Float16>::value) return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)m));
+        return m << 16;
+    }
+}
+
+// x / 127 for x of 2^-100 and above, rounded as a division is: a quotient from the nearest reciprocal, put right by what it
+// leaves (Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990).
+Q3T_DEVICE float by_127(float x) {
+    const float r = 1.f / 127.f, q = x * r;
+    return __builtin_fmaf(__builtin_fmaf(-q, 127.f, x), r, q);
+}
+// 127 / x for the same: of its mantissa alone, whose reciprocal is a normal number (tried for all 2^23 of them).
+Q3T_DEVICE float of_127(float x) {
+    const uint32_t bits = __float_as_uint(x);
+    const float m = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+    float r = __builtin_amdgcn_rcpf(m);
+    r = __builtin_fmaf(__builtin_fmaf(-m, r, 1.f), r, r);
+    float q = 127.f * r;
+    q = __builtin_fmaf(__builtin_fmaf(-q, m, 127.f), r, q);
+    return __uint_as_float(__float_as_uint(q) - ((bits >> 23) - 127) * (1u << 23));
 }
 
 // A row's scale and the lane's eight elements.
 template <bool E4M3> Q3T_DEVICE uint2 quantise(const float (&x)[8], uint32_t largest, float &scale) {
+#pragma clang fp contract(off)
     const bool finite = largest < 0x7f800000u;
     const uint32_t a = dpp_max(largest, 0x0d800000u);  // 2^-100
     float inverse;
@@ -85,8 +136,8 @@ template <bool E4M3> Q3T_DEVICE uint2 quantise(const float (&x)[8], uint32_t lar
         scale = __uint_as_float(exponent << 23);
         inverse = __uint_as_float((254 - exponent) << 23);
     } else {
-        scale = __uint_as_float(a) / 127.f;
-        inverse = 127.f / __uint_as_float(a);
+        scale = by_127(__uint_as_float(a));
+        inverse = of_127(__uint_as_float(a));
     }
     if (!finite) scale = __uint_as_float(0x7fc00000u);
     uint32_t w[2];
@@ -96,31 +147,53 @@ template <bool E4M3> Q3T_DEVICE uint2 quantise(const float (&x)[8], uint32_t lar
             w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inverse, x[4 * i + 1] * inverse, 0, false);
             w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inverse, x[4 * i + 3] * inverse, (int)w[i], true);
         } else {
-            w[i] = 0;
+            // products of at most 127, rounded to whole numbers by an addition to 1.5 2^23, whose low byte they then are
+            uint32_t u[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[i] |= ((uint32_t)(int)__builtin_rintf(x[4 * i + k] * inverse) & 0xffu) << 8 * k;
+            for (int k = 0; k < 4; ++k) u[k] = __float_as_uint(x[4 * i + k] * inverse + 0x1.8p23f);
+            w[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], 0x00000400u), __builtin_amdgcn_perm(u[1], u[0], 0x00000400u), 0x05040100u);
         }
         if (!finite) w[i] = 0;
     }
     return uint2{w[0], w[1]};
 }
 
-// A thread takes eight elements of one row of the keys and of the values; L of them have a row.
-template <typename T, int L, bool E4M3, bool VEC>
+// A thread takes eight elements of N rows of the keys and of the values, 256 / L rows apart; L threads have a row.  The rows are on
+// their way before the positions and page numbers are known; with two of them (launches that fill the card) those past a request's
+// length are not read.
+template <typename T, int L, bool E4M3, bool VEC, int N>
 __global__ void __launch_bounds__(kThreads) write_kernel(Params p) {
     for (uint32_t b = blockIdx.y; b < p.batch; b += gridDim.y) {
-        const uint32_t i = blockIdx.x * kThreads + threadIdx.x, row = i / L, unit = i % L;
-        const uint32_t t = divide(row, p.by_heads), h = row - t * p.heads;
-        const Place at = place(p, b, t);
-        if (at.page < 0) continue;  // (the same for all lanes of a row)
+        const int64_t start = p.positions[b];
+        const uint32_t used = used_rows(p, b), unit = threadIdx.x % L;
+        Eight<T> e[N][2];
+        uint32_t t[N], h[N];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const Rows &r = p.x[n];
-            float x[8], scale;
-            load8<T, VEC>(r.rows + b * r.r_sb + h * r.r_sh + t * r.r_st + unit * 8 * sizeof(T), x);
-            const uint2 w = quantise<E4M3>(x, row_largest<L>(x), scale);
-            *reinterpret_cast<uint2 *>(r.pages + at.page * r.p_sp + h * r.p_sh + at.row * r.p_st + unit * 8) = w;
-            if (unit == 0) r.scales[at.page * r.s_sp + h * r.s_sh + at.row * r.s_st] = scale;
+        for (int k = 0; k < N; ++k) {
+            const uint32_t row = ((blockIdx.x * N + k) * kThreads + threadIdx.x) / L;
+            t[k] = divide(row, p.by_heads);
+            h[k] = row - t[k] * p.heads;
+            if (t[k] >= (N == 1 ? p.tokens : used)) continue;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+                load8<VEC>(p.x[n].rows + b * p.x[n].r_sb + h[k] * p.x[n].r_sh + t[k] * p.x[n].r_st + unit * 8 * sizeof(T), e[k][n]);
+        }
+        Place at[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) at[k] = place(p, b, start, used, t[k]);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (at[k].page < 0) continue;  // (the same for all lanes of a row)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const Rows &r = p.x[n];
+                float x[8], scale;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = (float)e[k][n].x[i];
+                const uint2 w = quantise<E4M3>(x, row_largest<L>(e[k][n]), scale);
+                *reinterpret_cast<u32x2_t *>(r.pages + at[k].page * r.p_sp + h[k] * r.p_sh + at[k].row * r.p_st + unit * 8) = u32x2_t{w.x, w.y};
+                if (unit == 0) r.scales[at[k].page * r.s_sp + h[k] * r.s_sh + at[k].row * r.s_st] = scale;
+            }
         }
     }
 }
@@ -143,30 +216,45 @@ template <bool E4M3> Q3T_DEVICE void elements(uint2 w, float (&x)[8]) {
 template <typename T> Q3T_DEVICE T rounded(float x) { return (T)x; }
 template <> Q3T_DEVICE __bf16 rounded<__bf16>(float x) { return __builtin_bit_cast(__bf16, (uint16_t)float_to_bf16(x)); }
 
-template <typename T, int L, bool E4M3, bool VEC>
+template <typename T, int L, bool E4M3, bool VEC, int N>
 __global__ void __launch_bounds__(kThreads) read_kernel(Params p) {
     for (uint32_t b = blockIdx.y; b < p.batch; b += gridDim.y) {
-        const uint32_t i = blockIdx.x * kThreads + threadIdx.x, row = i / L, unit = i % L;
-        const uint32_t t = divide(row, p.by_heads), h = row - t * p.heads;
-        if (t >= p.tokens) continue;
-        const Place at = place(p, b, t);
+        const int64_t start = p.positions[b];
+        const uint32_t used = used_rows(p, b), unit = threadIdx.x % L;
+        uint32_t t[N], h[N];
+        Place at[N];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const Rows &r = p.x[n];
-            Eight<T> e = {};
-            if (at.page >= 0) {
-                float x[8];
-                elements<E4M3>(*reinterpret_cast<const uint2 *>(r.pages + at.page * r.p_sp + h * r.p_sh + at.row * r.p_st + unit * 8), x);
-                const float scale = r.scales[at.page * r.s_sp + h * r.s_sh + at.row * r.s_st];
+        for (int k = 0; k < N; ++k) {
+            const uint32_t row = ((blockIdx.x * N + k) * kThreads + threadIdx.x) / L;
+            t[k] = divide(row, p.by_heads);
+            h[k] = row - t[k] * p.heads;
+            at[k] = place(p, b, start, used, t[k]);
+        }
+        u32x2_t w[N][2];
+        float scale[N][2];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) e.x[k] = rounded<T>(x[k] * scale);
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const Rows &r = p.x[n];
+                w[k][n] = u32x2_t{0u, 0u};
+                scale[k][n] = 0.f;
+                if (at[k].page < 0) continue;
+                w[k][n] = *reinterpret_cast<const u32x2_t *>(r.pages + at[k].page * r.p_sp + h[k] * r.p_sh + at[k].row * r.p_st + unit * 8);
+                scale[k][n] = r.scales[at[k].page * r.s_sp + h[k] * r.s_sh + at[k].row * r.s_st];
             }
-            char *to = r.rows + b * r.r_sb + h * r.r_sh + t * r.r_st + unit * 8 * sizeof(T);
-            if constexpr (VEC) {
 #pragma unroll
-                for (int k = 0; k < (int)sizeof(e) / 16; ++k) reinterpret_cast<U4 *>(to)[k] = reinterpret_cast<U4 *>(&e)[k];
-            } else {
-                for (int k = 0; k < 8; ++k) reinterpret_cast<T *>(to)[k] = e.x[k];
+        for (int k = 0; k < N; ++k) {
+            if (t[k] >= p.tokens) continue;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const Rows &r = p.x[n];
+                float x[8];
+                elements<E4M3>(uint2{w[k][n][0], w[k][n][1]}, x);
+                Eight<T> e;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e.x[i] = at[k].page < 0 ? (T)0.f : rounded<T>(x[i] * scale[k][n]);
+                store8<VEC>(r.rows + b * r.r_sb + h[k] * r.r_sh + t[k] * r.r_st + unit * 8 * sizeof(T), e);
             }
         }
     }
@@ -177,21 +265,39 @@ template <int V> struct Unit { typedef uint32_t T __attribute__((ext_vector_type
 template <> struct Unit<4> { typedef uint32_t T; };
 template <> struct Unit<2> { typedef uint16_t T; };
 
-template <int V>
+template <int V, int N>
 __global__ void __launch_bounds__(kThreads) copy_kernel(Params p) {
     typedef typename Unit<V>::T T;
     for (uint32_t b = blockIdx.y; b < p.batch; b += gridDim.y) {
-        const uint32_t i = blockIdx.x * kThreads + threadIdx.x, row = divide(i, p.by_units);
-        const uint32_t t = divide(row, p.by_heads), h = row - t * p.heads;
-        const int64_t unit = (int64_t)(i - row * p.units) * V;
-        if (t >= p.tokens) continue;
-        const Place at = place(p, b, t);
+        const int64_t start = p.positions[b];
+        const uint32_t used = used_rows(p, b);
+        uint32_t t[N], h[N];
+        int64_t unit[N];
+        Place at[N];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const Rows &r = p.x[n];
-            T v = {};
-            if (at.page >= 0) v = *reinterpret_cast<const T *>(r.pages + at.page * r.p_sp + h * r.p_sh + at.row * r.p_st + unit);
-            *reinterpret_cast<T *>(r.rows + b * r.r_sb + h * r.r_sh + t * r.r_st + unit) = v;
+        for (int k = 0; k < N; ++k) {
+            const uint32_t i = (blockIdx.x * N + k) * kThreads + threadIdx.x, row = divide(i, p.by_units);
+            t[k] = divide(row, p.by_heads);
+            h[k] = row - t[k] * p.heads;
+            unit[k] = (int64_t)(i - row * p.units) * V;
+            at[k] = place(p, b, start, used, t[k]);
+        }
+        T v[N][2];
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const Rows &r = p.x[n];
+                v[k][n] = T{};
+                if (at[k].page >= 0)
+                    v[k][n] = __builtin_nontemporal_load(reinterpret_cast<const T *>(r.pages + at[k].page * r.p_sp + h[k] * r.p_sh + at[k].row * r.p_st + unit[k]));
+            }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (t[k] >= p.tokens) continue;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+                __builtin_nontemporal_store(v[k][n], reinterpret_cast<T *>(p.x[n].rows + b * p.x[n].r_sb + h[k] * p.x[n].r_sh + t[k] * p.x[n].r_st + unit[k]));
         }
     }
 }
@@ -240,18 +346,21 @@ static int64_t strides(const Params &p, bool pools) {
     return all;
 }
 
-// Launches `kernel` for `units` units of a row; Q3T_OK, or the status to return.
-template <typename K>
-static int launch(K kernel, Params &p, uint32_t units, void *stream) {
+// Launches one of two kernels, of one and of two units a thread, for `units` units of a row; Q3T_OK, or the status to return.
+constexpr int64_t kManyBlocks = 2048;  // workgroups of one unit a thread that the card holds at once
+template <typename K1, typename K2>
+static int launch(K1 one, K2 two, Params &p, uint32_t units, void *stream) {
     p.units = units;
     p.by_units = divisor(units);
     // units of a request stay below 2^31, and threads of a launch below 2^32
     if (p.heads > INT32_MAX / units || p.tokens > (INT32_MAX - 2 * kThreads) / (p.heads * units)) return Q3T_EUNSUPPORTED;
-    const int64_t blocks = ((int64_t)p.tokens * p.heads * units + kThreads - 1) / kThreads, most = ((int64_t)1 << 24) - 1;
+    const int64_t all = (int64_t)p.tokens * p.heads * units;
+    const bool many = all / kThreads * p.batch >= kManyBlocks;
+    const int64_t each = kThreads * (many ? 2 : 1), blocks = (all + each - 1) / each, most = ((int64_t)1 << 24) - 1;
     if (blocks > most) return Q3T_EUNSUPPORTED;
     int64_t across = p.batch < 65535 ? p.batch : 65535;
     if (across > most / blocks) across = most / blocks;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks, (uint32_t)across), dim3(kThreads), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL(many ? two : one, dim3((uint32_t)blocks, (uint32_t)across), dim3(kThreads), 0, (hipStream_t)stream, p);
     return launch_status();
 }
 
@@ -281,7 +390,9 @@ extern "C" int q3t_paged_write_quantized(const q3t_paged_write_args *a, int64_t 
     const int status = common(a, a->elem_size, 1, s, p);
     if (status != Q3T_OK || a->batch == 0 || a->tokens == 0) return status;
     return with(dtype, a->width, s->format, strides(p, false) % 16 == 0, [&](auto t, auto l, auto e, auto vec) {
-        return launch(write_kernel<decltype(t), decltype(l)::value, decltype(e)::value, decltype(vec)::value>, p, decltype(l)::value, stream);
+        constexpr int L = decltype(l)::value;
+        constexpr bool E = decltype(e)::value, VEC = decltype(vec)::value;
+        return launch(write_kernel<decltype(t), L, E, VEC, 1>, write_kernel<decltype(t), L, E, VEC, 2>, p, L, stream);
     });
 }
 
@@ -295,16 +406,18 @@ extern "C" int q3t_paged_read(const q3t_paged_read_args *a, const q3t_paged_scal
     if (status != Q3T_OK || a->batch == 0 || a->tokens == 0) return status;
     if (s)
         return with(a->dtype, a->width, s->format, strides(p, false) % 16 == 0, [&](auto t, auto l, auto e, auto vec) {
-            return launch(read_kernel<decltype(t), decltype(l)::value, decltype(e)::value, decltype(vec)::value>, p, decltype(l)::value, stream);
+            constexpr int L = decltype(l)::value;
+            constexpr bool E = decltype(e)::value, VEC = decltype(vec)::value;
+            return launch(read_kernel<decltype(t), L, E, VEC, 1>, read_kernel<decltype(t), L, E, VEC, 2>, p, L, stream);
         });
     const int64_t all = strides(p, true) | a->width * es;  // the widest unit that divides the row, every stride and every pointer
     int64_t v = 16;
     while (v > es && all % v) v >>= 1;
     const uint32_t units = (uint32_t)(a->width * es / v);
     switch (v) {
-        case 16: return launch(copy_kernel<16>, p, units, stream);
-        case 8: return launch(copy_kernel<8>, p, units, stream);
-        case 4: return launch(copy_kernel<4>, p, units, stream);
-        default: return launch(copy_kernel<2>, p, units, stream);
+        case 16: return launch(copy_kernel<16, 1>, copy_kernel<16, 2>, p, units, stream);
+        case 8: return launch(copy_kernel<8, 1>, copy_kernel<8, 2>, p, units, stream);
+        case 4: return launch(copy_kernel<4, 1>, copy_kernel<4, 2>, p, units, stream);
+        default: return launch(copy_kernel<2, 1>, copy_kernel<2, 2>, p, units, stream);
     }
 }
