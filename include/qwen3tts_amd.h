@@ -435,7 +435,7 @@ typedef struct q3t_paged_args {
     int64_t batch, q_heads, kv_heads, head_dim, dtype;
     int64_t ctx;   /* keys that a request may have, 1 ... table_width * page_size, below 2^30 */
     float scale;   /* softmax scale, normally head_dim ** -0.5 */
-    int32_t reserved; /* 0 */
+    int32_t reserved; /* 0 (q3t_paged_attention_with: Q3T_SHARE_*) */
     const void *query; /* (batch, q_heads, head_dim) */
     int64_t q_stride_b, q_stride_h;
     const void *key_pages, *value_pages;
@@ -516,12 +516,18 @@ int q3t_paged_read(const q3t_paged_read_args *args, const q3t_paged_scales *scal
 
 /*
  * q3t_paged_attention over pools of 8 bits (scales != NULL), the queries and the output having dtype; and for
- * a batch whose requests begin with the same pages (shared_pages > 0): the first shared_pages entries of every
- * request's row of page_table are taken to be those of request 0's row, and the keys on them are read
- * once for many requests.  Everything else is as q3t_paged_attention has it: a request attends its
- * keys 0 ... positions[b], also where that ends within the shared pages, under its own mask.
+ * a batch whose requests begin with the same pages (shared_pages > 0): the first shared_pages entries are the same in
+ * every request's row of page_table (any row's may be read).  Everything else is as q3t_paged_attention has it: a
+ * request attends its keys 0 ... positions[b], also where that ends within the shared pages, under its own mask.
  * shared_pages * page_size is below ctx.
+ *
+ * The keys on shared pages are read once for the batch, in a launch ahead of that for the requests' own keys, where that
+ * saves enough (Q3T_SHARE_AUTO in args->reserved), always or never; never over pools of 8 bits.  Weights of that launch
+ * are rounded to the type of 16 bits (half a step: 2^-8 in bf16, 2^-11 in fp16), and their sum is that of the rounded ones.
  */
+#define Q3T_SHARE_AUTO 0
+#define Q3T_SHARE_ALWAYS 1
+#define Q3T_SHARE_NEVER 2
 int64_t q3t_paged_workspace_bytes_with(const q3t_paged_args *args, const q3t_paged_scales *scales, int64_t shared_pages);
 int q3t_paged_attention_with(const q3t_paged_args *args, const q3t_paged_scales *scales, int64_t shared_pages, void *stream);
 

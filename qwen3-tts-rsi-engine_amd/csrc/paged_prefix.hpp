@@ -643,7 +643,7 @@ prefix_kernel(PrefixParams p) {
 
 // What a launch over a prefix does.
 struct PrefixPlan {
-    int64_t cw, kw, ct, columns, blocks, parts, chunk;
+    int64_t cw, kw, ct, columns, blocks, parts, chunk, step;  // step: keys of a stage for every group
     int64_t states, workgroups, bytes;  // states: in all
 };
 
@@ -659,8 +659,11 @@ static PrefixPlan prefix_plan(const q3t_paged_args *a, int64_t keys) {
     z.cw = z.columns <= 2 * kColumns ? 1 : 4;
     z.kw = z.cw == 4 ? 2 : 4;
     z.blocks = (z.columns + z.cw * z.ct * kColumns - 1) / (z.cw * z.ct * kColumns);
-    const int64_t step = z.kw * (sizeof(T) == 4 ? 16 : 32), workgroups = 256;
+    const int64_t step = z.step = z.kw * (sizeof(T) == 4 ? 16 : 32), workgroups = 256;
     int64_t parts = workgroups / (z.blocks * a->kv_heads);
+    // each request's end reads the states of its columns: up to eight for a thread of 512
+    const int64_t group = a->q_heads / a->kv_heads, most_parts = 16384 / ((group < kColumns ? group : kColumns) * a->head_dim);
+    if (parts > most_parts) parts = most_parts;
     if (parts < 1) parts = 1;
     z.chunk = (keys + parts - 1) / parts;
     if (z.chunk < kLeastChunk) z.chunk = kLeastChunk;

@@ -47,6 +47,7 @@ _pack_write = _lib.packer(_lib.PagedWriteArgs)
 _pack_read = _lib.packer(_lib.PagedReadArgs)
 _pack_scales = _lib.packer(_lib.PagedScales)
 _HELD = {torch.int8: _lib.Q3T_I8, torch.float8_e4m3fn: _lib.Q3T_E4M3}  # types of pools with scales
+_SHARE = {None: 0, True: 1, False: 2}  # Q3T_SHARE_*
 _TYPES = {torch.bfloat16: _lib.Q3T_BF16, torch.float16: _lib.Q3T_F16, torch.float32: _lib.Q3T_F32}
 
 
@@ -195,7 +196,7 @@ def paged_read(key_pages, value_pages, page_table, positions, tokens, lengths=No
 
 
 def paged_attention(query, key_pages, value_pages, page_table, positions, *, scale=None, mask=None, out=None,
-                    scales=None, shared_pages=0):
+                    scales=None, shared_pages=0, read_once=None):
     """Attention of one new token per request: query (B, 1, Hq, D) over the keys
     0 ... positions[b] of request b, which its row of ``page_table`` (B, width) int32 finds in
     key_pages/value_pages (pages, Hkv, page_size, D), by any strides with unit-stride rows.
@@ -214,12 +215,16 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     ``scales``: the pools are int8 or float8_e4m3fn, and the keys and values those that they stand for.
 
     ``shared_pages``: the first that many entries are the same pages in every row of ``page_table``, as where
-    all requests have one prompt in front.  They are taken from the first row, and their keys are read once
-    for many requests; what each request attends is as without it."""
-    return _attend(_attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out, scales, shared_pages))
+    all requests have one prompt in front.  What each request attends is as without it, but where it saves
+    enough (``read_once`` True or False: always, or never) the keys on them are read once for the whole
+    batch, their weights then rounded to the queries' type (of 16 bits) with the sum over them.  Pools of 8 bits are
+    attended request by request."""
+    return _attend(_attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out, scales, shared_pages,
+                                   read_once))
 
 
-def _attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out, scales=None, shared_pages=0):
+def _attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out, scales=None, shared_pages=0,
+                    read_once=None):
     """An attention launch whose arguments have been checked, for ``_attend``: (query, out, device index, fields,
     bytes of workspace, scales and shared pages if any); nothing has been launched on the pools yet."""
     if query.ndim != 4 or query.shape[1] != 1:
@@ -235,6 +240,8 @@ def _attention_call(query, key_pages, value_pages, page_table, positions, scale,
     held = _check_scales(scales, key_pages, value_pages, dtype)
     if isinstance(shared_pages, bool) or not isinstance(shared_pages, int) or not 0 <= shared_pages <= table_width:
         raise ValueError('shared_pages must be a number of entries of the page table')
+    if read_once not in _SHARE:
+        raise ValueError('read_once must be True, False or None')
     qs = query.stride()
     if qs[3] != 1:
         raise ValueError('rows must be unit-stride along head_dim')
@@ -272,7 +279,7 @@ def _attention_call(query, key_pages, value_pages, page_table, positions, scale,
         query = query.clone(memory_format=torch.contiguous_format)  # rows that 16-byte loads do not fit
         qs = query.stride()
     fields = (
-        batch, q_heads, kv_heads, head_dim, _TYPES[dtype], ctx, head_dim ** -0.5 if scale is None else scale, 0,
+        batch, q_heads, kv_heads, head_dim, _TYPES[dtype], ctx, head_dim ** -0.5 if scale is None else scale, _SHARE[read_once],
         query.data_ptr(), qs[0], qs[2], key_pages.data_ptr(), value_pages.data_ptr(),
         kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], pages, page_size,
         page_table.data_ptr(), table_width, ts, positions.data_ptr(), *mask_fields, out.data_ptr(), os[0], os[2])

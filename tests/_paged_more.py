@@ -65,12 +65,17 @@ def expected(p, mask=None, scale=None):
         keys, values = (x.detach().cpu().double() for x in (p.key_pages, p.value_pages))
     else:
         keys, values = (stands_for(x, s) for x, s in zip((p.key_pages, p.value_pages), p.scales))
-    call = lambda v: attention64(p.query, keys, v, p.table, p.positions, mask=mask, scale=scale)  # noqa: E731
+    query, size = p.query, scale
+    if scale is not None and scale < 0:  # (attention64's bound is for positive ones)
+        query, size = -query, -scale
+    call = lambda v: attention64(query, keys, v, p.table, p.positions, mask=mask, scale=size)  # noqa: E731
     out, tol = call(values)
     return out, tol + parts(p.query.dtype, p.shared > 0, values, call, p.table.shape[1] * p.page)
 
 
 def run(pkg, p, **kwargs):
+    if p.shared:
+        kwargs.setdefault('read_once', True)
     return pkg.paged_attention(p.query, p.key_pages, p.value_pages, p.table, p.positions, scales=p.scales,
                                shared_pages=p.shared, **kwargs)
 

@@ -108,6 +108,19 @@ def test_shared_pages_outside_the_table_are_refused(pkg, launches, shared):
     assert launches == []
 
 
+@pytest.mark.parametrize('once', [2, 'yes', 0.5], ids=repr)
+def test_other_ways_to_read_are_refused(pkg, launches, once):
+    with pytest.raises(ValueError):
+        _attend(pkg, pools=_pools(BF16), shared_pages=2, read_once=once)
+    assert launches == []
+
+
+def test_ways_to_read_are_passed_on(pkg, launches):
+    for once in (None, True, False):
+        _attend(pkg, pools=_pools(BF16), shared_pages=2, read_once=once)
+    assert [pkg._lib.PagedArgs.from_buffer_copy(call[1]).reserved for call in launches] == [0, 1, 2]
+
+
 def test_the_last_row_is_left_to_the_requests(pkg, launches):
     """Of pages that are all shared, and under a mask that ends within them."""
     _attend(pkg, pools=_pools(BF16), shared_pages=4)
@@ -207,7 +220,7 @@ def test_the_c_entry_points_refuse_types(pkg):
 
 @pytest.mark.parametrize('bad', BAD + [dict(ctx=65), dict(ctx=0), dict(head_dim=96), dict(dtype=3), dict(q_heads=12), dict(query=0), dict(out=0),
                                        dict(query=4104), dict(q_stride_h=4), dict(workspace=0), dict(workspace_bytes=8), dict(mask=4096, mask_dtype=9),
-                                       dict(o_stride_b=-1)], ids=str)
+                                       dict(o_stride_b=-1), dict(reserved=3), dict(reserved=-1)], ids=str)
 @pytest.mark.parametrize('held,shared', [(True, 0), (False, 2), (True, 2)])
 def test_the_c_entry_point_refuses_attention(pkg, bad, held, shared):
     a = _args(pkg, 'PagedArgs', **{**dict(workspace=1 << 20, workspace_bytes=1 << 40), **bad})
@@ -220,6 +233,8 @@ def test_the_c_entry_point_refuses_shared_pages(pkg):
         a = _args(pkg, 'PagedArgs', workspace=1 << 20, workspace_bytes=1 << 40)
         assert lib.q3t_paged_attention_with(a, None, shared, None) == -1
         assert lib.q3t_paged_workspace_bytes_with(a, None, shared) == -1
+    small, large = (lib.q3t_paged_workspace_bytes_with(_args(pkg, 'PagedArgs', reserved=way), None, 3) for way in (2, 1))
+    assert 0 < small < large
     assert lib.q3t_paged_workspace_bytes_with(_args(pkg, 'PagedArgs'), _c_scales(pkg), 3) > 0
     assert lib.q3t_paged_workspace_bytes_with(None, None, 0) == -1
 

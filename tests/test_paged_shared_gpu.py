@@ -99,6 +99,34 @@ def test_masks(pkg, device, width, dtype, heads, kind, batch):
     assert torch.equal(run(pkg, p, mask=strided), out)
 
 
+@pytest.mark.parametrize('scale', [0.0, -0.2, 1e-4])
+@pytest.mark.parametrize('dtype', [BF16, F32], ids=str)
+@pytest.mark.parametrize('masked', [False, True])
+def test_scales(pkg, device, scale, dtype, masked):
+    p = problem(device, _behind(320, [b % 30 for b in range(40)]), shared=20, dtype=dtype, seed=25)
+    mask = torch.ones(40, 1, 1, p.table.shape[1] * 16, dtype=torch.bool, device=device) if masked else None
+    assert_within(run(pkg, p, scale=scale, mask=mask), *expected(p, scale=scale, mask=mask))
+
+
+@pytest.mark.parametrize('dtype,width,heads', [(BF16, 128, (16, 8)), (F16, 64, (8, 8)), (F32, 128, (40, 2))], ids=str)
+@pytest.mark.parametrize('batch', [3, 20, 70])
+@pytest.mark.parametrize('odd', [math.nan, math.inf])
+def test_values_that_are_not_finite_behind_the_ends_of_some(pkg, device, dtype, width, heads, batch, odd):
+    """Requests that end within the shared pages before such a value, with it, and behind it."""
+    lengths = ([700, 705, 64, 65, 66, 640, 0, 900] * 10)[:batch]
+    p = problem(device, lengths, shared=40, dtype=dtype, width=width, q_heads=heads[0], kv_heads=heads[1], seed=26)
+    clean, tol = expected(p)
+    p.value_pages[int(p.table[0, 4]), 1, 0, 9] = odd  # key 64
+    out = run(pkg, p).cpu()
+    group = slice(heads[0] // heads[1], 2 * heads[0] // heads[1])
+    for b, n in enumerate(lengths):
+        if n > 64:
+            at = out[b, 0, group, 9]
+            assert (at.isnan() if math.isnan(odd) else at == odd).all()
+            out[b, 0, group, 9], clean[b, 0, group, 9] = 0, 0
+    assert_within(out, clean, tol)
+
+
 @pytest.mark.parametrize('dtype', [BF16, F32], ids=str)
 def test_a_value_hidden_from_some_requests_alone(pkg, device, dtype):
     """A NaN or an infinity among the shared values shows where it is attended, and nowhere else."""
@@ -158,11 +186,18 @@ def test_shared_pages_outside_the_pool_do_not_exist(pkg, device):
     assert_within(run(pkg, p), *expected(p))
 
 
-def test_the_first_rows_entries_are_everybodys(pkg, device):
-    p = problem(device, _behind(160, [5, 40, 1, 17] * 4), shared=10, seed=13)
-    want = run(pkg, p)
-    p.table[1:, :10] = -9
-    assert torch.equal(run(pkg, p), want)
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (F16, 64), (F32, 128)], ids=str)
+@pytest.mark.parametrize('prefix,batch', [(64, 40), (2048, 5), (2048, 40)])
+def test_by_the_librarys_choice_and_never(pkg, device, dtype, width, prefix, batch):
+    """Short and long prefixes, on either side of where the library reads them once."""
+    p = problem(device, _behind(prefix, [b % 50 for b in range(batch)]), shared=prefix // 16, dtype=dtype, width=width, seed=13)
+    never = run(pkg, p, read_once=False)
+    want = expected(p)
+    assert_within(never, *want)
+    assert torch.equal(never, pkg.paged_attention(p.query, p.key_pages, p.value_pages, p.table, p.positions))
+    chosen = run(pkg, p, read_once=None)
+    assert_within(chosen, *want)
+    assert torch.equal(chosen, never) or torch.equal(chosen, run(pkg, p))
 
 
 @pytest.mark.parametrize('held', HELD, ids=str)
