@@ -393,21 +393,23 @@ class PagedArena:
         rows = [list(pages) + [-1] * (width - len(pages)) for pages in requests]
         return torch.tensor(rows, dtype=torch.int32).reshape(len(rows), width).to(self.packed.device)
 
-    def load(self, page_table, cache, lengths):
+    def load(self, page_table, cache, lengths, start=None):
         """Copy the rows of a prefill cache (``cache.layers[i].keys`` / ``.values``, (B, kv_heads,
         length, head_dim)) into the pages of their requests: row b's first ``lengths[b]`` (int32,
-        device) positions, to positions 0 on."""
+        device) positions, to positions ``start[b]`` (int64, device; 0) on."""
         if len(cache.layers) != len(self.keys):
             raise ValueError('the cache and the arena must have the same layers')
-        start = torch.zeros(page_table.shape[0], device=page_table.device, dtype=torch.int64)
+        if start is None:
+            start = torch.zeros(page_table.shape[0], device=page_table.device, dtype=torch.int64)
         for layer, keys, values, scales in zip(cache.layers, self.keys, self.values, self.scales):
             paged_write(layer.keys, layer.values, keys, values, page_table, start, lengths, scales=scales)
 
-    def read(self, page_table, tokens, lengths=None):
-        """The rows of requests, the inverse of ``load``: their first ``tokens`` positions as a packed cache (2 *
-        layers, B, kv_heads, tokens, head_dim) of the model's dtype, as ``SlotArena.load_packed`` takes it,
-        zeros past the first ``lengths[b]`` (int32, device) rows of request b."""
-        start = torch.zeros(page_table.shape[0], device=page_table.device, dtype=torch.int64)
+    def read(self, page_table, tokens, lengths=None, start=None):
+        """The rows of requests, the inverse of ``load``: ``tokens`` positions from ``start[b]`` (int64, device; 0) on as a
+        packed cache (2 * layers, B, kv_heads, tokens, head_dim) of the model's dtype, as
+        ``SlotArena.load_packed`` takes it, zeros past the first ``lengths[b]`` (int32, device) rows of request b."""
+        if start is None:
+            start = torch.zeros(page_table.shape[0], device=page_table.device, dtype=torch.int64)
         layers, (_, heads, _, width) = len(self.keys), self.keys[0].shape
         packed = torch.empty((2 * layers, page_table.shape[0], heads, tokens, width), device=self.packed.device,
                              dtype=next(self.reference.parameters()).dtype)

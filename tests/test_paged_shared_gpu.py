@@ -255,3 +255,15 @@ def test_on_two_streams_at_once(pkg, device):
     torch.cuda.synchronize()
     for w, out in zip(want, outs):
         assert all(torch.equal(w, o) for o in out)
+
+
+def test_shared_pages_past_four_gigabytes(pkg, device):
+    pages = (1 << 32) // (8 * 16 * 128 * 2) + 16
+    near = problem(device, _behind(128, [5, 20, 1]), shared=8, seed=30)
+    pools = [torch.empty(pages, 8, 16, 128, dtype=BF16, device=device) for _ in range(2)]
+    for pool, given in zip(pools, (near.key_pages, near.value_pages)):
+        pool[-given.shape[0]:] = given
+    table = torch.where(near.table < 0, near.table, near.table + pages - near.key_pages.shape[0])
+    out = pkg.paged_attention(near.query, *pools, table, near.positions, shared_pages=8, read_once=True)
+    assert torch.equal(out, run(pkg, near))
+    assert_within(out, *expected(near))
