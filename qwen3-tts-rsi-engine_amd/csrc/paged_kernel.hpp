@@ -588,16 +588,24 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
     __shared__ Lds<T, D, MASK, W> s;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = (int)uniform(tid >> 6);
-    if constexpr (MORE && !HELD) {
-        uint32_t odd = 0;
-        for (uint32_t i = lane; i < p.odds; i += 64) odd |= p.odd[i];
-        if (__builtin_amdgcn_ballot_w64(odd != 0)) {  // the prefix' keys as all others
+    // Whether the states over the prefix are not to be used: on its way while the share is worked out as if they were.
+    uint32_t odd = 0;
+    if constexpr (MORE && !HELD)
+        for (uint32_t i = 0; i < p.odds; i += 256)
+#pragma unroll
+            for (uint32_t j = 0; j < 256; j += 64) odd |= p.odd[min(i + j + lane, p.odds - 1)];
+    auto without_prefix = [&] {  // its keys are then as all others
+        if constexpr (MORE && !HELD) {
+            if (!__builtin_amdgcn_ballot_w64(odd != 0)) return false;
+            odd = 0;
             ctx += p.skip;
             p.table -= p.skip_pages;
             if constexpr (MASK) p.mask -= (uint64_t)p.skip * p.m_st * (p.mask_dtype == Q3T_F32 ? 4 : p.mask_dtype == Q3T_BOOL ? 1 : 2);
             p.skip = p.parts = 0;
+            return true;
         }
-    }
+        return false;
+    };
 
     // ---- the share: every wave adds up all requests' stages and pieces for itself ---------------
     auto length_at = [&](uint32_t b) {
@@ -672,8 +680,10 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
         at = Cursor{blockIdx.x * kRoom, kRoom, b, blockIdx.x - b * p.heads, 0u};
         window = b;
         lengths = length_at(b + lane);
-    } else if (!find_share()) {
-        return;
+    } else {
+        bool some = find_share();
+        if (without_prefix()) some = find_share();
+        if (!some) return;
     }
     auto request_length = [&](uint32_t b) {
         return b - window < 64 ? (uint32_t)__builtin_amdgcn_readlane((int)lengths, (int)(b - window)) : uniform(length_at(b));
@@ -846,6 +856,11 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
         batches.key = wave * S::keys;
         batches.length = ctx;
         load_ids(0);
+        if (without_prefix()) {
+            lengths = length_at(at.b + lane);
+            batches.length = ctx;
+            load_ids(0);
+        }
     }
     next_batch();
     Batch now = batches;  // the batch whose rows are being loaded, its page numbers in half `half`
@@ -1014,7 +1029,7 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
     };
     const uint32_t state_size = p.columns * (D + 2);
     uint32_t p_parts = 0;
-    if constexpr (MORE) p_parts = p.parts;
+    if constexpr (MORE) p_parts = p.parts;  // (after without_prefix)
     // (a thread's place behind a wave's states, where groups of threads have some each)
     static_assert(!MORE || HELD || kThreads / (D / 4) * D * 4 / 2 + 64 * 32 <= S::stage, "");
 

@@ -579,9 +579,9 @@ prefix_kernel(PrefixParams p) {
             x.read_keys(buffer(n));
             if (n) x.values();
             scores();
-            if (!MASK && n + 3 < sets) exists[3] = locate(n + 3);
             __builtin_amdgcn_s_setprio(0);
             lds_barrier();
+            if (!MASK && n + 3 < sets) exists[3] = locate(n + 3);
             read_terms();
             softmax(n, exists[0]);
             if (MASK && n + 2 < sets) load(n + 2);
@@ -647,9 +647,10 @@ struct PrefixPlan {
     int64_t states, workgroups, bytes;  // states: in all
 };
 
-// By sizes alone: tiles for the columns that there are, and as many parts as fill the card with a chunk of kLeastChunk keys at least (a
-// state is written and read again for every part).
-constexpr int64_t kLeastChunk = 64;
+// By sizes alone: tiles for the columns that there are, and as many parts as fill the card, with some keys each at least: a
+// state is written and read again for every part.  us of both launches with 64 / 256 / 512 keys at least, bf16: 64 requests over 4096
+// keys 57.6 / 56.2 / 57.2, 64 over 2048 30.0 / 27.8 / 31.9, 32 over 1024 19.5 / 20.2 / 24.0, 128 over 1024 46.9 / 42.3 / 44.7; with 64 /
+// 128 / 256, float32 under a mask: 21 over 792 25.3 / 27.2 / 33.0.
 
 template <typename T>
 static PrefixPlan prefix_plan(const q3t_paged_args *a, int64_t keys) {
@@ -666,7 +667,8 @@ static PrefixPlan prefix_plan(const q3t_paged_args *a, int64_t keys) {
     if (parts > most_parts) parts = most_parts;
     if (parts < 1) parts = 1;
     z.chunk = (keys + parts - 1) / parts;
-    if (z.chunk < kLeastChunk) z.chunk = kLeastChunk;
+    const int64_t least = sizeof(T) == 4 ? 64 : 256;
+    if (z.chunk < least) z.chunk = least;
     z.chunk = (z.chunk + step - 1) / step * step;
     const int64_t most = (kEntries - 2) * a->page_size / step * step;  // whose page numbers a workgroup holds
     if (z.chunk > most) z.chunk = most;

@@ -129,7 +129,9 @@ def paged_write(keys, values, key_pages, value_pages, page_table, positions, len
     dtype = keys.dtype
     if dtype not in _TYPES or values.dtype != dtype:
         raise ValueError('paged K/V write supports bf16/fp16/fp32 tensors of one dtype')
-    held = _check_scales(scales, key_pages, value_pages, dtype)
+    held = None
+    if scales is not None or key_pages.dtype != dtype or value_pages.dtype != dtype:
+        held = _check_scales(scales, key_pages, value_pages, dtype)
     ks, vs = keys.stride(), values.stride()
     if ks[3] != 1 or vs[3] != 1:
         raise ValueError('K/V rows must be unit-stride along head_dim')
@@ -237,7 +239,9 @@ def _attention_call(query, key_pages, value_pages, page_table, positions, scale,
     dtype = query.dtype
     if dtype not in _TYPES:
         raise ValueError('paged attention supports bf16, fp16 or fp32 tensors of one dtype')
-    held = _check_scales(scales, key_pages, value_pages, dtype)
+    held = None
+    if scales is not None or key_pages.dtype != dtype or value_pages.dtype != dtype:
+        held = _check_scales(scales, key_pages, value_pages, dtype)
     if isinstance(shared_pages, bool) or not isinstance(shared_pages, int) or not 0 <= shared_pages <= table_width:
         raise ValueError('shared_pages must be a number of entries of the page table')
     if read_once not in _SHARE:

@@ -267,3 +267,24 @@ def test_shared_pages_past_four_gigabytes(pkg, device):
     out = pkg.paged_attention(near.query, *pools, table, near.positions, shared_pages=8, read_once=True)
     assert torch.equal(out, run(pkg, near))
     assert_within(out, *expected(near))
+
+
+@pytest.mark.parametrize('dtype,width,heads', [(BF16, 128, (16, 8)), (F16, 64, (20, 2)), (F32, 128, (4, 4))], ids=str)
+@pytest.mark.parametrize('masked', [False, True])
+def test_such_values_before_long_requests(pkg, device, dtype, width, heads, masked):
+    """Launches for requests of thousands of own keys that have to take the prefix as well."""
+    lengths = [5000, 3000, 2048, 100, 2600, 0, 2049, 4100] * 3
+    p = problem(device, lengths, shared=64, page=32, dtype=dtype, width=width, q_heads=heads[0], kv_heads=heads[1], seed=31)
+    mask = None
+    if masked:
+        mask = torch.ones(len(lengths), 1, 1, p.table.shape[1] * 32, dtype=torch.bool, device=device)
+        mask[::5, ..., 90:140] = False
+    clean, tol = expected(p, mask=mask)
+    p.value_pages[int(p.table[0, 4]), 0, 1, 9] = math.nan  # key 129
+    out = run(pkg, p, mask=mask).cpu()
+    group = slice(0, heads[0] // heads[1])
+    for b, n in enumerate(lengths):
+        if n > 129 and not (masked and b % 5 == 0):
+            assert out[b, 0, group, 9].isnan().all()
+            out[b, 0, group, 9], clean[b, 0, group, 9] = 0, 0
+    assert_within(out, clean, tol)
