@@ -515,11 +515,12 @@ prefix_kernel(PrefixParams p) {
         }
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-            const float from = X::shift - (m[ct] == -INFINITY ? 0.f : m[ct]) * unit;
+            // (under a mask the difference first: a mask's lowest term times the unit is no float32)
+            const float top = m[ct] == -INFINITY ? 0.f : m[ct], from = X::shift - top * unit;
 #pragma unroll
             for (int k = 0; k < TILES * 4; ++k) {
                 float &e = w[ct][k / 4][k % 4];
-                const float v = X::visible(fexp2(__builtin_fmaf(e, unit, from)));
+                const float v = X::visible(fexp2(MASK ? __builtin_fmaf(e - top, unit, X::shift) : __builtin_fmaf(e, unit, from)));
                 // (the smallest weight is for keys that are seen)
                 e = X::visible(0.f) != 0.f && e == -INFINITY ? 0.f : v;
             }

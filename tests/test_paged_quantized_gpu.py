@@ -237,6 +237,18 @@ def test_masks(pkg, device, held, width, dtype, kind, page):
 
 
 @pytest.mark.parametrize('held', HELD, ids=str)
+@pytest.mark.parametrize('dtype,kind', [(BF16, BF16), (F16, F16), (F32, F32)], ids=str)
+@pytest.mark.parametrize('lengths', [[100, 40, 300], [5000, 2000, 33]], ids=['short', 'cut'])
+def test_masks_of_the_types_lowest_value(pkg, device, held, dtype, kind, lengths):
+    """Terms that hide nothing where all keys of a request have them."""
+    p = problem(device, lengths, held=held, dtype=dtype, seed=12)
+    low = torch.rand(3, 1, 1, p.table.shape[1] * 16, generator=torch.Generator().manual_seed(13)) < 0.3
+    low[1] = True
+    mask = torch.where(low, torch.finfo(kind).min, 0.0).to(kind).to(device)
+    assert_within(run(pkg, p, mask=mask), *expected(p, mask=mask))
+
+
+@pytest.mark.parametrize('held', HELD, ids=str)
 @pytest.mark.parametrize('lengths', [[100, 40], [5000, 2000]], ids=['short', 'cut'])
 def test_rows_that_stand_for_nan_show(pkg, device, held, lengths):
     """An attended row of values whose scale is NaN makes its head's outputs NaN, and so does one of keys; others keep theirs."""

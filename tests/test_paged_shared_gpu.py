@@ -127,6 +127,18 @@ def test_values_that_are_not_finite_behind_the_ends_of_some(pkg, device, dtype, 
     assert_within(out, clean, tol)
 
 
+@pytest.mark.parametrize('dtype,kind', [(BF16, BF16), (BF16, F32), (F16, BF16), (F16, F16), (F32, F32), (F32, F16)], ids=str)
+@pytest.mark.parametrize('batch', [5, 40])
+def test_masks_of_the_types_lowest_value(pkg, device, dtype, kind, batch):
+    """Terms that hide nothing where all keys of a request have them, in the prefix, behind it or in both."""
+    p = problem(device, ([330, 340, 600, 321, 400] * 8)[:batch], shared=20, dtype=dtype, seed=32)
+    ctx = p.table.shape[1] * 16
+    low = torch.rand(batch, 1, 1, ctx, generator=torch.Generator().manual_seed(33)) < 0.3
+    low[0], low[1, ..., :320], low[2, ..., 320:] = True, True, True
+    mask = torch.where(low, torch.finfo(kind).min, 0.0).to(kind).to(device)
+    assert_within(run(pkg, p, mask=mask), *expected(p, mask=mask))
+
+
 @pytest.mark.parametrize('dtype', [BF16, F32], ids=str)
 def test_a_value_hidden_from_some_requests_alone(pkg, device, dtype):
     """A NaN or an infinity among the shared values shows where it is attended, and nowhere else."""
