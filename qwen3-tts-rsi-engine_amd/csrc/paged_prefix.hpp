@@ -402,7 +402,8 @@ prefix_kernel(PrefixParams p) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) m[ct] = -INFINITY;
     // exponents are unit (v - m) in log2 units: v the products themselves, or, under a mask, the natural scores
-    const float unit = MASK ? kLog2e : p.scale, threshold = X::threshold / unit;
+    // (a threshold that is finite: m is below any score at first)
+    const float unit = MASK ? kLog2e : p.scale, threshold = fminf(X::threshold / unit, __FLT_MAX__);
     bool odd = false;
     auto partial = [&](uint32_t key0) { return MASK || key0 + SK > least; };
     // Stage n, whose loads of this wave have ended.  Value rows of keys that do not exist become zeros: zero times NaN would

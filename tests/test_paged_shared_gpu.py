@@ -108,6 +108,13 @@ def test_scales(pkg, device, scale, dtype, masked):
     assert_within(run(pkg, p, scale=scale, mask=mask), *expected(p, scale=scale, mask=mask))
 
 
+@pytest.mark.parametrize('scale', [1e-38, -1e-38, 1e-41])
+@pytest.mark.parametrize('dtype', [BF16, F16, F32], ids=str)
+def test_scales_next_to_zero(pkg, device, scale, dtype):
+    p = problem(device, _behind(320, [b % 30 for b in range(40)]), shared=20, dtype=dtype, seed=27)
+    assert_within(run(pkg, p, scale=scale), *expected(p, scale=scale))
+
+
 @pytest.mark.parametrize('dtype,width,heads', [(BF16, 128, (16, 8)), (F16, 64, (8, 8)), (F32, 128, (40, 2))], ids=str)
 @pytest.mark.parametrize('batch', [3, 20, 70])
 @pytest.mark.parametrize('odd', [math.nan, math.inf])
