@@ -33,7 +33,7 @@ static int64_t bytes_with(const q3t_paged_args *a, const q3t_paged_scales *s, in
     const int status = s && s->format == Q3T_I8 ? sizes_int8(a, z) : sizes_e4m3(a, z);
     if (status != Q3T_OK) return status;
     if (shared_pages < 0 || shared_pages > a->table_width || shared_pages * a->page_size >= a->ctx) return Q3T_EINVAL;
-    if (s) return z.workspace;
+    if (s || a->batch == 0) return z.workspace;
     if (!once_for_all(a, shared_pages)) return q3t_paged_workspace_bytes(a);
     const int64_t keys = shared_pages * a->page_size;
     return a->dtype == Q3T_BF16 ? bytes_shared_bf16(a, keys) : a->dtype == Q3T_F16 ? bytes_shared_f16(a, keys) : bytes_shared_f32(a, keys);

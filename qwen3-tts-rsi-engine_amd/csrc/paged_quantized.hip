@@ -312,7 +312,8 @@ static int common(const A *a, int64_t es, int64_t held, const q3t_paged_scales *
     if (a->batch == 0 || a->tokens == 0) return Q3T_OK;
     if (!a->keys || !a->values || !a->key_pages || !a->value_pages || !a->page_table || !a->positions) return Q3T_EINVAL;
     if (s && (!s->key_scales || !s->value_scales || !aligned(s->key_scales, 4) || !aligned(s->value_scales, 4))) return Q3T_EINVAL;
-    if (a->pages > INT32_MAX || a->table_width > INT32_MAX / a->page_size || a->batch > INT32_MAX || a->width > 1 << 20)
+    if (a->pages > INT32_MAX || a->table_width > INT32_MAX / a->page_size || a->batch > INT32_MAX || a->heads > INT32_MAX ||
+        a->tokens > INT32_MAX || a->width > 1 << 20)
         return Q3T_EUNSUPPORTED;
     p.x[0] = {(char *)a->keys, (char *)a->key_pages, s ? s->key_scales : nullptr, a->k_stride_b * es, a->k_stride_h * es,
               a->k_stride_t * es, a->kp_stride_p * held, a->kp_stride_h * held, a->kp_stride_t * held,

@@ -161,10 +161,10 @@ def _args(pkg, cls, **changes):
         a.query = a.out = 4096
         a.q_stride_b, a.q_stride_h, a.o_stride_b, a.o_stride_h = 2048, 128, 2048, 128
     else:
-        a.batch, a.heads, a.tokens, a.width = 2, 8, 3, 128
+        a.batch, a.heads, a.tokens, a.width = 2, 8, 5, 128
         a.keys = a.values = 4096
-        a.k_stride_b, a.k_stride_h, a.k_stride_t = 3072, 384, 128
-        a.v_stride_b, a.v_stride_h, a.v_stride_t = 3072, 384, 128
+        a.k_stride_b, a.k_stride_h, a.k_stride_t = 5120, 640, 128
+        a.v_stride_b, a.v_stride_h, a.v_stride_t = 5120, 640, 128
     if cls == 'PagedWriteArgs':
         a.elem_size = 2
     a.key_pages = a.value_pages = a.page_table = a.positions = 4096
@@ -237,6 +237,23 @@ def test_the_c_entry_point_refuses_shared_pages(pkg):
     assert 0 < small < large
     assert lib.q3t_paged_workspace_bytes_with(_args(pkg, 'PagedArgs'), _c_scales(pkg), 3) > 0
     assert lib.q3t_paged_workspace_bytes_with(None, None, 0) == -1
+
+
+@pytest.mark.parametrize('way', [0, 1, 2])
+def test_attention_without_requests_is_none(pkg, way):
+    lib, a = pkg.library(), _args(pkg, 'PagedArgs', batch=0, reserved=way)
+    for held in (None, _c_scales(pkg)):
+        assert lib.q3t_paged_workspace_bytes_with(a, held, 2) >= 0
+        assert lib.q3t_paged_attention_with(a, held, 2, None) == 0
+
+
+@pytest.mark.parametrize('bad', [dict(heads=(1 << 32) + 8), dict(tokens=(1 << 32) + 5), dict(heads=1 << 40, tokens=0)], ids=str)
+def test_the_c_entry_points_refuse_counts_past_32_bits(pkg, bad):
+    lib, scales = pkg.library(), _c_scales(pkg)
+    expected = 0 if bad.get('tokens') == 0 else -2
+    assert lib.q3t_paged_write_quantized(_args(pkg, 'PagedWriteArgs', **bad), 0, scales, None) == expected
+    assert lib.q3t_paged_read(_args(pkg, 'PagedReadArgs', **bad), scales, None) == expected
+    assert lib.q3t_paged_read(_args(pkg, 'PagedReadArgs', **bad), None, None) == expected
 
 
 # ---- the arena -------------------------------------------------------------------------------
