@@ -14,6 +14,10 @@
 //   * A value that is not finite under a key that only some columns see would reach the others too, as zero times NaN.
 //     A launch that finds such a one says so, and its states are not used: the requests then attend the prefix each for
 //     itself.
+// The matrix cores bound it from some hundred columns on (4 * 16384 keys, 128 requests, 32 query heads over 8 KV heads of 128 in
+// bf16: 34.4 GFLOP in 50 us, 0.69 PFLOP/s and 0.8 past the start of 9 us, where a large library product reaches 1.2), the start and
+// the stages' chain below it (8 KV heads, 128 columns each, 4096 keys 16.8 us).  Waves that share a stage alternate between
+// matrix and vector instructions in two groups (with the addresses of a part worked out once, 65 -> 57 us then).
 #pragma once
 
 #include "paged_kernel.hpp"

@@ -30,8 +30,8 @@ and stands for scale times element.  A row with an infinity or a NaN in it stand
 
 Page numbers live on the device and are not checked on the host: a number outside the pool names
 no page, rows for it are not written and keys on it do not exist.  Two rows that are written to
-one place of a pool in one call leave either of the two.  Inference only, as the rest of the
-attention path.
+one place of a pool in one call leave either of the two (in 8 bits, of one the row and of the other
+the scale, perhaps).  Inference only, as the rest of the attention path.
 """
 from __future__ import annotations
 
@@ -216,11 +216,11 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
 
     ``scales``: the pools are int8 or float8_e4m3fn, and the keys and values those that they stand for.
 
-    ``shared_pages``: the first that many entries are the same pages in every row of ``page_table``, as where
-    all requests have one prompt in front.  What each request attends is as without it, but where it saves
-    enough (``read_once`` True or False: always, or never) the keys on them are read once for the whole
-    batch, their weights then rounded to the queries' type (of 16 bits) with the sum over them.  Pools of 8 bits are
-    attended request by request."""
+    ``shared_pages``: the first that many entries are the same pages in every row of ``page_table``, also in
+    rows of requests that attend nothing, as where all requests have one prompt in front.  What each
+    request attends is as without it, but where it saves enough (``read_once`` True or False: always, or
+    never) the keys on them are read once for the whole batch, their weights then rounded to the queries'
+    type (of 16 bits) with the sum over them.  Pools of 8 bits are attended request by request."""
     return _attend(_attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out, scales, shared_pages,
                                    read_once))
 
@@ -428,7 +428,7 @@ class PagedCache(Cache):
     ``positions[b]`` and returns the layer's pools; ``step`` attends over them too, as
     ``PackedAttention`` calls it.  ``page_table`` and ``positions`` are read at every step as they are
     then, so a captured step follows changes of their contents.  ``shared_pages``: entries that all rows of the
-    table begin with, as ``paged_attention`` takes them; no request may write to those pages.
+    table begin with, as ``paged_attention`` takes them (idle requests' rows too); no request may write to those pages.
 
     The lengths live on the device, so ``get_seq_length`` is 0: pass the model ``position_ids``, and as
     its mask None (a request then attends its keys up to its position) or one over the table's rows."""
