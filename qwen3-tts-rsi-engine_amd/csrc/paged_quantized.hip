@@ -218,6 +218,11 @@ template <bool E4M3> Q3T_DEVICE void elements(uint2 w, float (&x)[8]) {
 }
 
 template <typename T> Q3T_DEVICE T rounded(float x) { return (T)x; }
+// (a product and its rounding become one instruction otherwise, which adds a zero: -0 would be 0)
+template <> Q3T_DEVICE _Float16 rounded<_Float16>(float x) {
+    asm("" : "+v"(x));
+    return (_Float16)x;
+}
 template <> Q3T_DEVICE __bf16 rounded<__bf16>(float x) { return __builtin_bit_cast(__bf16, (uint16_t)float_to_bf16(x)); }
 
 template <typename T, int L, bool E4M3, bool VEC, int N>

@@ -138,6 +138,17 @@ def test_an_element_is_off_by_half_a_step_at_most(pkg, device, held):
         assert ((back - x).abs() <= half * (1 + 1e-5)).all()
 
 
+@pytest.mark.parametrize('dtype', [BF16, F16, F32], ids=str)
+def test_a_negative_zero_is_held_and_read(pkg, device, dtype):
+    pools, scales = _pools(device, 2, 1, 16, 64, torch.float8_e4m3fn)
+    x = torch.zeros(1, 1, 4, 64, device=device, dtype=dtype)
+    x[..., 1::2], x[..., 2, 0] = -0.0, -5.0
+    table, start = torch.ones(1, 1, dtype=torch.int32, device=device), torch.zeros(1, dtype=torch.int64, device=device)
+    pkg.paged_write(x, x, *pools, table, start, scales=scales)
+    for back in pkg.paged_read(*pools, table, start, 4, scales=scales, dtype=dtype):
+        assert torch.equal(bits(back), bits(x))
+
+
 @pytest.mark.parametrize('held', HELD, ids=str)
 def test_rows_off_16_bytes_and_pools_by_strides(pkg, device, held):
     big = torch.randn(2, 9, 3, 131, device=device).to(BF16)
