@@ -5,9 +5,9 @@
 // the scale NaN.  Read: scale * element, or the elements of an unquantised pool.
 // One pass each: a row lies in 8 or 16 lanes, whose maximum four steps over the lanes find, so it is read once and held in
 // registers.  Both are bound by HBM where rows are many and by the launch where they are few.  us per launch, the rows not in the
-// caches: 16 prompts of up to 1024 rows, 8 heads of 128, bf16 into int8 16.0 (3.5 TB/s), and read back behind the write, padding
-// and all, 16.1 (5.4); both in a graph 32.0 (4.45, nine tenths of a copy's rate); 48 requests of up to 777 rows, 12 heads of 64,
-// e4m3 into fp16 36.1 (4.1); one token of 64 requests 2.5 each way; 300 rows of one request 3.2.
+// caches: 16 prompts of up to 1024 rows, 8 heads of 128, bf16 into int8 16.4 (3.4 TB/s), and read back behind the write, padding
+// and all, 16.4 (5.3); both in a graph 33.0 (4.3, nine tenths of a copy's rate); 48 requests of up to 777 rows, 12 heads of 64,
+// e4m3 into fp16 34.4 (4.3); one token of 64 requests 2.5 each way; 300 rows of one request 3.2.
 #include "paged_index.hpp"
 #include "q3t_common.hpp"
 
@@ -30,8 +30,16 @@ struct Params {
     const int32_t *lengths, *table;
     int64_t table_sb, rows;  // rows: table_width * page_size
     uint32_t batch, heads, tokens, units, pages;
-    Divisor by_units, by_heads, by_page;
+    uint32_t token_last;  // rows are taken head by head, else token by token
+    Divisor by_units, by_inner, by_page;  // inner: tokens, or heads
 };
+
+// Token and head of a request's row in the order that rows are taken in, some past the end.
+Q3T_DEVICE void row_of(const Params &p, uint32_t row, uint32_t &t, uint32_t &h) {
+    const uint32_t outer = divide(row, p.by_inner), inner = row - outer * p.by_inner.d;
+    t = p.token_last ? inner : outer;
+    h = p.token_last ? outer : inner;
+}
 
 // Rows of a request that the call has.
 Q3T_DEVICE uint32_t used_rows(const Params &p, uint32_t b) {
@@ -39,9 +47,9 @@ Q3T_DEVICE uint32_t used_rows(const Params &p, uint32_t b) {
 }
 // Place of row t of request b, whose first row is at `start`: page and row of it, page -1 for a row that it has not.
 struct Place { int32_t page; uint32_t row; };
-Q3T_DEVICE Place place(const Params &p, uint32_t b, int64_t start, uint32_t used, uint32_t t) {
+Q3T_DEVICE Place place(const Params &p, uint32_t b, int64_t start, uint32_t used, uint32_t t, uint32_t h) {
     // (start + t overflows for no start that is left)
-    if (t >= used || start >= p.rows || start < -(int64_t)p.tokens || start + t < 0 || start + t >= p.rows) return {-1, 0u};
+    if (h >= p.heads || t >= used || start >= p.rows || start < -(int64_t)p.tokens || start + t < 0 || start + t >= p.rows) return {-1, 0u};
     const uint32_t j = (uint32_t)(start + t), entry = divide(j, p.by_page);
     const int32_t page = p.table[b * p.table_sb + entry];
     return {(uint32_t)page < p.pages ? page : -1, j - entry * p.by_page.d};
@@ -175,16 +183,15 @@ __global__ void __launch_bounds__(kThreads) write_kernel(Params p) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const uint32_t row = ((blockIdx.x * N + k) * kThreads + threadIdx.x) / L;
-            t[k] = divide(row, p.by_heads);
-            h[k] = row - t[k] * p.heads;
-            if (t[k] >= (N == 1 ? p.tokens : used)) continue;
+            row_of(p, row, t[k], h[k]);
+            if (h[k] >= p.heads || t[k] >= (N == 1 ? p.tokens : used)) continue;
 #pragma unroll
             for (int n = 0; n < 2; ++n)
                 load8<VEC>(p.x[n].rows + b * p.x[n].r_sb + h[k] * p.x[n].r_sh + t[k] * p.x[n].r_st + unit * 8 * sizeof(T), e[k][n]);
         }
         Place at[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) at[k] = place(p, b, start, used, t[k]);
+        for (int k = 0; k < N; ++k) at[k] = place(p, b, start, used, t[k], h[k]);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             if (at[k].page < 0) continue;  // (the same for all lanes of a row)
@@ -235,9 +242,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Params p) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const uint32_t row = ((blockIdx.x * N + k) * kThreads + threadIdx.x) / L;
-            t[k] = divide(row, p.by_heads);
-            h[k] = row - t[k] * p.heads;
-            at[k] = place(p, b, start, used, t[k]);
+            row_of(p, row, t[k], h[k]);
+            at[k] = place(p, b, start, used, t[k], h[k]);
         }
         u32x2_t w[N][2];
         float scale[N][2];
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Params p) {
             }
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            if (t[k] >= p.tokens) continue;
+            if (h[k] >= p.heads || t[k] >= p.tokens) continue;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const Rows &r = p.x[n];
@@ -286,10 +292,9 @@ __global__ void __launch_bounds__(kThreads) copy_kernel(Params p) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const uint32_t i = (blockIdx.x * N + k) * kThreads + threadIdx.x, row = divide(i, p.by_units);
-            t[k] = divide(row, p.by_heads);
-            h[k] = row - t[k] * p.heads;
+            row_of(p, row, t[k], h[k]);
             unit[k] = (int64_t)(i - row * p.units) * V;
-            at[k] = place(p, b, start, used, t[k]);
+            at[k] = place(p, b, start, used, t[k], h[k]);
         }
         T v[N][2];
 #pragma unroll
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(kThreads) copy_kernel(Params p) {
             }
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            if (t[k] >= p.tokens) continue;
+            if (h[k] >= p.heads || t[k] >= p.tokens) continue;
 #pragma unroll
             for (int n = 0; n < 2; ++n)
                 __builtin_nontemporal_store(v[k][n], reinterpret_cast<T *>(p.x[n].rows + b * p.x[n].r_sb + h[k] * p.x[n].r_sh + t[k] * p.x[n].r_st + unit[k]));
@@ -335,7 +340,12 @@ static int common(const A *a, int64_t es, int64_t held, const q3t_paged_scales *
     p.rows = a->table_width * a->page_size;
     p.batch = (uint32_t)a->batch; p.heads = (uint32_t)a->heads; p.tokens = (uint32_t)a->tokens;
     p.pages = (uint32_t)a->pages;
-    p.by_heads = divisor(p.heads);
+    // In the order of the call's rows: a projection's heads lie side by side, a prefill cache's tokens, as they do in pages.  us,
+    // token by token / head by head: written in int8, 16 prompts of 600 rows of a cache, 8 heads of 128, 16.6 / 16.1, 4 of 200 3.6 /
+    // 3.3, 48 of 700, 12 heads of 64, 37.5 / 35.6; the last read 35.7 / 33.1, 48 of up to 777 in e4m3 36.1 / 34.4; 16 of up to 1024
+    // read behind their write 15.8 / 16.4.
+    p.token_last = a->k_stride_t <= a->k_stride_h;
+    p.by_inner = divisor(p.token_last ? p.tokens : p.heads);
     p.by_page = divisor((uint32_t)a->page_size);
     if (!aligned(a->page_table, 4) || !aligned(a->positions, 8) || (a->lengths && !aligned(a->lengths, 4))) return Q3T_EINVAL;
     for (const Rows &r : p.x) {

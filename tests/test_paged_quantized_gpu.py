@@ -138,6 +138,29 @@ def test_an_element_is_off_by_half_a_step_at_most(pkg, device, held):
         assert ((back - x).abs() <= half * (1 + 1e-5)).all()
 
 
+@pytest.mark.parametrize('held', [*HELD, BF16], ids=str)
+@pytest.mark.parametrize('tokens', [1, 33, 700])  # (two rows a thread in the last)
+def test_either_order_of_tokens_and_heads(pkg, device, held, tokens):
+    """Rows of a prefill cache, head by head, and of a projection, token by token."""
+    batch, heads, width, page, wide = 26, 7, 64, 24, 31
+    rows = _rows(device, batch, heads, tokens, width, BF16)
+    pools, scales = _pools(device, batch * wide + 3, heads, page, width, torch.int8 if held == BF16 else held)
+    table = _table(device, batch, wide, batch * wide + 3)
+    positions = torch.arange(batch, device=device) * 2
+    lengths = (torch.arange(batch, device=device) * 29 % (tokens + 1)).to(torch.int32)
+    if held == BF16:
+        pools, scales = [x.to(BF16) for x in pools], None
+    else:
+        _check(pkg, [x.contiguous() for x in rows], pools, scales, table, positions, lengths)
+        by_head = [bits(x).clone() for x in (*pools, *scales)]
+        pkg.paged_write(*rows, *pools, table, positions, lengths, scales=scales)
+        assert all(torch.equal(bits(x), y) for x, y in zip((*pools, *scales), by_head))
+    want = pkg.paged_read(*pools, table, positions, tokens, lengths, scales=scales, dtype=BF16)
+    out = tuple(torch.full((batch, tokens, heads, width), 7.0, device=device, dtype=BF16).transpose(1, 2) for _ in range(2))
+    for x, y in zip(pkg.paged_read(*pools, table, positions, tokens, lengths, scales=scales, out=out), want):
+        assert torch.equal(bits(x), bits(y))
+
+
 @pytest.mark.parametrize('dtype', [BF16, F16, F32], ids=str)
 def test_a_negative_zero_is_held_and_read(pkg, device, dtype):
     pools, scales = _pools(device, 2, 1, 16, 64, torch.float8_e4m3fn)
