@@ -524,7 +524,7 @@ int q3t_paged_read(const q3t_paged_read_args *args, const q3t_paged_scales *scal
  *
  * The keys on shared pages are read once for the batch, in a launch ahead of that for the requests' own keys, where that
  * saves enough (Q3T_SHARE_AUTO in args->reserved), always or never; never over pools of 8 bits.  Weights of that launch
- * are rounded to the type of 16 bits (half a step: 2^-8 in bf16, 2^-11 in fp16), and their sum is that of the rounded ones.
+ * go in two parts of the type of 16 bits, 16 (bf16) or 22 (fp16) of a float32's 24 bits.
  */
 #define Q3T_SHARE_AUTO 0
 #define Q3T_SHARE_ALWAYS 1

@@ -11,7 +11,7 @@
 // with float32 queries under a mask, 12 heads of 64, e4m3 12.2 (1.2; float32 rows 18.0), one of 300 8.1 (7.6).
 //
 // A shared prefix is read once for the batch, by a launch ahead of that for the requests' own keys (paged_prefix.hpp): 128 requests
-// behind 16384 keys, 32 query heads, 88.7 us (50 for the prefix) where requests that each read it take 960, 64 behind 4096 56.3 (16.8)
+// behind 16384 keys, 32 query heads, 103 us (64 for the prefix) where requests that each read it take 960, 64 behind 4096 58.6 (18.6)
 // and 154.
 #include "paged_with.hpp"
 

@@ -7,17 +7,17 @@
 //     keys in LDS, each with CT tiles of 16 columns in registers; KW such groups take the stages in turn and are merged
 //     at the end.
 //   * Stages come straight from memory to LDS, ahead of the one that is multiplied.
-//   * The weights go into the second product in one part of the type's own bits (half a step of 2^-8 in bf16, as the
-//     prefill's weights have; float32 is multiplied as such): here, unlike in the attention of one request, the matrix
-//     cores are the bound.  Their sum is that of the rounded weights, by a product with ones, so that what rounding takes
-//     from a weight is taken from both.
-//   * A value that is not finite under a key that only some columns see would reach the others too, as zero times NaN.
-//     A launch that finds such a one says so, and its states are not used: the requests then attend the prefix each for
-//     itself.
+//   * The weights go into the second product in two parts of the type's bits, 16 of a float32's in bf16 and 22 in fp16 (float32 is
+//     multiplied as such), and their sum is that of the float32 weights: outputs are those of requests that each read the prefix, up to
+//     what the outputs' own rounding hides.  In one part the largest launch below takes 50 us for 64, but outputs are
+//     off by 0.0022 of their norm where the type's rounding alone is 0.0017.
+//   * A value that is not finite would reach, as zero times NaN, columns that do not see its key, and as infinity times a part that
+//     is zero those that do.  A launch that meets such a one says so, and its states are not used: the requests then attend the prefix
+//     each for itself.
 // The matrix cores bound it from some hundred columns on (4 * 16384 keys, 128 requests, 32 query heads over 8 KV heads of 128 in
-// bf16: 34.4 GFLOP in 50 us, 0.69 PFLOP/s and 0.8 past the start of 9 us, where a large library product reaches 1.2), the start and
-// the stages' chain below it (8 KV heads, 128 columns each, 4096 keys 16.8 us).  Waves that share a stage alternate between
-// matrix and vector instructions in two groups (with the addresses of a part worked out once, 65 -> 57 us then).
+// bf16: 51.5 GFLOP, the weights' two parts counted, in 64 us, 0.80 PFLOP/s and 0.94 past the start of 9 us, where a large library
+// product reaches 1.2), the start and the stages' chain below it (8 KV heads, 128 columns each, 4096 keys 18.6 us).  Waves that share a stage alternate between
+// matrix and vector instructions in two groups (with the addresses of a part worked out once, 65 -> 57 us, with weights in one part).
 #pragma once
 
 #include "paged_kernel.hpp"
@@ -47,8 +47,10 @@ template <typename T, int D, int CT> struct Wide {
     typedef Shape<T, D> S;
     static constexpr int tiles = 2, keys = 32;  // of 16 keys; keys of a stage
     static constexpr float shift = Half<T>::shift, threshold = Half<T>::threshold;
+    static constexpr int parts = 2;  // of a weight
     U4 q[CT][D / 32];
-    f32x4_t acc[CT][D / 16], sum[CT];
+    f32x4_t acc[CT][D / 16];
+    float sum[CT];
     uint32_t key_at[D / 32], value_at[D / 16];
 
     Q3T_DEVICE void load_query(int ct, const char *row, int g, bool live, bool flip) {
@@ -68,7 +70,7 @@ template <typename T, int D, int CT> struct Wide {
     Q3T_DEVICE void clear() {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-            sum[ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            sum[ct] = 0.f;
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) acc[ct][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         }
@@ -86,7 +88,7 @@ template <typename T, int D, int CT> struct Wide {
         for (int d = 0; d < D / 16; ++d)
             value_at[d] = (keys + r) * S::row + (((2 * d + ((c >> 1) & 1)) ^ S::value_swizzle(r)) & (S::chunks - 1)) * 16 + 8 * (c & 1);
     }
-    U4 k[tiles][D / 32], v[D / 16], p[CT];  // a stage's fragments of keys and values, its weights
+    U4 k[tiles][D / 32], v[D / 16], p[CT][parts];  // a stage's fragments of keys and values, its weights
     Q3T_DEVICE void read_keys(uint32_t stage) {
 #pragma unroll
         for (int t = 0; t < tiles; ++t)
@@ -114,35 +116,42 @@ template <typename T, int D, int CT> struct Wide {
         }
         together();
     }
-    // Rounded weights as an operand: inner index 8 g + j stands for key 4 g + j of the first tile (j < 4), and 4 g + j - 4 of the second.
-    Q3T_DEVICE static U4 pack(const float (&w)[tiles][4]) {
-        return U4{Half<T>::round2(w[0][0], w[0][1]), Half<T>::round2(w[0][2], w[0][3]), Half<T>::round2(w[1][0], w[1][1]),
-                  Half<T>::round2(w[1][2], w[1][3])};
-    }
-    // (worked out here, not where they are used)
+    // The weights as operands, in parts: inner index 8 g + j stands for key 4 g + j of the first tile (j < 4), and 4 g + j - 4 of
+    // the second.
     Q3T_DEVICE void weights(int ct, const float (&w)[tiles][4]) {
-        p[ct] = pack(w);
-        asm volatile("" : "+v"(p[ct].x), "+v"(p[ct].y), "+v"(p[ct].z), "+v"(p[ct].w));
+        float rest[tiles * 4];
+#pragma unroll
+        for (int k = 0; k < tiles * 4; ++k) rest[k] = w[k / 4][k % 4];
+        sum[ct] += ((rest[0] + rest[1]) + (rest[2] + rest[3])) + ((rest[4] + rest[5]) + (rest[6] + rest[7]));
+#pragma unroll
+        for (int n = 0; n < parts; ++n) {
+            uint32_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                u[i] = Half<T>::round2(rest[2 * i], rest[2 * i + 1]);
+                rest[2 * i] -= Half<T>::lo(u[i]);
+                rest[2 * i + 1] -= Half<T>::hi(u[i]);
+            }
+            p[ct][n] = U4{u[0], u[1], u[2], u[3]};
+            // (worked out here, not where they are used)
+            asm volatile("" : "+v"(p[ct][n].x), "+v"(p[ct][n].y), "+v"(p[ct][n].z), "+v"(p[ct][n].w));
+        }
     }
     Q3T_DEVICE void values() {
-        const uint32_t one = std::is_same<T, __bf16>::value ? 0x3f803f80u : 0x3c003c00u;
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d)
+        for (int n = 0; n < parts; ++n)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) acc[ct][d] = Half<T>::scores(v[d], p[ct], acc[ct][d]);
+            for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) sum[ct] = Half<T>::scores(U4{one, one, one, one}, p[ct], sum[ct]);
+                for (int ct = 0; ct < CT; ++ct) acc[ct][d] = Half<T>::scores(v[d], p[ct][n], acc[ct][d]);
     }
-    Q3T_DEVICE float total(int ct) const { return sum[ct][0]; }
+    Q3T_DEVICE float total(int ct) const {
+        const float l = sum[ct] + xor16(sum[ct]);
+        return l + xor32(l);
+    }
     // the values' dims, as they are stored: 16 bytes of acc[][a] from dim
     Q3T_DEVICE static int dim(int a, int g) { return 16 * a + 4 * g; }
     Q3T_DEVICE f32x4_t four(int ct, int a) const { return acc[ct][a]; }
-    Q3T_DEVICE static bool finite(U4 x) {
-        const uint32_t step = std::is_same<T, __bf16>::value ? 0x00800080u : 0x04000400u;  // carries an exponent of all ones into the sign
-        const uint32_t any = ((x.x & 0x7fff7fffu) + step) | ((x.y & 0x7fff7fffu) + step) | ((x.z & 0x7fff7fffu) + step) | ((x.w & 0x7fff7fffu) + step);
-        return !(any & 0x80008000u);
-    }
-    static Q3T_DEVICE float visible(float w) { return Half<T>::visible(w); }
 };
 
 template <int D, int CT> struct Wide<float, D, CT> {
@@ -235,11 +244,6 @@ template <int D, int CT> struct Wide<float, D, CT> {
         const int j = a & ~3, i = a & 3;
         return f32x4_t{acc[ct][j][i], acc[ct][j + 1][i], acc[ct][j + 2][i], acc[ct][j + 3][i]};
     }
-    Q3T_DEVICE static bool finite(U4 x) {
-        auto fine = [](uint32_t e) { return (e & 0x7fffffffu) < 0x7f800000u; };
-        return fine(x.x) && fine(x.y) && fine(x.z) && fine(x.w);
-    }
-    static Q3T_DEVICE float visible(float w) { return w; }
 };
 
 // Loads into LDS from an address per lane (load_rows and load_half, for rows that several workgroups read).
@@ -270,7 +274,7 @@ struct PrefixLds {
     };
     float ml[KW][CW][CT][2][64];
     uint64_t pages[kEntries][2];     // addresses of the head's first key and value row on a page, kBias short; odd for no page
-    uint32_t odd;                    // values that are not finite were found
+    uint32_t odd;                    // values that are not finite were met
     uint32_t least;                  // keys that all live columns see
     uint32_t holes;                  // entries that are no page
 };
@@ -408,20 +412,15 @@ prefix_kernel(PrefixParams p) {
     // exponents are unit (v - m) in log2 units: v the products themselves, or, under a mask, the natural scores
     // (a threshold that is finite: m is below any score at first)
     const float unit = MASK ? kLog2e : p.scale, threshold = fminf(X::threshold / unit, __FLT_MAX__);
-    bool odd = false;
     auto partial = [&](uint32_t key0) { return MASK || key0 + SK > least; };
     // Stage n, whose loads of this wave have ended.  Value rows of keys that do not exist become zeros: zero times NaN would
-    // be NaN.  Where some column does not see all keys, values that are not finite are looked for, for the same reason.
+    // be NaN.
     auto arrived = [&](uint32_t n, uint32_t here) {
-        const uint32_t key0 = begin + (n * KW + group) * SK, at = buffer(n);
-        if (here == kAll && !partial(key0)) return;
+        if (here == kAll) return;
+        const uint32_t at = buffer(n);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            if (!is_value(i)) continue;
-            const uint32_t to = at + (cw * LOADS + i) * 1024 + lane * 16;
-            if (!(here >> row_of(i) & 1u)) lds_write16(to, U4{0u, 0u, 0u, 0u});
-            else if (partial(key0) && !X::finite(lds_read16(to))) odd = true;
-        }
+        for (int i = 0; i < LOADS; ++i)
+            if (is_value(i) && !(here >> row_of(i) & 1u)) lds_write16(at + (cw * LOADS + i) * 1024 + lane * 16, U4{0u, 0u, 0u, 0u});
     };
     // The mask's words of stage n, four keys of a column at once where they lie so, and the terms in them.
     uint32_t words[CT][TILES][4] = {};
@@ -525,9 +524,7 @@ prefix_kernel(PrefixParams p) {
 #pragma unroll
             for (int k = 0; k < TILES * 4; ++k) {
                 float &e = w[ct][k / 4][k % 4];
-                const float v = X::visible(fexp2(MASK ? __builtin_fmaf(e - top, unit, X::shift) : __builtin_fmaf(e, unit, from)));
-                // (the smallest weight is for keys that are seen)
-                e = X::visible(0.f) != 0.f && e == -INFINITY ? 0.f : v;
+                e = fexp2(MASK ? __builtin_fmaf(e - top, unit, X::shift) : __builtin_fmaf(e, unit, from));
             }
             x.weights(ct, w[ct]);
         }
@@ -607,8 +604,17 @@ prefix_kernel(PrefixParams p) {
     // ---- the groups' states, into the first one's ----
     float l[CT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) l[ct] = x.total(ct);
-    if (odd) s.odd = 1;
+    for (int ct = 0; ct < CT; ++ct) {
+        l[ct] = x.total(ct);
+        // A value that is not finite leaves the sums of its dim so, whatever its weight.  (Where the weights are not either, so is
+        // what they should give.)
+        bool fine = true;
+#pragma unroll
+        for (int a = 0; a < D / 16; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fine &= __builtin_fabsf(x.acc[ct][a][i]) < INFINITY;
+        if (live[ct] && !fine && __builtin_fabsf(l[ct]) < INFINITY) s.odd = 1;
+    }
     lds_barrier();  // all have left the last stage
     if (tid == 0) p.odd[task * p.blocks + block] = s.odd;
     if constexpr (KW > 1) {

@@ -219,8 +219,8 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     ``shared_pages``: the first that many entries are the same pages in every row of ``page_table``, also in
     rows of requests that attend nothing, as where all requests have one prompt in front.  What each
     request attends is as without it, but where it saves enough (``read_once`` True or False: always, or
-    never) the keys on them are read once for the whole batch, their weights then rounded to the queries'
-    type (of 16 bits) with the sum over them.  Pools of 8 bits are attended request by request."""
+    never) the keys on them are read once for the whole batch, their weights then held in two parts of the queries'
+    type (of 16 bits): a relative 2^-16 in bf16, 2^-22 in fp16.  Pools of 8 bits are attended request by request."""
     return _attend(_attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out, scales, shared_pages,
                                    read_once))
 

@@ -1,0 +1,34 @@
+"""``paged_attention`` over shared pages where what the launch ahead of the requests' own keys does on its own shows: the bits
+of its weights."""
+import pytest
+import torch
+
+from tests._paged import assert_within, attention64
+from tests._paged_more import problem, run
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize('width', [64, 128])
+@pytest.mark.parametrize('batch', [5, 40])
+@pytest.mark.parametrize('masked', [False, True])
+def test_weights_keep_the_bits_that_outputs_show(pkg, device, dtype, width, batch, masked):
+    """Every second key scores a little more than the others and has a value of 1, the others -1: what is left of the values is the
+    difference of weights next to each other, which weights of the type's own bits get wrong by a sixth.
+
+    The scores are sums of one product, so that ``attention64``'s bound is small.  To it comes what two parts leave of a weight:
+    half a step each, 2^-16 of it in bf16, times A = sum_j w_j |v_j| = 1; in fp16 2^-22 (which the bound holds), and of weights
+    that are 2^8 times as large half of the smallest number, 2^-25, for each of 320 keys."""
+    p = problem(device, [321 + b % 7 for b in range(batch)], shared=20, dtype=dtype, width=width, seed=40)
+    p.query.zero_()
+    p.query[..., 0] = 0.01 + 0.004 * torch.arange(batch, device=device)[:, None, None] % 0.05
+    sign = torch.tensor([1.0, -1.0], device=device).repeat(8)[None, None, :, None]
+    p.key_pages.copy_(sign.expand(p.key_pages.shape))
+    p.value_pages.copy_(sign.expand(p.value_pages.shape))
+    mask = torch.ones(batch, 1, 1, p.table.shape[1] * 16, dtype=torch.bool, device=device) if masked else None
+    want, tol = attention64(p.query, p.key_pages, p.value_pages, p.table, p.positions, mask=mask)
+    tol += {BF16: 2.0 ** -16, F16: 320 * 2.0 ** -33, F32: 0.0}[dtype]
+    assert_within(run(pkg, p, mask=mask), want, tol)
