@@ -106,4 +106,9 @@ Q3T_BOTH Run next_run(Cursor &c, uint32_t stages, uint32_t heads, const Sharing 
     return r;
 }
 
+// The share of a workgroup that has one pair to itself, in one run: of any number of stages below 2^30.
+constexpr uint32_t kWholePair = 1u << 30;
+Q3T_BOTH Sharing whole_pair() { return {kWholePair, 0u, kWholePair, kWholePair}; }
+Q3T_BOTH Cursor whole_pair_at(uint32_t b, uint32_t head) { return {0u, kWholePair, b, head, 0u}; }
+
 }  // namespace q3t

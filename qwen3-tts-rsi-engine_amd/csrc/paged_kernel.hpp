@@ -674,10 +674,9 @@ paged_kernel(const int64_t *positions, uint32_t batch, uint32_t ctx, std::condit
         return at.left > 0;
     };
     if constexpr (SINGLE) {
-        constexpr uint32_t kRoom = 1u << (MORE ? 21 : kLogLeastSingle);  // holds any such pair's stages
-        sh = {kRoom, 0u, kRoom, batch * p.heads * kRoom};
         const uint32_t b = blockIdx.x / p.heads;
-        at = Cursor{blockIdx.x * kRoom, kRoom, b, blockIdx.x - b * p.heads, 0u};
+        sh = whole_pair();
+        at = whole_pair_at(b, blockIdx.x - b * p.heads);
         window = b;
         lengths = length_at(b + lane);
     } else {

@@ -1,5 +1,5 @@
 """``paged_attention`` over shared pages where what the launch ahead of the requests' own keys does on its own shows: the bits
-of its weights."""
+of its weights, and how long it may be."""
 import pytest
 import torch
 
@@ -32,3 +32,22 @@ def test_weights_keep_the_bits_that_outputs_show(pkg, device, dtype, width, batc
     want, tol = attention64(p.query, p.key_pages, p.value_pages, p.table, p.positions, mask=mask)
     tol += {BF16: 2.0 ** -16, F16: 320 * 2.0 ** -33, F32: 0.0}[dtype]
     assert_within(run(pkg, p, mask=mask), want, tol)
+
+
+@pytest.mark.parametrize('odd', [False, True])
+def test_prefixes_past_two_to_the_25_keys(pkg, device, odd):
+    """One page over and over, and at the end one whose key outweighs all others; a value after the request's end that is not finite
+    leaves all of them to the request's one workgroup."""
+    page, entries = 512, 65600  # (own keys that a workgroup has to itself)
+    pools = [torch.zeros(3, 1, page, 128, dtype=BF16, device=device) for _ in range(2)]
+    pools[0][1, 0, 7, 0] = 42.5  # a score of 30 over those of 3.4e7 others
+    pools[1][1, 0, 7] = torch.randn(128, device=device)
+    pools[1][1, 0, -1] = float('inf') if odd else 3.0
+    table = torch.zeros(2, entries + 1, dtype=torch.int32, device=device)
+    table[:, entries - 1], table[:, entries] = 1, 2
+    query = torch.zeros(2, 1, 1, 128, dtype=BF16, device=device)
+    query[..., 0] = 8
+    positions = torch.tensor([entries * page - 2, -1], device=device)
+    out = pkg.paged_attention(query, *pools, table, positions, shared_pages=entries, read_once=True)
+    want = pools[1][1, 0, 7].float()
+    assert ((out[0, 0, 0].float() - want).abs() <= want.abs() * (2.0 ** -8 + 1e-5)).all() and (out[1] == 0).all()
