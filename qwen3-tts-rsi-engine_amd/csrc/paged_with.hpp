@@ -55,7 +55,8 @@ template <typename T, typename With>
 static int64_t shared_bytes(const q3t_paged_args *a, int64_t keys, With with) {
     const q3t_paged_args b = behind(a, keys);
     Sizes z;
-    const int status = sizes_of(&b, z, with);
+    int status = sizes_of(a, z, with);  // of all keys too: the requests may have to attend the prefix each for itself
+    if (status == Q3T_OK) status = sizes_of(&b, z, with);
     return status != Q3T_OK ? status : (z.workspace + 15) / 16 * 16 + prefix_plan<T>(&b, keys).bytes;
 }
 

@@ -38,3 +38,31 @@ def test_a_workgroup_of_one_pair_has_all_of_its_stages(whole_pair, keys):
     stages = -(-keys // 16)
     for b, head, heads in ((0, 0, 1), (0, 1, 8), (31, 7, 8)):
         assert whole_pair(b, head, stages, heads) == [b, head, 0, stages, 1, 1, 0]
+
+
+def _args(pkg, **changes):
+    a = pkg._lib.PagedArgs()
+    a.batch, a.q_heads, a.kv_heads, a.head_dim, a.dtype, a.scale = 2, 16, 8, 128, pkg._lib.Q3T_BF16, 0.1
+    a.pages, a.page_size, a.table_width, a.table_stride_b, a.ctx = 10, 16, 4, 4, 64
+    for name, value in changes.items():
+        setattr(a, name, value)
+    a.ctx = changes.get('ctx', a.table_width * a.page_size)
+    return a
+
+
+def _bytes(pkg, shared, **changes):
+    return pkg.library().q3t_paged_workspace_bytes_with(_args(pkg, **changes), None, shared)
+
+
+@pytest.mark.parametrize('dtype,width', [('Q3T_BF16', 128), ('Q3T_F16', 128), ('Q3T_F32', 64), ('Q3T_F32', 128), ('Q3T_BF16', 64)])
+@pytest.mark.parametrize('once', ['Q3T_SHARE_AUTO', 'Q3T_SHARE_ALWAYS', 'Q3T_SHARE_NEVER'])
+def test_calls_of_too_many_stages_are_refused_however_much_is_shared(pkg, dtype, width, once):
+    """Stages are counted in 30 bits, those of the requests' shared keys too, which they may have to attend each for itself."""
+    ways = {'Q3T_SHARE_AUTO': 0, 'Q3T_SHARE_ALWAYS': 1, 'Q3T_SHARE_NEVER': 2}
+    keys = 32 if dtype != 'Q3T_F32' and width == 64 else 16  # of a stage
+    sizes = dict(batch=64512, q_heads=1, kv_heads=1, head_dim=width, dtype=getattr(pkg._lib, dtype), page_size=512, reserved=ways[once])
+    most = (1 << 30) // 64512  # stages of a request
+    fits, not_ = ((most - 40) * keys // 512, (most + 40) * keys // 512)
+    for entries, good in ((fits, True), (not_, False)):
+        for shared in (0, 1, entries - 1):
+            assert (_bytes(pkg, shared, table_width=entries, table_stride_b=entries, **sizes) >= 0) == good
