@@ -517,7 +517,8 @@ int q3t_paged_read(const q3t_paged_read_args *args, const q3t_paged_scales *scal
 /*
  * q3t_paged_attention over pools of 8 bits (scales != NULL), the queries and the output having dtype; and for
  * a batch whose requests begin with the same pages (shared_pages > 0): the first shared_pages entries are the same in
- * every request's row of page_table, also where a request attends nothing (any row's may be read).  Everything else is
+ * every request's row of page_table, also where a request attends nothing.  A row whose first entry names no page, where others'
+ * do, is one that a request has left: it attends none of the shared pages, whatever its others say.  Everything else is
  * as q3t_paged_attention has it: a request attends its keys 0 ... positions[b], also where that ends within the shared
  * pages, under its own mask.
  * shared_pages * page_size is below ctx.

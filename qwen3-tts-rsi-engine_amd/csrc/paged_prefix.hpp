@@ -27,7 +27,7 @@ namespace paged {
 
 struct PrefixParams {
     const char *q, *kp, *vp, *mask;
-    const int32_t *table;               // request 0's row
+    const int32_t *table;
     const int64_t *positions;
     float *states, *ml;                 // (part, KV head, column): D values; maximum and sum
     uint32_t *odd;                      // of each workgroup: its states are not to be used, nor any other
@@ -37,6 +37,7 @@ struct PrefixParams {
     uint32_t heads, columns, blocks;    // KV heads; columns of one, and their blocks
     uint32_t parts, keys, chunk;        // parts of `chunk` keys
     uint32_t pages, ctx;
+    uint32_t table_sb, batch;
     int32_t flip, zero;                 // unmasked: the scale is below zero, is zero
     Divisor by_page, by_group;
     float scale;                        // unmasked: its size times log2(e), 1 for none
@@ -277,6 +278,7 @@ struct PrefixLds {
     uint32_t odd;                    // values that are not finite were met
     uint32_t least;                  // keys that all live columns see
     uint32_t holes;                  // entries that are no page
+    uint32_t row;                    // the first of the table whose first entry is a page
 };
 
 // CW waves share the columns, KW groups of them the stages.
@@ -368,6 +370,7 @@ prefix_kernel(PrefixParams p) {
     bool live[CT];
     // what all of it starts with, on its way together: positions, query rows, page numbers
     int64_t position[CT];
+    uint32_t lead[CT];  // the first entry of the request's row of the table
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         column[ct] = (block * CW * CT + cw * CT + ct) * kColumns + c;
@@ -375,17 +378,37 @@ prefix_kernel(PrefixParams p) {
         request[ct] = real ? divide(column[ct], p.by_group) : 0;
         const uint32_t i = column[ct] - request[ct] * p.by_group.d;
         position[ct] = p.positions[request[ct]];
+        lead[ct] = (uint32_t)p.table[(uint64_t)request[ct] * p.table_sb];
         if (!real) position[ct] = -1;
         x.load_query(ct, p.q + ((uint64_t)request[ct] * p.q_sb + (uint64_t)(head * p.by_group.d + (real ? i : 0)) * p.q_sh) * 16, g, real && !p.zero, p.flip);
     }
-    const uint32_t first_id = (uint32_t)p.table[entry0 + min((uint32_t)tid, last_entry)];
+    uint32_t first_id = (uint32_t)p.table[entry0 + min((uint32_t)tid, last_entry)];
+    const bool first_leads = uniform((uint32_t)p.table[0]) < p.pages;
     if (tid == 0) {
         s.least = p.keys;
         s.odd = s.holes = 0;
+        s.row = p.batch;
     }
     __syncthreads();
+    // The entries are those of the first row whose first one is a page: a retired request's row holds none.  Where no row's is, row 0's.
+    uint32_t row = 0;
+    bool leads = first_leads;
+    if (!first_leads) {
+        for (uint32_t b = tid; b < p.batch; b += kThreads)
+            if ((uint32_t)p.table[(uint64_t)b * p.table_sb] < p.pages) {
+                atomicMin(&s.row, b);
+                break;
+            }
+        __syncthreads();
+        leads = uniform(s.row) < p.batch;
+        if (leads) {
+            row = uniform(s.row);
+            first_id = (uint32_t)p.table[(uint64_t)row * p.table_sb + entry0 + min((uint32_t)tid, last_entry)];
+        }
+    }
+    const int32_t *table = p.table + (uint64_t)row * p.table_sb + entry0;
     for (uint32_t i = tid; i <= last_entry; i += kThreads) {
-        const uint32_t id = i == (uint32_t)tid ? first_id : (uint32_t)p.table[entry0 + i], none = id >= p.pages;
+        const uint32_t id = i == (uint32_t)tid ? first_id : (uint32_t)table[i], none = id >= p.pages;
         auto first = [&](const char *pool, uint32_t page_stride, uint32_t head_stride) {
             return reinterpret_cast<uint64_t>(pool) + ((uint64_t)(none ? 0 : id) * page_stride + (uint64_t)head * head_stride) * 16 - kBias + none;
         };
@@ -395,7 +418,7 @@ prefix_kernel(PrefixParams p) {
     }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-        live[ct] = position[ct] >= 0 && position[ct] < (int64_t)p.ctx;
+        live[ct] = position[ct] >= 0 && position[ct] < (int64_t)p.ctx && (lead[ct] < p.pages) == leads;
         seen[ct] = live[ct] && position[ct] < (int64_t)p.keys ? (uint32_t)position[ct] + 1 : p.keys;
         if (seen[ct] < p.keys) atomicMin(&s.least, seen[ct]);
     }
@@ -711,6 +734,7 @@ static int prefix_run(const q3t_paged_args *a, const PrefixPlan &z, int64_t keys
     x.parts = (uint32_t)z.parts; x.keys = (uint32_t)keys; x.chunk = (uint32_t)z.chunk;
     x.pages = p.pages;
     x.ctx = (uint32_t)(a->ctx + keys);
+    x.table_sb = p.table_sb; x.batch = (uint32_t)a->batch;
     x.by_page = p.by_page;
     x.by_group = divisor(p.group);
     x.scale = p.scale;

@@ -217,7 +217,8 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     ``scales``: the pools are int8 or float8_e4m3fn, and the keys and values those that they stand for.
 
     ``shared_pages``: the first that many entries are the same pages in every row of ``page_table``, also in
-    rows of requests that attend nothing, as where all requests have one prompt in front.  What each
+    rows of requests that attend nothing, as where all requests have one prompt in front; only in rows that requests have
+    left may all entries be numbers of no page (-1), and nothing is attended by those.  What each
     request attends is as without it, but where it saves enough (``read_once`` True or False: always, or
     never) the keys on them are read once for the whole batch, their weights then held in two parts of the queries'
     type (of 16 bits): a relative 2^-16 in bf16, 2^-22 in fp16.  Pools of 8 bits are attended request by request."""
@@ -428,7 +429,7 @@ class PagedCache(Cache):
     ``positions[b]`` and returns the layer's pools; ``step`` attends over them too, as
     ``PackedAttention`` calls it.  ``page_table`` and ``positions`` are read at every step as they are
     then, so a captured step follows changes of their contents.  ``shared_pages``: entries that all rows of the
-    table begin with, as ``paged_attention`` takes them (idle requests' rows too); no request may write to those pages.
+    table begin with, as ``paged_attention`` takes them (all but retired requests' rows, of -1); no request may write to those pages.
 
     The lengths live on the device, so ``get_seq_length`` is 0: pass the model ``position_ids``, and as
     its mask None (a request then attends its keys up to its position) or one over the table's rows."""

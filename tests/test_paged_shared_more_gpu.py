@@ -1,10 +1,10 @@
 """``paged_attention`` over shared pages where what the launch ahead of the requests' own keys does on its own shows: the bits
-of its weights, and how long it may be."""
+of its weights, how long it may be, and whose row of the table it goes by."""
 import pytest
 import torch
 
 from tests._paged import assert_within, attention64
-from tests._paged_more import problem, run
+from tests._paged_more import expected, problem, run
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,50 @@ def test_prefixes_past_two_to_the_25_keys(pkg, device, odd):
     out = pkg.paged_attention(query, *pools, table, positions, shared_pages=entries, read_once=True)
     want = pools[1][1, 0, 7].float()
     assert ((out[0, 0, 0].float() - want).abs() <= want.abs() * (2.0 ** -8 + 1e-5)).all() and (out[1] == 0).all()
+
+
+@pytest.mark.parametrize('dtype,width,heads', [(BF16, 128, (16, 8)), (F16, 64, (20, 2)), (F32, 64, (3, 3))], ids=str)
+@pytest.mark.parametrize('batch,retired', [(5, [0]), (5, [0, 1, 2, 3]), (40, [0, 1, 17, 39]), (40, range(40)), (700, range(650))],
+                         ids=['0', 'all but one', 'some', 'all', 'past a workgroup'])
+@pytest.mark.parametrize('masked', [False, True])
+def test_rows_that_requests_have_left(pkg, device, dtype, width, heads, batch, retired, masked):
+    """Rows of -1, the first one's too, as the page table of an arena has them: they attend nothing, and no other loses a key."""
+    p = problem(device, [321 + 5 * b % 60 for b in range(batch)], shared=20, q_heads=heads[0], kv_heads=heads[1], dtype=dtype, width=width,
+                seed=41)
+    retired = list(retired)
+    p.table[retired] = -1
+    mask = torch.ones(batch, 1, 1, p.table.shape[1] * 16, dtype=torch.bool, device=device) if masked else None
+    want = expected(p, mask=mask)
+    for positions in (p.positions.clone(), p.positions.clone().index_fill(0, torch.tensor(retired, device=device), -1)):
+        p.positions = positions
+        out = run(pkg, p, mask=mask)
+        assert (out[retired] == 0).all()
+        assert_within(out, *want)
+
+
+def test_a_captured_launch_of_which_requests_retire(pkg, device):
+    """Through the table's contents alone, one after the other, a value that is not finite in between."""
+    p = problem(device, [1300 + b % 70 for b in range(30)], shared=80, seed=42)
+    run(pkg, p)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        out = run(pkg, p)
+    torch.cuda.current_stream().wait_stream(side)
+    for b in (0, 7, 1, 2):
+        p.table[b] = -1
+        p.query.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, run(pkg, p))
+        assert_within(out, *expected(p))
+    place = int(p.table[-1, 3]), 0, 5, 6
+    kept = p.value_pages[place].item()
+    p.value_pages[place] = float('inf')
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (out[:3] == 0).all() and (out[3:7, 0, :2, 6] == float('inf')).all()
+    p.value_pages[place] = kept
+    graph.replay()
+    torch.cuda.synchronize()
+    assert_within(out, *expected(p))
