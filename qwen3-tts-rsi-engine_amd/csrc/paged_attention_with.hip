@@ -18,21 +18,27 @@
 namespace q3t {
 namespace paged {
 
-// Whether the prefix is attended once for all: a launch of its own (9 us, and 1.1 for each set of stages that a workgroup has),
-// whose states every pair's end reads (16 ns a pair, 1.2 us for each time that a thread has four on their way), against the
-// time that reading the prefix again takes, at 5.5 TB/s.  us with / without it, requests x prefix, 8 KV heads of 128 and two
-// query heads each in bf16: 2 x 16384 28.6 / 29.4, 4 x 4096 19.3 / 19.9, 8 x 512 15.4 / 11.8, 8 x 2048 17.7 / 18.2, 8 x 4096
-// 19.6 / 24.0, 32 x 512 18.5 / 12.4, 32 x 1024 19.4 / 26.1, 64 x 256 23.8 / 16.3, 64 x 512 24.6 / 30.4, 64 x 4096 57.8 / 153, 128
-// x 256 38.9 / 36.0; one KV head of 16 query heads: 32 x 4096 30.0 / 19.2, 100 x 4096 32.5 / 35.5.
+// Whether the prefix is attended once for all: what its launch adds, against what reading the prefix again for every request takes.
+// The costs, in us, are those of a line through 478 pairs of times, of requests x prefix, heads, types, masks and pages of all kinds:
+// the choice is the quicker one or within 3% of it for all but 13 of them (0.35% off on average, 42% at worst, for 4720 columns under a
+// mask).  us once / for each, 8 KV heads of 128 and two query heads each in bf16 unless said: 2 x 16384 28.7 / 29.5, 8 x 512
+// 16.9 / 12.1, 8 x 4096 19.7 / 24.5, 64 x 512 28.8 / 31.1, 64 x 4096 32.3 / 108, float32 70.5 / 260, 64 x 512 under a mask 47.2 / 33.2;
+// one KV head of 16 query heads: 100 x 4096 35.7 / 34.3, float32 102 / 71; 40 query heads on 2: 16 x 4096 33.3 / 27.0, float32 99 / 49.
 static bool once_for_all(const q3t_paged_args *a, int64_t shared_pages) {
     if (shared_pages == 0 || a->reserved == Q3T_SHARE_NEVER) return false;
     if (a->reserved == Q3T_SHARE_ALWAYS) return true;
-    const int64_t size = a->dtype == Q3T_F32 ? 4 : 2, group = a->q_heads / a->kv_heads, keys = shared_pages * a->page_size;
-    const int64_t blocks = (group + kColumns - 1) / kColumns, columns = group < kColumns ? group : kColumns;
-    const PrefixPlan plan = size == 4 ? prefix_plan<float>(a, keys) : prefix_plan<__bf16>(a, keys);
-    const double again = 2.0 * (double)(a->head_dim * size * a->kv_heads) * (double)(a->batch * blocks - 1) * (double)keys / 5.5e6;
-    const double rounds = (double)((plan.parts * columns * a->head_dim / 4 + 2047) / 2048);
-    return again > 9.0 + 1.1 * (double)(plan.chunk / plan.step) + 0.016 * (double)(a->batch * a->kv_heads * blocks) + 1.2 * rounds;
+    const bool f32 = a->dtype == Q3T_F32;
+    const int64_t group = a->q_heads / a->kv_heads, keys = shared_pages * a->page_size, blocks = (group + kColumns - 1) / kColumns;
+    const PrefixPlan plan = f32 ? prefix_plan<float>(a, keys) : prefix_plan<__bf16>(a, keys);
+    const double width = (double)a->head_dim, pairs = (double)(a->batch * a->kv_heads * blocks);
+    // read again: 8.4 TB/s, out of the caches where it fits them
+    const double again = 2.0 * width * (f32 ? 4 : 2) * (pairs - (double)a->kv_heads) * (double)keys / 8.4e6;
+    // a set of stages: its start, the products (two a weight in 16 bits) at a CU's rate, the mask's terms
+    const double products = (f32 ? 4 : 6) * width * (double)(plan.cw * plan.ct * kColumns * plan.step) / (f32 ? 0.6e6 : 9.8e6);
+    const double set = 0.37 + 1.2 * products + (a->mask ? (f32 ? 0.72 : 1.15) * (double)plan.ct : 0.0);
+    const double sets = (double)((plan.workgroups + 255) / 256 * (plan.chunk / plan.step));
+    // a launch; the pairs' ends; the states, written and read
+    return again > 5.0 + sets * set + 0.0061 * pairs + (double)(plan.states * (a->head_dim + 2) * 4) / 0.7e6;
 }
 
 // Bytes of workspace, or the status to return.

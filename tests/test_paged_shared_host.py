@@ -66,3 +66,37 @@ def test_calls_of_too_many_stages_are_refused_however_much_is_shared(pkg, dtype,
     for entries, good in ((fits, True), (not_, False)):
         for shared in (0, 1, entries - 1):
             assert (_bytes(pkg, shared, table_width=entries, table_stride_b=entries, **sizes) >= 0) == good
+
+
+# (requests, keys shared, page, query heads, KV heads, width, type, masked, read once), and us read once / request by request
+CHOICES = [
+    ((8, 512, 16, 16, 8, 128, 'Q3T_BF16', False, False), '16.9 / 12.1'),
+    ((8, 4096, 16, 16, 8, 128, 'Q3T_BF16', False, True), '19.7 / 24.5'),
+    ((64, 4096, 16, 16, 8, 128, 'Q3T_BF16', False, True), '32.3 / 108'),
+    ((64, 4096, 16, 16, 8, 128, 'Q3T_F32', False, True), '70.5 / 260'),
+    ((128, 16384, 64, 32, 8, 128, 'Q3T_BF16', False, True), '103 / 965'),
+    ((64, 512, 16, 16, 8, 128, 'Q3T_BF16', True, False), '47.2 / 33.2'),
+    ((64, 4096, 16, 16, 8, 128, 'Q3T_BF16', True, True), '49.6 / 121'),
+    ((21, 792, 24, 12, 12, 64, 'Q3T_F32', True, True), '24.2 / 29.0'),
+    ((16, 4096, 16, 40, 2, 128, 'Q3T_F32', False, False), '98.6 / 49.2'),
+    ((16, 4096, 16, 40, 2, 128, 'Q3T_F16', False, False), '33.9 / 26.1'),
+    ((16, 4096, 16, 40, 2, 64, 'Q3T_F32', False, False), '40.5 / 29.0'),
+    ((26, 13568, 32, 8, 1, 128, 'Q3T_F32', True, False), '217 / 68'),
+    ((97, 2048, 256, 16, 1, 128, 'Q3T_BF16', False, False), '34.6 / 24.2'),
+    ((64, 4096, 1, 16, 8, 128, 'Q3T_BF16', False, True), '39.3 / 126'),
+    ((10, 389, 1, 64, 8, 128, 'Q3T_F32', False, False), '28.6 / 16.3'),
+]
+
+
+@pytest.mark.parametrize('case,times', CHOICES, ids=[str(c[0][:-1]) for c in CHOICES])
+def test_the_library_chooses_what_is_quicker(pkg, case, times):
+    """By the workspace that it asks for, which reading once needs more of."""
+    batch, keys, page, q_heads, kv_heads, width, dtype, masked, once = case
+    shared = keys // page
+    sizes = dict(batch=batch, q_heads=q_heads, kv_heads=kv_heads, head_dim=width, dtype=getattr(pkg._lib, dtype), page_size=page,
+                 pages=shared + 64 * batch, table_width=shared + 64)
+    if masked:
+        sizes.update(mask=4096, mask_dtype=pkg._lib.Q3T_BOOL, mask_stride_b=keys + 64 * page, mask_stride_t=1)
+    chosen, always, never = (_bytes(pkg, shared, reserved=way, **sizes) for way in (0, 1, 2))
+    assert 0 < never and 0 < always and never != always
+    assert chosen == (always if once else never)
