@@ -323,7 +323,7 @@ class PagedArena:
     ``packed`` is (2 * layers, pages, kv_heads, page_size, head_dim), keys first, as the slot
     arena's packed tensor is; a page number names the same page of every layer.
 
-    ``dtype``: torch.int8 or torch.float8_e4m3fn holds the rows in 8 bits; their scales are ``packed_scales``
+    ``dtype``: torch.int8 or torch.float8_e4m3fn holds the rows, of head_dim 64 or 128, in 8 bits; their scales are ``packed_scales``
     (2 * layers, pages, kv_heads, page_size), and ``scales[i]`` is layer i's pair of them (None otherwise)."""
 
     def __init__(self, reference, pages, page_size=16, dtype=None):
@@ -335,6 +335,8 @@ class PagedArena:
         weight, config = next(reference.parameters()), reference.config
         if dtype is not None and dtype != weight.dtype and dtype not in _HELD:
             raise ValueError('an arena holds rows of the model\'s dtype, int8 or float8_e4m3fn')
+        if dtype in _HELD and config.head_dim not in (64, 128):
+            raise ValueError('rows of 8 bits have a head_dim of 64 or 128')
         layers = len(reference.layers)
         shape = (2 * layers, pages, config.num_key_value_heads, page_size, config.head_dim)
         self.packed = torch.zeros(shape, device=weight.device, dtype=weight.dtype if dtype is None else dtype)

@@ -1,9 +1,12 @@
-"""Shared pages of the paged cache without a GPU: what launches of any length have for their work."""
+"""Shared pages of the paged cache without a GPU: what launches of any length have for their work, which calls are refused, and
+which way the library reads."""
 import ctypes
 import subprocess
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
+import torch
 
 CSRC = Path(__file__).resolve().parents[1] / 'qwen3-tts-rsi-engine_amd' / 'csrc'
 
@@ -100,3 +103,19 @@ def test_the_library_chooses_what_is_quicker(pkg, case, times):
     chosen, always, never = (_bytes(pkg, shared, reserved=way, **sizes) for way in (0, 1, 2))
     assert 0 < never and 0 < always and never != always
     assert chosen == (always if once else never)
+
+
+@pytest.mark.parametrize('held', [torch.int8, torch.float8_e4m3fn], ids=str)
+def test_arenas_of_8_bits_for_other_widths_are_refused(pkg, held):
+    """When they are made, not at the first row."""
+    module = torch.nn.Linear(2, 2).bfloat16()
+
+    def arena(width, **kwargs):
+        config = SimpleNamespace(num_key_value_heads=8, head_dim=width)
+        return pkg.PagedArena(SimpleNamespace(parameters=module.parameters, layers=[None], config=config), pages=3, **kwargs)
+    for width in (32, 96, 256):
+        with pytest.raises(ValueError):
+            arena(width, dtype=held)
+        assert arena(width).packed.shape[-1] == width
+    for width in (64, 128):
+        assert arena(width, dtype=held).packed.shape[-1] == width
