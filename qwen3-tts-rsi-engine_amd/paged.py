@@ -221,7 +221,8 @@ def paged_attention(query, key_pages, value_pages, page_table, positions, *, sca
     left may all entries be numbers of no page (-1), and nothing is attended by those.  What each
     request attends is as without it, but where it saves enough (``read_once`` True or False: always, or
     never) the keys on them are read once for the whole batch, their weights then held in two parts of the queries'
-    type (of 16 bits): a relative 2^-16 in bf16, 2^-22 in fp16.  Pools of 8 bits are attended request by request."""
+    type (of 16 bits): a relative 2^-16 in bf16, 2^-22 in fp16.  Pools of 8 bits are
+    attended request by request, whatever ``read_once`` says."""
     return _attend(_attention_call(query, key_pages, value_pages, page_table, positions, scale, mask, out, scales, shared_pages,
                                    read_once))
 
@@ -431,17 +432,19 @@ class PagedCache(Cache):
     ``positions[b]`` and returns the layer's pools; ``step`` attends over them too, as
     ``PackedAttention`` calls it.  ``page_table`` and ``positions`` are read at every step as they are
     then, so a captured step follows changes of their contents.  ``shared_pages``: entries that all rows of the
-    table begin with, as ``paged_attention`` takes them (all but retired requests' rows, of -1); no request may write to those pages.
+    table begin with, as ``paged_attention`` takes them (all but retired requests' rows, of -1), and its ``read_once``; no request
+    may write to those pages.
 
     The lengths live on the device, so ``get_seq_length`` is 0: pass the model ``position_ids``, and as
     its mask None (a request then attends its keys up to its position) or one over the table's rows."""
 
-    def __init__(self, arena, page_table, positions, shared_pages=0):
+    def __init__(self, arena, page_table, positions, shared_pages=0, read_once=None):
         super().__init__(layers=[])
         self.arena = arena
         self.page_table = page_table
         self.positions = positions
         self.shared_pages = shared_pages
+        self.read_once = read_once
 
     def update(self, keys, values, layer_idx, cache_kwargs=None):
         if keys.shape[2] != 1:
@@ -460,7 +463,8 @@ class PagedCache(Cache):
         if getattr(mask, 'shape', ())[-1:] == (1,) and self.page_table.shape[1] * self.arena.page_size > 1:
             raise ValueError('the mask of a paged step must end in the key dimension')
         call = _attention_call(query, self.arena.keys[layer_idx], self.arena.values[layer_idx], self.page_table,
-                               self.positions, scale, mask, None, self.arena.scales[layer_idx], self.shared_pages)
+                               self.positions, scale, mask, None, self.arena.scales[layer_idx], self.shared_pages,
+                               *(() if self.read_once is None else (self.read_once,)))
         self.update(keys, values, layer_idx)
         return _attend(call)
 

@@ -40,3 +40,21 @@ def test_the_first_request_retires(pkg, device, prefix):
         assert_within(out, *expected(p))
         assert all((out[b] == 0).all() for b in range(batch) if not owned[b])
         positions += 1
+
+
+@pytest.mark.parametrize('once', [True, False])
+def test_a_step_reads_as_it_is_told(pkg, device, once):
+    """At a size where the library would do the other."""
+    prefix, batch = (512, 6) if once else (4096, 32)
+    model = Talker(layers=1, hidden=256, seed=3, dtype=BF16).to(device).eval()
+    arena = pkg.PagedArena(model, pages=prefix // 16 + batch)
+    arena.packed.normal_()
+    shared = arena.allocate(prefix // 16)
+    table = arena.page_table([shared + arena.allocate(1) for _ in range(batch)])
+    positions = torch.full((batch,), prefix + 3, device=device)
+    query, rows = torch.randn(batch, 1, 16, 128, device=device).to(BF16), torch.randn(batch, 8, 1, 128, device=device).to(BF16)
+    out = pkg.PagedCache(arena, table, positions, len(shared), read_once=once).step(query, rows, rows, 0)
+    call = lambda once: pkg.paged_attention(query, arena.keys[0], arena.values[0], table, positions, shared_pages=len(shared),  # noqa: E731
+                                            read_once=once)
+    assert torch.equal(out, call(once))
+    assert torch.equal(call(None), call(not once)) and not torch.equal(out, call(None))
