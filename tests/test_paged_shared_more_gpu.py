@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests._paged import assert_within, attention64
-from tests._paged_more import expected, problem, run
+from tests._paged_more import HELD, expected, problem, run
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +98,42 @@ def test_a_captured_launch_of_which_requests_retire(pkg, device):
     graph.replay()
     torch.cuda.synchronize()
     assert_within(out, *expected(p))
+
+
+@pytest.mark.parametrize('held', HELD, ids=str)
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (F16, 64), (F32, 128)], ids=str)
+@pytest.mark.parametrize('batch', [3, 40])
+def test_pools_of_8_bits_are_read_by_each_request(pkg, device, held, dtype, width, batch):
+    """To the bound that they have without shared pages, and to the same bits."""
+    p = problem(device, [481 + b % 50 for b in range(batch)], shared=20, page=24, held=held, dtype=dtype, width=width, seed=43)
+    out = run(pkg, p)
+    p.shared = 0
+    assert torch.equal(out, run(pkg, p))
+    assert_within(out, *expected(p))
+
+
+@pytest.mark.parametrize('page,prefix,heads', [(1, 9000, (16, 1)), (1, 3000, (8, 4)), (2, 9000, (4, 1)), (3, 12000, (16, 1))], ids=str)
+@pytest.mark.parametrize('dtype', [BF16, F32], ids=str)
+@pytest.mark.parametrize('masked', [False, True])
+def test_parts_that_end_with_the_pages_that_a_workgroup_knows(pkg, device, page, prefix, heads, dtype, masked):
+    """Pages of few rows: 1022 of them hold fewer keys than a part would have otherwise, so that there are more parts."""
+    p = problem(device, [prefix + 1 + b for b in range(3)], shared=prefix // page, page=page, q_heads=heads[0], kv_heads=heads[1], dtype=dtype,
+                seed=44)
+    mask = None
+    if masked:
+        mask = torch.rand(3, 1, 1, p.table.shape[1] * page, generator=torch.Generator().manual_seed(45)).to(device) < 0.8
+    assert_within(run(pkg, p, mask=mask), *expected(p, mask=mask))
+
+
+@pytest.mark.parametrize('dtype,width', [(BF16, 128), (F16, 64), (F32, 64)], ids=str)
+@pytest.mark.parametrize('batch', [5, 40])
+@pytest.mark.parametrize('odd', [float('nan'), float('inf')])
+def test_queries_that_are_not_finite_stay_with_their_requests(pkg, device, dtype, width, batch, odd):
+    p = problem(device, [650 + b % 30 for b in range(batch)], shared=40, dtype=dtype, width=width, seed=46)
+    p.query[2, 0, 3, 5] = odd
+    out = run(pkg, p).cpu()
+    assert out[2, 0, 3].isnan().all()
+    p.query[2, 0, 3] = 0
+    want, tol = expected(p)
+    out[2, 0, 3], want[2, 0, 3] = 0, 0
+    assert_within(out, want, tol)
