@@ -493,7 +493,7 @@ int q3t_paged_write_quantized(const q3t_paged_write_args *args, int64_t dtype, c
  *   values[b, h, t, :] = value_pages[page_table[b, j / page_size], h, j % page_size, :]
  * for t < min(tokens, lengths[b]) (lengths == NULL: all tokens).  Rows past those, rows whose j lies
  * outside [0, table_width * page_size) and rows on no page are zeros.  scales == NULL: the pools have the
- * rows' type, and elements of elem_size bytes are copied; else the pools have 8 bits (head_dim 64 or 128, bases and
+ * rows' type, and elements of dtype are copied; else the pools have 8 bits (head_dim 64 or 128, bases and
  * strides multiples of 16 bytes), and elements are scale * element in float32, rounded to dtype.
  * The counterpart of q3t_copy_strided out of a slot (SlotArena.move, continuous.py:124-128).
  */

@@ -682,10 +682,12 @@ struct PrefixPlan {
     int64_t states, workgroups, bytes;  // states: in all
 };
 
-// By sizes alone: tiles for the columns that there are, and as many parts as fill the card, with some keys each at least: a
-// state is written and read again for every part.  us of both launches with 64 / 256 / 512 keys at least, bf16: 64 requests over 4096
-// keys 57.6 / 56.2 / 57.2, 64 over 2048 30.0 / 27.8 / 31.9, 32 over 1024 19.5 / 20.2 / 24.0, 128 over 1024 46.9 / 42.3 / 44.7; with 64 /
-// 128 / 256, float32 under a mask: 21 over 792 25.3 / 27.2 / 33.0.
+// By sizes alone: tiles for the columns that there are, and a part for each CU that blocks and heads leave, but some keys each at
+// least, as a state is written and read again for every part, and no more than a request's end reads at once (8 for groups of 16 query
+// heads of 128: with few KV heads the card is not filled).  Only pages of few rows, of which a workgroup knows 1022, make more parts:
+// 896 keys each in pages of one row.  us of both launches with 64 / 256 / 512 keys at least, bf16, weights in one part: 64 requests
+// over 4096 keys 57.6 / 56.2 / 57.2, 64 over 2048 30.0 / 27.8 / 31.9, 32 over 1024 19.5 / 20.2 / 24.0, 128 over 1024 46.9 / 42.3 / 44.7;
+// with 64 / 128 / 256, float32 under a mask: 21 over 792 25.3 / 27.2 / 33.0.
 
 template <typename T>
 static PrefixPlan prefix_plan(const q3t_paged_args *a, int64_t keys) {
@@ -697,7 +699,7 @@ static PrefixPlan prefix_plan(const q3t_paged_args *a, int64_t keys) {
     z.blocks = (z.columns + z.cw * z.ct * kColumns - 1) / (z.cw * z.ct * kColumns);
     const int64_t step = z.step = z.kw * (sizeof(T) == 4 ? 16 : 32), workgroups = 256;
     int64_t parts = workgroups / (z.blocks * a->kv_heads);
-    // each request's end reads the states of its columns: up to eight for a thread of 512
+    // each request's end reads the states of its columns: up to eight for a thread of 512, as far as pages allow
     const int64_t group = a->q_heads / a->kv_heads, most_parts = 16384 / ((group < kColumns ? group : kColumns) * a->head_dim);
     if (parts > most_parts) parts = most_parts;
     if (parts < 1) parts = 1;

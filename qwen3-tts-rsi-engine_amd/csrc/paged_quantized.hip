@@ -7,7 +7,8 @@
 // registers.  Both are bound by HBM where rows are many and by the launch where they are few.  us per launch, the rows not in the
 // caches: 16 prompts of up to 1024 rows, 8 heads of 128, bf16 into int8 16.4 (3.4 TB/s), and read back behind the write, padding
 // and all, 16.4 (5.3); both in a graph 33.0 (4.3, nine tenths of a copy's rate); 48 requests of up to 777 rows, 12 heads of 64,
-// e4m3 into fp16 34.4 (4.3); one token of 64 requests 2.5 each way; 300 rows of one request 3.2.
+// e4m3 into fp16 34.8 (4.3); one token of 64 requests 2.5 each way; 300 rows of one request 3.2.  Out of pools of the rows' own type:
+// the 48 requests in fp16 34.8 (5.1), in bf16 with 8 heads of 128 45.3 (5.2, a copy's rate and a little more); the one of 300 2.7.
 #include "paged_index.hpp"
 #include "q3t_common.hpp"
 
