@@ -8,8 +8,8 @@
 // to LDS, elements are widened to bf16 (exact) on the way into the products, and a key's scale multiplies its score and
 // a value's its weight, outside of them.  us per launch in a graph (TB/s of rows and scales; the same in bf16): 128 requests of
 // 100..4095 keys, 8 KV heads of 128, 32 query heads, int8 95 (5.7; 175), 64 of 64..1023 in e4m3 23.0 (3.4; 30.7), 21 of 1..700
-// with float32 queries under a mask, 12 heads of 64, e4m3 12.1 (1.2; float32 rows 18.0), one of 300 8.1 (7.6).  With fp16 queries the first two take 98 and 25.9, under a bool mask 94
-// and 25.9.
+// with float32 queries under a mask, 12 heads of 64, e4m3 12.1 (1.2; float32 rows 18.0), one of 300 8.1 (7.6).  With
+// fp16 queries the first two take 98 and 25.9, under a bool mask 94 and 25.9.
 //
 // A shared prefix is read once for the batch, by a launch ahead of that for the requests' own keys (paged_prefix.hpp): 128 requests
 // behind 16384 keys, 32 query heads, 102 us (64 for the prefix) where requests that each read it take 960, 64 behind 4096 58.1 (18.6)

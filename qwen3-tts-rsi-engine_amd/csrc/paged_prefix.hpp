@@ -16,8 +16,9 @@
 //     each for itself.
 // The matrix cores bound it from some hundred columns on (4 * 16384 keys, 128 requests, 32 query heads over 8 KV heads of 128 in
 // bf16: 51.5 GFLOP, the weights' two parts counted, in 64 us, 0.80 PFLOP/s and 0.94 past the start of 9 us, where a large library
-// product reaches 1.2), the start and the stages' chain below it (8 KV heads, 128 columns each, 4096 keys 18.6 us).  Waves that share a stage alternate between
-// matrix and vector instructions in two groups (with the addresses of a part worked out once, 65 -> 57 us, with weights in one part).
+// product reaches 1.2), the start and the stages' chain below it (8 KV heads, 128 columns each, 4096 keys 18.6 us).  Waves that
+// share a stage alternate between matrix and vector instructions in two groups (with the addresses of a part worked out once, 65 ->
+// 57 us, with weights in one part).
 #pragma once
 
 #include "paged_kernel.hpp"
